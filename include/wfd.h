@@ -38,10 +38,12 @@ typedef struct ihipStream_t* wfd_stream_t; /* == hipStream_t */
 enum { WFD_F32 = 0, WFD_BF16 = 1 };
 enum { WFD_OK = 0, WFD_BAD_ARG = -1, WFD_UNSUPPORTED = -2, WFD_LAUNCH = -3, WFD_WORKSPACE = -4 };
 enum { WFD_EPI_PLAIN = 0, WFD_EPI_SWIGLU = 1 };
+enum { WFD_E4M3 = 0, WFD_INT8 = 1 }; /* codes of an 8-bit slot cache */
 
 /* Message for the last failing call on this thread. */
 const char* wfd_last_error(void);
-/* Bumped whenever an entry point's signature changes or one is added (5: wfd_argmax's
+/* Bumped when an entry point's signature changes, and up to 8 when one was added (the
+   later ones -- wfd_*_q, wfd_attn_shared, wfd_sample -- are found by their symbols; 5: wfd_argmax's
    accept flags, wfd_attn_varlen_rows; 6: wfd_linear_argmax, wfd_argmax_groups;
    7: folded norm pairs -- wfd_linear_prep, wfd_norm_prep, the row-scale argument of
    wfd_linear, wfd_linear_qkv_rope_append and wfd_linear_argmax; 8: wfd_attn_varlen,
@@ -223,6 +225,60 @@ int wfd_attn_prefill(const void* q, const void* k_cache, const void* v_cache, in
  */
 int wfd_kv_append(const void* k, const void* v, void* k_cache, void* v_cache, int64_t kv_block_rows,
                   const int64_t* flat_row, int n, int Hkv, int Dh, int dtype, wfd_stream_t stream);
+
+/*
+ * The 8-bit slot cache. A row of Dh values x of one kv head is kept as Dh codes
+ * (WFD_E4M3: OCP e4m3, |code| <= 448; WFD_INT8: |code| <= 127) and one exponent
+ * byte b: value = code * 2^(b - 127), 2^(b - 127) the smallest power of two, not
+ * below 2^-126, with max|x| <= 448 (127) times it; a code is x / 2^(b - 127)
+ * rounded once to nearest, ties to even. A row that holds an infinity or NaN
+ * gets b = 255 and reads as NaN, it alone. (Rounding up may carry values beyond
+ * 1.9 * 2^127 to infinity.) The codes have the layout kv_block_rows gives a
+ * cache of one byte per element, the exponent bytes the same layout without Dh:
+ * (rows, Hkv), or (rows / B, Hkv, B). Dh 64 or 128; codes 16-byte aligned.
+ * It takes (Dh + 1) / (2 Dh) of a bf16 cache's bytes.
+ *
+ * wfd_kv_append_q: cache row flat_row[i] = k[i] / v[i], (Hkv, Dh) of `dtype` at
+ * row pitches ldk / ldv (elements). Rows of flat_row are distinct, except that
+ * rows never read (padding) may repeat: a row written twice in one call holds
+ * either's codes and either's exponent.
+ * wfd_qkv_rope_append_q: wfd_qkv_rope_append into an 8-bit cache: q_out as
+ * there, bit for bit; the codes of k are made from the rotation itself, without
+ * rounding it to `dtype` first. The rope tables are 16-byte aligned too.
+ * wfd_kv_read_q: k_out / v_out (n, Hkv, Dh) of `dtype` = the values of cache
+ * rows flat_row[i] (any rows, repeats allowed). Exact, save bf16 values below
+ * 2^-126.
+ * Replaces: nothing in the reference, whose caches keep the model's dtype; they
+ *   stand beside StaticKVCache.write_range / write_scatter / gather
+ *   (src/decoding/kv_cache.py:97-121) and BatchStaticKVCache.write_tokens
+ *   (src/decoding/batch_kv_cache.py:61-73).
+ */
+int wfd_kv_append_q(const void* k, int64_t ldk, const void* v, int64_t ldv, void* k_codes, void* v_codes,
+                    uint8_t* k_exp, uint8_t* v_exp, int code, int64_t kv_block_rows, const int64_t* flat_row, int n,
+                    int Hkv, int Dh, int dtype, wfd_stream_t stream);
+int wfd_qkv_rope_append_q(const void* qkv, int64_t ldq, const int32_t* pos, const float* rope_cos,
+                          const float* rope_sin, int rope_rows, const int64_t* flat_row, void* q_out, void* k_codes,
+                          void* v_codes, uint8_t* k_exp, uint8_t* v_exp, int code, int64_t kv_block_rows, int n, int H,
+                          int Hkv, int Dh, int dtype, wfd_stream_t stream);
+int wfd_kv_read_q(const void* k_codes, const void* v_codes, const uint8_t* k_exp, const uint8_t* v_exp, int code,
+                  int64_t kv_block_rows, const int64_t* flat_row, void* k_out, void* v_out, int n, int Hkv, int Dh,
+                  int dtype, wfd_stream_t stream);
+
+/*
+ * wfd_attn_decode over an 8-bit cache (codes, exponents, `code` and
+ * kv_block_rows as wfd_kv_append_q lays them out): q and out (n, H, Dh) of
+ * `dtype`, query i attends rows kv_row_base[i] .. + kv_len[i] - 1, a query with
+ * kv_len <= 0 gets a zero row. The values are used as they are stored (converted
+ * without rounding), with fp32 probabilities, sums and division. A key row
+ * marked non-finite makes the rows that attend it NaN, no others. H / Hkv in
+ * {1, 2, 4}, at most 32767 rows; workspace >= wfd_attn_workspace_bytes(n, H, Dh,
+ * kv_len_max). A row's bits depend on that row only.
+ * Replaces: what wfd_attn_decode replaces, over caches the reference does not have.
+ */
+int wfd_attn_decode_q(const void* q, const void* k_codes, const void* v_codes, const uint8_t* k_exp,
+                      const uint8_t* v_exp, int code, int64_t kv_block_rows, const int64_t* kv_row_base,
+                      const int32_t* kv_len, void* out, int n, int H, int Hkv, int Dh, int dtype, float scale,
+                      int kv_len_max, void* workspace, size_t ws_bytes, wfd_stream_t stream);
 
 /*
  * SwiGLU of n rows laid out [gate (F) | up (F)] with row stride ldg:

@@ -1,0 +1,133 @@
+"""Host-side refusals of the serving operators (CPU): in the front end before the
+library is reached, and in the C entry points before any launch."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from wavefront_decoding_amd import _lib, ops
+
+
+def _m(*shape, dtype=torch.bfloat16):
+    return torch.empty(*shape, dtype=dtype, device="meta")
+
+
+def _q(shape=(64, 2, 64), code=torch.int8):
+    e = lambda: _m(*shape[:-1], dtype=torch.uint8)  # noqa: E731
+    return ops.QuantKV(_m(*shape, dtype=code), _m(*shape, dtype=code), e(), e())
+
+
+@pytest.fixture
+def front(monkeypatch):
+    """The front end's checks alone: meta tensors pass as the current device's, the library is out of reach."""
+    monkeypatch.setattr(ops, "_need_cuda", lambda *ts: None)
+    monkeypatch.setattr(ops, "_need_current", lambda *ts: None)
+
+    def no_library():
+        raise AssertionError("validation should have rejected the call before the library is loaded")
+
+    monkeypatch.setattr(_lib, "load", no_library)
+
+
+def test_host_tensors_are_refused():
+    t = torch.zeros(2, 2, 64, dtype=torch.bfloat16)
+    cache = ops.QuantKV.zeros((8, 2, 64), device="cpu")
+    rows = torch.zeros(2, dtype=torch.int64)
+    for call in (lambda: ops.kv_append_q(t, t, cache, rows), lambda: ops.kv_read_q(cache, rows),
+                 lambda: ops.attn_decode_q(t, cache, rows, rows.int(), kv_len_max=4)):
+        with pytest.raises(_lib.WfdError, match="GPU tensors"):
+            call()
+
+
+def test_operands_on_another_device_are_refused(monkeypatch):
+    class Fake:
+        is_cuda, device = True, torch.device("cuda:1")
+
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    with pytest.raises(_lib.WfdError, match="current device is cuda:0"):
+        ops._need_current(Fake())
+
+
+def test_quant_cache_shapes():
+    c = ops.QuantKV.zeros((3, 2, 16, 64), code=torch.int8, device="cpu")
+    assert (c.Hkv, c.Dh, c.block_rows, c.code) == (2, 64, 16, _lib.INT8) and c.nbytes == 2 * 3 * 2 * 16 * 65
+    codes, exps = torch.zeros(4, 2, 64, dtype=torch.int8), torch.zeros(4, 2, dtype=torch.uint8)
+    for bad in ((codes.bfloat16(), codes.bfloat16(), exps, exps), (codes, codes[:2], exps, exps),
+                (codes, codes, exps[:, :1], exps), (codes, codes, exps, exps.int()),
+                (codes, codes.view(torch.float8_e4m3fn), exps, exps),
+                (codes, codes, torch.zeros(2, 4, dtype=torch.uint8).t(), exps)):
+        with pytest.raises(_lib.WfdError):
+            ops.QuantKV(*bad)
+    with pytest.raises(_lib.WfdError):
+        ops.QuantKV.zeros((4, 2, 64), code=torch.bfloat16, device="cpu")
+
+
+def test_quant_front_end_refusals(front):
+    c, rows = _q(), _m(4, dtype=torch.int64)
+    k = _m(4, 2, 64)
+    for bad in ((_m(4, 3, 64), k, rows), (k, _m(4, 2, 32), rows), (k, _m(5, 2, 64), rows), (k, k.float(), rows),
+                (k, k, _m(3, dtype=torch.int64)), (k, k, _m(4, dtype=torch.int32)),
+                (_m(4, 64, 2).transpose(1, 2), k, rows)):
+        with pytest.raises(_lib.WfdError):
+            ops.kv_append_q(bad[0], bad[1], c, bad[2])
+    with pytest.raises(_lib.WfdError, match="dtype"):
+        ops.kv_read_q(c, rows, dtype=torch.float16)
+    with pytest.raises(_lib.WfdError, match="k_out"):
+        ops.kv_read_q(c, rows, k_out=_m(3, 2, 64))
+    i32 = _m(4, dtype=torch.int32)
+    cos = _m(16, 32, dtype=torch.float32)
+    for bad in (dict(qkv=_m(4, 500)), dict(pos=rows), dict(cos=_m(16, 16, dtype=torch.float32)),
+                dict(H=7), dict(Hkv=1), dict(q_out=_m(3, 4, 64))):
+        a = dict(qkv=_m(4, 512), pos=i32, cos=cos, H=4, Hkv=2, q_out=None) | bad
+        with pytest.raises(_lib.WfdError):
+            ops.qkv_rope_append_q(a["qkv"], a["pos"], a["cos"], a["cos"], rows, c, a["H"], a["Hkv"], 64, a["q_out"])
+    q = _m(4, 4, 64)
+    for bad in (dict(q=_m(4, 4, 128)), dict(base=i32), dict(lens=rows), dict(lens=_m(3, dtype=torch.int32)),
+                dict(m=0), dict(out=_m(4, 4, 64, dtype=torch.float32)), dict(q=_m(4, 64, 4).transpose(1, 2)),
+                dict(q=_m(4, 4, 64, dtype=torch.float16), out=_m(4, 4, 64, dtype=torch.float16))):
+        a = dict(q=q, base=rows, lens=i32, m=8, out=None) | bad
+        with pytest.raises(_lib.WfdError):
+            ops.attn_decode_q(a["q"], c, a["base"], a["lens"], kv_len_max=a["m"], out=a["out"])
+    with pytest.raises(_lib.WfdError, match="exceeds the cache block"):
+        ops.attn_decode_q(q, _q((4, 2, 16, 64)), rows, i32, kv_len_max=17)
+
+
+def test_quant_entry_points_check_before_launch():
+    lib = _lib.load()
+    err = lib.wfd_last_error
+    app = lambda n=1, Hkv=2, Dh=64, dt=1, code=0, br=0, ld=128: lib.wfd_kv_append_q(  # noqa: E731
+        None, ld, None, ld, None, None, None, None, code, br, None, n, Hkv, Dh, dt, None)
+    assert app(n=-1) == -1 and app(Hkv=0) == -1 and app(Hkv=70000) == -1 and app(br=-1) == -1 and b"bad shape" in err()
+    assert app(Dh=96) == -2 and app(code=2) == -2 and app(dt=2) == -2 and b"dtype" in err()
+    assert app(ld=127) == -1 and b"row pitch" in err()
+    assert app(n=0) == 0 and app() == -1 and b"null pointer" in err()
+    rope = lambda n=1, H=4, S=8, ld=512: lib.wfd_qkv_rope_append_q(  # noqa: E731
+        None, ld, None, None, None, S, None, None, None, None, None, None, 0, 0, n, H, 2, 64, 1, None)
+    assert rope(H=0) == -1 and rope(S=0) == -1 and rope(ld=511) == -1 and b"ldq=511" in err()
+    assert rope(n=0) == 0 and rope() == -1 and b"null pointer" in err()
+    read = lambda n=1, dt=1: lib.wfd_kv_read_q(None, None, None, None, 1, 0, None, None, None, n, 2, 64, dt,  # noqa: E731
+                                               None)
+    assert read(dt=3) == -2 and read(n=0) == 0 and read() == -1
+    att = lambda n=1, H=4, Hkv=2, Dh=64, dt=1, m=8, br=0: lib.wfd_attn_decode_q(  # noqa: E731
+        None, None, None, None, None, 0, br, None, None, None, n, H, Hkv, Dh, dt, 0.1, m, None, 0, None)
+    assert att(H=3) == -1 and att(m=0) == -1 and att(br=4, m=5) == -1 and b"kv_block_rows=4" in err()
+    assert att(H=6) == -2 and att(dt=2) == -2 and att(Dh=32) == -2 and att(n=40000) == -2 and b"beyond" in err()
+    assert att(n=0) == 0 and att() == -1 and b"null pointer" in err()
+
+
+@pytest.mark.skipif(torch.cuda.device_count() > 0, reason="made-up device addresses: run only where no GPU is "
+                    "visible, so a regressed check cannot launch a kernel on them")
+def test_quant_alignment_is_checked():
+    lib = _lib.load()
+    p = [4096] * 4
+    assert lib.wfd_kv_append_q(4096 + 8, 128, 4096, 128, *p, 0, 0, 4096, 1, 2, 64, 1, None) == -1
+    assert lib.wfd_kv_append_q(4096, 132, 4096, 128, *p, 0, 0, 4096, 1, 2, 64, 1, None) == -1
+    assert lib.wfd_kv_append_q(4096, 128, 4096, 128, 4096 + 4, *p[1:], 0, 0, 4096, 1, 2, 64, 1, None) == -1
+    assert lib.wfd_qkv_rope_append_q(4096, 512, 4096, 4096 + 4, 4096, 8, 4096, 4096, *p, 0, 0, 1, 4, 2, 64, 1,
+                                     None) == -1
+    assert lib.wfd_kv_read_q(*p, 0, 0, 4096, 4096 + 2, 4096, 1, 2, 64, 1, None) == -1
+    assert lib.wfd_attn_decode_q(4096 + 2, *p, 0, 0, 4096, 4096, 4096, 1, 4, 2, 64, 1, 0.1, 8, 4096, 1 << 20,
+                                 None) == -1
+    assert b"16-byte aligned" in lib.wfd_last_error()
+    assert lib.wfd_attn_decode_q(4096, *p, 0, 0, 4096, 4096, 4096, 1, 4, 2, 64, 1, 0.1, 8, 4096, 16, None) == -4
+    assert b"workspace" in lib.wfd_last_error()

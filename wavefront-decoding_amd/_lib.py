@@ -19,6 +19,7 @@ LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libwfd.so")
 
 F32, BF16 = 0, 1
 EPI_PLAIN, EPI_SWIGLU = 0, 1
+E4M3, INT8 = 0, 1
 STATUS = {0: "ok", -1: "bad argument", -2: "unsupported", -3: "launch failure", -4: "workspace too small"}
 
 _vp = ctypes.c_void_p
@@ -48,6 +49,13 @@ SIGNATURES: dict[str, tuple] = {
     "wfd_swiglu": (_i32, [_vp, _i64, _vp, _i64, _i32, _i32, _i32, _vp]),
     "wfd_qkv_rope_append": (_i32, [_vp, _i64, _vp, _vp, _vp, _i32, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32,
                                    _i32, _i32, _vp]),
+    "wfd_kv_append_q": (_i32, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i32, _i64, _vp, _i32, _i32, _i32, _i32,
+                               _vp]),
+    "wfd_qkv_rope_append_q": (_i32, [_vp, _i64, _vp, _vp, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i64, _i32,
+                                     _i32, _i32, _i32, _i32, _vp]),
+    "wfd_kv_read_q": (_i32, [_vp, _vp, _vp, _vp, _i32, _i64, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _vp]),
+    "wfd_attn_decode_q": (_i32, [_vp, _vp, _vp, _vp, _vp, _i32, _i64, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32,
+                                 _f32, _i32, _vp, _sz, _vp]),
     "wfd_linear_k_multiple": (_i32, [_i32]),
     "wfd_linear_pack": (_i32, [_vp, _vp, _i32, _i32, _i32, _i32, _i32, _vp]),
     "wfd_linear": (_i32, [_vp, _vp, _i64, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _vp, _vp]),

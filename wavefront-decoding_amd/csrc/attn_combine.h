@@ -11,13 +11,16 @@ constexpr int kAttnSplit = 1024;  // keys per workgroup
 
 __device__ __forceinline__ float attn_finish(float O, float L) { return L > 0.f ? O / L : 0.f; }
 
+// The same where a NaN among a row's keys is to reach the row.
+__device__ __forceinline__ float attn_finish_nan(float O, float L) { return L == 0.f ? 0.f : O / L; }
+
 // Merge of a row's split partials, in split order: M = max m_s, then
 // L = sum l_s * 2^(m_s - M) and O = sum o_s * 2^(m_s - M), one fma per split.
 // The partials are read in batches of kCombineBatch independent loads, so a
 // row of many splits waits on memory twice per batch, not twice per split.
 constexpr int kCombineBatch = 8;
 
-template <typename T, int DH>
+template <typename T, int DH, bool KEEP_NAN = false>
 __global__ __launch_bounds__(DH) void attn_combine_kernel(const float* __restrict__ part_o,
                                                           const float* __restrict__ part_ml,
                                                           const int32_t* __restrict__ kv_len, T* __restrict__ out,
@@ -58,7 +61,7 @@ __global__ __launch_bounds__(DH) void attn_combine_kernel(const float* __restric
       }
     }
   }
-  Elem<T>::store(out + ((int64_t)i * H + h) * DH + d, attn_finish(O, L));
+  Elem<T>::store(out + ((int64_t)i * H + h) * DH + d, KEEP_NAN ? attn_finish_nan(O, L) : attn_finish(O, L));
 }
 
 // Row r of a packed varlen call (the FA varlen convention): query row r of
