@@ -511,6 +511,32 @@ int wfd_argmax(const float* logits, int64_t ld, int64_t* out, int64_t* ring, con
                int64_t ring_len, const int64_t* expect, int32_t* accept, int n, int vocab, wfd_stream_t stream);
 
 /*
+ * Tokens drawn from logits (n, vocab) fp32, row pitch ld: out[i] from row i, the
+ * caller's uniform number u[i] in [0, 1) and the row's parameters (device
+ * arrays; NULL: off). With w_j = exp((l_j - max l) / temperature[i]) and the
+ * tokens ordered by logit, largest first, the lower index first among equals,
+ * these are kept: the first top_k[i]; of these the shortest run whose sum of w
+ * reaches top_p[i] of theirs; of these the ones with w_j >= min_p[i], the first
+ * always. The token is the lowest kept index at which the running sum of w over
+ * the kept tokens, in index order, exceeds u[i] times their sum. So the same
+ * logits and the same u give the same token wherever the row is, and a draft
+ * can be verified by drawing it again. w is rounded to a multiple of 2^-44 (below
+ * 2^-45 a token is never drawn, whatever u), and the sums of these are exact.
+ * Off for a row: temperature 1, top_k <= 0 or >= vocab, top_p >= 1 or NaN, min_p
+ * <= 0 or NaN. temperature <= 0 or NaN: the greedy token (wfd_argmax's). top_p
+ * <= 0 keeps one token. u outside [0, 1) counts as the nearest inside, NaN as 0.
+ * Logits of -inf are never drawn; equal infinite largest logits share the draw;
+ * a row of nothing but -inf gives 0 and a row with a NaN the index of its first
+ * NaN, as wfd_argmax does. ring / ring_rows / ring_len and expect / accept as in
+ * wfd_argmax. vocab at most 524288.
+ * Replaces: the position-seeded draw of temperature sampling
+ *   (src/decoding/acceptance.py:61-214), with its .item() per token.
+ */
+int wfd_sample(const float* logits, int64_t ld, const float* u, const float* temperature, const int32_t* top_k,
+               const float* top_p, const float* min_p, int64_t* out, int64_t* ring, const int32_t* ring_rows,
+               int64_t ring_len, const int64_t* expect, int32_t* accept, int n, int vocab, wfd_stream_t stream);
+
+/*
  * Column groups of wfd_linear_argmax for this shape: the few-row launch's
  * workgroups (a 16-column tile, or half a tile when there are few tiles), or
  * 0 where wfd_linear would not take the few-row kernel (n above 16, a K too

@@ -131,3 +131,50 @@ def test_quant_alignment_is_checked():
     assert b"16-byte aligned" in lib.wfd_last_error()
     assert lib.wfd_attn_decode_q(4096, *p, 0, 0, 4096, 4096, 4096, 1, 4, 2, 64, 1, 0.1, 8, 4096, 16, None) == -4
     assert b"workspace" in lib.wfd_last_error()
+
+
+# ---------------------------------------------------------------------------
+# drawing tokens
+# ---------------------------------------------------------------------------
+def test_sample_front_end_refusals(front):
+    l, u = _m(4, 100, dtype=torch.float32), _m(4, dtype=torch.float32)
+    i32, i64 = _m(4, dtype=torch.int32), _m(4, dtype=torch.int64)
+    for kw in (dict(logits=_m(4, 100)), dict(logits=l.t()), dict(logits=l[0]), dict(u=u[:3]), dict(u=u.double()),
+               dict(temperature=u[:3]), dict(top_k=i64), dict(top_k=u), dict(top_p=i32), dict(min_p=u.double()),
+               dict(n=5), dict(n=-1), dict(out=i32), dict(out=i64[:3]), dict(ring=i64), dict(expect=i64),
+               dict(accept=i32), dict(expect=i64, accept=i64), dict(temperature=_m(8, dtype=torch.float32)[::2])):
+        a = dict(logits=l, u=u) | kw
+        with pytest.raises(_lib.WfdError):
+            ops.sample(a.pop("logits"), a.pop("u"), **a)
+
+
+def test_sample_entry_point_checks_before_launch():
+    lib = _lib.load()
+    call = lambda n=1, V=10, ld=10, ring=None, expect=None: lib.wfd_sample(  # noqa: E731
+        None, ld, None, None, None, None, None, None, ring, None, 0, expect, None, n, V, None)
+    assert call(n=-1) == -1 and call(V=0) == -1 and call(ld=9) == -1 and b"ld=9" in lib.wfd_last_error()
+    assert call(V=(1 << 19) + 1, ld=1 << 20) == -2 and b"at most 524288" in lib.wfd_last_error()
+    assert call(n=0) == 0 and call() == -1 and b"null pointer" in lib.wfd_last_error()
+
+
+def test_sampler_parameters_and_numbers():
+    from wavefront_decoding_amd.acceptance import SeededSampler
+    from wavefront_decoding_amd.policy import SampledPolicy, SsdPolicy
+
+    for bad in (dict(temperature=-0.1), dict(top_k=-1), dict(top_p=0.0), dict(top_p=1.1), dict(min_p=-0.1),
+                dict(min_p=1.5), dict(temperature=float("nan"))):
+        with pytest.raises(ValueError):
+            SeededSampler(0, **bad)
+        with pytest.raises(ValueError):
+            SampledPolicy(8, 2, **bad)
+    with pytest.raises(ValueError):
+        SsdPolicy(8, 2, mode="sample")
+    with pytest.raises(ValueError):
+        SampledPolicy(8, 2, mode="greedy")
+    a, b, c = SeededSampler(3), SeededSampler(3), SeededSampler(4)
+    at = [0, 1, 4095, 4096, 100000]
+    assert [a.uniform(p) for p in at] == [b.uniform(p) for p in reversed(at)][::-1]
+    assert all(0.0 <= a.uniform(p) < 1.0 for p in at) and a.uniform(0) != c.uniform(0)
+    assert len({a.uniform(p) for p in at}) == len(at)
+    made = SampledPolicy(8, 2, sample_seed=5, temperature=0.5, top_k=7).make_sampler()
+    assert (made.seed, made.temperature, made.top_k, made.top_p) == (5, 0.5, 7, 1.0)

@@ -346,4 +346,27 @@ __device__ __forceinline__ void argmax_merge(float& bv, int& bi, float ov, int o
   }
 }
 
+// Row i's id ix: out[i], the accept flag, the token ring.
+__device__ __forceinline__ void argmax_finish(int i, int ix, int64_t* __restrict__ out, int64_t* __restrict__ ring,
+                                              const int32_t* __restrict__ ring_rows, int64_t ring_len,
+                                              const int64_t* __restrict__ expect, int32_t* __restrict__ accept) {
+  out[i] = (int64_t)ix;
+  if (accept) {
+    // greedy acceptance on the device: the token speculated at the next
+    // position is a plain id (>= 0) or a ring handle -(slot + 1) written by
+    // an earlier pass; anything else is "nothing to compare" (reads 0)
+    const int64_t e = expect[i];
+    int64_t want = -1;
+    if (e >= 0)
+      want = e;
+    else if (ring && e >= -ring_len)
+      want = ring[-e - 1];
+    accept[i] = want == (int64_t)ix ? 1 : 0;
+  }
+  if (ring) {
+    const int32_t r = ring_rows[i];
+    if (r >= 0 && r < ring_len) ring[r] = (int64_t)ix;
+  }
+}
+
 }  // namespace wfd

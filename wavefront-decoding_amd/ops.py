@@ -864,6 +864,34 @@ def argmax(logits: torch.Tensor, *, n: int | None = None, out: torch.Tensor | No
     return out
 
 
+def sample(logits: torch.Tensor, u: torch.Tensor, *, temperature: torch.Tensor | None = None,
+           top_k: torch.Tensor | None = None, top_p: torch.Tensor | None = None, min_p: torch.Tensor | None = None,
+           n: int | None = None, out: torch.Tensor | None = None, ring: torch.Tensor | None = None,
+           ring_rows: torch.Tensor | None = None, expect: torch.Tensor | None = None,
+           accept: torch.Tensor | None = None, accept_mapped: tuple[int, int] | None = None) -> torch.Tensor:
+    """out[i] = the token drawn from logits[i] with the uniform number u[i]
+    (wfd_sample has the definition): parameters per row, on the device
+    (float32, top_k int32; None: off), temperature 0 greedy. The outputs are
+    argmax's: with `ring`, ring[ring_rows[i]] = out[i]; with `expect`, accept
+    flags of the drawn tokens."""
+    _need_current(logits, u, temperature, top_k, top_p, min_p, out, ring, ring_rows, expect, accept)
+    _need(logits.dtype == torch.float32 and logits.dim() == 2 and logits.stride(1) == 1, "logits: float32 (n, V)")
+    n = logits.shape[0] if n is None else n
+    _need(0 <= n <= logits.shape[0], f"n={n} outside the {logits.shape[0]} logits rows")
+    for name, t, dt in (("u", u, torch.float32), ("temperature", temperature, torch.float32),
+                        ("top_k", top_k, torch.int32), ("top_p", top_p, torch.float32),
+                        ("min_p", min_p, torch.float32)):
+        if t is not None:
+            _need(t.dtype == dt and t.is_contiguous() and t.numel() >= n, f"{name}: {dt} contiguous (>= {n},)")
+    out, acc = _argmax_outputs(n, logits.device, out, ring, ring_rows, expect, accept, accept_mapped)
+    ld = logits.stride(0) if logits.shape[0] > 1 else logits.shape[1]
+    rc = _lib.load().wfd_sample(logits.data_ptr(), ld, u.data_ptr(), _p(temperature), _p(top_k), _p(top_p), _p(min_p),
+                                out.data_ptr(), _p(ring), _p(ring_rows), ring.numel() if ring is not None else 0,
+                                _p(expect), acc, n, logits.shape[1], _stream())
+    _lib.check(rc, "wfd_sample")
+    return out
+
+
 def _argmax_outputs(n, device, out, ring, ring_rows, expect, accept, accept_mapped):
     """Checks argmax's ring / expect / accept operands; returns (out, accept address)."""
     if ring is not None:
