@@ -196,6 +196,36 @@ int wfd_attn_varlen(const void* q, const void* k, const void* v, const int32_t* 
                     void* workspace, size_t ws_bytes, wfd_stream_t stream);
 
 /*
+ * Decode attention of rows that share a prefix (several answers to one prompt,
+ * whose keys are stored once). Group j = query rows [group_first[j],
+ * group_first[j+1]) of q (n, H, Dh), consecutive and in order; its rows attend
+ * the cache rows prefix_row_base[j] .. + prefix_len[j] - 1, read once for the
+ * group, and then each row the cache rows kv_row_base[i] .. + kv_len[i] - 1 of
+ * its own, one softmax over both. A row outside every group attends its own keys
+ * alone; lengths <= 0 are empty, and a row without any key gets a zero row.
+ * The caches are in the kv_block_rows layout (with blocks, a prefix lies in one
+ * block, and so do a row's own keys). Device tables: prefix_row_base int64 and
+ * prefix_len int32 (ngroups), group_first int32 (ngroups + 1), kv_row_base int64
+ * and kv_len int32 (n). prefix_len_max, kv_len_max >= the lengths (0: none has
+ * any) and group_max >= every group's rows size the grid. workspace >=
+ * wfd_attn_shared_workspace_bytes(...). Dh 64 or 128, H / Hkv up to 16, any
+ * scale; at most 65535 rows. fp32 statistics, sums and division; for bf16 the
+ * probabilities meet V as bf16 (as in wfd_attn_prefill). A row's bits depend on
+ * its own q, keys and lengths and on Hkv, not on its group's other rows (they
+ * are not wfd_attn_decode's, whose key order differs). Infinities and NaN in K
+ * and V reach only the rows that attend them.
+ * Replaces: what wfd_attn_decode replaces for sequences whose prompts are equal;
+ *   the reference stores and reads such a prompt once per sequence
+ *   (src/decoding/huginn_blocks_batch.py:179-203,265-285).
+ */
+size_t wfd_attn_shared_workspace_bytes(int n, int H, int Hkv, int Dh, int prefix_len_max, int kv_len_max);
+int wfd_attn_shared(const void* q, const void* k_cache, const void* v_cache, int64_t kv_block_rows,
+                    const int64_t* prefix_row_base, const int32_t* prefix_len, const int32_t* group_first, int ngroups,
+                    int group_max, const int64_t* kv_row_base, const int32_t* kv_len, void* out, int n, int H,
+                    int Hkv, int Dh, int dtype, float scale, int prefix_len_max, int kv_len_max, void* workspace,
+                    size_t ws_bytes, wfd_stream_t stream);
+
+/*
  * Causal prefill attention on MFMA (bf16; Dh 64 or 128; any H / Hkv).
  * Segment s owns query rows [seg_q_start[s], seg_q_start[s+1]) of q (n, H, Dh)
  * at positions seg_pos0[s], seg_pos0[s] + 1, ... of one slot whose cache rows

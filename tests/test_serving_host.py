@@ -178,3 +178,59 @@ def test_sampler_parameters_and_numbers():
     assert len({a.uniform(p) for p in at}) == len(at)
     made = SampledPolicy(8, 2, sample_seed=5, temperature=0.5, top_k=7).make_sampler()
     assert (made.seed, made.temperature, made.top_k, made.top_p) == (5, 0.5, 7, 1.0)
+
+
+# ---------------------------------------------------------------------------
+# shared prefixes
+# ---------------------------------------------------------------------------
+def test_shared_front_end_refusals(front):
+    i32, i64 = (lambda n: _m(n, dtype=torch.int32)), (lambda n: _m(n, dtype=torch.int64))
+    ok = dict(q=_m(6, 4, 64), k=_m(100, 2, 64), v=_m(100, 2, 64), pb=i64(2), pl=i32(2), gf=i32(3), rb=i64(6), rl=i32(6),
+              prefix_len_max=50, kv_len_max=10)
+    for bad in (dict(q=_m(6, 4, 128)), dict(q=_m(4, 6, 64).transpose(0, 1)), dict(k=_m(100, 2, 64).float()),
+                dict(k=_m(90, 2, 64)), dict(pb=i32(2)), dict(pl=i64(2)), dict(pl=i32(1)), dict(gf=i32(2)),
+                dict(gf=i64(3)), dict(rb=i64(5)), dict(rl=i32(5)), dict(rl=i32(12)[::2]), dict(prefix_len_max=-1),
+                dict(kv_len_max=-1), dict(group_max=-1), dict(out=_m(5, 4, 64)),
+                dict(k=_m(4, 2, 32, 64), v=_m(4, 2, 32, 64)),
+                dict(q=_m(6, 4, 64, dtype=torch.float16), k=_m(100, 2, 64, dtype=torch.float16),
+                     v=_m(100, 2, 64, dtype=torch.float16))):
+        a = ok | bad
+        operands = [a.pop(x) for x in ("q", "k", "v", "pb", "pl", "gf", "rb", "rl")]
+        with pytest.raises(_lib.WfdError):
+            ops.attn_shared(*operands, **a)
+
+
+def test_shared_entry_point_checks_before_launch():
+    lib = _lib.load()
+    err = lib.wfd_last_error
+
+    def call(n=2, H=4, Hkv=2, Dh=64, dt=1, ng=1, gm=2, pm=10, om=10, br=0):
+        return lib.wfd_attn_shared(None, None, None, br, None, None, None, ng, gm, None, None, None, n, H, Hkv, Dh, dt,
+                                   0.1, pm, om, None, 0, None)
+
+    for bad in (dict(n=-1), dict(H=0), dict(H=3), dict(ng=-1), dict(gm=-1), dict(pm=-1), dict(om=-1), dict(br=-1)):
+        assert call(**bad) == -1 and b"bad shape" in err(), bad
+    assert call(br=8) == -1 and b"exceed a block" in err()
+    assert call(dt=2) == -2 and call(Dh=32) == -2 and call(H=34) == -2 and b"G=17" in err()
+    assert call(n=0) == 0 and call() == -1 and b"null pointer" in err()
+    # the parts: 256 / Hkv chunks at most while they are below 1024 keys, then 1024 keys each; own keys apart
+    size = lambda parts: sum(-(-x // 256) * 256 for x in (parts * 64 * 4, parts * 8))  # noqa: E731
+    ws = lib.wfd_attn_shared_workspace_bytes
+    assert ws(2, 4, 2, 64, 0, 0) == 0 and ws(0, 4, 2, 64, 100, 100) == 0 and ws(2, 4, 2, 64, -1, 0) == 0
+    assert ws(2, 4, 2, 64, 128, 0) == size(8) and ws(2, 4, 2, 64, 129, 0) == size(16)
+    assert ws(2, 4, 2, 64, 200 * 1024, 0) == size(8 * 200)
+
+
+@pytest.mark.skipif(torch.cuda.device_count() > 0, reason="made-up device addresses: run only where no GPU is "
+                    "visible, so a regressed check cannot launch a kernel on them")
+def test_shared_alignment_workspace_and_grid_are_checked():
+    lib = _lib.load()
+
+    def call(q=4096, ws=4096, size=1 << 30, n=2, ng=1, gm=2, pm=10, om=10):
+        return lib.wfd_attn_shared(q, 4096, 4096, 0, 4096, 4096, 4096, ng, gm, 4096, 4096, 4096, n, 4, 2, 64, 1, 0.1,
+                                   pm, om, ws, size, None)
+
+    assert call(q=4096 + 2) == -1 and call(ws=4096 + 8) == -1 and b"16-byte aligned" in lib.wfd_last_error()
+    assert call(size=16) == -4 and b"workspace" in lib.wfd_last_error()
+    assert call(n=70000, size=1 << 60) == -2 and b"beyond the grid" in lib.wfd_last_error()
+    assert call(n=60000, gm=60000, ng=60000, pm=1 << 24, size=1 << 60) == -2

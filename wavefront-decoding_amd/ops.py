@@ -149,7 +149,10 @@ def attn_workspace(n: int, H: int, Dh: int, kv_len_max: int, device) -> torch.Te
     two streams nor the two kernels of a split launch, between which another
     thread may enqueue its own on the same stream, ever share one. A stream
     under capture gets a fresh one, which the graph owns."""
-    need = attn_workspace_bytes(n, H, Dh, kv_len_max)
+    return _workspace(attn_workspace_bytes(n, H, Dh, kv_len_max), device)
+
+
+def _workspace(need: int, device) -> torch.Tensor:
     dev = device if isinstance(device, torch.device) else torch.device(device)
     if torch.cuda.is_current_stream_capturing():
         return torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
@@ -259,6 +262,53 @@ def attn_varlen(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.T
                              ws.data_ptr(), ws_bytes, _stream())
     _lib.check(rc, "wfd_attn_varlen")
     return out
+
+
+def attn_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, prefix_row_base: torch.Tensor,
+                prefix_len: torch.Tensor, group_first: torch.Tensor, kv_row_base: torch.Tensor, kv_len: torch.Tensor,
+                *, prefix_len_max: int, kv_len_max: int, group_max: int | None = None, scale: float | None = None,
+                out: torch.Tensor | None = None, workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """Decode attention of rows that share a prefix (wfd_attn_shared): the query
+    rows [group_first[j], group_first[j+1]) attend cache rows
+    prefix_row_base[j] + [0, prefix_len[j]), read once for the group, and each
+    row its own rows kv_row_base[i] + [0, kv_len[i]). prefix_len_max and
+    kv_len_max bound the lengths (0: none has any), group_max a group's rows
+    (None: n)."""
+    _need_current(q, k_cache, v_cache, prefix_row_base, prefix_len, group_first, kv_row_base, kv_len, out, workspace)
+    _need(q.dim() == 3 and q.is_contiguous(), "q must be contiguous (n, H, Dh)")
+    n, H, Dh = q.shape
+    Hkv, cDh, br = kv_layout(k_cache, v_cache)
+    _need(cDh == Dh and k_cache.dtype == q.dtype, "q/k/v dtype or head_dim mismatch")
+    ng = prefix_row_base.numel()
+    for name, t, dt, size in (("prefix_row_base", prefix_row_base, torch.int64, ng),
+                              ("prefix_len", prefix_len, torch.int32, ng),
+                              ("group_first", group_first, torch.int32, ng + 1),
+                              ("kv_row_base", kv_row_base, torch.int64, n), ("kv_len", kv_len, torch.int32, n)):
+        _need(t.dtype == dt and t.is_contiguous() and t.numel() >= size, f"{name}: {dt} contiguous (>= {size},)")
+    _need(prefix_len_max >= 0 and kv_len_max >= 0, "prefix_len_max and kv_len_max must be >= 0")
+    _need(br == 1 or max(prefix_len_max, kv_len_max) <= br,
+          f"prefix_len_max {prefix_len_max} or kv_len_max {kv_len_max} exceeds the cache block ({br} rows)")
+    group_max = n if group_max is None else int(group_max)
+    _need(group_max >= 0, "group_max must be >= 0")
+    if out is None:
+        out = torch.empty_like(q)
+    _need(out.shape == q.shape and out.dtype == q.dtype and out.is_contiguous(), "bad out")
+    dt, lib = _dt(q), _lib.load()
+    if workspace is None:
+        workspace = _workspace(lib.wfd_attn_shared_workspace_bytes(n, H, Hkv, Dh, prefix_len_max, kv_len_max),
+                               q.device)
+    sc = 1.0 / math.sqrt(Dh) if scale is None else float(scale)
+    rc = lib.wfd_attn_shared(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), br, prefix_row_base.data_ptr(),
+                             prefix_len.data_ptr(), group_first.data_ptr(), ng, group_max, kv_row_base.data_ptr(),
+                             kv_len.data_ptr(), out.data_ptr(), n, H, Hkv, Dh, dt, sc, int(prefix_len_max),
+                             int(kv_len_max), workspace.data_ptr(), workspace.numel() * workspace.element_size(),
+                             _stream())
+    _lib.check(rc, "wfd_attn_shared")
+    return out
+
+
+def attn_shared_workspace_bytes(n: int, H: int, Hkv: int, Dh: int, prefix_len_max: int, kv_len_max: int) -> int:
+    return int(_lib.load().wfd_attn_shared_workspace_bytes(n, H, Hkv, Dh, prefix_len_max, kv_len_max))
 
 
 def attn_prefill(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, seg_row_base: torch.Tensor,
