@@ -6,8 +6,8 @@
 // Softmax over a union is a merge of softmaxes over its parts: a part leaves its
 // maximum m, sum l and unnormalised output o, and the row is sum o 2^(m - M) /
 // sum l 2^(m - M) over its parts. The prefix is cut into chunks of keys, a
-// workgroup computes one chunk for up to kShRows (query row, query head) pairs of
-// a group and one kv head -- each key is read once for all of them -- and a row's
+// workgroup computes one chunk for up to 32 (fp32: 16) (query row, query head)
+// pairs of a group and one kv head -- each key is read once for all of them -- and a row's
 // own keys are cut likewise, for that row alone; attn_shared_combine merges a
 // row's parts in the order of its keys.
 //
@@ -18,13 +18,15 @@
 
 namespace wfd {
 
-constexpr int kShRows = 16;      // (query row, head) pairs per workgroup
+constexpr int kShRowsF32 = 16;   // (query row, head) pairs per workgroup
+constexpr int kShRowsBF16 = 32;
 constexpr int kShWaves = 4;      // key streams per workgroup
 constexpr int kShMinChunk = 128;
 constexpr int kShMaxChunk = 1024;
 constexpr int kShOwnChunk = 512;
 constexpr int kShTarget = 256;   // chunks x kv heads aimed at
 constexpr int kShMaxG = 16;
+constexpr int kShMaxHeads = 4096;  // a chunk's keys stay within 32-bit offsets of its first
 
 // Keys per chunk of a prefix of P keys: enough chunks for a workgroup per CU over
 // the kv heads while they are at least 128 keys; long prefixes take 1024, where
@@ -58,8 +60,96 @@ struct ShArgs {
   float scale_log2;
 };
 
-template <typename T, int DH>
-__global__ __launch_bounds__(64 * kShWaves) void attn_shared_kernel(ShArgs a) {
+// What one workgroup computes: keys [k0, k1) of the slot rows from `base`, for nr
+// pairs from pair p0 of the query rows from row0 (pair r: query row row0 + r / G,
+// head g G + r % G), left as the rows' part `part`.
+struct ShItem {
+  int g, row0, p0, nr, k0, k1, part;
+  int64_t base;
+};
+
+// The workgroup's item; false if it has none (a shorter prefix, a smaller group).
+// Prefix items first, RT pairs each. The tiles of one (group, chunk, head) read
+// the same keys: they are 8 workgroups apart, so they run on one XCD at about the
+// same time, and one of them brings the keys to its L2.
+template <int RT>
+__device__ __forceinline__ bool sh_item(const ShArgs& a, ShItem& it) {
+  const int G = a.H / a.Hkv;
+  const int64_t x = blockIdx.x;
+  const int64_t nkeys = (int64_t)a.ng * a.pchunks * a.Hkv;
+  const int64_t nprefix = (nkeys + 7) / 8 * 8 * a.tiles;
+  if (x < nprefix) {
+    const int64_t q = x / 8;
+    const int tile = (int)(q % a.tiles);
+    const int64_t kg = q / a.tiles * 8 + x % 8;
+    if (kg >= nkeys) return false;
+    it.g = (int)(kg % a.Hkv);
+    const int64_t jc = kg / a.Hkv;
+    const int c = (int)(jc % a.pchunks), j = (int)(jc / a.pchunks);
+    const int P = min(a.plen[j], a.pmax);
+    const int ck = prefix_chunk(P, a.Hkv);
+    it.row0 = a.gfirst[j];
+    it.p0 = tile * RT;
+    it.nr = min((min(a.gfirst[j + 1], a.n) - it.row0) * G - it.p0, RT);
+    it.k0 = c * ck;
+    it.k1 = min(it.k0 + ck, P);
+    it.part = c;
+    it.base = a.pbase[j];
+  } else {
+    const int64_t y = x - nprefix;
+    it.g = (int)(y % a.Hkv);
+    const int64_t ic = y / a.Hkv;
+    const int c = (int)(ic % a.ochunks);
+    it.row0 = (int)(ic / a.ochunks);
+    it.p0 = 0;
+    it.nr = G;
+    it.k0 = c * kShOwnChunk;
+    it.k1 = min(it.k0 + kShOwnChunk, min(a.rlen[it.row0], a.omax));
+    it.part = a.pchunks + c;
+    it.base = a.rbase[it.row0];
+  }
+  return it.k0 < it.k1 && it.nr > 0;
+}
+
+__device__ __forceinline__ int64_t sh_pair(const ShArgs& a, const ShItem& it, int r) {
+  const int G = a.H / a.Hkv;
+  const int row = (it.p0 + r) / G;
+  return (int64_t)(it.row0 + row) * a.H + it.g * G + (it.p0 + r - row * G);
+}
+
+// Merges the workgroup's key streams, one per wave, and leaves the part: o_lds
+// [wave][pair][DH, pitch OP], m / l [wave][pair].
+template <int DH, int OP, int RT>
+__device__ __forceinline__ void sh_leave(const ShArgs& a, const ShItem& it, const float* o_lds, const float* m_lds,
+                                         const float* l_lds) {
+  const int ms = a.pchunks + a.ochunks;
+  for (int idx = threadIdx.x; idx < it.nr * DH; idx += 64 * kShWaves) {
+    const int r = idx / DH, d = idx - r * DH;
+    float M = -INFINITY, O = 0.f, L = 0.f;
+#pragma unroll
+    for (int w = 0; w < kShWaves; ++w) M = fmaxf(M, m_lds[w * RT + r]);
+#pragma unroll
+    for (int w = 0; w < kShWaves; ++w) {
+      const float mw = m_lds[w * RT + r];
+      const float f = mw == -INFINITY ? 0.f : exp2f(mw - M);
+      O = fmaf(o_lds[(w * RT + r) * OP + d], f, O);
+      L = fmaf(l_lds[w * RT + r], f, L);
+    }
+    const int64_t at = sh_pair(a, it, r) * ms + it.part;
+    a.po[at * DH + d] = O;
+    if (d == 0) {
+      a.pml[2 * at] = M;
+      a.pml[2 * at + 1] = L;
+    }
+  }
+}
+
+// fp32: 16 pairs per workgroup on the fp32 MFMA (scores as in wfd_attn_decode;
+// P.V on the 16x16x4 form, P through LDS), operands straight from the cache.
+template <int DH>
+__global__ __launch_bounds__(64 * kShWaves) void attn_shared_f32_kernel(ShArgs a) {
+  using T = float;
+  constexpr int RT = kShRowsF32;
   constexpr int V = Elem<T>::kVec;
   constexpr int KSTEP = 4 * V;
   constexpr int NDS = DH / KSTEP;
@@ -68,55 +158,18 @@ __global__ __launch_bounds__(64 * kShWaves) void attn_shared_kernel(ShArgs a) {
   __shared__ float o_lds[kShWaves][16][DH];
   __shared__ float m_lds[kShWaves][16];
   __shared__ float l_lds[kShWaves][16];
-  const int G = a.H / a.Hkv;
-  const int g = blockIdx.x % a.Hkv;
-  int64_t item = blockIdx.x / a.Hkv;
-  const int64_t nprefix = (int64_t)a.ng * a.pchunks * a.tiles;
-  int row0, nr, k0, k1, part;  // first query row, pairs, keys, the part's place
-  int64_t base;
-  if (item < nprefix) {
-    const int tile = (int)(item % a.tiles);
-    item /= a.tiles;
-    const int c = (int)(item % a.pchunks), j = (int)(item / a.pchunks);
-    const int P = min(a.plen[j], a.pmax);
-    const int first = a.gfirst[j];
-    const int pairs = (min(a.gfirst[j + 1], a.n) - first) * G;
-    const int ck = prefix_chunk(P, a.Hkv);
-    k0 = c * ck;
-    k1 = min(k0 + ck, P);
-    if (k0 >= k1 || tile * kShRows >= pairs) return;  // uniform
-    row0 = first;
-    nr = pairs;
-    part = c;
-    base = a.pbase[j];
-    // pairs tile * kShRows .. of the group
-    item = tile * kShRows;
-  } else {
-    item -= nprefix;
-    const int c = (int)(item % a.ochunks), i = (int)(item / a.ochunks);
-    const int L = min(a.rlen[i], a.omax);
-    k0 = c * kShOwnChunk;
-    k1 = min(k0 + kShOwnChunk, L);
-    if (k0 >= k1) return;
-    row0 = i;
-    nr = G;
-    part = a.pchunks + c;
-    base = a.rbase[i];
-    item = 0;
-  }
-  const int p0 = (int)item;
-  nr = min(nr - p0, kShRows);
+  ShItem it;
+  if (!sh_item<RT>(a, it)) return;  // uniform
+  const int g = it.g, nr = it.nr, k0 = it.k0, k1 = it.k1;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4;
-  const int64_t hb = kv_offset(base, g, a.Hkv, DH, a.br);
+  const int64_t hb = kv_offset(it.base, g, a.Hkv, DH, a.br);
   const int64_t rs = a.br > 1 ? (int64_t)DH : (int64_t)a.Hkv * DH;
   const T* kb = (const T*)a.kc + hb;
   const T* vb = (const T*)a.vc + hb;
-  auto pair_row = [&](int r) { return (int64_t)(row0 + (p0 + r) / G) * a.H + g * G + (p0 + r) % G; };
-
   u32x4 qf[NDS];
 #pragma unroll
   for (int s = 0; s < NDS; ++s)
-    qf[s] = col < nr ? ld16((const T*)a.q + pair_row(col) * DH + grp * V + s * KSTEP) : zero16();
+    qf[s] = col < nr ? ld16((const T*)a.q + sh_pair(a, it, col) * DH + grp * V + s * KSTEP) : zero16();
 
   float mrun[4], lrun[4];
   f32x4 o[NC];
@@ -182,25 +235,175 @@ __global__ __launch_bounds__(64 * kShWaves) void attn_shared_kernel(ShArgs a) {
     }
   }
   __syncthreads();
-  const int ms = a.pchunks + a.ochunks;
-  for (int idx = threadIdx.x; idx < nr * DH; idx += 64 * kShWaves) {
-    const int r = idx / DH, d = idx - r * DH;
-    float M = -INFINITY, O = 0.f, L = 0.f;
+  sh_leave<DH, DH, RT>(a, it, &o_lds[0][0][0], &m_lds[0][0], &l_lds[0][0]);
+}
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+__device__ __forceinline__ f32x16 sh_mfma32(const u32x4& x, const u32x4& y, f32x16 acc) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, y), acc, 0,
+                                                 0, 0);
+}
+
+// bf16: 32 pairs per workgroup, one per column of the 32x32x16 MFMA, and four
+// waves that each stream 32-key tiles of the chunk (wave w tiles w, w + 4, ...)
+// through LDS of their own: whole rows to registers a tile ahead, to LDS as
+// loaded, no workgroup barrier before the merge. A wave computes S^T = K Q^T and
+// O^T = V^T P^T; the K rows of a tile are taken in the order that makes a lane's
+// S^T registers the 8 consecutive keys its P^T operand wants (result register r of
+// lane half hf is key 16 (r / 8) + 8 hf + r % 8), so P never leaves its lane, and
+// V^T comes out of the row-major tile by transposing LDS reads. Keys past the
+// chunk read as zeros and score -inf.
+template <int DH>
+__global__ __launch_bounds__(64 * kShWaves) __attribute__((amdgpu_waves_per_eu(2))) void attn_shared_bf16_kernel(
+    ShArgs a) {
+  constexpr int RT = kShRowsBF16;
+  constexpr int TK = 32;
+  constexpr int NDS = DH / 16;
+  constexpr int NDB = DH / 32;
+  constexpr int KP = DH + 8;    // LDS row pitches: K reads 16 bytes of 32 rows, V^T 64 bytes of 8 rows,
+  constexpr int VP = DH + 32;   // each spread over all banks
+  constexpr int CPR = DH / 8;   // 16-byte pieces per row
+  constexpr int RPI = 64 / CPR;
+  constexpr int NLD = TK / RPI;
+  constexpr int OP = DH + 4;
+  constexpr int kWaveEls = TK * (KP + VP);
+  constexpr size_t kStage = sizeof(bf16_t) * kWaveEls * kShWaves, kMerge = sizeof(float) * kShWaves * RT * OP;
+  __shared__ __align__(16) unsigned char lds[kStage > kMerge ? kStage : kMerge];
+  __shared__ float m_lds[kShWaves * RT];
+  __shared__ float l_lds[kShWaves * RT];
+  ShItem it;
+  if (!sh_item<RT>(a, it)) return;  // uniform
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, col = lane & 31, hf = lane >> 5;
+  bf16_t* k_lds = reinterpret_cast<bf16_t*>(lds) + wave * kWaveEls;
+  bf16_t* v_lds = k_lds + TK * KP;
+
+  // K / V of this head from key k0; the resources end with key k1 - 1
+  const int64_t rs = a.br > 1 ? (int64_t)DH : (int64_t)a.Hkv * DH;
+  const int64_t at = kv_offset(it.base, it.g, a.Hkv, DH, a.br) + it.k0 * rs;
+  const int nk = it.k1 - it.k0;
+  const uint32_t rsb = (uint32_t)(rs * sizeof(bf16_t));
+  const uint32_t span = (uint32_t)(nk - 1) * rsb + DH * sizeof(bf16_t);
+  auto rsrc = [&](const void* p) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<bf16_t*>((const bf16_t*)p + at), (short)0, span, 0x00020000);
+  };
+  const __amdgpu_buffer_rsrc_t kr = rsrc(a.kc), vr = rsrc(a.vc);
+  const int lr = lane / CPR, lp = lane % CPR;  // row within a load, piece
+  u32x4 kreg[NLD], vreg[NLD];
+  auto fetch = [&](int t0) {
 #pragma unroll
-    for (int w = 0; w < kShWaves; ++w) M = fmaxf(M, m_lds[w][r]);
-#pragma unroll
-    for (int w = 0; w < kShWaves; ++w) {
-      const float f = m_lds[w][r] == -INFINITY ? 0.f : exp2f(m_lds[w][r] - M);
-      O = fmaf(o_lds[w][r][d], f, O);
-      L = fmaf(l_lds[w][r], f, L);
+    for (int s = 0; s < NLD; ++s) {
+      const uint32_t off = (uint32_t)(t0 + RPI * s + lr) * rsb + (uint32_t)lp * 16u;
+      kreg[s] = buf_ld16(kr, off);
+      vreg[s] = buf_ld16(vr, off);
     }
-    const int64_t at = pair_row(r) * ms + part;
-    a.po[at * DH + d] = O;
-    if (d == 0) {
-      a.pml[2 * at] = M;
-      a.pml[2 * at + 1] = L;
+  };
+  fetch(TK * wave);
+
+  u32x4 qf[NDS];
+  {
+    const bf16_t* qp = (const bf16_t*)a.q + sh_pair(a, it, min(col, it.nr - 1)) * DH + 8 * hf;
+#pragma unroll
+    for (int s = 0; s < NDS; ++s) qf[s] = ld16(qp + 16 * s);
+  }
+  const int krow = 16 * (col >> 4) + 8 * ((col >> 2) & 1) + 4 * ((col >> 3) & 1) + (col & 3);
+  const int tg = lane >> 4, ti = lane & 15;
+  const int v_lane = ((tg >> 1) * 8 + (ti >> 2)) * VP + 16 * (tg & 1) + 4 * (ti & 3);
+  auto vt_frag = [&](int db, int s) {
+    typedef short s16x4 __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+    typedef const __attribute__((address_space(3))) void* lds_ptr;
+    const bf16_t* p = v_lds + v_lane + 16 * s * VP + 32 * db;
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(lds_ptr)p);
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(lds_ptr)(p + 4 * VP));
+    const uint2 x = __builtin_bit_cast(uint2, lo), y = __builtin_bit_cast(uint2, hi);
+    return u32x4{x.x, x.y, y.x, y.y};
+  };
+
+  float mrun = -INFINITY, lrun = 0.f;
+  f32x16 o[NDB];
+#pragma unroll
+  for (int c = 0; c < NDB; ++c)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o[c][r] = 0.f;
+
+  for (int t0 = TK * wave; t0 < nk; t0 += TK * kShWaves) {  // uniform over the wave
+#pragma unroll
+    for (int s = 0; s < NLD; ++s) {
+      *reinterpret_cast<u32x4*>(k_lds + (RPI * s + lr) * KP + 8 * lp) = kreg[s];
+      *reinterpret_cast<u32x4*>(v_lds + (RPI * s + lr) * VP + 8 * lp) = vreg[s];
+    }
+    fetch(t0 + TK * kShWaves);  // zeros past the chunk
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    f32x16 sc;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) sc[r] = 0.f;
+#pragma unroll
+    for (int s = 0; s < NDS; ++s)
+      sc = sh_mfma32(*reinterpret_cast<const u32x4*>(k_lds + krow * KP + 16 * s + 8 * hf), qf[s], sc);
+    float mt = -INFINITY;
+    const bool full = t0 + TK <= nk;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      sc[r] *= a.scale_log2;
+      if (!full && t0 + 16 * (r >> 3) + 8 * hf + (r & 7) >= nk) sc[r] = -INFINITY;
+      mt = fmaxf(mt, sc[r]);
+    }
+    mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
+    const float mnew = fmaxf(mrun, mt);
+    const float mref = mnew == -INFINITY ? 0.f : mnew;
+    // v_exp_f32 flushes below 2^-126: far under a bf16 probability's resolution
+    const float corr = __builtin_amdgcn_exp2f(mrun - mref);
+    float lt = 0.f;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      sc[r] = __builtin_amdgcn_exp2f(sc[r] - mref);
+      lt += sc[r];
+    }
+    lt += __shfl_xor(lt, 32, 64);
+    lrun = fmaf(lrun, corr, lt);
+    mrun = mnew;
+    // the one rounding before the output's: P meets V as bf16 (half a step: 2^-8
+    // of P, at random signs), where fp32 products would take 8 times the MFMA time
+    u32x4 pb[2];
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) pb[s][e] = f32x2_to_bf16x2_bits(sc[8 * s + 2 * e], sc[8 * s + 2 * e + 1]);
+    if (__builtin_amdgcn_ballot_w64(corr != 1.f)) {
+#pragma unroll
+      for (int db = 0; db < NDB; ++db)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[db][r] *= corr;
+    }
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int db = 0; db < NDB; ++db) o[db] = sh_mfma32(vt_frag(db, s), pb[s], o[db]);
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();  // the next tile overwrites this one
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  }
+
+  __syncthreads();  // every wave's tiles are done: the merge takes their LDS
+  float* o_lds = reinterpret_cast<float*>(lds);
+  if (col < it.nr) {
+#pragma unroll
+    for (int db = 0; db < NDB; ++db)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        *reinterpret_cast<f32x4*>(o_lds + (wave * RT + col) * OP + 32 * db + 8 * r + 4 * hf) =
+            f32x4{o[db][4 * r], o[db][4 * r + 1], o[db][4 * r + 2], o[db][4 * r + 3]};
+    if (hf == 0) {
+      m_lds[wave * RT + col] = mrun;
+      l_lds[wave * RT + col] = lrun;
     }
   }
+  __syncthreads();
+  sh_leave<DH, OP, RT>(a, it, o_lds, m_lds, l_lds);
 }
 
 // Group of row i (the last one that starts at or before it and ends after it), or -1.
@@ -260,10 +463,13 @@ __global__ __launch_bounds__(DH) void attn_shared_combine(ShArgs a) {
 }
 
 template <typename T, int DH>
-static void launch_shared(const ShArgs& a, hipStream_t st) {
-  const int64_t items = (int64_t)a.ng * a.pchunks * a.tiles + (int64_t)a.n * a.ochunks;
-  if (items)
-    hipLaunchKernelGGL((attn_shared_kernel<T, DH>), dim3((unsigned)(items * a.Hkv)), dim3(64 * kShWaves), 0, st, a);
+static void launch_shared(const ShArgs& a, int64_t wgs, hipStream_t st) {
+  if (wgs) {
+    if constexpr (sizeof(T) == 2)
+      hipLaunchKernelGGL((attn_shared_bf16_kernel<DH>), dim3((unsigned)wgs), dim3(64 * kShWaves), 0, st, a);
+    else
+      hipLaunchKernelGGL((attn_shared_f32_kernel<DH>), dim3((unsigned)wgs), dim3(64 * kShWaves), 0, st, a);
+  }
   hipLaunchKernelGGL((attn_shared_combine<T, DH>), dim3(a.H, a.n), dim3(DH), 0, st, a);
 }
 
@@ -285,7 +491,7 @@ int wfd_attn_shared(const void* q, const void* k_cache, const void* v_cache, int
                     size_t ws_bytes, hipStream_t stream) {
   using namespace wfd;
   const char* me = "wfd_attn_shared";
-  if (n < 0 || H <= 0 || Hkv <= 0 || H % Hkv != 0 || H > 65535 || ngroups < 0 || group_max < 0 || kv_block_rows < 0 ||
+  if (n < 0 || H <= 0 || Hkv <= 0 || H % Hkv != 0 || H > kShMaxHeads || ngroups < 0 || group_max < 0 || kv_block_rows < 0 ||
       prefix_len_max < 0 || kv_len_max < 0) {
     set_error("%s: bad shape n=%d H=%d Hkv=%d ngroups=%d group_max=%d prefix_len_max=%d kv_len_max=%d", me, n, H, Hkv,
               ngroups, group_max, prefix_len_max, kv_len_max);
@@ -332,7 +538,8 @@ int wfd_attn_shared(const void* q, const void* k_cache, const void* v_cache, int
   a.Hkv = Hkv;
   a.ng = ngroups;
   const int64_t pairs = (int64_t)(group_max < n ? group_max : n) * G;
-  const int64_t tiles = (pairs + kShRows - 1) / kShRows;
+  const int rt = dtype == kBF16 ? kShRowsBF16 : kShRowsF32;
+  const int64_t tiles = (pairs + rt - 1) / rt;
   a.pchunks = max_prefix_chunks(prefix_len_max, Hkv);
   a.ochunks = div_up(kv_len_max, kShOwnChunk);
   a.pmax = prefix_len_max;
@@ -341,18 +548,18 @@ int wfd_attn_shared(const void* q, const void* k_cache, const void* v_cache, int
   a.po = (float*)workspace;
   a.pml = (float*)((char*)workspace + align256((size_t)n * H * (a.pchunks + a.ochunks) * Dh * sizeof(float)));
   // in double: the product of four counts may pass 64 bits
-  const double wgs = ((double)ngroups * a.pchunks * (double)tiles + (double)n * a.ochunks) * Hkv;
-  if (wgs > 2147483647.0 || n > 65535) {
+  const double most = (((double)ngroups * a.pchunks * Hkv + 8) * (double)tiles + (double)n * a.ochunks * Hkv);
+  if (most > 2147483647.0 || n > 65535) {
     set_error("%s: n=%d ngroups=%d group_max=%d prefix_len_max=%d kv_len_max=%d beyond the grid", me, n, ngroups,
               group_max, prefix_len_max, kv_len_max);
     return kUnsupported;
   }
   a.tiles = (int)tiles;
-  if (a.pchunks == 0 || tiles == 0) a.ng = 0;
+  const int64_t wgs = ((int64_t)ngroups * a.pchunks * Hkv + 7) / 8 * 8 * tiles + (int64_t)n * a.ochunks * Hkv;
   if (dtype == kBF16)
-    Dh == 64 ? launch_shared<bf16_t, 64>(a, stream) : launch_shared<bf16_t, 128>(a, stream);
+    Dh == 64 ? launch_shared<bf16_t, 64>(a, wgs, stream) : launch_shared<bf16_t, 128>(a, wgs, stream);
   else
-    Dh == 64 ? launch_shared<float, 64>(a, stream) : launch_shared<float, 128>(a, stream);
+    Dh == 64 ? launch_shared<float, 64>(a, wgs, stream) : launch_shared<float, 128>(a, wgs, stream);
   return launch_status(me);
 }
 
