@@ -24,7 +24,7 @@ constexpr int kShWaves = 4;      // key streams per workgroup
 constexpr int kShMinChunk = 128;
 constexpr int kShMaxChunk = 1024;
 constexpr int kShOwnChunk = 512;
-constexpr int kShTarget = 256;   // chunks x kv heads aimed at
+constexpr int kShTarget = 128;   // chunks x kv heads aimed at
 constexpr int kShMaxG = 16;
 constexpr int kShMaxHeads = 4096;  // a chunk's keys stay within 32-bit offsets of its first
 
@@ -40,7 +40,7 @@ __host__ __device__ inline int prefix_chunk(int P, int Hkv) {
 __host__ __device__ inline int div_up(int a, int b) { return a <= 0 ? 0 : (a + b - 1) / b; }
 
 // The most chunks any prefix of up to P keys makes (a chunk has at least
-// P Hkv / 256 keys unless it has 1024).
+// P Hkv / kShTarget keys unless it has 1024).
 inline int max_prefix_chunks(int P, int Hkv) {
   const int few = div_up(P, kShMinChunk), target = div_up(kShTarget, Hkv), many = div_up(P, kShMaxChunk);
   const int b = few < target ? few : target;
@@ -74,35 +74,35 @@ struct ShItem {
 // same time, and one of them brings the keys to its L2.
 template <int RT>
 __device__ __forceinline__ bool sh_item(const ShArgs& a, ShItem& it) {
-  const int G = a.H / a.Hkv;
-  const int64_t x = blockIdx.x;
-  const int64_t nkeys = (int64_t)a.ng * a.pchunks * a.Hkv;
-  const int64_t nprefix = (nkeys + 7) / 8 * 8 * a.tiles;
+  const uint32_t G = a.H / a.Hkv;
+  const uint32_t x = blockIdx.x;  // the host keeps the grid below 2^31
+  const uint32_t nkeys = (uint32_t)a.ng * a.pchunks * a.Hkv;
+  const uint32_t nprefix = (nkeys + 7) / 8 * 8 * a.tiles;
   if (x < nprefix) {
-    const int64_t q = x / 8;
-    const int tile = (int)(q % a.tiles);
-    const int64_t kg = q / a.tiles * 8 + x % 8;
+    const uint32_t q = x / 8;
+    const uint32_t tile = q % a.tiles;
+    const uint32_t kg = q / a.tiles * 8 + x % 8;
     if (kg >= nkeys) return false;
     it.g = (int)(kg % a.Hkv);
-    const int64_t jc = kg / a.Hkv;
+    const uint32_t jc = kg / a.Hkv;
     const int c = (int)(jc % a.pchunks), j = (int)(jc / a.pchunks);
     const int P = min(a.plen[j], a.pmax);
     const int ck = prefix_chunk(P, a.Hkv);
     it.row0 = a.gfirst[j];
     it.p0 = tile * RT;
-    it.nr = min((min(a.gfirst[j + 1], a.n) - it.row0) * G - it.p0, RT);
+    it.nr = min((min(a.gfirst[j + 1], a.n) - it.row0) * (int)G - it.p0, RT);
     it.k0 = c * ck;
     it.k1 = min(it.k0 + ck, P);
     it.part = c;
     it.base = a.pbase[j];
   } else {
-    const int64_t y = x - nprefix;
+    const uint32_t y = x - nprefix;
     it.g = (int)(y % a.Hkv);
-    const int64_t ic = y / a.Hkv;
+    const uint32_t ic = y / a.Hkv;
     const int c = (int)(ic % a.ochunks);
     it.row0 = (int)(ic / a.ochunks);
     it.p0 = 0;
-    it.nr = G;
+    it.nr = (int)G;
     it.k0 = c * kShOwnChunk;
     it.k1 = min(it.k0 + kShOwnChunk, min(a.rlen[it.row0], a.omax));
     it.part = a.pchunks + c;
@@ -118,29 +118,43 @@ __device__ __forceinline__ int64_t sh_pair(const ShArgs& a, const ShItem& it, in
 }
 
 // Merges the workgroup's key streams, one per wave, and leaves the part: o_lds
-// [wave][pair][DH, pitch OP], m / l [wave][pair].
+// [wave][pair][DH, pitch OP], m / l [wave][pair]. A thread first has one pair's
+// weights and place (it would otherwise compute them for every value), then takes
+// four columns of a pair at a time.
 template <int DH, int OP, int RT>
 __device__ __forceinline__ void sh_leave(const ShArgs& a, const ShItem& it, const float* o_lds, const float* m_lds,
-                                         const float* l_lds) {
+                                         float* l_lds, int64_t* at_lds) {
   const int ms = a.pchunks + a.ochunks;
-  for (int idx = threadIdx.x; idx < it.nr * DH; idx += 64 * kShWaves) {
-    const int r = idx / DH, d = idx - r * DH;
-    float M = -INFINITY, O = 0.f, L = 0.f;
+  if (threadIdx.x < it.nr) {
+    const int r = threadIdx.x;
+    float M = -INFINITY, L = 0.f, f[kShWaves];
 #pragma unroll
     for (int w = 0; w < kShWaves; ++w) M = fmaxf(M, m_lds[w * RT + r]);
 #pragma unroll
     for (int w = 0; w < kShWaves; ++w) {
       const float mw = m_lds[w * RT + r];
-      const float f = mw == -INFINITY ? 0.f : exp2f(mw - M);
-      O = fmaf(o_lds[(w * RT + r) * OP + d], f, O);
-      L = fmaf(l_lds[w * RT + r], f, L);
+      f[w] = mw == -INFINITY ? 0.f : exp2f(mw - M);
+      L = fmaf(l_lds[w * RT + r], f[w], L);
     }
     const int64_t at = sh_pair(a, it, r) * ms + it.part;
-    a.po[at * DH + d] = O;
-    if (d == 0) {
-      a.pml[2 * at] = M;
-      a.pml[2 * at + 1] = L;
+    a.pml[2 * at] = M;
+    a.pml[2 * at + 1] = L;
+    at_lds[r] = at;
+#pragma unroll
+    for (int w = 0; w < kShWaves; ++w) l_lds[w * RT + r] = f[w];
+  }
+  __syncthreads();
+  for (int idx = threadIdx.x; idx < it.nr * (DH / 4); idx += 64 * kShWaves) {
+    const int r = idx / (DH / 4), d = 4 * (idx % (DH / 4));
+    f32x4 O = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < kShWaves; ++w) {
+      const float f = l_lds[w * RT + r];
+      const f32x4 ow = *reinterpret_cast<const f32x4*>(o_lds + (w * RT + r) * OP + d);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) O[e] = fmaf(ow[e], f, O[e]);
     }
+    *reinterpret_cast<f32x4*>(a.po + at_lds[r] * DH + d) = O;
   }
 }
 
@@ -155,9 +169,10 @@ __global__ __launch_bounds__(64 * kShWaves) void attn_shared_f32_kernel(ShArgs a
   constexpr int NDS = DH / KSTEP;
   constexpr int NC = DH / 16;
   __shared__ float p_lds[kShWaves][16][17];
-  __shared__ float o_lds[kShWaves][16][DH];
+  __shared__ __align__(16) float o_lds[kShWaves][16][DH];
   __shared__ float m_lds[kShWaves][16];
   __shared__ float l_lds[kShWaves][16];
+  __shared__ int64_t at_lds[RT];
   ShItem it;
   if (!sh_item<RT>(a, it)) return;  // uniform
   const int g = it.g, nr = it.nr, k0 = it.k0, k1 = it.k1;
@@ -235,7 +250,7 @@ __global__ __launch_bounds__(64 * kShWaves) void attn_shared_f32_kernel(ShArgs a
     }
   }
   __syncthreads();
-  sh_leave<DH, DH, RT>(a, it, &o_lds[0][0][0], &m_lds[0][0], &l_lds[0][0]);
+  sh_leave<DH, DH, RT>(a, it, &o_lds[0][0][0], &m_lds[0][0], &l_lds[0][0], at_lds);
 }
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -272,6 +287,7 @@ __global__ __launch_bounds__(64 * kShWaves) __attribute__((amdgpu_waves_per_eu(2
   __shared__ __align__(16) unsigned char lds[kStage > kMerge ? kStage : kMerge];
   __shared__ float m_lds[kShWaves * RT];
   __shared__ float l_lds[kShWaves * RT];
+  __shared__ int64_t at_lds[RT];
   ShItem it;
   if (!sh_item<RT>(a, it)) return;  // uniform
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -291,21 +307,28 @@ __global__ __launch_bounds__(64 * kShWaves) __attribute__((amdgpu_waves_per_eu(2
   const __amdgpu_buffer_rsrc_t kr = rsrc(a.kc), vr = rsrc(a.vc);
   const int lr = lane / CPR, lp = lane % CPR;  // row within a load, piece
   u32x4 kreg[NLD], vreg[NLD];
-  auto fetch = [&](int t0) {
+  uint32_t off[NLD];
+#pragma unroll
+  for (int s = 0; s < NLD; ++s) off[s] = (uint32_t)(TK * wave + RPI * s + lr) * rsb + (uint32_t)lp * 16u;
+  auto fetch = [&]() {  // this wave's next tile; zeros past the chunk
 #pragma unroll
     for (int s = 0; s < NLD; ++s) {
-      const uint32_t off = (uint32_t)(t0 + RPI * s + lr) * rsb + (uint32_t)lp * 16u;
-      kreg[s] = buf_ld16(kr, off);
-      vreg[s] = buf_ld16(vr, off);
+      kreg[s] = buf_ld16(kr, off[s]);
+      vreg[s] = buf_ld16(vr, off[s]);
+      off[s] += (uint32_t)(TK * kShWaves) * rsb;
     }
   };
-  fetch(TK * wave);
+  fetch();
 
+  // Q as the B operand; a negative scale's sign goes to q, so that scores order as
+  // their products do, and a zero one is a tiny one, under which -inf stays -inf
+  const float scale = fmaxf(fabsf(a.scale_log2), 1e-37f);
+  const uint32_t flip = a.scale_log2 < 0.f ? 0x80008000u : 0u;
   u32x4 qf[NDS];
   {
     const bf16_t* qp = (const bf16_t*)a.q + sh_pair(a, it, min(col, it.nr - 1)) * DH + 8 * hf;
 #pragma unroll
-    for (int s = 0; s < NDS; ++s) qf[s] = ld16(qp + 16 * s);
+    for (int s = 0; s < NDS; ++s) qf[s] = ld16(qp + 16 * s) ^ flip;
   }
   const int krow = 16 * (col >> 4) + 8 * ((col >> 2) & 1) + 4 * ((col >> 3) & 1) + (col & 3);
   const int tg = lane >> 4, ti = lane & 15;
@@ -321,7 +344,12 @@ __global__ __launch_bounds__(64 * kShWaves) __attribute__((amdgpu_waves_per_eu(2
     return u32x4{x.x, x.y, y.x, y.y};
   };
 
-  float mrun = -INFINITY, lrun = 0.f;
+  // The reference point of a pair's exponentials: the maximum when it was last
+  // moved, which is when a tile exceeds it by more than 2^8. Probabilities up to
+  // 2^8 lose nothing in fp32 sums or bf16, and most tiles rescale nothing (with
+  // the running maximum itself some pair of the 32 moves in nearly every tile).
+  // It depends on the pair's own scores only.
+  float mref = -INFINITY, lrun = 0.f;
   f32x16 o[NDB];
 #pragma unroll
   for (int c = 0; c < NDB; ++c)
@@ -334,7 +362,7 @@ __global__ __launch_bounds__(64 * kShWaves) __attribute__((amdgpu_waves_per_eu(2
       *reinterpret_cast<u32x4*>(k_lds + (RPI * s + lr) * KP + 8 * lp) = kreg[s];
       *reinterpret_cast<u32x4*>(v_lds + (RPI * s + lr) * VP + 8 * lp) = vreg[s];
     }
-    fetch(t0 + TK * kShWaves);  // zeros past the chunk
+    fetch();
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
@@ -344,28 +372,34 @@ __global__ __launch_bounds__(64 * kShWaves) __attribute__((amdgpu_waves_per_eu(2
 #pragma unroll
     for (int s = 0; s < NDS; ++s)
       sc = sh_mfma32(*reinterpret_cast<const u32x4*>(k_lds + krow * KP + 16 * s + 8 * hf), qf[s], sc);
-    float mt = -INFINITY;
-    const bool full = t0 + TK <= nk;
+    if (t0 + TK > nk) {  // the chunk's last tile (uniform)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      sc[r] *= a.scale_log2;
-      if (!full && t0 + 16 * (r >> 3) + 8 * hf + (r & 7) >= nk) sc[r] = -INFINITY;
-      mt = fmaxf(mt, sc[r]);
+      for (int r = 0; r < 16; ++r)
+        if (t0 + 16 * (r >> 3) + 8 * hf + (r & 7) >= nk) sc[r] = -INFINITY;
     }
-    mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
-    const float mnew = fmaxf(mrun, mt);
-    const float mref = mnew == -INFINITY ? 0.f : mnew;
+    float mt = -INFINITY;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) mt = fmaxf(mt, sc[r]);
+    mt = fmaxf(mt, __shfl_xor(mt, 32, 64)) * scale;
+    if (__builtin_amdgcn_ballot_w64(mt > mref + 8.f)) {
+      const float mnew = mt > mref + 8.f ? mt : mref;
+      const float corr = mref == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mref - mnew);
+      mref = mnew;
+      lrun *= corr;
+#pragma unroll
+      for (int db = 0; db < NDB; ++db)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[db][r] *= corr;
+    }
+    const float ref = mref == -INFINITY ? 0.f : mref;
     // v_exp_f32 flushes below 2^-126: far under a bf16 probability's resolution
-    const float corr = __builtin_amdgcn_exp2f(mrun - mref);
     float lt = 0.f;
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-      sc[r] = __builtin_amdgcn_exp2f(sc[r] - mref);
+      sc[r] = __builtin_amdgcn_exp2f(fmaf(sc[r], scale, -ref));
       lt += sc[r];
     }
-    lt += __shfl_xor(lt, 32, 64);
-    lrun = fmaf(lrun, corr, lt);
-    mrun = mnew;
+    lrun += lt + __shfl_xor(lt, 32, 64);
     // the one rounding before the output's: P meets V as bf16 (half a step: 2^-8
     // of P, at random signs), where fp32 products would take 8 times the MFMA time
     u32x4 pb[2];
@@ -373,12 +407,6 @@ __global__ __launch_bounds__(64 * kShWaves) __attribute__((amdgpu_waves_per_eu(2
     for (int s = 0; s < 2; ++s)
 #pragma unroll
       for (int e = 0; e < 4; ++e) pb[s][e] = f32x2_to_bf16x2_bits(sc[8 * s + 2 * e], sc[8 * s + 2 * e + 1]);
-    if (__builtin_amdgcn_ballot_w64(corr != 1.f)) {
-#pragma unroll
-      for (int db = 0; db < NDB; ++db)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) o[db][r] *= corr;
-    }
 #pragma unroll
     for (int s = 0; s < 2; ++s)
 #pragma unroll
@@ -398,58 +426,52 @@ __global__ __launch_bounds__(64 * kShWaves) __attribute__((amdgpu_waves_per_eu(2
         *reinterpret_cast<f32x4*>(o_lds + (wave * RT + col) * OP + 32 * db + 8 * r + 4 * hf) =
             f32x4{o[db][4 * r], o[db][4 * r + 1], o[db][4 * r + 2], o[db][4 * r + 3]};
     if (hf == 0) {
-      m_lds[wave * RT + col] = mrun;
+      m_lds[wave * RT + col] = mref;
       l_lds[wave * RT + col] = lrun;
     }
   }
   __syncthreads();
-  sh_leave<DH, OP, RT>(a, it, o_lds, m_lds, l_lds);
+  sh_leave<DH, OP, RT>(a, it, o_lds, m_lds, l_lds, at_lds);
 }
 
-// Group of row i (the last one that starts at or before it and ends after it), or -1.
-__device__ __forceinline__ int row_group(const int32_t* __restrict__ gfirst, int ng, int i) {
-  if (ng == 0 || i < gfirst[0] || i >= gfirst[ng]) return -1;
-  int lo = 0, hi = ng;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (gfirst[mid] <= i)
-      lo = mid;
-    else
-      hi = mid;
-  }
-  return lo;
-}
-
-// One row's parts, prefix chunks then its own, merged in that order.
+// One row's parts, prefix chunks then its own, merged in that order, kCombineBatch
+// at a time (loads together, one rescale of the sums per batch). The row's group
+// is found by one wave-wide look at group_first per 64 groups.
 template <typename T, int DH>
 __global__ __launch_bounds__(DH) void attn_shared_combine(ShArgs a) {
   constexpr int B = kCombineBatch;
-  const int h = blockIdx.x, i = blockIdx.y, d = threadIdx.x;
-  const int j = row_group(a.gfirst, a.ng, i);
-  const int P = j < 0 ? 0 : min(a.plen[j], a.pmax);
-  const int np = P > 0 ? div_up(P, prefix_chunk(P, a.Hkv)) : 0;
-  const int ns = np + div_up(min(a.rlen[i], a.omax), kShOwnChunk);
-  const int64_t base = ((int64_t)i * a.H + h) * (a.pchunks + a.ochunks);
-  auto at = [&](int s) { return base + (s < np ? s : a.pchunks + s - np); };
-  float M = -INFINITY;
-  for (int s0 = 0; s0 < ns; s0 += B) {
-    float mv[B];
-#pragma unroll
-    for (int b = 0; b < B; ++b) mv[b] = s0 + b < ns ? a.pml[2 * at(s0 + b)] : -INFINITY;
-#pragma unroll
-    for (int b = 0; b < B; ++b) M = fmaxf(M, mv[b]);
+  const int h = blockIdx.x, i = blockIdx.y, d = threadIdx.x, lane = threadIdx.x & 63;
+  const int own = div_up(min(a.rlen[i], a.omax), kShOwnChunk);
+  int P = 0;
+  for (int j0 = 0; j0 < a.ng; j0 += 64) {  // uniform
+    const int j = min(j0 + lane, a.ng - 1);
+    const uint64_t hit = __ballot(j0 + lane < a.ng && a.gfirst[j] <= i && i < a.gfirst[j + 1]);
+    const int len = a.plen[j];
+    if (hit) P = __shfl(len, __builtin_ctzll(hit), 64);
   }
-  float O = 0.f, L = 0.f;
+  P = min(P, a.pmax);
+  const int np = P > 0 ? div_up(P, prefix_chunk(P, a.Hkv)) : 0;
+  const int ns = np + own;
+  const int64_t base = ((int64_t)i * a.H + h) * (a.pchunks + a.ochunks);
+  float M = -INFINITY, O = 0.f, L = 0.f;
   for (int s0 = 0; s0 < ns; s0 += B) {
     float mv[B], lv[B], ov[B];
+    float mb = M;
 #pragma unroll
     for (int b = 0; b < B; ++b) {
-      const bool ok = s0 + b < ns;
-      const int64_t p = ok ? at(s0 + b) : base;
-      mv[b] = ok ? a.pml[2 * p] : -INFINITY;
-      lv[b] = ok ? a.pml[2 * p + 1] : 0.f;
-      ov[b] = ok ? a.po[p * DH + d] : 0.f;
+      const int s = min(s0 + b, ns - 1);
+      const int64_t p = base + (s < np ? s : a.pchunks + s - np);
+      const float2 ml = *reinterpret_cast<const float2*>(a.pml + 2 * p);
+      ov[b] = a.po[p * DH + d];
+      mv[b] = s0 + b < ns ? ml.x : -INFINITY;
+      lv[b] = ml.y;
     }
+#pragma unroll
+    for (int b = 0; b < B; ++b) mb = fmaxf(mb, mv[b]);
+    const float corr = M == -INFINITY ? 1.f : exp2f(M - mb);  // nothing but zeros (or a NaN to keep) so far
+    O *= corr;
+    L *= corr;
+    M = mb;
 #pragma unroll
     for (int b = 0; b < B; ++b) {
       if (s0 + b < ns) {
@@ -463,12 +485,17 @@ __global__ __launch_bounds__(DH) void attn_shared_combine(ShArgs a) {
 }
 
 template <typename T, int DH>
-static void launch_shared(const ShArgs& a, int64_t wgs, hipStream_t st) {
-  if (wgs) {
-    if constexpr (sizeof(T) == 2)
-      hipLaunchKernelGGL((attn_shared_bf16_kernel<DH>), dim3((unsigned)wgs), dim3(64 * kShWaves), 0, st, a);
-    else
-      hipLaunchKernelGGL((attn_shared_f32_kernel<DH>), dim3((unsigned)wgs), dim3(64 * kShWaves), 0, st, a);
+static void launch_shared(ShArgs a, int64_t pairs, hipStream_t st) {
+  const int64_t nkeys = (int64_t)a.ng * a.pchunks * a.Hkv, own = (int64_t)a.n * a.ochunks * a.Hkv;
+  auto tiles = [&](int rt) { return (int)((pairs + rt - 1) / rt); };
+  auto grid = [&](int64_t prefix_tiles) { return dim3((unsigned)((nkeys + 7) / 8 * 8 * prefix_tiles + own)); };
+  const dim3 block(64 * kShWaves);
+  if constexpr (sizeof(T) == 4) {
+    a.tiles = tiles(kShRowsF32);
+    if (grid(a.tiles).x) hipLaunchKernelGGL((attn_shared_f32_kernel<DH>), grid(a.tiles), block, 0, st, a);
+  } else {
+    a.tiles = tiles(kShRowsBF16);
+    if (grid(a.tiles).x) hipLaunchKernelGGL((attn_shared_bf16_kernel<DH>), grid(a.tiles), block, 0, st, a);
   }
   hipLaunchKernelGGL((attn_shared_combine<T, DH>), dim3(a.H, a.n), dim3(DH), 0, st, a);
 }
@@ -554,12 +581,10 @@ int wfd_attn_shared(const void* q, const void* k_cache, const void* v_cache, int
               group_max, prefix_len_max, kv_len_max);
     return kUnsupported;
   }
-  a.tiles = (int)tiles;
-  const int64_t wgs = ((int64_t)ngroups * a.pchunks * Hkv + 7) / 8 * 8 * tiles + (int64_t)n * a.ochunks * Hkv;
   if (dtype == kBF16)
-    Dh == 64 ? launch_shared<bf16_t, 64>(a, wgs, stream) : launch_shared<bf16_t, 128>(a, wgs, stream);
+    Dh == 64 ? launch_shared<bf16_t, 64>(a, pairs, stream) : launch_shared<bf16_t, 128>(a, pairs, stream);
   else
-    Dh == 64 ? launch_shared<float, 64>(a, wgs, stream) : launch_shared<float, 128>(a, wgs, stream);
+    Dh == 64 ? launch_shared<float, 64>(a, pairs, stream) : launch_shared<float, 128>(a, pairs, stream);
   return launch_status(me);
 }
 
