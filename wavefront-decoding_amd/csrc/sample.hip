@@ -14,11 +14,15 @@
 // kernel's layout, the companions or the run -- and a border is off by 2^-45 per
 // token. u, p and their products with the sums are exact (64 x 64 -> 128 bits).
 //
-// One workgroup per row; no sort: the prefix is found by a radix select over
-// the logits' order-preserving keys, 8 bits a pass from the top, with the count
-// (top-k) or the weight (top-p) of each digit's tokens in LDS; only the tokens
-// that share the digits found so far take part. Ties with the last kept key are
-// kept in index order.
+// One workgroup per row; no sort. The last kept token is found in two steps:
+// a histogram of the logits' distance from the largest, over the range that
+// holds any weight, says which of 1024 bins it lies in, by count (top-k) or by
+// weight (top-p); the tokens of that bin -- with top-k, of all bins up to it --
+// go to a list in LDS, and a radix select over the list's keys, 10 bits a pass,
+// finds it. A list that would overflow (thousands of nearly equal logits at the
+// border) is replaced by the row itself. Ties with the last kept key are kept in
+// index order. What follows a top-k that fits the list never looks at the rest
+// of the row.
 #include "wfd_common.h"
 
 namespace wfd {
@@ -59,26 +63,64 @@ struct SmArgs {
   int V;
 };
 
-// NR > 0: the row's chunks live in registers (V <= NR * kSmChunk); 0: they are
-// read again in every pass (from L2).
-template <int NR>
+constexpr int kSmBins = 1024;   // one per thread
+constexpr int kSmList = 2048;
+constexpr float kSmSpan = 100.f;  // logits this far below the largest share the last bin
+
+__device__ __forceinline__ uint64_t sm_wave_sum(uint64_t v) {
+#pragma unroll
+  for (int m = 32; m >= 1; m >>= 1) v += sm_shfl_xor(v, m);
+  return v;
+}
+
+// 2^x for x <= 0 in units of 2^-44, rounded to nearest: x = m / 32 + r, 2^r by its
+// series to r^5 (the rest is below 3e-15 of it), 2^(m / 32) from the table.
+__device__ __forceinline__ uint64_t sm_exp2(double x, const double* __restrict__ tab) {
+  if (!(x > -46.)) return 0;  // also NaN
+  const double m = rint(x * 32.);
+  const double r = fma(m, -0.03125, x);
+  const int k = (int)m;
+  double p = fma(r, 0.0013333558146428443, 0.009618129107628477);
+  p = fma(p, r, 0.05550410866482158);
+  p = fma(p, r, 0.24022650695910072);
+  p = fma(p, r, 0.6931471805599453);
+  p = fma(p, r, 1.0);
+  const double w = ldexp(p * tab[k & 31], (k >> 5) + 44);
+  return __double_as_longlong(w + 4503599627370496.0) - 0x4330000000000000ll;  // + 2^52: rounded to an integer
+}
+
+// floor(s f) for f in [0, 1), and whether anything was cut off
+__device__ __forceinline__ uint64_t sm_mul_frac(uint64_t s, float f, bool& rest) {
+  const uint64_t q = (uint64_t)((double)f * 18446744073709551616.0);
+  rest = s * q != 0;
+  return __umul64hi(s, q);
+}
+
+// CAP > 0: the row is kept in LDS (V <= CAP); 0: it is read again in every pass
+// (from L2). In registers, 32 logits a thread, the passes' code spilled.
+template <int CAP>
 __global__ __launch_bounds__(kSmThreads) void sample_kernel(SmArgs a) {
-  __shared__ unsigned long long hist[256];
-  __shared__ unsigned long long seg[kSmMaxVocab / 256];  // per 256 logits, in index order
-  __shared__ float s_max[kSmWaves];
+  __shared__ unsigned long long hist[kSmBins];
+  __shared__ unsigned long long seg[(CAP > 0 ? CAP : kSmMaxVocab) / 256];  // per 256 logits, in index order
+  __shared__ __align__(16) u32x4 keep[CAP > 0 ? CAP / 4 : 1];
+  __shared__ uint32_t list_key[kSmList];
+  __shared__ uint32_t list_idx[kSmList];
+  __shared__ double tab[32];
+  __shared__ float s_max[kSmWaves], s_min[kSmWaves];
   __shared__ int s_idx[kSmWaves];
   __shared__ unsigned long long s_sum[kSmWaves];
-  __shared__ unsigned long long s_u64[2];
-  __shared__ uint32_t s_u32[2];
+  __shared__ uint32_t s_lo[kSmWaves], s_hi[kSmWaves];
+  __shared__ unsigned long long s_u64;
+  __shared__ uint32_t s_u32, s_count;
   const int i = blockIdx.x;
   const int t = threadIdx.x;
-  const int wave = t >> 6, lane = t & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63;
   const int V = a.V;
   const float* row = a.logits + (int64_t)i * a.ld;
   const bool vec = ((uintptr_t)row & 15) == 0;
   const int nchunks = (V + kSmChunk - 1) / kSmChunk;
 
-  auto fetch = [&](int c, float (&x)[4]) {  // logits 4096 c + 4 t ..; past the row: NaN-free filler, masked by index
+  auto fetch = [&](int c, float (&x)[4]) {  // logits 4096 c + 4 t ..; -inf past the row, and never used there
     const int e = c * kSmChunk + 4 * t;
     if (vec && e + 4 <= V) {
       Elem<float>::unpack(ld16(row + e), x);
@@ -87,22 +129,30 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SmArgs a) {
       for (int k = 0; k < 4; ++k) x[k] = e + k < V ? row[e + k] : -INFINITY;
     }
   };
-  float reg[NR > 0 ? NR : 1][4];
-  if constexpr (NR > 0) {
+  if constexpr (CAP > 0) {  // every load first; a thread reads back only what it stores
+    float x[CAP / kSmChunk][4];
 #pragma unroll
-    for (int c = 0; c < NR; ++c) fetch(c, reg[c]);
+    for (int c = 0; c < CAP / kSmChunk; ++c) fetch(c, x[c]);
+#pragma unroll
+    for (int c = 0; c < CAP / kSmChunk; ++c) keep[c * kSmThreads + t] = Elem<float>::pack(x[c]);
   }
+  if (t < 32) tab[t] = exp2((double)t * 0.03125);
   // f(chunk, first index, the 4 logits) over the row, in index order per thread
   auto each = [&](auto f) {
-    if constexpr (NR > 0) {
-#pragma unroll
-      for (int c = 0; c < NR; ++c)
-        if (c < nchunks) f(c, c * kSmChunk + 4 * t, reg[c]);
-    } else {
+    float x[4];
+    if constexpr (CAP > 0) {
       for (int c = 0; c < nchunks; ++c) {
-        float x[4];
-        fetch(c, x);
+        Elem<float>::unpack(keep[c * kSmThreads + t], x);
         f(c, c * kSmChunk + 4 * t, x);
+      }
+    } else {
+      fetch(0, x);
+      for (int c = 0; c < nchunks; ++c) {  // a chunk ahead
+        float y[4];
+        fetch(min(c + 1, nchunks - 1), y);
+        f(c, c * kSmChunk + 4 * t, x);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[k] = y[k];
       }
     }
   };
@@ -124,6 +174,7 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SmArgs a) {
   __syncthreads();
   best = s_max[0];
   bi = s_idx[0];
+#pragma unroll
   for (int w = 1; w < kSmWaves; ++w) argmax_merge(best, bi, s_max[w], s_idx[w]);
 
   const float T = a.temperature ? a.temperature[i] : 1.f;
@@ -132,20 +183,24 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SmArgs a) {
     if (t == 0) argmax_finish(i, bi, a.out, a.ring, a.ring_rows, a.ring_len, a.expect, a.accept);
     return;
   }
-  const double mx = (double)best;
   const double inv = 1.4426950408889634 / (double)T;
-  auto weight_of = [&](float l, float floor_w) -> uint64_t {
+  auto weight = [&](float l) -> uint64_t {
     if (l == best) return (uint64_t)kSmOne;  // also of infinite logits
     if (l == -INFINITY) return 0;
-    const double w = exp2(((double)l - mx) * inv);
-    if (floor_w > 0.f && w < (double)floor_w) return 0;
-    return w > 0. ? (uint64_t)(w * kSmOne + 0.5) : 0;  // NaN (infinite temperature under an infinite logit): 0
+    return sm_exp2(((double)l - (double)best) * inv, tab);
   };
-  auto weight = [&](float l) { return weight_of(l, 0.f); };
+  const int k = a.top_k ? a.top_k[i] : 0;
+  const bool has_k = k > 0 && k < V;
+  const float p = a.top_p ? a.top_p[i] : 1.f;
+  const bool has_p = p < 1.f;
+  const float minp = a.min_p ? a.min_p[i] : 0.f;
+  // min_p on the integer weights' scale: w >= min_p for w on or above it
+  const uint64_t wmin = minp > 0.f ? (minp < 1.f ? (uint64_t)ceil((double)minp * kSmOne) : (uint64_t)kSmOne) : 0;
+  float u = a.u[i];
+  u = u > 0.f ? (u < 1.f ? u : 0.99999994f) : 0.f;
 
   auto block_sum = [&](uint64_t v) -> uint64_t {
-#pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) v += sm_shfl_xor(v, m);
+    v = sm_wave_sum(v);
     __syncthreads();
     if (lane == 0) s_sum[wave] = v;
     __syncthreads();
@@ -154,107 +209,221 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SmArgs a) {
     for (int w = 0; w < kSmWaves; ++w) s += s_sum[w];
     return s;
   };
+  // The bin (thread t holds bin t's sum v) in which base plus the running sum reaches need; before: the sum before it.
+  auto find_bin = [&](uint64_t v, uint64_t base, uint64_t need, uint64_t& before) -> uint32_t {
+    uint64_t inc = v;
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) {
+      const uint64_t o = sm_shfl_up(inc, m);
+      if (lane >= m) inc += o;
+    }
+    __syncthreads();
+    if (lane == 63) s_sum[wave] = inc;
+    __syncthreads();
+    for (int w = 0; w < wave; ++w) base += s_sum[w];
+    const uint64_t run = base + inc - v;
+    if (run < need && run + v >= need) {
+      s_u32 = t;
+      s_u64 = run;
+    }
+    __syncthreads();
+    before = s_u64;
+    return s_u32;
+  };
 
   // Kept so far: keys above kk, and the first `ties` tokens with key kk.
   uint32_t kk = 0;
   uint64_t ties = 0;
 
-  // The shortest prefix of the kept tokens whose measure (1 or the weight) reaches need > 0.
-  auto select = [&](uint64_t need, bool by_weight) {
+  // The shortest prefix of the kept tokens whose measure (1 or the weight), on
+  // top of base, reaches need. over(f) calls f(key) for tokens that include all
+  // that may end it; equal keys may all be there, the kept ties count as ties.
+  auto refine = [&](auto over, uint64_t base, uint64_t need, bool by_weight) {
     const uint32_t k0 = kk;
     const uint64_t t0 = ties;
-    uint32_t prefix = 0;
-    uint64_t above = 0;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      __syncthreads();
-      if (t < 256) hist[t] = 0;
-      __syncthreads();
-      each([&](int, int e, const float (&x)[4]) {
+    uint32_t lo = 0xffffffffu, hi = 0;
+    over([&](uint32_t key) {
+      if (key > k0 || (t0 && key == k0)) {
+        lo = min(lo, key);
+        hi = max(hi, key);
+      }
+    });
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const uint32_t key = sm_key(x[k]);
-          if (e + k < V && key > k0 && (shift == 24 || (key >> (shift + 8)) == (prefix >> (shift + 8)))) {
-            const uint64_t m = by_weight ? weight(x[k]) : 1;
-            if (m) atomicAdd(&hist[(key >> shift) & 255], (unsigned long long)m);
-          }
+    for (int m = 32; m >= 1; m >>= 1) {
+      lo = min(lo, (uint32_t)__shfl_xor((int)lo, m, 64));
+      hi = max(hi, (uint32_t)__shfl_xor((int)hi, m, 64));
+    }
+    __syncthreads();
+    if (lane == 0) {
+      s_lo[wave] = lo;
+      s_hi[wave] = hi;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kSmWaves; ++w) {
+      lo = min(lo, s_lo[w]);
+      hi = max(hi, s_hi[w]);
+    }
+    // digits of hi - key, so that larger keys come first
+    const int bits = 32 - __clz((int)((hi - lo) | 1u));
+    int shift = bits;
+    uint32_t prefix = 0;
+    while (shift > 0) {  // uniform
+      const int width = min(10, shift), next = shift - width;
+      const uint32_t mask = (1u << width) - 1;
+      __syncthreads();
+      hist[t] = 0;
+      __syncthreads();
+      auto add = [&](uint32_t key, uint64_t m) {
+        const uint32_t off = hi - key;
+        if (shift == bits || off >> shift == prefix) atomicAdd(&hist[(off >> next) & mask], (unsigned long long)m);
+      };
+      over([&](uint32_t key) {
+        if (key > k0 && key >= lo && key <= hi) {
+          const uint64_t m = by_weight ? weight(sm_logit(key)) : 1;
+          if (m) add(key, m);
         }
       });
-      if (t == 0 && t0 && (shift == 24 || (k0 >> (shift + 8)) == (prefix >> (shift + 8)))) {
-        // the kept ties, as one
-        atomicAdd(&hist[(k0 >> shift) & 255], (unsigned long long)(t0 * (by_weight ? weight(sm_logit(k0)) : 1)));
-      }
+      if (t == 0 && t0 && k0 >= lo && k0 <= hi) add(k0, t0 * (by_weight ? weight(sm_logit(k0)) : 1));
       __syncthreads();
-      if (wave == 0) {  // lane b holds digits 255 - 4 b .. 252 - 4 b: the running sum from the top
-        uint64_t v[4], own = 0;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) own += v[k] = hist[255 - 4 * lane - k];
-        uint64_t inc = own;
-#pragma unroll
-        for (int m = 1; m < 64; m <<= 1) {
-          const uint64_t o = sm_shfl_up(inc, m);
-          if (lane >= m) inc += o;
-        }
-        uint64_t run = above + inc - own;
-        const uint64_t hit = __ballot(run < need && run + own >= need);  // one lane: the sums reach need
-        if (hit >> lane & 1) {
-          int d = 255 - 4 * lane;
-#pragma unroll
-          for (int k = 0; k < 3; ++k)
-            if (run + v[k] < need && d == 255 - 4 * lane - k) {
-              run += v[k];
-              --d;
-            }
-          s_u32[0] = prefix | ((uint32_t)d << shift);
-          s_u64[0] = run;
-        }
-      }
-      __syncthreads();
-      prefix = s_u32[0];
-      above = s_u64[0];
+      const uint32_t d = find_bin(hist[t], base, need, base);
+      prefix = (prefix << width) | d;
+      shift = next;
     }
-    kk = prefix;
-    const uint64_t each_w = by_weight ? weight(sm_logit(kk)) : 1;
-    ties = (need - above + each_w - 1) / each_w;  // >= 1; no more than there are, since they reach need
+    kk = hi - prefix;
+    const uint64_t one = by_weight ? weight(sm_logit(kk)) : 1;
+    ties = (need - base + one - 1) / one;  // >= 1; no more than there are, since they reach need
   };
 
-  const int k = a.top_k ? a.top_k[i] : 0;
-  if (k > 0 && k < V) select((uint64_t)k, false);
-
-  auto mul_frac = [](uint64_t s, float f, uint64_t& lo) -> uint64_t {  // floor(s * f), f in [0, 1), and the rest
-    const uint64_t q = (uint64_t)((double)f * 18446744073709551616.0);
-    lo = s * q;
-    return __umul64hi(s, q);
+  // bins of the distance from the largest logit, the lowest within kSmSpan in the last but one
+  float scale = 0.f;
+  auto bin_of = [&](float l) -> int { return l == best ? 0 : (int)fminf((best - l) * scale, (float)(kSmBins - 1)); };
+  if (has_k || has_p) {
+    float low = best;
+    each([&](int, int, const float (&x)[4]) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        if (x[q] >= best - kSmSpan) low = fminf(low, x[q]);
+    });
+#pragma unroll
+    for (int m = 32; m >= 1; m >>= 1) low = fminf(low, __shfl_xor(low, m, 64));
+    if (lane == 0) s_min[wave] = low;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kSmWaves; ++w) low = fminf(low, s_min[w]);
+    scale = best > low ? (float)(kSmBins - 2) / (best - low) : 0.f;
+  }
+  // Tokens of bins [b0, b1] to the list; false if they are too many.
+  int nlist = 0;
+  auto collect = [&](int b0, int b1) -> bool {
+    __syncthreads();
+    if (t == 0) s_count = 0;
+    __syncthreads();
+    each([&](int, int e, const float (&x)[4]) {
+      bool in[4];
+      int mine = 0;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int b = bin_of(x[q]);
+        in[q] = e + q < V && b >= b0 && b <= b1;
+        mine += in[q];
+      }
+      if (mine) {
+        uint32_t at = atomicAdd(&s_count, (uint32_t)mine);
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          if (in[q]) {
+            if (at < kSmList) {
+              list_key[at] = sm_key(x[q]);
+              list_idx[at] = e + q;
+            }
+            ++at;
+          }
+      }
+    });
+    __syncthreads();
+    nlist = (int)min(s_count, (uint32_t)kSmList);
+    return s_count <= kSmList;
   };
-  auto kept_sum = [&](float floor_w) -> uint64_t {
-    uint64_t s = 0;
+  auto over_list = [&](auto f) {
+    for (int e = t; e < nlist; e += kSmThreads) f(list_key[e]);
+  };
+  auto over_row = [&](auto f) {
     each([&](int, int e, const float (&x)[4]) {
 #pragma unroll
       for (int q = 0; q < 4; ++q)
-        if (e + q < V && sm_key(x[q]) > kk) s += weight_of(x[q], floor_w);
+        if (e + q < V) f(sm_key(x[q]));
     });
-    s = block_sum(s);
-    return ties ? s + ties * weight_of(sm_logit(kk), floor_w) : s;
   };
-  const float p = a.top_p ? a.top_p[i] : 1.f;
-  if (p < 1.f) {
-    uint64_t lo;
-    const uint64_t s = kept_sum(0.f);
-    uint64_t need = mul_frac(s, p > 0.f ? p : 0.f, lo);
-    if (lo || need == 0) ++need;
-    select(need, true);
-  }
 
-  // the last kept tie's index, if some of the ties are left out
-  auto find = [&](uint64_t target, auto measure) -> int {  // lowest index whose running sum exceeds target
-    each([&](int c, int e, const float (&x)[4]) {
-      uint64_t v = 0;
+  bool all_listed = false;  // every kept token is in the list
+  if (has_k) {
+    hist[t] = 0;
+    __syncthreads();
+    each([&](int, int e, const float (&x)[4]) {
 #pragma unroll
       for (int q = 0; q < 4; ++q)
-        if (e + q < V) v += measure(e + q, x[q]);
-#pragma unroll
-      for (int m = 32; m >= 1; m >>= 1) v += sm_shfl_xor(v, m);
-      if (lane == 0) seg[c * kSmWaves + wave] = v;
+        if (e + q < V) atomicAdd(&hist[bin_of(x[q])], 1ull);
     });
+    __syncthreads();
+    uint64_t before;
+    const uint32_t b = find_bin(hist[t], 0, (uint64_t)k, before);
+    const uint64_t upto = before + hist[b];
+    all_listed = upto <= kSmList;
+    if (all_listed) {
+      collect(0, b);
+      refine(over_list, 0, (uint64_t)k, false);
+    } else if (collect(b, b)) {
+      refine(over_list, before, (uint64_t)k, false);
+    } else {
+      refine(over_row, 0, (uint64_t)k, false);
+    }
+  }
+  auto kept_sum = [&](auto over) -> uint64_t {
+    uint64_t s = 0;
+    over([&](uint32_t key) {
+      if (key > kk) s += weight(sm_logit(key));
+    });
+    s = block_sum(s);
+    return ties ? s + ties * weight(sm_logit(kk)) : s;
+  };
+  if (has_p) {
+    bool rest;
+    auto need_of = [&](uint64_t s) -> uint64_t {
+      const uint64_t need = sm_mul_frac(s, p > 0.f ? p : 0.f, rest);
+      return rest || need == 0 ? need + 1 : need;
+    };
+    if (all_listed) {
+      refine(over_list, 0, need_of(kept_sum(over_list)), true);
+    } else {
+      const uint32_t k0 = kk;
+      const uint64_t t0 = ties;
+      __syncthreads();
+      hist[t] = 0;
+      __syncthreads();
+      each([&](int, int e, const float (&x)[4]) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          if (e + q < V && sm_key(x[q]) > k0) {
+            const uint64_t w = weight(x[q]);
+            if (w) atomicAdd(&hist[bin_of(x[q])], (unsigned long long)w);
+          }
+      });
+      if (t == 0 && t0) atomicAdd(&hist[bin_of(sm_logit(k0))], (unsigned long long)(t0 * weight(sm_logit(k0))));
+      __syncthreads();
+      const uint64_t mine = hist[t];
+      const uint64_t need = need_of(block_sum(mine));
+      uint64_t before;
+      const uint32_t b = find_bin(mine, 0, need, before);
+      if (collect(b, b)) refine(over_list, before, need, true);
+      else refine(over_row, 0, need, true);
+    }
+  }
+
+  // the index up to which ties are kept
+  int last_tie = 0x7fffffff;
+  // Lowest index whose running sum of measure(index, logit), in index order, exceeds target; seg holds the sums.
+  auto find = [&](uint64_t target, auto measure) -> int {
     __syncthreads();
     if (wave == 0) {
       uint64_t base = 0;
@@ -290,30 +459,58 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SmArgs a) {
           if (r2 <= target && r2 + mine > target) {
             int q = 0;
             while (q < 3 && r2 + v[q] <= target) r2 += v[q++];
-            s_u32[0] = (uint32_t)(e + q);
+            s_u32 = (uint32_t)(e + q);
           }
           break;
         }
-        base = (uint64_t)__shfl((unsigned long long)inc, 63, 64) + base;
+        base += (uint64_t)__shfl((unsigned long long)inc, 63, 64);
       }
     }
     __syncthreads();
-    const int r = (int)s_u32[0];
-    __syncthreads();
-    return r;
+    return (int)s_u32;
   };
-  int last_tie = -1;
-  if (ties) last_tie = find(ties - 1, [&](int, float l) -> uint64_t { return sm_key(l) == kk ? 1 : 0; });
-  const float minp = a.min_p ? a.min_p[i] : 0.f;
-  const uint64_t total = kept_sum(minp);
-  float u = a.u[i];
-  u = u > 0.f ? (u < 1.f ? u : 0.99999994f) : 0.f;
-  uint64_t lo;
-  const uint64_t target = mul_frac(total, u, lo);
-  const int id = find(target, [&](int e, float l) -> uint64_t {
+  auto fill = [&](auto measure) -> uint64_t {  // seg from the row; their sum
+    uint64_t sum = 0;
+    each([&](int c, int e, const float (&x)[4]) {
+      uint64_t v = 0;
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        if (e + q < V) v += measure(e + q, x[q]);
+      sum += v;
+      if (__ballot(v != 0)) v = sm_wave_sum(v);
+      if (lane == 0) seg[c * kSmWaves + wave] = v;
+    });
+    return block_sum(sum);
+  };
+  if (ties) {
+    auto is_tie = [&](int, float l) -> uint64_t { return sm_key(l) == kk ? 1 : 0; };
+    __syncthreads();
+    if (fill(is_tie) > ties) last_tie = find(ties - 1, is_tie);
+    __syncthreads();
+  }
+  auto kept = [&](int e, float l) -> uint64_t {
     const uint32_t key = sm_key(l);
-    return key > kk || (key == kk && e <= last_tie) ? weight_of(l, minp) : 0;
-  });
+    if (!(key > kk || (key == kk && e <= last_tie))) return 0;
+    const uint64_t w = weight(l);
+    return w >= wmin ? w : 0;
+  };
+  uint64_t total;
+  if (all_listed) {
+    const int ns = nchunks * kSmWaves;
+    for (int e = t; e < ns; e += kSmThreads) seg[e] = 0;
+    __syncthreads();
+    uint64_t sum = 0;
+    for (int e = t; e < nlist; e += kSmThreads) {
+      const uint64_t w = kept((int)list_idx[e], sm_logit(list_key[e]));
+      sum += w;
+      if (w) atomicAdd(&seg[list_idx[e] >> 8], (unsigned long long)w);
+    }
+    total = block_sum(sum);
+  } else {
+    total = fill(kept);
+  }
+  bool rest;
+  const int id = find(sm_mul_frac(total, u, rest), kept);
   if (t == 0) argmax_finish(i, id, a.out, a.ring, a.ring_rows, a.ring_len, a.expect, a.accept);
 }
 
@@ -354,9 +551,9 @@ int wfd_sample(const float* logits, int64_t ld, const float* u, const float* tem
   a.accept = accept;
   a.V = vocab;
   if (vocab <= 2 * kSmChunk)
-    hipLaunchKernelGGL(sample_kernel<2>, dim3(n), dim3(kSmThreads), 0, stream, a);
+    hipLaunchKernelGGL(sample_kernel<2 * kSmChunk>, dim3(n), dim3(kSmThreads), 0, stream, a);
   else if (vocab <= 8 * kSmChunk)
-    hipLaunchKernelGGL(sample_kernel<8>, dim3(n), dim3(kSmThreads), 0, stream, a);
+    hipLaunchKernelGGL(sample_kernel<8 * kSmChunk>, dim3(n), dim3(kSmThreads), 0, stream, a);
   else
     hipLaunchKernelGGL(sample_kernel<0>, dim3(n), dim3(kSmThreads), 0, stream, a);
   return launch_status("wfd_sample");
