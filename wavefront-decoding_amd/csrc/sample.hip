@@ -14,15 +14,16 @@
 // kernel's layout, the companions or the run -- and a border is off by 2^-45 per
 // token. u, p and their products with the sums are exact (64 x 64 -> 128 bits).
 //
-// One workgroup per row; no sort. The last kept token is found in two steps:
-// a histogram of the logits' distance from the largest, over the range that
-// holds any weight, says which of 1024 bins it lies in, by count (top-k) or by
-// weight (top-p); the tokens of that bin -- with top-k, of all bins up to it --
-// go to a list in LDS, and a radix select over the list's keys, 10 bits a pass,
-// finds it. A list that would overflow (thousands of nearly equal logits at the
-// border) is replaced by the row itself. Ties with the last kept key are kept in
-// index order. What follows a top-k that fits the list never looks at the rest
-// of the row.
+// One workgroup per row. Where the kept tokens are few -- top-k, or a top-p whose
+// tokens hold enough of the weight -- they are found without ordering the row: of
+// the 1024 threads' largest logits, at least k are no smaller than the k-th, so
+// every one of the first k tokens is at or above it, and few others are. Those go
+// to a list in LDS, which is sorted (one entry a thread), and top-k, top-p and
+// min_p are positions in it.
+// Otherwise a histogram of the logits' distance from the largest says which of
+// 1024 bins the last kept token lies in, by count or by weight, and a radix select
+// over that bin's tokens (over the row, if they are too many) finds its key; ties
+// with it are kept in index order.
 #include "wfd_common.h"
 
 namespace wfd {
@@ -65,7 +66,9 @@ struct SmArgs {
 
 constexpr int kSmBins = 1024;   // one per thread
 constexpr int kSmList = 2048;
-constexpr float kSmSpan = 100.f;  // logits this far below the largest share the last bin
+constexpr int kSmSort = kSmThreads;  // entries of a list that is sorted
+constexpr int kSmGuess = 600;        // tokens aimed at for a top-p list
+constexpr float kSmMasked = -1e4f;  // logits down to here spread the bins; the others share the last
 
 __device__ __forceinline__ uint64_t sm_wave_sum(uint64_t v) {
 #pragma unroll
@@ -107,7 +110,6 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SmArgs a) {
   __shared__ uint32_t list_idx[kSmList];
   __shared__ double tab[32];
   __shared__ float s_max[kSmWaves], s_min[kSmWaves];
-  __shared__ int s_idx[kSmWaves];
   __shared__ unsigned long long s_sum[kSmWaves];
   __shared__ uint32_t s_lo[kSmWaves], s_hi[kSmWaves];
   __shared__ unsigned long long s_u64;
@@ -157,30 +159,55 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SmArgs a) {
     }
   };
 
-  // the largest logit and its first index; a NaN ranks above everything, as in wfd_argmax
-  float best = -INFINITY;
-  int bi = 0x7fffffff;
-  each([&](int, int e, const float (&x)[4]) {
+  // the largest logit (of the thread, of the row), whether there is a NaN, the range of the bins
+  float mine = -INFINITY, low = INFINITY;
+  bool nan = false;
+  each([&](int, int, const float (&x)[4]) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-      if (e + k < V) argmax_merge(best, bi, x[k], e + k);
+    for (int q = 0; q < 4; ++q) {
+      nan |= x[q] != x[q];
+      mine = fmaxf(mine, x[q]);
+      low = fminf(low, x[q] > kSmMasked ? x[q] : INFINITY);
+    }
   });
+  float best = mine;
 #pragma unroll
-  for (int m = 32; m >= 1; m >>= 1) argmax_merge(best, bi, __shfl_xor(best, m, 64), __shfl_xor(bi, m, 64));
+  for (int m = 32; m >= 1; m >>= 1) {
+    best = fmaxf(best, __shfl_xor(best, m, 64));
+    low = fminf(low, __shfl_xor(low, m, 64));
+  }
+  nan = __ballot(nan) != 0;
   if (lane == 0) {
-    s_max[wave] = best;
-    s_idx[wave] = bi;
+    s_max[wave] = nan ? __uint_as_float(0x7fc00000u) : best;
+    s_min[wave] = low;
   }
   __syncthreads();
-  best = s_max[0];
-  bi = s_idx[0];
+  nan = false;
 #pragma unroll
-  for (int w = 1; w < kSmWaves; ++w) argmax_merge(best, bi, s_max[w], s_idx[w]);
+  for (int w = 0; w < kSmWaves; ++w) {
+    nan |= s_max[w] != s_max[w];
+    best = fmaxf(best, s_max[w]);
+    low = fminf(low, s_min[w]);
+  }
 
   const float T = a.temperature ? a.temperature[i] : 1.f;
-  // greedy rows; rows with a NaN (its index, visibly) or without any possible token (index 0)
-  if (!(T > 0.f) || best != best || best == -INFINITY) {  // uniform
-    if (t == 0) argmax_finish(i, bi, a.out, a.ring, a.ring_rows, a.ring_len, a.expect, a.accept);
+  if (nan || !(T > 0.f) || best == -INFINITY) {  // uniform
+    // greedy rows: the first of the largest; a row with a NaN: its first, visibly, as
+    // in wfd_argmax; a row without any possible token: 0
+    int bi = 0x7fffffff;
+    each([&](int, int e, const float (&x)[4]) {
+#pragma unroll
+      for (int q = 3; q >= 0; --q)
+        if (e + q < V && (nan ? x[q] != x[q] : x[q] == best)) bi = min(bi, e + q);
+    });
+#pragma unroll
+    for (int m = 32; m >= 1; m >>= 1) bi = min(bi, __shfl_xor(bi, m, 64));
+    if (lane == 0) s_lo[wave] = (uint32_t)bi;
+    __syncthreads();
+    if (t == 0) {
+      for (int w = 0; w < kSmWaves; ++w) bi = min(bi, (int)s_lo[w]);
+      argmax_finish(i, bi, a.out, a.ring, a.ring_rows, a.ring_len, a.expect, a.accept);
+    }
     return;
   }
   const double inv = 1.4426950408889634 / (double)T;
@@ -209,8 +236,8 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SmArgs a) {
     for (int w = 0; w < kSmWaves; ++w) s += s_sum[w];
     return s;
   };
-  // The bin (thread t holds bin t's sum v) in which base plus the running sum reaches need; before: the sum before it.
-  auto find_bin = [&](uint64_t v, uint64_t base, uint64_t need, uint64_t& before) -> uint32_t {
+  // The sum of the threads' v before this one.
+  auto block_scan = [&](uint64_t v) -> uint64_t {
     uint64_t inc = v;
 #pragma unroll
     for (int m = 1; m < 64; m <<= 1) {
@@ -220,8 +247,14 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SmArgs a) {
     __syncthreads();
     if (lane == 63) s_sum[wave] = inc;
     __syncthreads();
-    for (int w = 0; w < wave; ++w) base += s_sum[w];
-    const uint64_t run = base + inc - v;
+    uint64_t before = lane < wave ? (uint64_t)s_sum[lane] : 0;  // 16 waves
+#pragma unroll
+    for (int m = 8; m >= 1; m >>= 1) before += sm_shfl_xor(before, m);
+    return (uint64_t)__shfl((unsigned long long)before, 0, 64) + inc - v;
+  };
+  // The bin (thread t holds bin t's sum v) in which base plus the running sum reaches need; before: the sum before it.
+  auto find_bin = [&](uint64_t v, uint64_t base, uint64_t need, uint64_t& before) -> uint32_t {
+    const uint64_t run = base + block_scan(v);
     if (run < need && run + v >= need) {
       s_u32 = t;
       s_u64 = run;
@@ -295,41 +328,25 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SmArgs a) {
     ties = (need - base + one - 1) / one;  // >= 1; no more than there are, since they reach need
   };
 
-  // bins of the distance from the largest logit, the lowest within kSmSpan in the last but one
-  float scale = 0.f;
+  const float scale = best > low ? (float)(kSmBins - 2) / (best - low) : 1.f;
   auto bin_of = [&](float l) -> int { return l == best ? 0 : (int)fminf((best - l) * scale, (float)(kSmBins - 1)); };
-  if (has_k || has_p) {
-    float low = best;
-    each([&](int, int, const float (&x)[4]) {
-#pragma unroll
-      for (int q = 0; q < 4; ++q)
-        if (x[q] >= best - kSmSpan) low = fminf(low, x[q]);
-    });
-#pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) low = fminf(low, __shfl_xor(low, m, 64));
-    if (lane == 0) s_min[wave] = low;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kSmWaves; ++w) low = fminf(low, s_min[w]);
-    scale = best > low ? (float)(kSmBins - 2) / (best - low) : 0.f;
-  }
   // Tokens of bins [b0, b1] to the list; false if they are too many.
   int nlist = 0;
-  auto collect = [&](int b0, int b1) -> bool {
+  auto collect = [&](int b0, int b1, uint32_t room = kSmList) -> bool {
     __syncthreads();
     if (t == 0) s_count = 0;
     __syncthreads();
     each([&](int, int e, const float (&x)[4]) {
       bool in[4];
-      int mine = 0;
+      int n_in = 0;
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const int b = bin_of(x[q]);
         in[q] = e + q < V && b >= b0 && b <= b1;
-        mine += in[q];
+        n_in += in[q];
       }
-      if (mine) {
-        uint32_t at = atomicAdd(&s_count, (uint32_t)mine);
+      if (n_in) {
+        uint32_t at = atomicAdd(&s_count, (uint32_t)n_in);
 #pragma unroll
         for (int q = 0; q < 4; ++q)
           if (in[q]) {
@@ -343,7 +360,7 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SmArgs a) {
     });
     __syncthreads();
     nlist = (int)min(s_count, (uint32_t)kSmList);
-    return s_count <= kSmList;
+    return s_count <= room;
   };
   auto over_list = [&](auto f) {
     for (int e = t; e < nlist; e += kSmThreads) f(list_key[e]);
@@ -356,8 +373,84 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SmArgs a) {
     });
   };
 
+  auto need_of = [&](uint64_t s) -> uint64_t {  // the weight that top-p asks of s, at least the least
+    bool rest;
+    const uint64_t need = sm_mul_frac(s, p > 0.f ? p : 0.f, rest);
+    return rest || need == 0 ? need + 1 : need;
+  };
   bool all_listed = false;  // every kept token is in the list
-  if (has_k) {
+  int last_tie = 0x7fffffff;  // ties are kept up to this index
+  bool selected = !has_k && !has_p;
+  uint64_t row_sum = 0;
+
+  // the list of the first tokens, sorted
+  const int guess = has_k ? k : kSmGuess;
+  if (!selected && (V <= kSmSort || guess <= min(kSmThreads, V / 4))) {  // V / 4 threads hold 4 logits each
+    uint32_t b = kSmBins - 1;
+    if (V > kSmSort) {
+      hist[t] = 0;
+      __syncthreads();
+      if (4 * t < V) atomicAdd(&hist[bin_of(mine)], 1ull);
+      __syncthreads();
+      uint64_t before;
+      b = find_bin(hist[t], 0, (uint64_t)guess, before);
+    }
+    bool enough = true;
+    if (!has_k) {  // does their weight reach p of the row's?
+      uint64_t all = 0, top = 0;
+      each([&](int, int e, const float (&x)[4]) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          if (e + q < V) {
+            const uint64_t w = weight(x[q]);
+            all += w;
+            top += bin_of(x[q]) <= (int)b ? w : 0;
+          }
+      });
+      row_sum = block_sum(all);
+      enough = block_sum(top) >= need_of(row_sum);
+    }
+    if (enough && collect(0, b, kSmSort)) {
+      // larger keys first, lower indexes first among equals; nothing behind the list
+      uint64_t v = t < nlist ? ((uint64_t)list_key[t] << 32) | (uint32_t)~list_idx[t] : 0;
+      unsigned long long* swap = hist;
+#pragma unroll
+      for (int size = 2; size <= kSmSort; size <<= 1) {
+#pragma unroll
+        for (int step = size >> 1; step > 0; step >>= 1) {
+          uint64_t o;
+          if (step < 64) {
+            o = sm_shfl_xor(v, step);
+          } else {
+            __syncthreads();
+            swap[t] = v;
+            __syncthreads();
+            o = swap[t ^ step];
+          }
+          const bool first = (t & step) == 0, falling = (t & size) == 0;
+          v = (first == falling) == (v > o) ? v : o;
+        }
+      }
+      __syncthreads();
+      swap[t] = v;
+      const uint64_t w = t < nlist ? weight(sm_logit((uint32_t)(v >> 32))) : 0;
+      const uint64_t before = block_scan(w);
+      if (has_k && t == k - 1) s_u64 = before + w;
+      __syncthreads();
+      uint64_t keep_n = has_k ? (uint64_t)k : 0;
+      if (has_p) {
+        const uint64_t need = need_of(has_k ? (uint64_t)s_u64 : row_sum);
+        if (before < need && before + w >= need) s_u32 = t;
+        __syncthreads();
+        keep_n = s_u32 + 1;
+      }
+      const uint64_t last = swap[keep_n - 1];
+      kk = (uint32_t)(last >> 32);
+      last_tie = (int)~(uint32_t)last;
+      all_listed = selected = true;
+    }
+  }
+  if (has_k && !selected) {
     hist[t] = 0;
     __syncthreads();
     each([&](int, int e, const float (&x)[4]) {
@@ -387,12 +480,7 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SmArgs a) {
     s = block_sum(s);
     return ties ? s + ties * weight(sm_logit(kk)) : s;
   };
-  if (has_p) {
-    bool rest;
-    auto need_of = [&](uint64_t s) -> uint64_t {
-      const uint64_t need = sm_mul_frac(s, p > 0.f ? p : 0.f, rest);
-      return rest || need == 0 ? need + 1 : need;
-    };
+  if (has_p && !selected) {
     if (all_listed) {
       refine(over_list, 0, need_of(kept_sum(over_list)), true);
     } else {
@@ -420,8 +508,6 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SmArgs a) {
     }
   }
 
-  // the index up to which ties are kept
-  int last_tie = 0x7fffffff;
   // Lowest index whose running sum of measure(index, logit), in index order, exceeds target; seg holds the sums.
   auto find = [&](uint64_t target, auto measure) -> int {
     __syncthreads();
