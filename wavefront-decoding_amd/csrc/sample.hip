@@ -30,7 +30,7 @@ namespace wfd {
 
 constexpr int kSmThreads = 1024;
 constexpr int kSmWaves = kSmThreads / 64;
-constexpr int kSmChunk = 4 * kSmThreads;  // logits per round of the workgroup: 4 consecutive ones a thread
+constexpr int kSmChunk = 4 * kSmThreads;  // logits per round of the workgroup, 4 consecutive ones a thread
 constexpr int kSmMaxVocab = 1 << 19;      // sums of 2^19 weights of 2^44 fit 63 bits
 constexpr double kSmOne = 17592186044416.0;  // 2^44
 
@@ -67,7 +67,7 @@ struct SmArgs {
 constexpr int kSmBins = 1024;   // one per thread
 constexpr int kSmList = 2048;
 constexpr int kSmSort = kSmThreads;  // entries of a list that is sorted
-constexpr int kSmGuess = 600;        // tokens aimed at for a top-p list
+constexpr int kSmGuess = 600;        // top-k up to which the list is tried: ~900 tokens are then above the k-th thread's
 constexpr float kSmMasked = -1e4f;  // logits down to here spread the bins; the others share the last
 
 __device__ __forceinline__ uint64_t sm_wave_sum(uint64_t v) {
@@ -77,19 +77,21 @@ __device__ __forceinline__ uint64_t sm_wave_sum(uint64_t v) {
 }
 
 // 2^x for x <= 0 in units of 2^-44, rounded to nearest: x = m / 32 + r, 2^r by its
-// series to r^5 (the rest is below 3e-15 of it), 2^(m / 32) from the table.
+// series to r^5 (the rest is below 3e-15 of it), 2^(m / 32) from the table with
+// the exponent added to its bits. Adding 1.5 2^52 (2^52) leaves the nearest integer
+// in the low bits of the sum.
 __device__ __forceinline__ uint64_t sm_exp2(double x, const double* __restrict__ tab) {
-  if (!(x > -46.)) return 0;  // also NaN
-  const double m = rint(x * 32.);
-  const double r = fma(m, -0.03125, x);
-  const int k = (int)m;
+  x = fmax(x, -900.);  // also of NaN; far below the least weight
+  const double t = fma(x, 32., 6755399441055744.);
+  const int k = (int)(uint32_t)__double_as_longlong(t);
+  const double r = fma(t - 6755399441055744., -0.03125, x);
   double p = fma(r, 0.0013333558146428443, 0.009618129107628477);
   p = fma(p, r, 0.05550410866482158);
   p = fma(p, r, 0.24022650695910072);
   p = fma(p, r, 0.6931471805599453);
   p = fma(p, r, 1.0);
-  const double w = ldexp(p * tab[k & 31], (k >> 5) + 44);
-  return __double_as_longlong(w + 4503599627370496.0) - 0x4330000000000000ll;  // + 2^52: rounded to an integer
+  const double two = __longlong_as_double(__double_as_longlong(tab[k & 31]) + ((long long)((k >> 5) + 44) << 52));
+  return (uint64_t)__double_as_longlong(fma(p, two, 4503599627370496.)) & 0xfffffffffffffull;
 }
 
 // floor(s f) for f in [0, 1), and whether anything was cut off
@@ -104,7 +106,7 @@ __device__ __forceinline__ uint64_t sm_mul_frac(uint64_t s, float f, bool& rest)
 template <int CAP>
 __global__ __launch_bounds__(kSmThreads) void sample_kernel(SmArgs a) {
   __shared__ unsigned long long hist[kSmBins];
-  __shared__ unsigned long long seg[(CAP > 0 ? CAP : kSmMaxVocab) / 256];  // per 256 logits, in index order
+  __shared__ unsigned long long seg[(CAP > 0 ? CAP : kSmMaxVocab) / 256];  // the running sums' steps, in index order
   __shared__ __align__(16) u32x4 keep[CAP > 0 ? CAP / 4 : 1];
   __shared__ uint32_t list_key[kSmList];
   __shared__ uint32_t list_idx[kSmList];
@@ -120,15 +122,19 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SmArgs a) {
   const int V = a.V;
   const float* row = a.logits + (int64_t)i * a.ld;
   const bool vec = ((uintptr_t)row & 15) == 0;
-  const int nchunks = (V + kSmChunk - 1) / kSmChunk;
+  // wave w holds the logits [w per_wave, (w + 1) per_wave): index order is wave, round, lane
+  const int per_wave = (V + 63) / 64 * 4;
+  const int w_end = min((wave + 1) * per_wave, V);
+  const int nchunks = (per_wave + 255) / 256;
+  auto first_of = [&](int c) { return wave * per_wave + 256 * c + 4 * lane; };
 
-  auto fetch = [&](int c, float (&x)[4]) {  // logits 4096 c + 4 t ..; -inf past the row, and never used there
-    const int e = c * kSmChunk + 4 * t;
-    if (vec && e + 4 <= V) {
+  auto fetch = [&](int c, float (&x)[4]) {  // 4 logits; -inf past the wave's
+    const int e = first_of(c);
+    if (vec && e + 4 <= w_end) {
       Elem<float>::unpack(ld16(row + e), x);
     } else {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) x[k] = e + k < V ? row[e + k] : -INFINITY;
+      for (int k = 0; k < 4; ++k) x[k] = e + k < w_end ? row[e + k] : -INFINITY;
     }
   };
   if constexpr (CAP > 0) {  // every load first; a thread reads back only what it stores
@@ -139,20 +145,21 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SmArgs a) {
     for (int c = 0; c < CAP / kSmChunk; ++c) keep[c * kSmThreads + t] = Elem<float>::pack(x[c]);
   }
   if (t < 32) tab[t] = exp2((double)t * 0.03125);
-  // f(chunk, first index, the 4 logits) over the row, in index order per thread
+  // f(first index, the 4 logits) over the row, in index order per thread; -inf fills the
+  // places past the wave's share, which no weight, bin or key below counts
   auto each = [&](auto f) {
     float x[4];
     if constexpr (CAP > 0) {
       for (int c = 0; c < nchunks; ++c) {
         Elem<float>::unpack(keep[c * kSmThreads + t], x);
-        f(c, c * kSmChunk + 4 * t, x);
+        f(first_of(c), x);
       }
     } else {
       fetch(0, x);
       for (int c = 0; c < nchunks; ++c) {  // a chunk ahead
         float y[4];
         fetch(min(c + 1, nchunks - 1), y);
-        f(c, c * kSmChunk + 4 * t, x);
+        f(first_of(c), x);
 #pragma unroll
         for (int k = 0; k < 4; ++k) x[k] = y[k];
       }
@@ -162,7 +169,7 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SmArgs a) {
   // the largest logit (of the thread, of the row), whether there is a NaN, the range of the bins
   float mine = -INFINITY, low = INFINITY;
   bool nan = false;
-  each([&](int, int, const float (&x)[4]) {
+  each([&](int, const float (&x)[4]) {
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       nan |= x[q] != x[q];
@@ -195,10 +202,10 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SmArgs a) {
     // greedy rows: the first of the largest; a row with a NaN: its first, visibly, as
     // in wfd_argmax; a row without any possible token: 0
     int bi = 0x7fffffff;
-    each([&](int, int e, const float (&x)[4]) {
+    each([&](int e, const float (&x)[4]) {
 #pragma unroll
       for (int q = 3; q >= 0; --q)
-        if (e + q < V && (nan ? x[q] != x[q] : x[q] == best)) bi = min(bi, e + q);
+        if (e + q < w_end && (nan ? x[q] != x[q] : x[q] == best)) bi = min(bi, e + q);
     });
 #pragma unroll
     for (int m = 32; m >= 1; m >>= 1) bi = min(bi, __shfl_xor(bi, m, 64));
@@ -210,11 +217,11 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SmArgs a) {
     }
     return;
   }
-  const double inv = 1.4426950408889634 / (double)T;
+  const double inv = fmin(1.4426950408889634 / (double)T, 1e300);  // finite: 0 times it is 0
+  const bool endless = best == INFINITY;  // infinite logits share everything
   auto weight = [&](float l) -> uint64_t {
-    if (l == best) return (uint64_t)kSmOne;  // also of infinite logits
-    if (l == -INFINITY) return 0;
-    return sm_exp2(((double)l - (double)best) * inv, tab);
+    if (endless) return l == best ? (uint64_t)kSmOne : 0;
+    return sm_exp2(((double)l - (double)best) * inv, tab);  // of the largest itself: exactly one
   };
   const int k = a.top_k ? a.top_k[i] : 0;
   const bool has_k = k > 0 && k < V;
@@ -266,7 +273,7 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SmArgs a) {
 
   // Kept so far: keys above kk, and the first `ties` tokens with key kk.
   uint32_t kk = 0;
-  uint64_t ties = 0;
+  uint64_t ties = 0, ties_left = 0;  // and the ones with key kk that are not
 
   // The shortest prefix of the kept tokens whose measure (1 or the weight), on
   // top of base, reaches need. over(f) calls f(key) for tokens that include all
@@ -326,6 +333,9 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SmArgs a) {
     kk = hi - prefix;
     const uint64_t one = by_weight ? weight(sm_logit(kk)) : 1;
     ties = (need - base + one - 1) / one;  // >= 1; no more than there are, since they reach need
+    uint64_t equal = 0;
+    over([&](uint32_t key) { equal += key == kk; });
+    ties_left = block_sum(equal) - ties;
   };
 
   const float scale = best > low ? (float)(kSmBins - 2) / (best - low) : 1.f;
@@ -336,13 +346,13 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SmArgs a) {
     __syncthreads();
     if (t == 0) s_count = 0;
     __syncthreads();
-    each([&](int, int e, const float (&x)[4]) {
+    each([&](int e, const float (&x)[4]) {
       bool in[4];
       int n_in = 0;
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const int b = bin_of(x[q]);
-        in[q] = e + q < V && b >= b0 && b <= b1;
+        in[q] = e + q < w_end && b >= b0 && b <= b1;
         n_in += in[q];
       }
       if (n_in) {
@@ -366,10 +376,10 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SmArgs a) {
     for (int e = t; e < nlist; e += kSmThreads) f(list_key[e]);
   };
   auto over_row = [&](auto f) {
-    each([&](int, int e, const float (&x)[4]) {
+    each([&](int e, const float (&x)[4]) {
 #pragma unroll
       for (int q = 0; q < 4; ++q)
-        if (e + q < V) f(sm_key(x[q]));
+        if (e + q < w_end) f(sm_key(x[q]));
     });
   };
 
@@ -381,82 +391,67 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SmArgs a) {
   bool all_listed = false;  // every kept token is in the list
   int last_tie = 0x7fffffff;  // ties are kept up to this index
   bool selected = !has_k && !has_p;
-  uint64_t row_sum = 0;
 
-  // the list of the first tokens, sorted
-  const int guess = has_k ? k : kSmGuess;
-  if (!selected && (V <= kSmSort || guess <= min(kSmThreads, V / 4))) {  // V / 4 threads hold 4 logits each
+  // the list of the first tokens, sorted, and the kept ones in it: of the k first
+  // (k > 0, else of all), those that reach need(weight of these)
+  auto from_list = [&](int kept_of, auto need) {
+    // larger keys first, lower indexes first among equals; nothing behind the list
+    uint64_t v = t < nlist ? ((uint64_t)list_key[t] << 32) | (uint32_t)~list_idx[t] : 0;
+    unsigned long long* swap = hist;
+#pragma unroll
+    for (int size = 2; size <= kSmSort; size <<= 1) {
+#pragma unroll
+      for (int step = size >> 1; step > 0; step >>= 1) {
+        uint64_t o;
+        if (step < 64) {
+          o = sm_shfl_xor(v, step);
+        } else {
+          __syncthreads();
+          swap[t] = v;
+          __syncthreads();
+          o = swap[t ^ step];
+        }
+        const bool first = (t & step) == 0, falling = (t & size) == 0;
+        v = (first == falling) == (v > o) ? v : o;
+      }
+    }
+    __syncthreads();
+    swap[t] = v;
+    const uint64_t w = t < nlist ? weight(sm_logit((uint32_t)(v >> 32))) : 0;
+    const uint64_t before = block_scan(w);
+    if (t == kept_of - 1) s_u64 = before + w;
+    __syncthreads();
+    int n_kept = kept_of;
+    if (has_p) {
+      const uint64_t least = need((uint64_t)s_u64);
+      if (before < least && before + w >= least) s_u32 = t;
+      __syncthreads();
+      n_kept = (int)s_u32 + 1;
+    }
+    const uint64_t last = swap[n_kept - 1];
+    kk = (uint32_t)(last >> 32);
+    last_tie = (int)~(uint32_t)last;
+    all_listed = selected = true;
+  };
+  if (has_k && (V <= kSmSort || k <= min(kSmGuess, V / 4))) {  // V / 4 threads, or 960, hold logits
     uint32_t b = kSmBins - 1;
     if (V > kSmSort) {
       hist[t] = 0;
       __syncthreads();
-      if (4 * t < V) atomicAdd(&hist[bin_of(mine)], 1ull);
+      if (first_of(0) < w_end) atomicAdd(&hist[bin_of(mine)], 1ull);
       __syncthreads();
       uint64_t before;
-      b = find_bin(hist[t], 0, (uint64_t)guess, before);
+      b = find_bin(hist[t], 0, (uint64_t)k, before);
     }
-    bool enough = true;
-    if (!has_k) {  // does their weight reach p of the row's?
-      uint64_t all = 0, top = 0;
-      each([&](int, int e, const float (&x)[4]) {
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-          if (e + q < V) {
-            const uint64_t w = weight(x[q]);
-            all += w;
-            top += bin_of(x[q]) <= (int)b ? w : 0;
-          }
-      });
-      row_sum = block_sum(all);
-      enough = block_sum(top) >= need_of(row_sum);
-    }
-    if (enough && collect(0, b, kSmSort)) {
-      // larger keys first, lower indexes first among equals; nothing behind the list
-      uint64_t v = t < nlist ? ((uint64_t)list_key[t] << 32) | (uint32_t)~list_idx[t] : 0;
-      unsigned long long* swap = hist;
-#pragma unroll
-      for (int size = 2; size <= kSmSort; size <<= 1) {
-#pragma unroll
-        for (int step = size >> 1; step > 0; step >>= 1) {
-          uint64_t o;
-          if (step < 64) {
-            o = sm_shfl_xor(v, step);
-          } else {
-            __syncthreads();
-            swap[t] = v;
-            __syncthreads();
-            o = swap[t ^ step];
-          }
-          const bool first = (t & step) == 0, falling = (t & size) == 0;
-          v = (first == falling) == (v > o) ? v : o;
-        }
-      }
-      __syncthreads();
-      swap[t] = v;
-      const uint64_t w = t < nlist ? weight(sm_logit((uint32_t)(v >> 32))) : 0;
-      const uint64_t before = block_scan(w);
-      if (has_k && t == k - 1) s_u64 = before + w;
-      __syncthreads();
-      uint64_t keep_n = has_k ? (uint64_t)k : 0;
-      if (has_p) {
-        const uint64_t need = need_of(has_k ? (uint64_t)s_u64 : row_sum);
-        if (before < need && before + w >= need) s_u32 = t;
-        __syncthreads();
-        keep_n = s_u32 + 1;
-      }
-      const uint64_t last = swap[keep_n - 1];
-      kk = (uint32_t)(last >> 32);
-      last_tie = (int)~(uint32_t)last;
-      all_listed = selected = true;
-    }
+    if (collect(0, b, kSmSort)) from_list(k, need_of);
   }
   if (has_k && !selected) {
     hist[t] = 0;
     __syncthreads();
-    each([&](int, int e, const float (&x)[4]) {
+    each([&](int e, const float (&x)[4]) {
 #pragma unroll
       for (int q = 0; q < 4; ++q)
-        if (e + q < V) atomicAdd(&hist[bin_of(x[q])], 1ull);
+        if (e + q < w_end) atomicAdd(&hist[bin_of(x[q])], 1ull);
     });
     __syncthreads();
     uint64_t before;
@@ -489,31 +484,41 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SmArgs a) {
       __syncthreads();
       hist[t] = 0;
       __syncthreads();
-      each([&](int, int e, const float (&x)[4]) {
+      each([&](int, const float (&x)[4]) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
-          if (e + q < V && sm_key(x[q]) > k0) {
-            const uint64_t w = weight(x[q]);
-            if (w) atomicAdd(&hist[bin_of(x[q])], (unsigned long long)w);
-          }
+        for (int q = 0; q < 4; ++q) {
+          const uint64_t w = weight(x[q]);
+          if (w && sm_key(x[q]) > k0) atomicAdd(&hist[bin_of(x[q])], (unsigned long long)w);
+        }
       });
       if (t == 0 && t0) atomicAdd(&hist[bin_of(sm_logit(k0))], (unsigned long long)(t0 * weight(sm_logit(k0))));
       __syncthreads();
-      const uint64_t mine = hist[t];
-      const uint64_t need = need_of(block_sum(mine));
+      const uint64_t own = hist[t];
+      const uint64_t need = need_of(block_sum(own));
       uint64_t before;
-      const uint32_t b = find_bin(mine, 0, need, before);
-      if (collect(b, b)) refine(over_list, before, need, true);
-      else refine(over_row, 0, need, true);
+      const uint32_t b = find_bin(own, 0, need, before);
+      uint64_t upto = 0;
+      each([&](int e, const float (&x)[4]) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) upto += e + q < w_end && bin_of(x[q]) <= (int)b;
+      });
+      if (!has_k && block_sum(upto) <= kSmSort) {
+        collect(0, b, kSmSort);
+        from_list(nlist, [&](uint64_t) { return need; });
+      } else if (collect(b, b)) {
+        refine(over_list, before, need, true);
+      } else {
+        refine(over_row, 0, need, true);
+      }
     }
   }
 
-  // Lowest index whose running sum of measure(index, logit), in index order, exceeds target; seg holds the sums.
-  auto find = [&](uint64_t target, auto measure) -> int {
+  // Lowest index of [from, to), in steps of 256 that seg has the sums of, whose
+  // running sum of measure(index, logit), from base on, exceeds target.
+  auto find_in = [&](int from, int to, uint64_t base, uint64_t target, auto measure) -> int {
     __syncthreads();
     if (wave == 0) {
-      uint64_t base = 0;
-      const int ns = nchunks * kSmWaves;
+      const int ns = (to - from + 255) / 256;
       for (int s0 = 0; s0 < ns; s0 += 64) {
         const uint64_t own = s0 + lane < ns ? (uint64_t)seg[s0 + lane] : 0;
         uint64_t inc = own;
@@ -527,22 +532,22 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SmArgs a) {
         if (hit) {
           const int b = __builtin_ctzll(hit);
           const uint64_t at = (uint64_t)__shfl((unsigned long long)run, b, 64);
-          // the segment's 256 logits again, 4 a lane
-          const int e = (s0 + b) * 256 + 4 * lane;
-          uint64_t v[4], mine = 0;
+          // the step's 256 logits again, 4 a lane
+          const int e = from + (s0 + b) * 256 + 4 * lane;
+          uint64_t v[4], sum = 0;
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
-            v[q] = e + q < V ? measure(e + q, row[e + q]) : 0;
-            mine += v[q];
+            v[q] = e + q < to ? measure(e + q, row[e + q]) : 0;
+            sum += v[q];
           }
-          uint64_t in2 = mine;
+          uint64_t in2 = sum;
 #pragma unroll
           for (int m = 1; m < 64; m <<= 1) {
             const uint64_t o = sm_shfl_up(in2, m);
             if (lane >= m) in2 += o;
           }
-          uint64_t r2 = at + in2 - mine;
-          if (r2 <= target && r2 + mine > target) {
+          uint64_t r2 = at + in2 - sum;
+          if (r2 <= target && r2 + sum > target) {
             int q = 0;
             while (q < 3 && r2 + v[q] <= target) r2 += v[q++];
             s_u32 = (uint32_t)(e + q);
@@ -555,23 +560,35 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SmArgs a) {
     __syncthreads();
     return (int)s_u32;
   };
-  auto fill = [&](auto measure) -> uint64_t {  // seg from the row; their sum
+  // The same over the row, for the target that goal(sum over the row) gives: the
+  // waves' sums say whose share it is in, the workgroup adds up that share's steps.
+  auto find = [&](auto measure, auto goal) -> int {
     uint64_t sum = 0;
-    each([&](int c, int e, const float (&x)[4]) {
+    each([&](int e, const float (&x)[4]) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) sum += e + q < w_end ? measure(e + q, x[q]) : 0;
+    });
+    const uint64_t target = goal(block_sum(sum));
+    uint64_t base = 0, upto = 0;
+    int w = -1;
+    do {  // at most 16 waves; their sums exceed target
+      base = upto;
+      upto += s_sum[++w];
+    } while (upto <= target && w < kSmWaves - 1);
+    const int from = w * per_wave, to = min(from + per_wave, V);
+    for (int c = wave; c * 256 < to - from; c += kSmWaves) {
+      const int e = from + 256 * c + 4 * lane;
       uint64_t v = 0;
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
-        if (e + q < V) v += measure(e + q, x[q]);
-      sum += v;
-      if (__ballot(v != 0)) v = sm_wave_sum(v);
-      if (lane == 0) seg[c * kSmWaves + wave] = v;
-    });
-    return block_sum(sum);
+      for (int q = 0; q < 4; ++q) v += e + q < to ? measure(e + q, row[e + q]) : 0;
+      v = sm_wave_sum(v);
+      if (lane == 0) seg[c] = v;
+    }
+    return find_in(from, to, base, target, measure);
   };
-  if (ties) {
-    auto is_tie = [&](int, float l) -> uint64_t { return sm_key(l) == kk ? 1 : 0; };
-    __syncthreads();
-    if (fill(is_tie) > ties) last_tie = find(ties - 1, is_tie);
+  if (ties && ties_left) {
+    const uint64_t nth = ties - 1;
+    last_tie = find([&](int, float l) -> uint64_t { return sm_key(l) == kk ? 1 : 0; }, [&](uint64_t) { return nth; });
     __syncthreads();
   }
   auto kept = [&](int e, float l) -> uint64_t {
@@ -580,9 +597,14 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SmArgs a) {
     const uint64_t w = weight(l);
     return w >= wmin ? w : 0;
   };
-  uint64_t total;
+  auto goal = [&](uint64_t total) -> uint64_t {
+    bool rest;
+    return sm_mul_frac(total, u, rest);
+  };
+  int id;
   if (all_listed) {
-    const int ns = nchunks * kSmWaves;
+    const int ns = (V + 255) / 256;
+    __syncthreads();
     for (int e = t; e < ns; e += kSmThreads) seg[e] = 0;
     __syncthreads();
     uint64_t sum = 0;
@@ -591,12 +613,10 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SmArgs a) {
       sum += w;
       if (w) atomicAdd(&seg[list_idx[e] >> 8], (unsigned long long)w);
     }
-    total = block_sum(sum);
+    id = find_in(0, V, 0, goal(block_sum(sum)), kept);
   } else {
-    total = fill(kept);
+    id = find(kept, goal);
   }
-  bool rest;
-  const int id = find(sm_mul_frac(total, u, rest), kept);
   if (t == 0) argmax_finish(i, id, a.out, a.ring, a.ring_rows, a.ring_len, a.expect, a.accept);
 }
 
