@@ -299,9 +299,10 @@ int wfd_kv_read_q(const void* k_codes, const void* v_codes, const uint8_t* k_exp
  * kv_block_rows as wfd_kv_append_q lays them out): q and out (n, H, Dh) of
  * `dtype`, query i attends rows kv_row_base[i] .. + kv_len[i] - 1, a query with
  * kv_len <= 0 gets a zero row. The values are used as they are stored (converted
- * without rounding), with fp32 probabilities, sums and division. A key row
- * marked non-finite makes the rows that attend it NaN, no others. H / Hkv in
- * {1, 2, 4}, at most 32767 rows; workspace >= wfd_attn_workspace_bytes(n, H, Dh,
+ * without rounding), with fp32 statistics, sums and division; probabilities meet
+ * V with 16 significant bits (fp32 queries: 24). A key row marked non-finite
+ * makes the rows that attend it NaN, no others. H / Hkv up to 16, H up to 4096,
+ * at most 65535 rows, any scale; workspace >= wfd_attn_workspace_bytes(n, H, Dh,
  * kv_len_max). A row's bits depend on that row only.
  * Replaces: what wfd_attn_decode replaces, over caches the reference does not have.
  */

@@ -163,7 +163,7 @@ def _filled(rows, Hkv, Dh, code, gpu, seed, block=0):
 @pytest.mark.parametrize("code", CODES)
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("H,Hkv,Dh,block", [(4, 4, 64, 0), (4, 2, 64, 2600), (8, 2, 128, 0), (3, 3, 128, 2600),
-                                            (4, 2, 128, 2600), (4, 1, 64, 0)])
+                                            (4, 2, 128, 2600), (4, 1, 64, 0), (16, 1, 128, 0), (10, 2, 64, 2600)])
 def test_attention_lengths_and_layouts(gpu, code, dtype, H, Hkv, Dh, block):
     """Lengths around a tile, a split and the zero row; each row as if it were alone."""
     lens = [0, 1, 2, 15, 16, 17, 63, 64, 65, 500, 1023, 1024, 1025, 2049, 2600, -3]
@@ -176,7 +176,8 @@ def test_attention_lengths_and_layouts(gpu, code, dtype, H, Hkv, Dh, block):
     out = ops.attn_decode_q(q.to(gpu), cache, *args(slice(None)), kv_len_max=2600)
     for i, L in enumerate(lens):
         span = slice(int(base[i]), int(base[i]) + max(L, 0))
-        ref, bound = attend(q[i].double(), k[span].transpose(0, 1), v[span].transpose(0, 1), 1 / math.sqrt(Dh))
+        ref, bound = attend(q[i].double(), k[span].transpose(0, 1), v[span].transpose(0, 1), 1 / math.sqrt(Dh),
+                            2.0 ** -16 if dtype == torch.bfloat16 else 0.0)
         check_attention(out[i], ref, bound)
         one = slice(i, i + 1)
         alone = ops.attn_decode_q(q[one].to(gpu), cache, *args(one), kv_len_max=2600)
@@ -211,6 +212,20 @@ def test_attention_marked_row_reaches_rows_of_several_splits(gpu):
     q = torch.randn(2, H, Dh, generator=_gen(2)).bfloat16().to(gpu)
     nan = ops.attn_decode_q(q, cache, torch.zeros(2, dtype=torch.int64, device=gpu), lens, kv_len_max=S).isnan()
     assert bool(nan[0, 1].all()) and not bool(nan[0, 0].any()) and not bool(nan[1].any())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("scale", [0.0, -0.2, 3.0])
+def test_attention_any_scale_and_large_scores(gpu, dtype, scale):
+    H, Hkv, Dh, S = 4, 2, 64, 1100
+    cache, (k, v) = _filled(S, Hkv, Dh, "int8", gpu, 5)
+    q = (torch.randn(3, H, Dh, generator=_gen(4)) * 3).to(dtype)
+    lens = [1100, 40, 7]
+    got = ops.attn_decode_q(q.to(gpu), cache, torch.zeros(3, dtype=torch.int64, device=gpu),
+                            torch.tensor(lens, dtype=torch.int32, device=gpu), kv_len_max=S, scale=scale)
+    for i, L in enumerate(lens):
+        check_attention(got[i], *attend(q[i].double(), k[:L].transpose(0, 1), v[:L].transpose(0, 1), scale,
+                                        2.0 ** -16 if dtype == torch.bfloat16 else 0.0))
 
 
 def test_attention_scale_and_workspace_and_out(gpu):

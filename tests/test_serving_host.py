@@ -111,7 +111,7 @@ def test_quant_entry_points_check_before_launch():
     att = lambda n=1, H=4, Hkv=2, Dh=64, dt=1, m=8, br=0: lib.wfd_attn_decode_q(  # noqa: E731
         None, None, None, None, None, 0, br, None, None, None, n, H, Hkv, Dh, dt, 0.1, m, None, 0, None)
     assert att(H=3) == -1 and att(m=0) == -1 and att(br=4, m=5) == -1 and b"kv_block_rows=4" in err()
-    assert att(H=6) == -2 and att(dt=2) == -2 and att(Dh=32) == -2 and att(n=40000) == -2 and b"beyond" in err()
+    assert att(H=34) == -2 and att(dt=2) == -2 and att(Dh=32) == -2 and att(n=70000) == -2 and b"beyond" in err()
     assert att(n=0) == 0 and att() == -1 and b"null pointer" in err()
 
 

@@ -3,260 +3,25 @@
 //   o[i,h,:] = softmax_t(q[i,h,:] . K_t * scale) V_t,   K_t = kcode_t 2^(ke_t - 127), V_t likewise.
 //
 // Codes are exact in bf16 and the scales are powers of two, so the products are
-// those of a cache that held the values themselves: q . kcode runs on MFMA in
-// q's type (the codes converted, not q), the score takes its key's scale, and
-// the probability its key's V scale before it multiplies V's codes in fp32 on
-// the VALU. Statistics and sums are fp32; the one rounding is the output's.
+// those of a cache that held the values themselves: a score takes its key's
+// scale after q . kcode, a probability its key's V scale before it meets V's
+// codes. Both products run on the 16x16x32 bf16 MFMA, S^T = K Q^T and O^T = V^T
+// P^T, the query heads of the kv head as the 16 columns. fp32 queries are split
+// into three bf16 terms, which hold all their bits; probabilities into two (a
+// half step of 2^-16 of each) or, for fp32, three. Statistics and sums are fp32.
 //
-// Bound by HBM: (Dh + 1) bytes of K and of V per key and kv head. Work split as
-// in wfd_attn_decode: a workgroup of 8 waves owns one (1024-key split, kv head,
-// query row), its waves take 64-key tiles round-robin, a split's waves merge
-// through LDS in fixed order and a row's splits in attn_combine_kernel, all a
-// function of kv_len only, so a row's bits do not depend on the launch.
+// Bound by HBM: (Dh + 1) bytes of K and of V per key and kv head. P.V on the
+// VALU, as in wfd_attn_decode, took 1600 vector instructions per 64 keys of four
+// heads and held 64 rows over 32k keys at 3.3 TB/s; a tile here takes a fifth.
+// Work split as there: a workgroup of 8 waves owns one (1024-key split, kv head,
+// query row), its waves take 32-key tiles round-robin, each through LDS of its
+// own a tile ahead; the waves merge through LDS in fixed order and a row's splits
+// in attn_combine_kernel, all a function of kv_len only, so a row's bits do not
+// depend on the launch.
 #include "attn_combine.h"
 #include "quant.h"
 
 namespace wfd {
-
-// Codes of a 16-byte piece as MFMA operand fragments: piece p of a key holds
-// its values 16 p .. 16 p + 15; step t of its steps takes kVec of them.
-template <typename T, int CODE>
-__device__ __forceinline__ u32x4 code_frag(const u32x4& w, int t) {
-  if constexpr (sizeof(T) == 2) {
-    float f[8];
-    decode4<CODE>(w[2 * t], f);
-    decode4<CODE>(w[2 * t + 1], f + 4);
-    return Elem<bf16_t>::pack(f);
-  } else {
-    float f[4];
-    decode4<CODE>(w[t], f);
-    return Elem<float>::pack(f);
-  }
-}
-
-template <typename T, int CODE, int DH, int G>
-__global__ __launch_bounds__(512) void attn_q_split_kernel(
-    const T* __restrict__ q, const uint8_t* __restrict__ kc, const uint8_t* __restrict__ vc,
-    const uint8_t* __restrict__ ke, const uint8_t* __restrict__ ve, const int64_t* __restrict__ row_base,
-    const int32_t* __restrict__ kv_len, float* __restrict__ part_o, float* __restrict__ part_ml, T* __restrict__ out,
-    int H, int Hkv, int max_splits, float scale_log2, int64_t block_rows, int vsplit) {
-  constexpr int NW = 8;
-  constexpr int TK = 64;
-  constexpr int V = Elem<T>::kVec;
-  constexpr int NJ = TK / 16;       // 16-key blocks per tile
-  constexpr int LPK = DH / 16;      // 16-byte pieces (lanes) per key row
-  constexpr int KPI = 64 / LPK;     // key rows per load instruction
-  constexpr int NLD = TK / KPI;     // load instructions per tile and tensor
-  constexpr int NP = LPK / 4;       // pieces per lane of a fragment (its lane group's)
-  constexpr int STEPS = 16 / V;     // MFMA steps per piece
-  constexpr int SW = 16 / LPK;      // key rows per 256 bytes of LDS
-  __shared__ __align__(16) u32x4 k_lds[NW][TK * LPK];
-  __shared__ float p_lds[NW][G][TK];
-  __shared__ float o_lds[NW][G][DH];
-  __shared__ float m_lds[NW][G];
-  __shared__ float l_lds[NW][G];
-
-  const int split = blockIdx.x;
-  const int g = blockIdx.y;
-  const int nz = gridDim.z / vsplit;
-  const int vp = blockIdx.z / nz;
-  const int i = blockIdx.z - vp * nz;
-  const int DV = DH / vsplit;
-  const int d0 = vp * DV;  // output columns [d0, d0 + DV) are this workgroup's
-  const int len = kv_len[i];
-  if (split * kAttnSplit >= len) {  // uniform
-    if (split == 0)                 // no keys: a zero row
-      for (int idx = threadIdx.x; idx < G * DV; idx += 64 * NW)
-        Elem<T>::store(out + ((int64_t)i * H + g * G + idx / DV) * DH + d0 + idx % DV, 0.f);
-    return;
-  }
-  const int kend = min(len, (split + 1) * kAttnSplit);
-  const int ntiles = (kend - split * kAttnSplit + TK - 1) / TK;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int lane = threadIdx.x & 63;
-  const int col = lane & 15;
-  const int grp = lane >> 4;
-  const int vg = lane / LPK;    // V row of this lane within a load
-  const int dseg = lane % LPK;  // its 16 columns
-  const bool vmine = dseg * 16 >= d0 && dseg * 16 < d0 + DV;
-  const int64_t hb = kv_offset(row_base[i], g, Hkv, DH, block_rows);
-  const int64_t rs = block_rows > 1 ? (int64_t)DH : (int64_t)Hkv * DH;  // key stride, bytes
-  const int64_t es = block_rows > 1 ? 1 : Hkv;                          // exponent stride
-  const uint8_t* kb = kc + hb;
-  const uint8_t* vb = vc + hb;
-  const uint8_t* keb = ke + hb / DH;
-  const uint8_t* veb = ve + hb / DH;
-
-  // Q as the A operand, row = query head g G + col, in the codes' k order
-  u32x4 qf[NP][STEPS];
-  {
-    const bool real = col < G;
-    const T* qp = q + ((int64_t)i * H + g * G + (real ? col : 0)) * DH + 16 * grp;
-#pragma unroll
-    for (int p = 0; p < NP; ++p)
-#pragma unroll
-      for (int t = 0; t < STEPS; ++t) qf[p][t] = real ? ld16(qp + 64 * p + V * t) : zero16();
-  }
-
-  float mrun[G], lrun[G], o[G][16];
-#pragma unroll
-  for (int m = 0; m < G; ++m) {
-    mrun[m] = -INFINITY;
-    lrun[m] = 0.f;
-#pragma unroll
-    for (int e = 0; e < 16; ++e) o[m][e] = 0.f;
-  }
-
-  for (int t = wave; t < ntiles; t += NW) {  // uniform over the wave
-    const int t0 = split * kAttnSplit + t * TK;
-    u32x4 kf[NLD], vf[NLD];
-    uint32_t kx[NJ], vx[NJ];
-#pragma unroll
-    for (int s = 0; s < NLD; ++s) {  // whole key rows; the piece order keeps the fragment reads off each other's banks
-      const int r = KPI * s + lane / LPK;
-      const int key = min(t0 + r, kend - 1);
-      kf[s] = ld16(kb + (int64_t)key * rs + ((lane % LPK) ^ ((r / SW) % LPK)) * 16);
-    }
-#pragma unroll
-    for (int j = 0; j < NJ; ++j) {
-      const int key = min(t0 + 16 * j + col, kend - 1);
-      kx[j] = keb[key * es];
-      vx[j] = veb[key * es];
-    }
-#pragma unroll
-    for (int s = 0; s < NLD; ++s) {
-      const int key = min(t0 + KPI * s + vg, kend - 1);
-      vf[s] = vmine ? ld16(vb + (int64_t)key * rs + dseg * 16) : zero16();
-    }
-    // the LDS executes one wave's accesses in order
-    asm volatile("" ::: "memory");
-#pragma unroll
-    for (int s = 0; s < NLD; ++s) k_lds[wave][64 * s + lane] = kf[s];
-    asm volatile("" ::: "memory");
-    // scores: lane (grp, col) holds S[row 4 grp + r][key 16 j + col]
-    f32x4 acc[NJ];
-#pragma unroll
-    for (int j = 0; j < NJ; ++j) {
-      acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-      const int r = 16 * j + col;
-#pragma unroll
-      for (int p = 0; p < NP; ++p) {
-        const u32x4 w = k_lds[wave][r * LPK + ((4 * p + grp) ^ ((r / SW) % LPK))];
-#pragma unroll
-        for (int st = 0; st < STEPS; ++st) acc[j] = mfma_step<T>(qf[p][st], code_frag<T, CODE>(w, st), acc[j]);
-      }
-    }
-    // rows 0 .. G - 1 sit in lane group 0: it reduces them, the others follow
-    float p4[NJ][4];
-    float corr[G];
-#pragma unroll
-    for (int m = 0; m < G; ++m) {
-      float mt = -INFINITY;
-#pragma unroll
-      for (int j = 0; j < NJ; ++j) {
-        const bool valid = t0 + 16 * j + col < kend;
-        const float sv = valid ? acc[j][m] * (scale_log2 * code_scale(kx[j])) : -INFINITY;
-        p4[j][m] = sv;
-        mt = fmaxf(mt, sv);
-      }
-#pragma unroll
-      for (int sh = 8; sh >= 1; sh >>= 1) mt = fmaxf(mt, __shfl_xor(mt, sh, 64));
-      mt = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(mt)));
-      const float mnew = fmaxf(mrun[m], mt);
-      corr[m] = (mrun[m] == -INFINITY) ? 0.f : exp2f(mrun[m] - mnew);
-      mrun[m] = mnew;
-      float lt = 0.f;
-#pragma unroll
-      for (int j = 0; j < NJ; ++j) {
-        const float p = (p4[j][m] == -INFINITY) ? 0.f : exp2f(p4[j][m] - mnew);
-        lt += p;
-        // a key past the end contributes nothing whatever scale it was clamped to
-        p4[j][m] = t0 + 16 * j + col < kend ? p * code_scale(vx[j]) : 0.f;
-      }
-#pragma unroll
-      for (int sh = 8; sh >= 1; sh >>= 1) lt += __shfl_xor(lt, sh, 64);
-      lt = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(lt)));
-      lrun[m] = fmaf(lrun[m], corr[m], lt);
-    }
-    if (grp == 0) {
-#pragma unroll
-      for (int m = 0; m < G; ++m)
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-          const int kt = 16 * j + col;
-          p_lds[wave][m][(kt % KPI) * NLD + kt / KPI] = p4[j][m];  // in the V lanes' key order
-        }
-    }
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-#pragma unroll
-    for (int m = 0; m < G; ++m)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) o[m][e] *= corr[m];
-#pragma unroll
-    for (int s = 0; s < NLD; ++s) {
-      float v[16];
-#pragma unroll
-      for (int w = 0; w < 4; ++w) decode4<CODE>(vf[s][w], v + 4 * w);
-#pragma unroll
-      for (int m = 0; m < G; ++m) {
-        const float p = p_lds[wave][m][vg * NLD + s];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) o[m][e] = fmaf(p, v[e], o[m][e]);
-      }
-    }
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();  // the next tile rewrites P and K
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-  }
-#pragma unroll
-  for (int m = 0; m < G; ++m) {
-#pragma unroll
-    for (int sh = LPK; sh < 64; sh <<= 1)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) o[m][e] += __shfl_xor(o[m][e], sh, 64);
-    if (vg == 0) {
-#pragma unroll
-      for (int e = 0; e < 16; ++e) o_lds[wave][m][dseg * 16 + e] = o[m][e];
-    }
-    if (lane == 0) {
-      m_lds[wave][m] = mrun[m];
-      l_lds[wave][m] = lrun[m];
-    }
-  }
-  __syncthreads();
-
-  // merge the waves in fixed order: the row itself if its keys fit one split,
-  // this split's unnormalised partial otherwise
-  const int ns = min((len + kAttnSplit - 1) / kAttnSplit, max_splits);
-  for (int idx = threadIdx.x; idx < G * DV; idx += 64 * NW) {
-    const int m = idx / DV;
-    const int d = d0 + (idx - m * DV);
-    float M = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < NW; ++w) M = fmaxf(M, m_lds[w][m]);
-    float O = 0.f, L = 0.f;
-#pragma unroll
-    for (int w = 0; w < NW; ++w) {
-      const float mw = m_lds[w][m];
-      const float f = (mw == -INFINITY) ? 0.f : exp2f(mw - M);
-      O = fmaf(o_lds[w][m][d], f, O);
-      L = fmaf(l_lds[w][m], f, L);
-    }
-    const int64_t row = (int64_t)i * H + g * G + m;
-    if (ns == 1) {
-      Elem<T>::store(out + row * DH + d, attn_finish_nan(O, L));
-    } else {
-      const int64_t pidx = row * max_splits + split;
-      part_o[pidx * DH + d] = O;
-      if (d == 0) {
-        part_ml[pidx * 2] = M;
-        part_ml[pidx * 2 + 1] = L;
-      }
-    }
-  }
-}
 
 struct AttnQArgs {
   const void* q;
@@ -270,32 +35,293 @@ struct AttnQArgs {
   int64_t br;
 };
 
-template <typename T, int CODE, int DH, int G>
-static void launch_attn_q(const AttnQArgs& a, hipStream_t st) {
-  const int vs = 1;
-  hipLaunchKernelGGL((attn_q_split_kernel<T, CODE, DH, G>), dim3(a.ms, a.Hkv, a.n * vs), dim3(512), 0, st,
-                     (const T*)a.q, a.kc, a.vc, a.ke, a.ve, a.rb, a.kl, a.po, a.pml, (T*)a.out, a.H, a.Hkv, a.ms,
-                     a.scale_log2, a.br, vs);
-  if (a.ms > 1)  // some query may span several splits
-    hipLaunchKernelGGL((attn_combine_kernel<T, DH, true>), dim3(a.H, a.n), dim3(DH), 0, st, a.po, a.pml, a.kl, (T*)a.out,
-                       a.H, a.ms);
+constexpr int kAqWaves = 8;
+constexpr int kAqMaxG = 16;        // columns of the MFMA
+constexpr int kAqMaxHeads = 4096;  // a split's keys stay within 32-bit offsets of its first
+
+// Eight codes (two dwords) as a bf16 operand fragment, exact.
+template <int CODE>
+__device__ __forceinline__ u32x4 code_frag(uint32_t w0, uint32_t w1) {
+  if constexpr (CODE == WFD_E4M3) {
+    // two codes an instruction; taken as the dword it is
+    auto pair = [](uint32_t w, bool hi) {
+      return hi ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, true))
+                : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false));
+    };
+    return u32x4{pair(w0, false), pair(w0, true), pair(w1, false), pair(w1, true)};
+  } else {
+    float f[8];
+    decode4<CODE>(w0, f);
+    decode4<CODE>(w1, f + 4);
+    return Elem<bf16_t>::pack(f);
+  }
 }
 
-template <typename T, int CODE>
-static bool dispatch_attn_q(int Dh, int G, const AttnQArgs& a, hipStream_t st) {
-#define WFD_ATTNQ_CASE(DHV, GV)             \
-  if (Dh == DHV && G == GV) {               \
-    launch_attn_q<T, CODE, DHV, GV>(a, st); \
-    return true;                            \
+// The next bf16 term of eight values: x's rounding, which x then loses.
+__device__ __forceinline__ u32x4 take_term(float (&x)[8], bool last) {
+  const u32x4 w = Elem<bf16_t>::pack(x);
+  if (!last) {
+    float r[8];
+    Elem<bf16_t>::unpack(w, r);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] -= r[e];
   }
-  WFD_ATTNQ_CASE(64, 1)
-  WFD_ATTNQ_CASE(64, 2)
-  WFD_ATTNQ_CASE(64, 4)
-  WFD_ATTNQ_CASE(128, 1)
-  WFD_ATTNQ_CASE(128, 2)
-  WFD_ATTNQ_CASE(128, 4)
-#undef WFD_ATTNQ_CASE
-  return false;
+  return w;
+}
+
+template <typename T, int CODE, int DH>
+__global__ __launch_bounds__(64 * kAqWaves) __attribute__((amdgpu_waves_per_eu(sizeof(T) == 2 ? 4 : 2))) void
+attn_q_split_kernel(AttnQArgs a) {
+  constexpr int NW = kAqWaves;
+  constexpr int TK = 32;
+  constexpr int QT = sizeof(T) == 2 ? 1 : 3;  // bf16 terms of a query
+  constexpr int PT = sizeof(T) == 2 ? 2 : 3;  // and of a probability
+  constexpr int LPK = DH / 16;   // 16-byte pieces (lanes) per row of codes
+  constexpr int RPI = 64 / LPK;  // rows per load instruction
+  constexpr int NLD = TK / RPI;
+  constexpr int NP = LPK / 4;    // pieces per lane of a K fragment, two MFMA steps each
+  constexpr int NDB = DH / 16;
+  constexpr int SW = 16 / LPK;   // rows per 256 bytes of LDS
+  constexpr int OP = DH + 4;
+  constexpr int kTile = TK * DH;
+  constexpr size_t kStage = (size_t)NW * 2 * kTile, kMerge = sizeof(float) * NW * kAqMaxG * OP;
+  __shared__ __align__(16) uint8_t lds[kStage > kMerge ? kStage : kMerge];
+  __shared__ __align__(16) float s_lds[NW][2 * TK];  // a tile's K and V scales
+  __shared__ float m_lds[NW][kAqMaxG];
+  __shared__ float l_lds[NW][kAqMaxG];
+
+  const int split = blockIdx.x, g = blockIdx.y, i = blockIdx.z;
+  const int G = a.H / a.Hkv;
+  const int64_t row0 = (int64_t)i * a.H + g * G;
+  const int len = a.kl[i];
+  if (split * kAttnSplit >= len) {  // uniform
+    if (split == 0)                 // no keys: zero rows
+      for (int idx = threadIdx.x; idx < G * DH; idx += 64 * NW) Elem<T>::store((T*)a.out + row0 * DH + idx, 0.f);
+    return;
+  }
+  const int nk = min(len - split * kAttnSplit, kAttnSplit);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4;
+  uint8_t* k_lds = lds + wave * 2 * kTile;
+  uint8_t* v_lds = k_lds + kTile;
+
+  // codes of this head from the split's first key; the resources end with its last,
+  // so that later rows read as zeros
+  const uint32_t rs = a.br > 1 ? DH : a.Hkv * DH;  // key stride, bytes
+  const int64_t at = kv_offset(a.rb[i], g, a.Hkv, DH, a.br) + (int64_t)split * kAttnSplit * rs;
+  const uint32_t span = (uint32_t)(nk - 1) * rs + DH;
+  auto rsrc = [&](const uint8_t* p) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p + at), (short)0, span, 0x00020000);
+  };
+  const __amdgpu_buffer_rsrc_t kr = rsrc(a.kc), vr = rsrc(a.vc);
+  const uint8_t* eb = (lane < TK ? a.ke : a.ve) + at / DH;  // lane: the K (V) scale of key lane % 32
+  const uint32_t es = rs / DH;
+  // whole rows, a row's pieces in an order that keeps the fragment reads off each
+  // other's banks: piece p of row r sits at place p ^ (r / SW)
+  uint32_t off[NLD];
+#pragma unroll
+  for (int s = 0; s < NLD; ++s) {
+    const int r = RPI * s + lane / LPK;
+    off[s] = (uint32_t)(TK * wave + r) * rs + (uint32_t)(((lane % LPK) ^ ((r / SW) % LPK)) * 16);
+  }
+  u32x4 kreg[NLD], vreg[NLD];
+  uint32_t ereg;
+  int t0 = TK * wave;
+  auto fetch = [&](int t) {  // this wave's next tile
+#pragma unroll
+    for (int s = 0; s < NLD; ++s) {
+      kreg[s] = buf_ld16(kr, off[s]);
+      vreg[s] = buf_ld16(vr, off[s]);
+      off[s] += (uint32_t)(TK * NW) * rs;
+    }
+    ereg = eb[(uint64_t)min(t + (lane % TK), nk - 1) * es];
+  };
+  fetch(t0);
+
+  // Q as the B operand, column = query head, in the codes' k order
+  u32x4 qf[QT][NP][2];
+#pragma unroll
+  for (int p = 0; p < NP; ++p)
+#pragma unroll
+    for (int st = 0; st < 2; ++st) {
+      const T* qp = (const T*)a.q + (row0 + (col < G ? col : 0)) * DH + 64 * p + 16 * grp + 8 * st;
+      if constexpr (QT == 1) {
+        qf[0][p][st] = ld16(qp);
+      } else {
+        float x[8];
+        float lo[4], hi[4];
+        Elem<float>::unpack(ld16(qp), lo);
+        Elem<float>::unpack(ld16(qp + 4), hi);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          x[e] = lo[e];
+          x[4 + e] = hi[e];
+        }
+#pragma unroll
+        for (int c = 0; c < QT; ++c) qf[c][p][st] = take_term(x, c == QT - 1);
+      }
+    }
+  // V^T fragment of 16 dims: the transposing read gives lane i of a 16-lane group byte
+  // i % 8 of what lanes i / 8 + 2 e address, e < 8. Lane j addresses half j % 2 of the
+  // piece in row key(j / 2), key(e) = 16 (e / 4) + 4 grp + e % 4: the keys whose scores the
+  // group's lanes hold, in their order.
+  const int vkey = 16 * (col >> 3) + 4 * grp + ((col >> 1) & 3);
+  const uint32_t v_row = (uint32_t)(vkey * DH + 8 * (col & 1)), v_swz = (uint32_t)(((vkey / SW) % LPK) * 16);
+  auto vt_frag = [&](int db) {
+    typedef int i32x2 __attribute__((ext_vector_type(2)));
+    typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
+    typedef const __attribute__((address_space(3))) void* lds_ptr;
+    const i32x2 w = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+        (lds_i32x2*)(lds_ptr)(v_lds + v_row + ((uint32_t)(16 * db) ^ v_swz)));
+    return code_frag<CODE>((uint32_t)w[0], (uint32_t)w[1]);
+  };
+
+  // lane (grp, col): of query head col, the keys 16 j + 4 grp + r of a tile and the dims
+  // 16 db + 4 grp + r of the output; lrun its share of the sum. mref is the head's
+  // maximum when a tile last exceeded it by more than 2^8 (see attn_shared.hip).
+  float mref = -INFINITY, lrun = 0.f;
+  f32x4 o[NDB];
+#pragma unroll
+  for (int db = 0; db < NDB; ++db) o[db] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  for (; t0 < nk; t0 += TK * NW) {  // uniform over the wave
+#pragma unroll
+    for (int s = 0; s < NLD; ++s) {
+      *reinterpret_cast<u32x4*>(k_lds + 1024 * s + 16 * lane) = kreg[s];
+      *reinterpret_cast<u32x4*>(v_lds + 1024 * s + 16 * lane) = vreg[s];
+    }
+    // a key past the end weighs nothing, whatever its clamped scale says
+    const float sc = code_scale(ereg);
+    s_lds[wave][lane] = lane < TK ? sc * a.scale_log2 : (t0 + (lane % TK) < nk ? sc : 0.f);
+    fetch(t0 + TK * NW);
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    f32x4 acc[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+      const int r = 16 * j + col;
+#pragma unroll
+      for (int p = 0; p < NP; ++p) {
+        const u32x4 w =
+            *reinterpret_cast<const u32x4*>(k_lds + r * DH + (((4 * p + grp) ^ ((r / SW) % LPK)) * 16));
+#pragma unroll
+        for (int st = 0; st < 2; ++st) {
+          const u32x4 kf = code_frag<CODE>(w[2 * st], w[2 * st + 1]);
+#pragma unroll
+          for (int c = QT - 1; c >= 0; --c) acc[j] = mfma_step<bf16_t>(kf, qf[c][p][st], acc[j]);
+        }
+      }
+    }
+    float mt = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const f32x4 ks = *reinterpret_cast<const f32x4*>(&s_lds[wave][16 * j + 4 * grp]);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) acc[j][r] *= ks[r];
+    }
+    if (t0 + TK > nk) {  // the last tile (uniform)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (t0 + 16 * j + 4 * grp + r >= nk) acc[j][r] = -INFINITY;
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) mt = fmaxf(mt, acc[j][r]);
+    if (__builtin_amdgcn_ballot_w64(mt > mref + 8.f)) {
+      mt = fmaxf(mt, __shfl_xor(mt, 16, 64));
+      mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
+      const float mnew = mt > mref + 8.f ? mt : mref;
+      const float corr = mref == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mref - mnew);
+      mref = mnew;
+      lrun *= corr;
+#pragma unroll
+      for (int db = 0; db < NDB; ++db)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o[db][r] *= corr;
+    }
+    const float ref = mref == -INFINITY ? 0.f : mref;
+    float pv[8];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const f32x4 vs = *reinterpret_cast<const f32x4*>(&s_lds[wave][TK + 16 * j + 4 * grp]);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float p = __builtin_amdgcn_exp2f(acc[j][r] - ref);
+        lrun += p;
+        pv[4 * j + r] = p * vs[r];
+      }
+    }
+    u32x4 pb[PT];
+#pragma unroll
+    for (int c = 0; c < PT; ++c) pb[c] = take_term(pv, c == PT - 1);
+#pragma unroll
+    for (int db = 0; db < NDB; ++db) {
+      const u32x4 vf = vt_frag(db);
+#pragma unroll
+      for (int c = PT - 1; c >= 0; --c) o[db] = mfma_step<bf16_t>(vf, pb[c], o[db]);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();  // the next tile overwrites this one
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  }
+  lrun += __shfl_xor(lrun, 16, 64);
+  lrun += __shfl_xor(lrun, 32, 64);
+
+  __syncthreads();  // every wave's tiles are done: the merge takes their LDS
+  float* o_lds = reinterpret_cast<float*>(lds);
+  if (col < G) {
+#pragma unroll
+    for (int db = 0; db < NDB; ++db)
+      *reinterpret_cast<f32x4*>(o_lds + (wave * kAqMaxG + col) * OP + 16 * db + 4 * grp) = o[db];
+    if (grp == 0) {
+      m_lds[wave][col] = mref;
+      l_lds[wave][col] = lrun;
+    }
+  }
+  __syncthreads();
+  // merge the waves in fixed order: the row itself if its keys fit one split,
+  // this split's unnormalised partial otherwise
+  const int ns = min((len + kAttnSplit - 1) / kAttnSplit, a.ms);
+  for (int idx = threadIdx.x; idx < G * (DH / 4); idx += 64 * NW) {
+    const int m = idx / (DH / 4), d = 4 * (idx % (DH / 4));
+    float M = -INFINITY, L = 0.f;
+    f32x4 O = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < NW; ++w) M = fmaxf(M, m_lds[w][m]);
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      const float mw = m_lds[w][m];
+      const float f = mw == -INFINITY ? 0.f : exp2f(mw - M);
+      const f32x4 ow = *reinterpret_cast<const f32x4*>(o_lds + (w * kAqMaxG + m) * OP + d);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) O[e] = fmaf(ow[e], f, O[e]);
+      L = fmaf(l_lds[w][m], f, L);
+    }
+    if (ns == 1) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) Elem<T>::store((T*)a.out + (row0 + m) * DH + d + e, attn_finish_nan(O[e], L));
+    } else {
+      const int64_t pidx = (row0 + m) * a.ms + split;
+      *reinterpret_cast<f32x4*>(a.po + pidx * DH + d) = O;
+      if (d == 0) {
+        a.pml[pidx * 2] = M;
+        a.pml[pidx * 2 + 1] = L;
+      }
+    }
+  }
+}
+
+template <typename T, int CODE, int DH>
+static void launch_attn_q(const AttnQArgs& a, hipStream_t st) {
+  hipLaunchKernelGGL((attn_q_split_kernel<T, CODE, DH>), dim3(a.ms, a.Hkv, a.n), dim3(64 * kAqWaves), 0, st, a);
+  if (a.ms > 1)  // some query may span several splits
+    hipLaunchKernelGGL((attn_combine_kernel<T, DH, true>), dim3(a.H, a.n), dim3(DH), 0, st, a.po, a.pml, a.kl,
+                       (T*)a.out, a.H, a.ms);
 }
 
 }  // namespace wfd
@@ -309,19 +335,19 @@ int wfd_attn_decode_q(const void* q, const void* k_codes, const void* v_codes, c
   using namespace wfd;
   const char* me = "wfd_attn_decode_q";
   if (int rc = check_qcache(me, n, Hkv, Dh, code, kv_block_rows)) return rc;
-  if (H <= 0 || H > kMaxHeads || H % Hkv != 0 || kv_len_max < 1 ||
+  if (H <= 0 || H > kAqMaxHeads || H % Hkv != 0 || kv_len_max < 1 ||
       (kv_block_rows > 1 && kv_len_max > kv_block_rows)) {
     set_error("%s: bad shape H=%d Hkv=%d kv_len_max=%d kv_block_rows=%lld", me, H, Hkv, kv_len_max,
               (long long)kv_block_rows);
     return kBadArg;
   }
   const int G = H / Hkv;
-  if ((dtype != kBF16 && dtype != kF32) || (G != 1 && G != 2 && G != 4)) {
-    set_error("%s: unsupported dtype=%d G=%d (G = H / Hkv 1/2/4)", me, dtype, G);
+  if ((dtype != kBF16 && dtype != kF32) || G > kAqMaxG) {
+    set_error("%s: unsupported dtype=%d G=%d (G = H / Hkv up to %d)", me, dtype, G, kAqMaxG);
     return kUnsupported;
   }
-  if (n > 32767) {
-    set_error("%s: n=%d beyond the grid (32767 rows)", me, n);
+  if (n > 65535) {
+    set_error("%s: n=%d beyond the grid (65535 rows)", me, n);
     return kUnsupported;
   }
   if (n == 0) return kOk;
@@ -355,12 +381,16 @@ int wfd_attn_decode_q(const void* q, const void* k_codes, const void* v_codes, c
   a.pml = (float*)((char*)workspace + align256((size_t)n * H * a.ms * Dh * sizeof(float)));
   a.scale_log2 = scale * 1.4426950408889634f;
   a.br = kv_block_rows;
-  if (dtype == kBF16)
-    code == WFD_E4M3 ? dispatch_attn_q<bf16_t, WFD_E4M3>(Dh, G, a, stream)
-                     : dispatch_attn_q<bf16_t, WFD_INT8>(Dh, G, a, stream);
-  else
-    code == WFD_E4M3 ? dispatch_attn_q<float, WFD_E4M3>(Dh, G, a, stream)
-                     : dispatch_attn_q<float, WFD_INT8>(Dh, G, a, stream);
+#define WFD_ATTNQ_CASE(TT, DT, CODE)                            \
+  if (dtype == DT && code == CODE) {                             \
+    if (Dh == 64) launch_attn_q<TT, CODE, 64>(a, stream);        \
+    else launch_attn_q<TT, CODE, 128>(a, stream);                \
+  }
+  WFD_ATTNQ_CASE(bf16_t, kBF16, WFD_E4M3)
+  WFD_ATTNQ_CASE(bf16_t, kBF16, WFD_INT8)
+  WFD_ATTNQ_CASE(float, kF32, WFD_E4M3)
+  WFD_ATTNQ_CASE(float, kF32, WFD_INT8)
+#undef WFD_ATTNQ_CASE
   return launch_status(me);
 }
 
