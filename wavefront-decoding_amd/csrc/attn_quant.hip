@@ -30,7 +30,7 @@ struct AttnQArgs {
   const int32_t* kl;
   void* out;
   float *po, *pml;
-  int n, H, Hkv, ms;
+  int n, H, Hkv, ms, spw;
   float scale_log2;
   int64_t br;
 };
@@ -81,34 +81,38 @@ attn_q_split_kernel(AttnQArgs a) {
   constexpr int NLD = TK / RPI;
   constexpr int NP = LPK / 4;    // pieces per lane of a K fragment, two MFMA steps each
   constexpr int NDB = DH / 16;
-  constexpr int SW = 16 / LPK;   // rows per 256 bytes of LDS
+  constexpr int RP = DH + 16;    // LDS row pitch: 16 rows start on 16 different 16-byte bank groups
   constexpr int OP = DH + 4;
-  constexpr int kTile = TK * DH;
+  constexpr int kTile = TK * RP;
   constexpr size_t kStage = (size_t)NW * 2 * kTile, kMerge = sizeof(float) * NW * kAqMaxG * OP;
   __shared__ __align__(16) uint8_t lds[kStage > kMerge ? kStage : kMerge];
   __shared__ __align__(16) float s_lds[NW][2 * TK];  // a tile's K and V scales
+  __shared__ __align__(16) u32x4 q_lds[QT == 1 ? NP : 1][2][64];
   __shared__ float m_lds[NW][kAqMaxG];
   __shared__ float l_lds[NW][kAqMaxG];
 
-  const int split = blockIdx.x, g = blockIdx.y, i = blockIdx.z;
+  const int split0 = blockIdx.x * a.spw, g = blockIdx.y, i = blockIdx.z;
   const int G = a.H / a.Hkv;
   const int64_t row0 = (int64_t)i * a.H + g * G;
-  const int len = a.kl[i];
-  if (split * kAttnSplit >= len) {  // uniform
-    if (split == 0)                 // no keys: zero rows
+  const int len = min(a.kl[i], a.ms * kAttnSplit);
+  if (split0 * kAttnSplit >= len) {  // uniform
+    if (split0 == 0)                 // no keys: zero rows
       for (int idx = threadIdx.x; idx < G * DH; idx += 64 * NW) Elem<T>::store((T*)a.out + row0 * DH + idx, 0.f);
     return;
   }
-  const int nk = min(len - split * kAttnSplit, kAttnSplit);
+  // keys from split0's first, nk of them: the workgroup's splits, nsp of them
+  const int nk = min(len - split0 * kAttnSplit, a.spw * kAttnSplit);
+  const int nsp = (nk + kAttnSplit - 1) / kAttnSplit;
+  const int ns = (len + kAttnSplit - 1) / kAttnSplit;  // the row's
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4;
   uint8_t* k_lds = lds + wave * 2 * kTile;
   uint8_t* v_lds = k_lds + kTile;
 
-  // codes of this head from the split's first key; the resources end with its last,
-  // so that later rows read as zeros
+  // codes of this head from the first split's first key; the resources end with the
+  // last one, so that later rows read as zeros
   const uint32_t rs = a.br > 1 ? DH : a.Hkv * DH;  // key stride, bytes
-  const int64_t at = kv_offset(a.rb[i], g, a.Hkv, DH, a.br) + (int64_t)split * kAttnSplit * rs;
+  const int64_t at = kv_offset(a.rb[i], g, a.Hkv, DH, a.br) + (int64_t)split0 * kAttnSplit * rs;
   const uint32_t span = (uint32_t)(nk - 1) * rs + DH;
   auto rsrc = [&](const uint8_t* p) {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p + at), (short)0, span, 0x00020000);
@@ -116,14 +120,10 @@ attn_q_split_kernel(AttnQArgs a) {
   const __amdgpu_buffer_rsrc_t kr = rsrc(a.kc), vr = rsrc(a.vc);
   const uint8_t* eb = (lane < TK ? a.ke : a.ve) + at / DH;  // lane: the K (V) scale of key lane % 32
   const uint32_t es = rs / DH;
-  // whole rows, a row's pieces in an order that keeps the fragment reads off each
-  // other's banks: piece p of row r sits at place p ^ (r / SW)
+  const int lr = lane / LPK, lp = lane % LPK;  // row within a load, piece
   uint32_t off[NLD];
 #pragma unroll
-  for (int s = 0; s < NLD; ++s) {
-    const int r = RPI * s + lane / LPK;
-    off[s] = (uint32_t)(TK * wave + r) * rs + (uint32_t)(((lane % LPK) ^ ((r / SW) % LPK)) * 16);
-  }
+  for (int s = 0; s < NLD; ++s) off[s] = (uint32_t)(TK * wave + RPI * s + lr) * rs + (uint32_t)lp * 16u;
   u32x4 kreg[NLD], vreg[NLD];
   uint32_t ereg;
   int t0 = TK * wave;
@@ -138,20 +138,24 @@ attn_q_split_kernel(AttnQArgs a) {
   };
   fetch(t0);
 
-  // Q as the B operand, column = query head, in the codes' k order
+  // Q as the B operand, column = query head, in the codes' k order: three terms in
+  // registers, or bf16 in LDS, whose registers would cost a wave per SIMD. Columns
+  // past the last head repeat it; nothing of theirs is kept.
+  const T* qp = (const T*)a.q + (row0 + min(col, G - 1)) * DH + 16 * grp;
   u32x4 qf[QT][NP][2];
+  if constexpr (QT == 1) {
+    if (wave < NP)
 #pragma unroll
-  for (int p = 0; p < NP; ++p)
+      for (int st = 0; st < 2; ++st) q_lds[wave][st][lane] = ld16(qp + 64 * wave + 8 * st);
+    __syncthreads();
+  } else {
 #pragma unroll
-    for (int st = 0; st < 2; ++st) {
-      const T* qp = (const T*)a.q + (row0 + (col < G ? col : 0)) * DH + 64 * p + 16 * grp + 8 * st;
-      if constexpr (QT == 1) {
-        qf[0][p][st] = ld16(qp);
-      } else {
-        float x[8];
-        float lo[4], hi[4];
-        Elem<float>::unpack(ld16(qp), lo);
-        Elem<float>::unpack(ld16(qp + 4), hi);
+    for (int p = 0; p < NP; ++p)
+#pragma unroll
+      for (int st = 0; st < 2; ++st) {
+        float x[8], lo[4], hi[4];
+        Elem<float>::unpack(ld16(qp + 64 * p + 8 * st), lo);
+        Elem<float>::unpack(ld16(qp + 64 * p + 8 * st + 4), hi);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           x[e] = lo[e];
@@ -160,35 +164,38 @@ attn_q_split_kernel(AttnQArgs a) {
 #pragma unroll
         for (int c = 0; c < QT; ++c) qf[c][p][st] = take_term(x, c == QT - 1);
       }
-    }
+  }
   // V^T fragment of 16 dims: the transposing read gives lane i of a 16-lane group byte
   // i % 8 of what lanes i / 8 + 2 e address, e < 8. Lane j addresses half j % 2 of the
   // piece in row key(j / 2), key(e) = 16 (e / 4) + 4 grp + e % 4: the keys whose scores the
   // group's lanes hold, in their order.
   const int vkey = 16 * (col >> 3) + 4 * grp + ((col >> 1) & 3);
-  const uint32_t v_row = (uint32_t)(vkey * DH + 8 * (col & 1)), v_swz = (uint32_t)(((vkey / SW) % LPK) * 16);
+  const uint32_t v_at = (uint32_t)(vkey * RP + 8 * (col & 1));
   auto vt_frag = [&](int db) {
     typedef int i32x2 __attribute__((ext_vector_type(2)));
     typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
     typedef const __attribute__((address_space(3))) void* lds_ptr;
     const i32x2 w = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
-        (lds_i32x2*)(lds_ptr)(v_lds + v_row + ((uint32_t)(16 * db) ^ v_swz)));
+        (lds_i32x2*)(lds_ptr)(v_lds + v_at + 16 * db));
     return code_frag<CODE>((uint32_t)w[0], (uint32_t)w[1]);
   };
 
   // lane (grp, col): of query head col, the keys 16 j + 4 grp + r of a tile and the dims
   // 16 db + 4 grp + r of the output; lrun its share of the sum. mref is the head's
   // maximum when a tile last exceeded it by more than 2^8 (see attn_shared.hip).
+  float* o_lds = reinterpret_cast<float*>(lds);
+  for (int sp = 0; sp < nsp; ++sp) {  // uniform over the workgroup
+  const int t_end = min((sp + 1) * kAttnSplit, nk);
   float mref = -INFINITY, lrun = 0.f;
   f32x4 o[NDB];
 #pragma unroll
   for (int db = 0; db < NDB; ++db) o[db] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-  for (; t0 < nk; t0 += TK * NW) {  // uniform over the wave
+  for (; t0 < t_end; t0 += TK * NW) {  // uniform over the wave
 #pragma unroll
     for (int s = 0; s < NLD; ++s) {
-      *reinterpret_cast<u32x4*>(k_lds + 1024 * s + 16 * lane) = kreg[s];
-      *reinterpret_cast<u32x4*>(v_lds + 1024 * s + 16 * lane) = vreg[s];
+      *reinterpret_cast<u32x4*>(k_lds + (RPI * s + lr) * RP + 16 * lp) = kreg[s];
+      *reinterpret_cast<u32x4*>(v_lds + (RPI * s + lr) * RP + 16 * lp) = vreg[s];
     }
     // a key past the end weighs nothing, whatever its clamped scale says
     const float sc = code_scale(ereg);
@@ -205,12 +212,13 @@ attn_q_split_kernel(AttnQArgs a) {
 #pragma unroll
       for (int p = 0; p < NP; ++p) {
         const u32x4 w =
-            *reinterpret_cast<const u32x4*>(k_lds + r * DH + (((4 * p + grp) ^ ((r / SW) % LPK)) * 16));
+            *reinterpret_cast<const u32x4*>(k_lds + r * RP + (4 * p + grp) * 16);
 #pragma unroll
         for (int st = 0; st < 2; ++st) {
           const u32x4 kf = code_frag<CODE>(w[2 * st], w[2 * st + 1]);
 #pragma unroll
-          for (int c = QT - 1; c >= 0; --c) acc[j] = mfma_step<bf16_t>(kf, qf[c][p][st], acc[j]);
+          for (int c = QT - 1; c >= 0; --c)
+            acc[j] = mfma_step<bf16_t>(kf, QT == 1 ? q_lds[p][st][lane] : qf[c][p][st], acc[j]);
         }
       }
     }
@@ -273,7 +281,6 @@ attn_q_split_kernel(AttnQArgs a) {
   lrun += __shfl_xor(lrun, 32, 64);
 
   __syncthreads();  // every wave's tiles are done: the merge takes their LDS
-  float* o_lds = reinterpret_cast<float*>(lds);
   if (col < G) {
 #pragma unroll
     for (int db = 0; db < NDB; ++db)
@@ -286,7 +293,6 @@ attn_q_split_kernel(AttnQArgs a) {
   __syncthreads();
   // merge the waves in fixed order: the row itself if its keys fit one split,
   // this split's unnormalised partial otherwise
-  const int ns = min((len + kAttnSplit - 1) / kAttnSplit, a.ms);
   for (int idx = threadIdx.x; idx < G * (DH / 4); idx += 64 * NW) {
     const int m = idx / (DH / 4), d = 4 * (idx % (DH / 4));
     float M = -INFINITY, L = 0.f;
@@ -306,7 +312,7 @@ attn_q_split_kernel(AttnQArgs a) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) Elem<T>::store((T*)a.out + (row0 + m) * DH + d + e, attn_finish_nan(O[e], L));
     } else {
-      const int64_t pidx = (row0 + m) * a.ms + split;
+      const int64_t pidx = (row0 + m) * a.ms + split0 + sp;
       *reinterpret_cast<f32x4*>(a.po + pidx * DH + d) = O;
       if (d == 0) {
         a.pml[pidx * 2] = M;
@@ -314,12 +320,48 @@ attn_q_split_kernel(AttnQArgs a) {
       }
     }
   }
+  __syncthreads();  // the next split's tiles take the LDS; this one's partial is written
+  }
+  if (ns == 1 || nsp < ns) return;
+  // a row whose splits were all this workgroup's: attn_combine_kernel's sums, on
+  // partials that this workgroup wrote
+  for (int idx = threadIdx.x; idx < G * (DH / 4); idx += 64 * NW) {
+    const int m = idx / (DH / 4), d = 4 * (idx % (DH / 4));
+    const int64_t base = (row0 + m) * a.ms;
+    float M = -INFINITY, L = 0.f;
+    f32x4 O = {0.f, 0.f, 0.f, 0.f};
+    for (int sp = 0; sp < ns; ++sp) M = fmaxf(M, a.pml[(base + sp) * 2]);
+    for (int sp = 0; sp < ns; ++sp) {
+      const float mv = a.pml[(base + sp) * 2];
+      const float f = mv == -INFINITY ? 0.f : exp2f(mv - M);
+      const f32x4 ov = *reinterpret_cast<const f32x4*>(a.po + (base + sp) * DH + d);
+      L = fmaf(a.pml[(base + sp) * 2 + 1], f, L);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) O[e] = fmaf(ov[e], f, O[e]);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) Elem<T>::store((T*)a.out + (row0 + m) * DH + d + e, attn_finish_nan(O[e], L));
+  }
+}
+
+// Splits a workgroup takes, one after the other. A row of up to four splits is one
+// workgroup's where the rows alone make 1024 splits (two rounds of workgroups): it
+// finishes the row itself, with the combine kernel's arithmetic, and neither that
+// launch nor workgroups that find no keys are needed. 112 rows x 16 heads x 128-1200
+// keys: 104 -> 82 us. Longer rows keep a workgroup per split (64 rows x 4 heads x 32k
+// keys, four splits each: 400 -> 410 us), and so do fewer rows, whose splits are what
+// fills the chip.
+constexpr int kAqRowSplits = 4;
+constexpr int kAqFill = 1024;
+static int splits_per_workgroup(int ms, int64_t rows) {
+  return ms <= kAqRowSplits && ms * rows >= kAqFill ? ms : 1;
 }
 
 template <typename T, int CODE, int DH>
 static void launch_attn_q(const AttnQArgs& a, hipStream_t st) {
-  hipLaunchKernelGGL((attn_q_split_kernel<T, CODE, DH>), dim3(a.ms, a.Hkv, a.n), dim3(64 * kAqWaves), 0, st, a);
-  if (a.ms > 1)  // some query may span several splits
+  const int wgs = (a.ms + a.spw - 1) / a.spw;
+  hipLaunchKernelGGL((attn_q_split_kernel<T, CODE, DH>), dim3(wgs, a.Hkv, a.n), dim3(64 * kAqWaves), 0, st, a);
+  if (wgs > 1)  // some query may span several workgroups
     hipLaunchKernelGGL((attn_combine_kernel<T, DH, true>), dim3(a.H, a.n), dim3(DH), 0, st, a.po, a.pml, a.kl,
                        (T*)a.out, a.H, a.ms);
 }
@@ -379,6 +421,7 @@ int wfd_attn_decode_q(const void* q, const void* k_codes, const void* v_codes, c
   a.ms = max_splits_for(kv_len_max);
   a.po = (float*)workspace;
   a.pml = (float*)((char*)workspace + align256((size_t)n * H * a.ms * Dh * sizeof(float)));
+  a.spw = splits_per_workgroup(a.ms, (int64_t)n * Hkv);
   a.scale_log2 = scale * 1.4426950408889634f;
   a.br = kv_block_rows;
 #define WFD_ATTNQ_CASE(TT, DT, CODE)                            \
