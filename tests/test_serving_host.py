@@ -29,7 +29,8 @@ def front(monkeypatch):
     monkeypatch.setattr(_lib, "load", no_library)
 
 
-def test_host_tensors_are_refused():
+def test_host_tensors_are_refused(monkeypatch):
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
     t = torch.zeros(2, 2, 64, dtype=torch.bfloat16)
     cache = ops.QuantKV.zeros((8, 2, 64), device="cpu")
     rows = torch.zeros(2, dtype=torch.int64)
@@ -42,6 +43,7 @@ def test_host_tensors_are_refused():
 def test_operands_on_another_device_are_refused(monkeypatch):
     class Fake:
         is_cuda, device = True, torch.device("cuda:1")
+        get_device = staticmethod(lambda: 1)
 
     monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
     with pytest.raises(_lib.WfdError, match="current device is cuda:0"):

@@ -54,11 +54,16 @@ def _need(cond: bool, msg: str) -> None:
 
 def _need_current(*ts: torch.Tensor | None) -> None:
     """GPU tensors, all on the device whose stream the launch goes to."""
-    _need_cuda(*ts)
     dev = torch.cuda.current_device()
     for t in ts:
-        if t is not None and t.device.index != dev:
+        if t is not None and t.get_device() != dev:
+            _need_cuda(t)
             raise _lib.WfdError(f"operand on {t.device}, but the current device is cuda:{dev}")
+
+
+def _table(name: str, t: torch.Tensor, dtype: torch.dtype, size: int) -> None:
+    if t.dtype != dtype or t.numel() < size or not t.is_contiguous():
+        raise _lib.WfdError(f"{name}: {dtype} contiguous (>= {size},)")
 
 
 def _rows(t: torch.Tensor | None, n: int, name: str) -> None:
@@ -280,14 +285,15 @@ def attn_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, p
     Hkv, cDh, br = kv_layout(k_cache, v_cache)
     _need(cDh == Dh and k_cache.dtype == q.dtype, "q/k/v dtype or head_dim mismatch")
     ng = prefix_row_base.numel()
-    for name, t, dt, size in (("prefix_row_base", prefix_row_base, torch.int64, ng),
-                              ("prefix_len", prefix_len, torch.int32, ng),
-                              ("group_first", group_first, torch.int32, ng + 1),
-                              ("kv_row_base", kv_row_base, torch.int64, n), ("kv_len", kv_len, torch.int32, n)):
-        _need(t.dtype == dt and t.is_contiguous() and t.numel() >= size, f"{name}: {dt} contiguous (>= {size},)")
+    _table("prefix_row_base", prefix_row_base, torch.int64, ng)
+    _table("prefix_len", prefix_len, torch.int32, ng)
+    _table("group_first", group_first, torch.int32, ng + 1)
+    _table("kv_row_base", kv_row_base, torch.int64, n)
+    _table("kv_len", kv_len, torch.int32, n)
     _need(prefix_len_max >= 0 and kv_len_max >= 0, "prefix_len_max and kv_len_max must be >= 0")
-    _need(br == 1 or max(prefix_len_max, kv_len_max) <= br,
-          f"prefix_len_max {prefix_len_max} or kv_len_max {kv_len_max} exceeds the cache block ({br} rows)")
+    if 1 < br < max(prefix_len_max, kv_len_max):
+        raise _lib.WfdError(f"prefix_len_max {prefix_len_max} or kv_len_max {kv_len_max} exceeds the cache block "
+                            f"({br} rows)")
     group_max = n if group_max is None else int(group_max)
     _need(group_max >= 0, "group_max must be >= 0")
     if out is None:
@@ -445,7 +451,7 @@ class QuantKV:
     `v_exp` (uint8), the codes' shape without its last dimension; a value is
     code * 2^(exp - 127)."""
 
-    __slots__ = ("k", "v", "k_exp", "v_exp", "code", "Hkv", "Dh", "block_rows")
+    __slots__ = ("k", "v", "k_exp", "v_exp", "code", "Hkv", "Dh", "block_rows", "tensors", "_ptrs")
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_exp: torch.Tensor, v_exp: torch.Tensor):
         _need(k.dtype in _CODES, f"8-bit cache: codes float8_e4m3fn or int8, not {k.dtype}")
@@ -455,6 +461,8 @@ class QuantKV:
                   "8-bit cache: exponents uint8, contiguous, shaped like the codes without their last dimension")
         _need(k.device == v.device == k_exp.device == v_exp.device, "8-bit cache: its tensors are on one device")
         self.k, self.v, self.k_exp, self.v_exp, self.code = k, v, k_exp, v_exp, _CODES[k.dtype]
+        self.tensors = (k, v, k_exp, v_exp)
+        self._ptrs = tuple(t.data_ptr() for t in self.tensors)
 
     @classmethod
     def zeros(cls, shape, *, code: torch.dtype = torch.float8_e4m3fn, device="cuda") -> "QuantKV":
@@ -469,32 +477,26 @@ class QuantKV:
     def nbytes(self) -> int:
         return 2 * (self.k.numel() + self.k_exp.numel())
 
-    @property
-    def tensors(self) -> tuple:
-        return self.k, self.v, self.k_exp, self.v_exp
-
-    def _ptrs(self) -> tuple:
-        return self.k.data_ptr(), self.v.data_ptr(), self.k_exp.data_ptr(), self.v_exp.data_ptr()
-
 
 def _kv_rows(t: torch.Tensor, cache: QuantKV, name: str) -> None:
-    _need(t.dim() == 3 and t.shape[1:] == (cache.Hkv, cache.Dh) and t.stride(2) == 1
-          and (t.stride(1) == cache.Dh or cache.Hkv == 1), f"{name}: (n, Hkv, Dh) rows of the cache's heads")
+    if not (t.dim() == 3 and t.shape[1:] == (cache.Hkv, cache.Dh) and t.stride(2) == 1
+            and (t.stride(1) == cache.Dh or cache.Hkv == 1)):
+        raise _lib.WfdError(f"{name}: (n, Hkv, Dh) rows of the cache's heads")
 
 
 def kv_append_q(k: torch.Tensor, v: torch.Tensor, cache: QuantKV, flat_row: torch.Tensor) -> None:
     """Cache row flat_row[i] = k[i] / v[i], quantised (wfd_kv_append_q): k, v
     (n, Hkv, Dh), each row contiguous (views of a fused qkv row will do);
     flat_row int64, distinct rows."""
-    _need_current(k, v, flat_row, *cache.tensors)
+    _need_current(k, v, flat_row, cache.k)
     n = k.shape[0]
     _kv_rows(k, cache, "k")
     _kv_rows(v, cache, "v")
     _need(v.shape[0] == n and k.dtype == v.dtype, "k and v: as many rows of one dtype")
-    _need(flat_row.dtype == torch.int64 and flat_row.numel() >= n and flat_row.is_contiguous(), "flat_row: int64 (n,)")
+    _table("flat_row", flat_row, torch.int64, n)
     width = cache.Hkv * cache.Dh
     ldk, ldv = (t.stride(0) if n > 1 else width for t in (k, v))
-    rc = _lib.load().wfd_kv_append_q(k.data_ptr(), ldk, v.data_ptr(), ldv, *cache._ptrs(), cache.code,
+    rc = _lib.load().wfd_kv_append_q(k.data_ptr(), ldk, v.data_ptr(), ldv, *cache._ptrs, cache.code,
                                      cache.block_rows, flat_row.data_ptr(), n, cache.Hkv, cache.Dh, _dt(k), _stream())
     _lib.check(rc, "wfd_kv_append_q")
 
@@ -504,11 +506,11 @@ def qkv_rope_append_q(qkv: torch.Tensor, pos: torch.Tensor, rope_cos: torch.Tens
                       q_out: torch.Tensor | None = None) -> torch.Tensor:
     """qkv_rope_append into an 8-bit cache (wfd_qkv_rope_append_q): returns the
     rotated q (the same bits), k (rotated) and v go to rows flat_row."""
-    _need_current(qkv, pos, rope_cos, rope_sin, flat_row, q_out, *cache.tensors)
+    _need_current(qkv, pos, rope_cos, rope_sin, flat_row, q_out, cache.k)
     n = qkv.shape[0]
     _need(qkv.dim() == 2 and qkv.stride(1) == 1 and qkv.shape[1] >= (H + 2 * Hkv) * Dh, "qkv (n, (H+2Hkv)Dh)")
-    _need(pos.dtype == torch.int32 and pos.numel() >= n and pos.is_contiguous(), "pos: int32")
-    _need(flat_row.dtype == torch.int64 and flat_row.numel() >= n and flat_row.is_contiguous(), "flat_row: int64 (n,)")
+    _table("pos", pos, torch.int32, n)
+    _table("flat_row", flat_row, torch.int64, n)
     _need(rope_cos.dtype == torch.float32 == rope_sin.dtype and rope_cos.shape == rope_sin.shape
           and rope_cos.dim() == 2 and rope_cos.shape[1] == Dh // 2 and rope_cos.is_contiguous()
           and rope_sin.is_contiguous(), "rope tables: float32 (S, Dh/2)")
@@ -519,7 +521,7 @@ def qkv_rope_append_q(qkv: torch.Tensor, pos: torch.Tensor, rope_cos: torch.Tens
     ldq = qkv.stride(0) if n > 1 else (H + 2 * Hkv) * Dh
     rc = _lib.load().wfd_qkv_rope_append_q(qkv.data_ptr(), ldq, pos.data_ptr(), rope_cos.data_ptr(),
                                            rope_sin.data_ptr(), rope_cos.shape[0], flat_row.data_ptr(),
-                                           q_out.data_ptr(), *cache._ptrs(), cache.code, cache.block_rows, n, H, Hkv,
+                                           q_out.data_ptr(), *cache._ptrs, cache.code, cache.block_rows, n, H, Hkv,
                                            Dh, _dt(qkv), _stream())
     _lib.check(rc, "wfd_qkv_rope_append_q")
     return q_out
@@ -528,15 +530,17 @@ def qkv_rope_append_q(qkv: torch.Tensor, pos: torch.Tensor, rope_cos: torch.Tens
 def kv_read_q(cache: QuantKV, flat_row: torch.Tensor, *, dtype: torch.dtype = torch.bfloat16,
               k_out: torch.Tensor | None = None, v_out: torch.Tensor | None = None):
     """(k, v), each (n, Hkv, Dh) of `dtype`: the values of cache rows flat_row (wfd_kv_read_q)."""
-    _need_current(flat_row, k_out, v_out, *cache.tensors)
+    _need_current(flat_row, k_out, v_out, cache.k)
     _need(flat_row.dtype == torch.int64 and flat_row.dim() == 1 and flat_row.is_contiguous(), "flat_row: int64 (n,)")
-    _need(dtype in _DT, f"unsupported dtype {dtype} (float32 / bfloat16)")
+    if dtype not in _DT:
+        raise _lib.WfdError(f"unsupported dtype {dtype} (float32 / bfloat16)")
     n, shape = flat_row.numel(), (flat_row.numel(), cache.Hkv, cache.Dh)
     k_out, v_out = (torch.empty(shape, dtype=dtype, device=cache.k.device) if t is None else t
                     for t in (k_out, v_out))
     for name, t in (("k_out", k_out), ("v_out", v_out)):
-        _need(t.shape == shape and t.is_contiguous() and t.dtype == dtype, f"{name}: (n, Hkv, Dh) of {dtype}")
-    rc = _lib.load().wfd_kv_read_q(*cache._ptrs(), cache.code, cache.block_rows, flat_row.data_ptr(),
+        if not (t.shape == shape and t.is_contiguous() and t.dtype == dtype):
+            raise _lib.WfdError(f"{name}: (n, Hkv, Dh) of {dtype}")
+    rc = _lib.load().wfd_kv_read_q(*cache._ptrs, cache.code, cache.block_rows, flat_row.data_ptr(),
                                    k_out.data_ptr(), v_out.data_ptr(), n, cache.Hkv, cache.Dh, _DT[dtype], _stream())
     _lib.check(rc, "wfd_kv_read_q")
     return k_out, v_out
@@ -547,15 +551,14 @@ def attn_decode_q(q: torch.Tensor, cache: QuantKV, kv_row_base: torch.Tensor, kv
                   workspace: torch.Tensor | None = None) -> torch.Tensor:
     """attn_decode over an 8-bit cache (wfd_attn_decode_q): q (n, H, Dh), query i
     reads cache rows kv_row_base[i] + [0, kv_len[i])."""
-    _need_current(q, kv_row_base, kv_len, out, workspace, *cache.tensors)
+    _need_current(q, kv_row_base, kv_len, out, workspace, cache.k)
     _need(q.dim() == 3 and q.is_contiguous(), "q must be contiguous (n, H, Dh)")
     n, H, Dh = q.shape
-    _need(cache.Dh == Dh, f"head_dim mismatch: q {Dh}, cache {cache.Dh}")
-    _need(cache.block_rows == 1 or kv_len_max <= cache.block_rows,
-          f"kv_len_max {kv_len_max} exceeds the cache block ({cache.block_rows} rows)")
-    _need(kv_row_base.dtype == torch.int64 and kv_row_base.numel() >= n and kv_row_base.is_contiguous(),
-          "kv_row_base: int64 (n,)")
-    _need(kv_len.dtype == torch.int32 and kv_len.numel() >= n and kv_len.is_contiguous(), "kv_len: int32 (n,)")
+    _need(cache.Dh == Dh, "q and cache head_dim mismatch")
+    if 1 < cache.block_rows < kv_len_max:
+        raise _lib.WfdError(f"kv_len_max {kv_len_max} exceeds the cache block ({cache.block_rows} rows)")
+    _table("kv_row_base", kv_row_base, torch.int64, n)
+    _table("kv_len", kv_len, torch.int32, n)
     _need(kv_len_max >= 1, "kv_len_max must be >= 1")
     if out is None:
         out = torch.empty_like(q)
@@ -564,7 +567,7 @@ def attn_decode_q(q: torch.Tensor, cache: QuantKV, kv_row_base: torch.Tensor, kv
     if workspace is None:
         workspace = attn_workspace(n, H, Dh, kv_len_max, q.device)
     sc = 1.0 / math.sqrt(Dh) if scale is None else float(scale)
-    rc = _lib.load().wfd_attn_decode_q(q.data_ptr(), *cache._ptrs(), cache.code, cache.block_rows,
+    rc = _lib.load().wfd_attn_decode_q(q.data_ptr(), *cache._ptrs, cache.code, cache.block_rows,
                                        kv_row_base.data_ptr(), kv_len.data_ptr(), out.data_ptr(), n, H, cache.Hkv, Dh,
                                        dt, sc, int(kv_len_max), workspace.data_ptr(),
                                        workspace.numel() * workspace.element_size(), _stream())
@@ -927,12 +930,17 @@ def sample(logits: torch.Tensor, u: torch.Tensor, *, temperature: torch.Tensor |
     _need_current(logits, u, temperature, top_k, top_p, min_p, out, ring, ring_rows, expect, accept)
     _need(logits.dtype == torch.float32 and logits.dim() == 2 and logits.stride(1) == 1, "logits: float32 (n, V)")
     n = logits.shape[0] if n is None else n
-    _need(0 <= n <= logits.shape[0], f"n={n} outside the {logits.shape[0]} logits rows")
-    for name, t, dt in (("u", u, torch.float32), ("temperature", temperature, torch.float32),
-                        ("top_k", top_k, torch.int32), ("top_p", top_p, torch.float32),
-                        ("min_p", min_p, torch.float32)):
-        if t is not None:
-            _need(t.dtype == dt and t.is_contiguous() and t.numel() >= n, f"{name}: {dt} contiguous (>= {n},)")
+    if not 0 <= n <= logits.shape[0]:
+        raise _lib.WfdError(f"n={n} outside the {logits.shape[0]} logits rows")
+    _table("u", u, torch.float32, n)
+    if temperature is not None:
+        _table("temperature", temperature, torch.float32, n)
+    if top_k is not None:
+        _table("top_k", top_k, torch.int32, n)
+    if top_p is not None:
+        _table("top_p", top_p, torch.float32, n)
+    if min_p is not None:
+        _table("min_p", min_p, torch.float32, n)
     out, acc = _argmax_outputs(n, logits.device, out, ring, ring_rows, expect, accept, accept_mapped)
     ld = logits.stride(0) if logits.shape[0] > 1 else logits.shape[1]
     rc = _lib.load().wfd_sample(logits.data_ptr(), ld, u.data_ptr(), _p(temperature), _p(top_k), _p(top_p), _p(min_p),
