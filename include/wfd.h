@@ -559,13 +559,17 @@ int wfd_argmax(const float* logits, int64_t ld, int64_t* out, int64_t* ring, con
  * Logits of -inf are never drawn; equal infinite largest logits share the draw;
  * a row of nothing but -inf gives 0 and a row with a NaN the index of its first
  * NaN, as wfd_argmax does. ring / ring_rows / ring_len and expect / accept as in
- * wfd_argmax. vocab at most 524288.
+ * wfd_argmax. vocab at most 524288, n at most 65535. workspace >=
+ * wfd_sample_workspace_bytes(n, vocab), 16-byte aligned (0 bytes, and NULL will
+ * do, up to 32768 logits a row).
  * Replaces: the position-seeded draw of temperature sampling
  *   (src/decoding/acceptance.py:61-214), with its .item() per token.
  */
+size_t wfd_sample_workspace_bytes(int n, int vocab);
 int wfd_sample(const float* logits, int64_t ld, const float* u, const float* temperature, const int32_t* top_k,
                const float* top_p, const float* min_p, int64_t* out, int64_t* ring, const int32_t* ring_rows,
-               int64_t ring_len, const int64_t* expect, int32_t* accept, int n, int vocab, wfd_stream_t stream);
+               int64_t ring_len, const int64_t* expect, int32_t* accept, int n, int vocab, void* workspace,
+               size_t ws_bytes, wfd_stream_t stream);
 
 /*
  * Column groups of wfd_linear_argmax for this shape: the few-row launch's

@@ -153,10 +153,24 @@ def test_sample_front_end_refusals(front):
 def test_sample_entry_point_checks_before_launch():
     lib = _lib.load()
     call = lambda n=1, V=10, ld=10, ring=None, expect=None: lib.wfd_sample(  # noqa: E731
-        None, ld, None, None, None, None, None, None, ring, None, 0, expect, None, n, V, None)
+        None, ld, None, None, None, None, None, None, ring, None, 0, expect, None, n, V, None, 0, None)
     assert call(n=-1) == -1 and call(V=0) == -1 and call(ld=9) == -1 and b"ld=9" in lib.wfd_last_error()
     assert call(V=(1 << 19) + 1, ld=1 << 20) == -2 and b"at most 524288" in lib.wfd_last_error()
-    assert call(n=0) == 0 and call() == -1 and b"null pointer" in lib.wfd_last_error()
+    assert call(n=70000) == -2 and call(n=0) == 0 and call() == -1 and b"null pointer" in lib.wfd_last_error()
+    ws = lib.wfd_sample_workspace_bytes  # long rows only; as much for each
+    assert ws(100, 32768) == 0 and ws(0, 50000) == 0 and ws(3, 1 << 20) == 0
+    assert ws(1, 32769) > 8 * 1024 + 8 * 8192 and ws(7, 500000) == 7 * ws(1, 32769)
+
+
+@pytest.mark.skipif(torch.cuda.device_count() > 0, reason="made-up device addresses: run only where no GPU is "
+                    "visible, so a regressed check cannot launch a kernel on them")
+def test_sample_workspace_is_checked():
+    lib = _lib.load()
+    call = lambda ws, size: lib.wfd_sample(4096, 50000, 4096, None, None, None, None, 4096, None, None, 0,  # noqa: E731
+                                           None, None, 2, 50000, ws, size, None)
+    assert call(None, 1 << 30) == -1 and b"null pointer" in lib.wfd_last_error()
+    assert call(4096 + 8, 1 << 30) == -1 and b"16-byte aligned" in lib.wfd_last_error()
+    assert call(4096, 1000) == -4 and b"workspace 1000 bytes" in lib.wfd_last_error()
 
 
 def test_sampler_parameters_and_numbers():

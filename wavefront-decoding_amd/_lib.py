@@ -78,7 +78,9 @@ SIGNATURES: dict[str, tuple] = {
                                  _vp, _i64, _i32, _i32, _i32, _f32, _i32, _vp]),
     "wfd_copy_rows": (_i32, [_vp, _vp, _i64, _vp, _vp, _i64, _i32, _i32, _i32, _vp]),
     "wfd_argmax": (_i32, [_vp, _i64, _vp, _vp, _vp, _i64, _vp, _vp, _i32, _i32, _vp]),
-    "wfd_sample": (_i32, [_vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _vp, _i32, _i32, _vp]),
+    "wfd_sample_workspace_bytes": (_sz, [_i32, _i32]),
+    "wfd_sample": (_i32, [_vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _vp, _i32, _i32, _vp, _sz,
+                          _vp]),
     "wfd_linear_argmax_groups": (_i32, [_i32, _i32, _i32, _i32]),
     "wfd_linear_argmax": (_i32, [_vp, _vp, _i64, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _vp, _vp, _vp, _vp]),
     "wfd_argmax_groups": (_i32, [_vp, _vp, _i32, _vp, _vp, _vp, _i64, _vp, _vp, _i32, _vp]),

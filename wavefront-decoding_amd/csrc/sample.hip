@@ -14,16 +14,22 @@
 // kernel's layout, the companions or the run -- and a border is off by 2^-45 per
 // token. u, p and their products with the sums are exact (64 x 64 -> 128 bits).
 //
-// One workgroup per row. Where the kept tokens are few -- top-k, or a top-p whose
-// tokens hold enough of the weight -- they are found without ordering the row: of
-// the 1024 threads' largest logits, at least k are no smaller than the k-th, so
-// every one of the first k tokens is at or above it, and few others are. Those go
-// to a list in LDS, which is sorted (one entry a thread), and top-k, top-p and
-// min_p are positions in it.
-// Otherwise a histogram of the logits' distance from the largest says which of
-// 1024 bins the last kept token lies in, by count or by weight, and a radix select
-// over that bin's tokens (over the row, if they are too many) finds its key; ties
-// with it are kept in index order.
+// Where the kept tokens are few -- top-k, or a top-p whose tokens hold enough of
+// the weight -- they are found without ordering the row: of the 1024 threads'
+// largest logits, at least k are no smaller than the k-th, so every one of the
+// first k tokens is at or above it, and few others are. Those go to a list in LDS,
+// which is sorted (one entry a thread), and top-k, top-p and min_p are positions
+// in it. Otherwise a histogram of the logits' distance from the largest says which
+// of 1024 bins the last kept token lies in, by count or by weight, and a radix
+// select over that bin's tokens (over the row, if they are too many) finds its
+// key; ties with it are kept in index order.
+//
+// Rows of up to 32768 logits are one workgroup's, which keeps them in LDS. Longer
+// ones are cut into slabs of 8192, a workgroup each, in five launches that leave
+// their results in the workspace: the slabs' largest logits; the k candidates or
+// the histogram; the tokens of the border's bin; the weights up to the border; the
+// row's token. What no slab could prepare (a top-k beyond kSmGuess, a list that
+// overflows) the last launch does by itself as for a short row.
 #include "wfd_common.h"
 
 namespace wfd {
@@ -65,9 +71,12 @@ struct SmArgs {
 };
 
 constexpr int kSmBins = 1024;   // one per thread
-constexpr int kSmList = 2048;
 constexpr int kSmSort = kSmThreads;  // entries of a list that is sorted
-constexpr int kSmGuess = 600;        // top-k up to which the list is tried: ~900 tokens are then above the k-th thread's
+constexpr int kSmLong = 32768;       // longest row of one workgroup
+constexpr int kSmSlab = 8192;
+constexpr int kSmSlabs = kSmMaxVocab / kSmSlab;
+constexpr int kSmRowList = 8192;     // tokens that the slabs of a row may list
+constexpr int kSmGuess = 600;        // top-k up to which the list is tried: ~900 tokens are at or above the 600th thread's
 constexpr float kSmMasked = -1e4f;  // logits down to here spread the bins; the others share the last
 
 __device__ __forceinline__ uint64_t sm_wave_sum(uint64_t v) {
@@ -101,106 +110,222 @@ __device__ __forceinline__ uint64_t sm_mul_frac(uint64_t s, float f, bool& rest)
   return __umul64hi(s, q);
 }
 
-// CAP > 0: the row is kept in LDS (V <= CAP); 0: it is read again in every pass
-// (from L2). In registers, 32 logits a thread, the passes' code spilled.
-template <int CAP>
-__global__ __launch_bounds__(kSmThreads) void sample_kernel(SmArgs a) {
-  __shared__ unsigned long long hist[kSmBins];
-  __shared__ unsigned long long seg[(CAP > 0 ? CAP : kSmMaxVocab) / 256];  // the running sums' steps, in index order
-  __shared__ __align__(16) u32x4 keep[CAP > 0 ? CAP / 4 : 1];
-  __shared__ uint32_t list_key[kSmList];
-  __shared__ uint32_t list_idx[kSmList];
-  __shared__ double tab[32];
-  __shared__ float s_max[kSmWaves], s_min[kSmWaves];
-  __shared__ unsigned long long s_sum[kSmWaves];
-  __shared__ uint32_t s_lo[kSmWaves], s_hi[kSmWaves];
-  __shared__ unsigned long long s_u64;
-  __shared__ uint32_t s_u32, s_count;
-  const int i = blockIdx.x;
-  const int t = threadIdx.x;
-  const int wave = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63;
-  const int V = a.V;
-  const float* row = a.logits + (int64_t)i * a.ld;
-  const bool vec = ((uintptr_t)row & 15) == 0;
-  // wave w holds the logits [w per_wave, (w + 1) per_wave): index order is wave, round, lane
-  const int per_wave = (V + 63) / 64 * 4;
-  const int w_end = min((wave + 1) * per_wave, V);
-  const int nchunks = (per_wave + 255) / 256;
-  auto first_of = [&](int c) { return wave * per_wave + 256 * c + 4 * lane; };
+// What a long row's launches leave each other.
+struct SmRowWs {
+  unsigned long long hist[kSmBins];
+  unsigned long long share[kSmSlabs * kSmWaves];  // weights kept in the waves' shares, slab after slab
+  float max[kSmSlabs], min[kSmSlabs];
+  uint32_t nan[kSmSlabs];
+  uint32_t count;  // of the list; more than kSmRowList: it is incomplete
+  uint32_t kk;
+  int32_t last_tie;
+  uint32_t pad;
+  uint32_t key[kSmRowList], idx[kSmRowList];
+};
 
-  auto fetch = [&](int c, float (&x)[4]) {  // 4 logits; -inf past the wave's
+// CAP > 0: the logits at hand are kept in LDS, at most CAP; 0: they are read again
+// in every pass (from L2). In registers, 32 a thread, the passes' code spilled.
+template <int CAP, int LIST>
+struct SmShared {
+  unsigned long long hist[kSmBins];
+  unsigned long long seg[(CAP > 0 ? CAP : kSmMaxVocab) / 256];  // the running sums' steps, in index order
+  u32x4 keep[CAP > 0 ? CAP / 4 : 1];
+  uint32_t list_key[LIST], list_idx[LIST];
+  double tab[32];
+  float max[kSmWaves], min[kSmWaves];
+  unsigned long long sum[kSmWaves];
+  uint32_t lo[kSmWaves], hi[kSmWaves];
+  unsigned long long u64;
+  uint32_t u32, count;
+};
+
+// A workgroup's work on logits [begin, end) of a row: wave w holds [begin + w
+// per_wave, begin + (w + 1) per_wave), 4 consecutive ones a lane and round, so
+// that index order is wave, round, lane. Every method is called by all threads.
+template <int CAP, int LIST>
+struct Sm {
+  const SmArgs& a;
+  SmShared<CAP, LIST>& s;
+  const int i, t, wave, lane, V, begin, end, per_wave, w_end, rounds;
+  const float* row;
+  const bool vec;
+  // the row's largest logit and the bins' range, and the thread's own largest
+  float best, low, mine;
+  bool nan;
+  // parameters
+  float T, p, minp, u, scale;
+  int k;
+  bool has_k, has_p, endless;
+  double inv;
+  uint64_t wmin;
+  // Kept: keys above kk, and the first `ties` tokens with key kk, of which ties_left
+  // more are not kept; last_tie: the index of the last kept one.
+  uint32_t kk = 0;
+  uint64_t ties = 0, ties_left = 0;
+  int last_tie = 0x7fffffff;
+  bool ties_listed = false;  // every token with key kk is in the list
+  int nlist = 0;
+
+  __device__ __forceinline__ Sm(const SmArgs& args, SmShared<CAP, LIST>& sh, int row_i, int lo, int hi)
+      : a(args), s(sh), i(row_i), t(threadIdx.x), wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)),
+        lane(threadIdx.x & 63), V(args.V), begin(lo), end(hi), per_wave((hi - lo + 63) / 64 * 4),
+        w_end(min(lo + (wave + 1) * per_wave, hi)), rounds((per_wave + 255) / 256),
+        row(args.logits + (int64_t)row_i * args.ld), vec(((uintptr_t)(row + lo) & 15) == 0) {
+    if constexpr (CAP > 0) {  // every load first; a thread reads back only what it stores
+      float x[CAP / kSmChunk][4];
+#pragma unroll
+      for (int c = 0; c < CAP / kSmChunk; ++c) fetch(c, x[c]);
+#pragma unroll
+      for (int c = 0; c < CAP / kSmChunk; ++c) s.keep[c * kSmThreads + t] = Elem<float>::pack(x[c]);
+    }
+    if (t < 32) s.tab[t] = exp2((double)t * 0.03125);
+  }
+
+  __device__ __forceinline__ int first_of(int c) const { return begin + wave * per_wave + 256 * c + 4 * lane; }
+  __device__ __forceinline__ void fetch(int c, float (&x)[4]) const {  // 4 logits; -inf past the wave's
     const int e = first_of(c);
     if (vec && e + 4 <= w_end) {
       Elem<float>::unpack(ld16(row + e), x);
     } else {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) x[k] = e + k < w_end ? row[e + k] : -INFINITY;
+      for (int q = 0; q < 4; ++q) x[q] = e + q < w_end ? row[e + q] : -INFINITY;
     }
-  };
-  if constexpr (CAP > 0) {  // every load first; a thread reads back only what it stores
-    float x[CAP / kSmChunk][4];
-#pragma unroll
-    for (int c = 0; c < CAP / kSmChunk; ++c) fetch(c, x[c]);
-#pragma unroll
-    for (int c = 0; c < CAP / kSmChunk; ++c) keep[c * kSmThreads + t] = Elem<float>::pack(x[c]);
   }
-  if (t < 32) tab[t] = exp2((double)t * 0.03125);
-  // f(first index, the 4 logits) over the row, in index order per thread; -inf fills the
-  // places past the wave's share, which no weight, bin or key below counts
-  auto each = [&](auto f) {
+  // f(first index, 4 logits), in index order per thread; -inf fills the places past the
+  // wave's share, which no weight, bin or key below counts
+  template <typename F>
+  __device__ __forceinline__ void each(F f) {
     float x[4];
     if constexpr (CAP > 0) {
-      for (int c = 0; c < nchunks; ++c) {
-        Elem<float>::unpack(keep[c * kSmThreads + t], x);
+      for (int c = 0; c < rounds; ++c) {
+        Elem<float>::unpack(s.keep[c * kSmThreads + t], x);
         f(first_of(c), x);
       }
     } else {
       fetch(0, x);
-      for (int c = 0; c < nchunks; ++c) {  // a chunk ahead
+      for (int c = 0; c < rounds; ++c) {  // a round ahead
         float y[4];
-        fetch(min(c + 1, nchunks - 1), y);
+        fetch(min(c + 1, rounds - 1), y);
         f(first_of(c), x);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) x[k] = y[k];
+        for (int q = 0; q < 4; ++q) x[q] = y[q];
       }
     }
-  };
+  }
 
-  // the largest logit (of the thread, of the row), whether there is a NaN, the range of the bins
-  float mine = -INFINITY, low = INFINITY;
-  bool nan = false;
-  each([&](int, const float (&x)[4]) {
+  // --- the workgroup's sums -------------------------------------------------
+  __device__ __forceinline__ uint64_t block_sum(uint64_t v) {
+    v = sm_wave_sum(v);
+    __syncthreads();
+    if (lane == 0) s.sum[wave] = v;
+    __syncthreads();
+    uint64_t all = 0;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      nan |= x[q] != x[q];
-      mine = fmaxf(mine, x[q]);
-      low = fminf(low, x[q] > kSmMasked ? x[q] : INFINITY);
+    for (int w = 0; w < kSmWaves; ++w) all += s.sum[w];
+    return all;
+  }
+  __device__ __forceinline__ uint64_t wave_scan(uint64_t v) const {  // inclusive
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) {
+      const uint64_t o = sm_shfl_up(v, m);
+      if (lane >= m) v += o;
     }
-  });
-  float best = mine;
-#pragma unroll
-  for (int m = 32; m >= 1; m >>= 1) {
-    best = fmaxf(best, __shfl_xor(best, m, 64));
-    low = fminf(low, __shfl_xor(low, m, 64));
+    return v;
   }
-  nan = __ballot(nan) != 0;
-  if (lane == 0) {
-    s_max[wave] = nan ? __uint_as_float(0x7fc00000u) : best;
-    s_min[wave] = low;
-  }
-  __syncthreads();
-  nan = false;
+  __device__ __forceinline__ uint64_t block_scan(uint64_t v) {  // the sum of the threads' v before this one
+    const uint64_t inc = wave_scan(v);
+    __syncthreads();
+    if (lane == 63) s.sum[wave] = inc;
+    __syncthreads();
+    uint64_t before = lane < wave ? (uint64_t)s.sum[lane] : 0;  // 16 waves
 #pragma unroll
-  for (int w = 0; w < kSmWaves; ++w) {
-    nan |= s_max[w] != s_max[w];
-    best = fmaxf(best, s_max[w]);
-    low = fminf(low, s_min[w]);
+    for (int m = 8; m >= 1; m >>= 1) before += sm_shfl_xor(before, m);
+    return (uint64_t)__shfl((unsigned long long)before, 0, 64) + inc - v;
+  }
+  // The bin (thread t holds bin t's sum v) in which base plus the running sum reaches need; before: the sum before it.
+  __device__ __forceinline__ uint32_t find_bin(uint64_t v, uint64_t base, uint64_t need, uint64_t& before) {
+    const uint64_t run = base + block_scan(v);
+    if (run < need && run + v >= need) {
+      s.u32 = t;
+      s.u64 = run;
+    }
+    __syncthreads();
+    before = s.u64;
+    return s.u32;
   }
 
-  const float T = a.temperature ? a.temperature[i] : 1.f;
-  if (nan || !(T > 0.f) || best == -INFINITY) {  // uniform
-    // greedy rows: the first of the largest; a row with a NaN: its first, visibly, as
-    // in wfd_argmax; a row without any possible token: 0
+  // --- the row's largest logit, whether there is a NaN, the range of the bins --
+  __device__ __forceinline__ void largest() {
+    mine = -INFINITY;
+    float lo = INFINITY;
+    bool bad = false;
+    each([&](int, const float (&x)[4]) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        bad |= x[q] != x[q];
+        mine = fmaxf(mine, x[q]);
+        lo = fminf(lo, x[q] > kSmMasked ? x[q] : INFINITY);
+      }
+    });
+    float hi = mine;
+#pragma unroll
+    for (int m = 32; m >= 1; m >>= 1) {
+      hi = fmaxf(hi, __shfl_xor(hi, m, 64));
+      lo = fminf(lo, __shfl_xor(lo, m, 64));
+    }
+    bad = __ballot(bad) != 0;
+    if (lane == 0) {
+      s.max[wave] = hi;
+      s.min[wave] = lo;
+      s.lo[wave] = bad;
+    }
+    __syncthreads();
+    nan = false;
+    best = -INFINITY;
+    low = INFINITY;
+#pragma unroll
+    for (int w = 0; w < kSmWaves; ++w) {
+      nan |= s.lo[w] != 0;
+      best = fmaxf(best, s.max[w]);
+      low = fminf(low, s.min[w]);
+    }
+    __syncthreads();
+  }
+  // The same of a long row, from its slabs'.
+  __device__ __forceinline__ void largest_of(const SmRowWs& ws, int slabs) {
+    nan = false;
+    best = -INFINITY;
+    low = INFINITY;
+    const int l = min(lane, slabs - 1);  // at most 64
+    nan = __ballot(ws.nan[l] != 0) != 0;
+    best = ws.max[l];
+    low = ws.min[l];
+#pragma unroll
+    for (int m = 32; m >= 1; m >>= 1) {
+      best = fmaxf(best, __shfl_xor(best, m, 64));
+      low = fminf(low, __shfl_xor(low, m, 64));
+    }
+  }
+  // false: a greedy row, or one with a NaN or without any possible token
+  __device__ __forceinline__ bool parameters() {
+    T = a.temperature ? a.temperature[i] : 1.f;
+    if (nan || !(T > 0.f) || best == -INFINITY) return false;
+    inv = fmin(1.4426950408889634 / (double)T, 1e300);  // finite: 0 times it is 0
+    endless = best == INFINITY;                          // infinite logits share everything
+    k = a.top_k ? a.top_k[i] : 0;
+    has_k = k > 0 && k < V;
+    p = a.top_p ? a.top_p[i] : 1.f;
+    has_p = p < 1.f;
+    minp = a.min_p ? a.min_p[i] : 0.f;
+    // on the integer weights' scale: w >= min_p for w on or above it
+    wmin = minp > 0.f ? (minp < 1.f ? (uint64_t)ceil((double)minp * kSmOne) : (uint64_t)kSmOne) : 0;
+    u = a.u[i];
+    u = u > 0.f ? (u < 1.f ? u : 0.99999994f) : 0.f;
+    scale = best > low ? (float)(kSmBins - 2) / (best - low) : 1.f;
+    return true;
+  }
+  // The first index of the largest logit, or of a NaN.
+  __device__ __forceinline__ int first_best() {
     int bi = 0x7fffffff;
     each([&](int e, const float (&x)[4]) {
 #pragma unroll
@@ -209,76 +334,140 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SmArgs a) {
     });
 #pragma unroll
     for (int m = 32; m >= 1; m >>= 1) bi = min(bi, __shfl_xor(bi, m, 64));
-    if (lane == 0) s_lo[wave] = (uint32_t)bi;
     __syncthreads();
-    if (t == 0) {
-      for (int w = 0; w < kSmWaves; ++w) bi = min(bi, (int)s_lo[w]);
-      argmax_finish(i, bi, a.out, a.ring, a.ring_rows, a.ring_len, a.expect, a.accept);
-    }
-    return;
+    if (lane == 0) s.lo[wave] = (uint32_t)bi;
+    __syncthreads();
+    for (int w = 0; w < kSmWaves; ++w) bi = min(bi, (int)s.lo[w]);
+    return bi;
   }
-  const double inv = fmin(1.4426950408889634 / (double)T, 1e300);  // finite: 0 times it is 0
-  const bool endless = best == INFINITY;  // infinite logits share everything
-  auto weight = [&](float l) -> uint64_t {
+
+  // --- weights and bins ------------------------------------------------------
+  __device__ __forceinline__ uint64_t weight(float l) const {
     if (endless) return l == best ? (uint64_t)kSmOne : 0;
-    return sm_exp2(((double)l - (double)best) * inv, tab);  // of the largest itself: exactly one
-  };
-  const int k = a.top_k ? a.top_k[i] : 0;
-  const bool has_k = k > 0 && k < V;
-  const float p = a.top_p ? a.top_p[i] : 1.f;
-  const bool has_p = p < 1.f;
-  const float minp = a.min_p ? a.min_p[i] : 0.f;
-  // min_p on the integer weights' scale: w >= min_p for w on or above it
-  const uint64_t wmin = minp > 0.f ? (minp < 1.f ? (uint64_t)ceil((double)minp * kSmOne) : (uint64_t)kSmOne) : 0;
-  float u = a.u[i];
-  u = u > 0.f ? (u < 1.f ? u : 0.99999994f) : 0.f;
+    return sm_exp2(((double)l - (double)best) * inv, s.tab);  // of the largest itself: exactly one
+  }
+  __device__ __forceinline__ int bin_of(float l) const {  // by the distance from the largest
+    return l == best ? 0 : (int)fminf((best - l) * scale, (float)(kSmBins - 1));
+  }
+  __device__ __forceinline__ bool above(int e, float l) const {
+    const uint32_t key = sm_key(l);
+    return key > kk || (key == kk && e <= last_tie);
+  }
+  __device__ __forceinline__ uint64_t kept(int e, float l) const {
+    if (!above(e, l)) return 0;
+    const uint64_t w = weight(l);
+    return w >= wmin ? w : 0;
+  }
+  __device__ __forceinline__ uint64_t need_of(uint64_t sum) const {  // the weight that top-p asks of sum, at least the least
+    bool rest;
+    const uint64_t need = sm_mul_frac(sum, p > 0.f ? p : 0.f, rest);
+    return rest || need == 0 ? need + 1 : need;
+  }
+  __device__ __forceinline__ uint64_t goal(uint64_t total) const {
+    bool rest;
+    return sm_mul_frac(total, u, rest);
+  }
 
-  auto block_sum = [&](uint64_t v) -> uint64_t {
-    v = sm_wave_sum(v);
+  // --- the list ----------------------------------------------------------------
+  // Tokens of bins [b0, b1] to the list; false if they are more than room.
+  __device__ __forceinline__ bool collect(int b0, int b1, uint32_t room) {
     __syncthreads();
-    if (lane == 0) s_sum[wave] = v;
+    if (t == 0) s.count = 0;
     __syncthreads();
-    uint64_t s = 0;
+    each([&](int e, const float (&x)[4]) {
+      bool in[4];
+      int n_in = 0;
 #pragma unroll
-    for (int w = 0; w < kSmWaves; ++w) s += s_sum[w];
-    return s;
-  };
-  // The sum of the threads' v before this one.
-  auto block_scan = [&](uint64_t v) -> uint64_t {
-    uint64_t inc = v;
+      for (int q = 0; q < 4; ++q) {
+        const int b = bin_of(x[q]);
+        in[q] = e + q < w_end && b >= b0 && b <= b1;
+        n_in += in[q];
+      }
+      if (n_in) {
+        uint32_t at = atomicAdd(&s.count, (uint32_t)n_in);
 #pragma unroll
-    for (int m = 1; m < 64; m <<= 1) {
-      const uint64_t o = sm_shfl_up(inc, m);
-      if (lane >= m) inc += o;
+        for (int q = 0; q < 4; ++q)
+          if (in[q]) {
+            if (at < LIST) {
+              s.list_key[at] = sm_key(x[q]);
+              s.list_idx[at] = e + q;
+            }
+            ++at;
+          }
+      }
+    });
+    __syncthreads();
+    nlist = (int)min(s.count, (uint32_t)LIST);
+    return s.count <= room;
+  }
+  // The bin that holds the k-th of the threads' largest logits (of `mine`, of the threads
+  // that hold any): every one of the first k tokens is in it or before.
+  __device__ __forceinline__ int guess_bin(uint64_t of) {
+    __syncthreads();
+    s.hist[t] = 0;
+    __syncthreads();
+    if (first_of(0) < w_end) atomicAdd(&s.hist[bin_of(mine)], 1ull);
+    __syncthreads();
+    uint64_t before;
+    return (int)find_bin(s.hist[t], 0, of, before);
+  }
+  template <typename F>
+  __device__ __forceinline__ void over_list(F f) const {
+    for (int e = t; e < nlist; e += kSmThreads) f(s.list_key[e]);
+  }
+  template <typename F>
+  __device__ __forceinline__ void over_row(F f) {
+    each([&](int e, const float (&x)[4]) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        if (e + q < w_end) f(sm_key(x[q]));
+    });
+  }
+  // Sorts a list of at most kSmSort tokens and cuts it: of the n_kept first (all, without
+  // top-k) those whose weight reaches need(weight of these), with top-p.
+  template <typename N>
+  __device__ __forceinline__ void cut_list(int n_kept, N need) {
+    // larger keys first, lower indexes first among equals; nothing behind the list
+    __syncthreads();
+    uint64_t v = t < nlist ? ((uint64_t)s.list_key[t] << 32) | (uint32_t)~s.list_idx[t] : 0;
+    for (int size = 2; size < 2 * nlist; size <<= 1) {
+      for (int step = size >> 1; step > 0; step >>= 1) {
+        uint64_t o;
+        if (step < 64) {
+          o = sm_shfl_xor(v, step);
+        } else {
+          __syncthreads();
+          s.hist[t] = v;
+          __syncthreads();
+          o = s.hist[t ^ step];
+        }
+        const bool first = (t & step) == 0, falling = (t & size) == 0;
+        v = (first == falling) == (v > o) ? v : o;
+      }
     }
     __syncthreads();
-    if (lane == 63) s_sum[wave] = inc;
-    __syncthreads();
-    uint64_t before = lane < wave ? (uint64_t)s_sum[lane] : 0;  // 16 waves
-#pragma unroll
-    for (int m = 8; m >= 1; m >>= 1) before += sm_shfl_xor(before, m);
-    return (uint64_t)__shfl((unsigned long long)before, 0, 64) + inc - v;
-  };
-  // The bin (thread t holds bin t's sum v) in which base plus the running sum reaches need; before: the sum before it.
-  auto find_bin = [&](uint64_t v, uint64_t base, uint64_t need, uint64_t& before) -> uint32_t {
-    const uint64_t run = base + block_scan(v);
-    if (run < need && run + v >= need) {
-      s_u32 = t;
-      s_u64 = run;
+    s.hist[t] = v;
+    const uint64_t w = t < nlist ? weight(sm_logit((uint32_t)(v >> 32))) : 0;
+    const uint64_t before = block_scan(w);
+    if (has_p) {
+      if (t == n_kept - 1) s.u64 = before + w;
+      __syncthreads();
+      const uint64_t least = need((uint64_t)s.u64);
+      if (before < least && before + w >= least) s.u32 = t;
+      __syncthreads();
+      n_kept = (int)s.u32 + 1;
     }
-    __syncthreads();
-    before = s_u64;
-    return s_u32;
-  };
+    const uint64_t last = s.hist[n_kept - 1];
+    kk = (uint32_t)(last >> 32);
+    last_tie = (int)~(uint32_t)last;
+    ties = 0;
+  }
 
-  // Kept so far: keys above kk, and the first `ties` tokens with key kk.
-  uint32_t kk = 0;
-  uint64_t ties = 0, ties_left = 0;  // and the ones with key kk that are not
-
-  // The shortest prefix of the kept tokens whose measure (1 or the weight), on
-  // top of base, reaches need. over(f) calls f(key) for tokens that include all
-  // that may end it; equal keys may all be there, the kept ties count as ties.
-  auto refine = [&](auto over, uint64_t base, uint64_t need, bool by_weight) {
+  // The shortest prefix of the kept tokens whose measure (1 or the weight), on top of
+  // base, reaches need. over(f) calls f(key) for tokens that include all that may end
+  // it; equal keys may all be there, the kept ties count as ties.
+  template <typename O>
+  __device__ __forceinline__ void refine(O over, uint64_t base, uint64_t need, bool by_weight) {
     const uint32_t k0 = kk;
     const uint64_t t0 = ties;
     uint32_t lo = 0xffffffffu, hi = 0;
@@ -295,14 +484,14 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SmArgs a) {
     }
     __syncthreads();
     if (lane == 0) {
-      s_lo[wave] = lo;
-      s_hi[wave] = hi;
+      s.lo[wave] = lo;
+      s.hi[wave] = hi;
     }
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < kSmWaves; ++w) {
-      lo = min(lo, s_lo[w]);
-      hi = max(hi, s_hi[w]);
+      lo = min(lo, s.lo[w]);
+      hi = max(hi, s.hi[w]);
     }
     // digits of hi - key, so that larger keys come first
     const int bits = 32 - __clz((int)((hi - lo) | 1u));
@@ -312,11 +501,11 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SmArgs a) {
       const int width = min(10, shift), next = shift - width;
       const uint32_t mask = (1u << width) - 1;
       __syncthreads();
-      hist[t] = 0;
+      s.hist[t] = 0;
       __syncthreads();
       auto add = [&](uint32_t key, uint64_t m) {
         const uint32_t off = hi - key;
-        if (shift == bits || off >> shift == prefix) atomicAdd(&hist[(off >> next) & mask], (unsigned long long)m);
+        if (shift == bits || off >> shift == prefix) atomicAdd(&s.hist[(off >> next) & mask], (unsigned long long)m);
       };
       over([&](uint32_t key) {
         if (key > k0 && key >= lo && key <= hi) {
@@ -326,7 +515,7 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SmArgs a) {
       });
       if (t == 0 && t0 && k0 >= lo && k0 <= hi) add(k0, t0 * (by_weight ? weight(sm_logit(k0)) : 1));
       __syncthreads();
-      const uint32_t d = find_bin(hist[t], base, need, base);
+      const uint32_t d = find_bin(s.hist[t], base, need, base);
       prefix = (prefix << width) | d;
       shift = next;
     }
@@ -336,197 +525,47 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SmArgs a) {
     uint64_t equal = 0;
     over([&](uint32_t key) { equal += key == kk; });
     ties_left = block_sum(equal) - ties;
-  };
-
-  const float scale = best > low ? (float)(kSmBins - 2) / (best - low) : 1.f;
-  auto bin_of = [&](float l) -> int { return l == best ? 0 : (int)fminf((best - l) * scale, (float)(kSmBins - 1)); };
-  // Tokens of bins [b0, b1] to the list; false if they are too many.
-  int nlist = 0;
-  auto collect = [&](int b0, int b1, uint32_t room = kSmList) -> bool {
-    __syncthreads();
-    if (t == 0) s_count = 0;
-    __syncthreads();
-    each([&](int e, const float (&x)[4]) {
-      bool in[4];
-      int n_in = 0;
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int b = bin_of(x[q]);
-        in[q] = e + q < w_end && b >= b0 && b <= b1;
-        n_in += in[q];
-      }
-      if (n_in) {
-        uint32_t at = atomicAdd(&s_count, (uint32_t)n_in);
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-          if (in[q]) {
-            if (at < kSmList) {
-              list_key[at] = sm_key(x[q]);
-              list_idx[at] = e + q;
-            }
-            ++at;
-          }
-      }
-    });
-    __syncthreads();
-    nlist = (int)min(s_count, (uint32_t)kSmList);
-    return s_count <= room;
-  };
-  auto over_list = [&](auto f) {
-    for (int e = t; e < nlist; e += kSmThreads) f(list_key[e]);
-  };
-  auto over_row = [&](auto f) {
-    each([&](int e, const float (&x)[4]) {
-#pragma unroll
-      for (int q = 0; q < 4; ++q)
-        if (e + q < w_end) f(sm_key(x[q]));
-    });
-  };
-
-  auto need_of = [&](uint64_t s) -> uint64_t {  // the weight that top-p asks of s, at least the least
-    bool rest;
-    const uint64_t need = sm_mul_frac(s, p > 0.f ? p : 0.f, rest);
-    return rest || need == 0 ? need + 1 : need;
-  };
-  bool all_listed = false;  // every kept token is in the list
-  int last_tie = 0x7fffffff;  // ties are kept up to this index
-  bool selected = !has_k && !has_p;
-
-  // the list of the first tokens, sorted, and the kept ones in it: of the k first
-  // (k > 0, else of all), those that reach need(weight of these)
-  auto from_list = [&](int kept_of, auto need) {
-    // larger keys first, lower indexes first among equals; nothing behind the list
-    uint64_t v = t < nlist ? ((uint64_t)list_key[t] << 32) | (uint32_t)~list_idx[t] : 0;
-    unsigned long long* swap = hist;
-#pragma unroll
-    for (int size = 2; size <= kSmSort; size <<= 1) {
-#pragma unroll
-      for (int step = size >> 1; step > 0; step >>= 1) {
-        uint64_t o;
-        if (step < 64) {
-          o = sm_shfl_xor(v, step);
-        } else {
-          __syncthreads();
-          swap[t] = v;
-          __syncthreads();
-          o = swap[t ^ step];
-        }
-        const bool first = (t & step) == 0, falling = (t & size) == 0;
-        v = (first == falling) == (v > o) ? v : o;
-      }
-    }
-    __syncthreads();
-    swap[t] = v;
-    const uint64_t w = t < nlist ? weight(sm_logit((uint32_t)(v >> 32))) : 0;
-    const uint64_t before = block_scan(w);
-    if (t == kept_of - 1) s_u64 = before + w;
-    __syncthreads();
-    int n_kept = kept_of;
-    if (has_p) {
-      const uint64_t least = need((uint64_t)s_u64);
-      if (before < least && before + w >= least) s_u32 = t;
-      __syncthreads();
-      n_kept = (int)s_u32 + 1;
-    }
-    const uint64_t last = swap[n_kept - 1];
-    kk = (uint32_t)(last >> 32);
-    last_tie = (int)~(uint32_t)last;
-    all_listed = selected = true;
-  };
-  if (has_k && (V <= kSmSort || k <= min(kSmGuess, V / 4))) {  // V / 4 threads, or 960, hold logits
-    uint32_t b = kSmBins - 1;
-    if (V > kSmSort) {
-      hist[t] = 0;
-      __syncthreads();
-      if (first_of(0) < w_end) atomicAdd(&hist[bin_of(mine)], 1ull);
-      __syncthreads();
-      uint64_t before;
-      b = find_bin(hist[t], 0, (uint64_t)k, before);
-    }
-    if (collect(0, b, kSmSort)) from_list(k, need_of);
   }
-  if (has_k && !selected) {
-    hist[t] = 0;
-    __syncthreads();
-    each([&](int e, const float (&x)[4]) {
-#pragma unroll
-      for (int q = 0; q < 4; ++q)
-        if (e + q < w_end) atomicAdd(&hist[bin_of(x[q])], 1ull);
-    });
-    __syncthreads();
-    uint64_t before;
-    const uint32_t b = find_bin(hist[t], 0, (uint64_t)k, before);
-    const uint64_t upto = before + hist[b];
-    all_listed = upto <= kSmList;
-    if (all_listed) {
-      collect(0, b);
-      refine(over_list, 0, (uint64_t)k, false);
-    } else if (collect(b, b)) {
-      refine(over_list, before, (uint64_t)k, false);
-    } else {
-      refine(over_row, 0, (uint64_t)k, false);
-    }
+  __device__ __forceinline__ void refine_list(uint64_t base, uint64_t need, bool by_weight) {
+    refine([&](auto f) { over_list(f); }, base, need, by_weight);
+    ties_listed = true;
   }
-  auto kept_sum = [&](auto over) -> uint64_t {
-    uint64_t s = 0;
-    over([&](uint32_t key) {
-      if (key > kk) s += weight(sm_logit(key));
+  __device__ __forceinline__ void refine_row(uint64_t need, bool by_weight) {
+    refine([&](auto f) { over_row(f); }, 0, need, by_weight);
+    ties_listed = false;
+  }
+  __device__ __forceinline__ uint64_t list_sum() {  // weight of the kept tokens, all of them listed
+    uint64_t sum = 0;
+    over_list([&](uint32_t key) {
+      if (key > kk) sum += weight(sm_logit(key));
     });
-    s = block_sum(s);
-    return ties ? s + ties * weight(sm_logit(kk)) : s;
-  };
-  if (has_p && !selected) {
-    if (all_listed) {
-      refine(over_list, 0, need_of(kept_sum(over_list)), true);
-    } else {
-      const uint32_t k0 = kk;
-      const uint64_t t0 = ties;
-      __syncthreads();
-      hist[t] = 0;
-      __syncthreads();
-      each([&](int, const float (&x)[4]) {
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const uint64_t w = weight(x[q]);
-          if (w && sm_key(x[q]) > k0) atomicAdd(&hist[bin_of(x[q])], (unsigned long long)w);
-        }
-      });
-      if (t == 0 && t0) atomicAdd(&hist[bin_of(sm_logit(k0))], (unsigned long long)(t0 * weight(sm_logit(k0))));
-      __syncthreads();
-      const uint64_t own = hist[t];
-      const uint64_t need = need_of(block_sum(own));
-      uint64_t before;
-      const uint32_t b = find_bin(own, 0, need, before);
-      uint64_t upto = 0;
-      each([&](int e, const float (&x)[4]) {
-#pragma unroll
-        for (int q = 0; q < 4; ++q) upto += e + q < w_end && bin_of(x[q]) <= (int)b;
-      });
-      if (!has_k && block_sum(upto) <= kSmSort) {
-        collect(0, b, kSmSort);
-        from_list(nlist, [&](uint64_t) { return need; });
-      } else if (collect(b, b)) {
-        refine(over_list, before, need, true);
-      } else {
-        refine(over_row, 0, need, true);
-      }
+    sum = block_sum(sum);
+    return ties ? sum + ties * weight(sm_logit(kk)) : sum;
+  }
+  // The index of the last kept tie, from a list that holds all of them.
+  __device__ __forceinline__ void last_listed_tie() {
+    int lo = 0, hi = V - 1;
+    while (lo < hi) {  // uniform: the least index up to which there are enough
+      const int mid = (lo + hi) >> 1;
+      uint64_t n = 0;
+      for (int e = t; e < nlist; e += kSmThreads) n += s.list_key[e] == kk && (int)s.list_idx[e] <= mid;
+      if (block_sum(n) >= ties) hi = mid;
+      else lo = mid + 1;
     }
+    last_tie = lo;
   }
 
+  // --- the token ---------------------------------------------------------------
   // Lowest index of [from, to), in steps of 256 that seg has the sums of, whose
   // running sum of measure(index, logit), from base on, exceeds target.
-  auto find_in = [&](int from, int to, uint64_t base, uint64_t target, auto measure) -> int {
+  template <typename M>
+  __device__ __forceinline__ int find_in(int from, int to, uint64_t base, uint64_t target, M measure) {
     __syncthreads();
     if (wave == 0) {
       const int ns = (to - from + 255) / 256;
       for (int s0 = 0; s0 < ns; s0 += 64) {
-        const uint64_t own = s0 + lane < ns ? (uint64_t)seg[s0 + lane] : 0;
-        uint64_t inc = own;
-#pragma unroll
-        for (int m = 1; m < 64; m <<= 1) {
-          const uint64_t o = sm_shfl_up(inc, m);
-          if (lane >= m) inc += o;
-        }
+        const uint64_t own = s0 + lane < ns ? (uint64_t)s.seg[s0 + lane] : 0;
+        const uint64_t inc = wave_scan(own);
         const uint64_t run = base + inc - own;
         const uint64_t hit = __ballot(run <= target && run + own > target);
         if (hit) {
@@ -540,17 +579,11 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SmArgs a) {
             v[q] = e + q < to ? measure(e + q, row[e + q]) : 0;
             sum += v[q];
           }
-          uint64_t in2 = sum;
-#pragma unroll
-          for (int m = 1; m < 64; m <<= 1) {
-            const uint64_t o = sm_shfl_up(in2, m);
-            if (lane >= m) in2 += o;
-          }
-          uint64_t r2 = at + in2 - sum;
+          uint64_t r2 = at + wave_scan(sum) - sum;
           if (r2 <= target && r2 + sum > target) {
             int q = 0;
             while (q < 3 && r2 + v[q] <= target) r2 += v[q++];
-            s_u32 = (uint32_t)(e + q);
+            s.u32 = (uint32_t)(e + q);
           }
           break;
         }
@@ -558,88 +591,357 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SmArgs a) {
       }
     }
     __syncthreads();
-    return (int)s_u32;
-  };
-  // The same over the row, for the target that goal(sum over the row) gives: the
-  // waves' sums say whose share it is in, the workgroup adds up that share's steps.
-  auto find = [&](auto measure, auto goal) -> int {
-    uint64_t sum = 0;
-    each([&](int e, const float (&x)[4]) {
-#pragma unroll
-      for (int q = 0; q < 4; ++q) sum += e + q < w_end ? measure(e + q, x[q]) : 0;
-    });
-    const uint64_t target = goal(block_sum(sum));
-    uint64_t base = 0, upto = 0;
-    int w = -1;
-    do {  // at most 16 waves; their sums exceed target
-      base = upto;
-      upto += s_sum[++w];
-    } while (upto <= target && w < kSmWaves - 1);
-    const int from = w * per_wave, to = min(from + per_wave, V);
+    return (int)s.u32;
+  }
+  // The same over one share [from, to), whose steps the workgroup adds up first.
+  template <typename M>
+  __device__ __forceinline__ int find_share(int from, int to, uint64_t base, uint64_t target, M measure) {
     for (int c = wave; c * 256 < to - from; c += kSmWaves) {
       const int e = from + 256 * c + 4 * lane;
       uint64_t v = 0;
 #pragma unroll
       for (int q = 0; q < 4; ++q) v += e + q < to ? measure(e + q, row[e + q]) : 0;
       v = sm_wave_sum(v);
-      if (lane == 0) seg[c] = v;
+      if (lane == 0) s.seg[c] = v;
     }
     return find_in(from, to, base, target, measure);
-  };
-  if (ties && ties_left) {
-    const uint64_t nth = ties - 1;
-    last_tie = find([&](int, float l) -> uint64_t { return sm_key(l) == kk ? 1 : 0; }, [&](uint64_t) { return nth; });
-    __syncthreads();
   }
-  auto kept = [&](int e, float l) -> uint64_t {
-    const uint32_t key = sm_key(l);
-    if (!(key > kk || (key == kk && e <= last_tie))) return 0;
-    const uint64_t w = weight(l);
-    return w >= wmin ? w : 0;
-  };
-  auto goal = [&](uint64_t total) -> uint64_t {
-    bool rest;
-    return sm_mul_frac(total, u, rest);
-  };
-  int id;
-  if (all_listed) {
+  template <typename M>
+  __device__ __forceinline__ uint64_t own_sum(M measure) {  // the thread's
+    uint64_t sum = 0;
+    each([&](int e, const float (&x)[4]) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) sum += e + q < w_end ? measure(e + q, x[q]) : 0;
+    });
+    return sum;
+  }
+  // The same over the row, for the target that aim(sum over the row) gives: the waves'
+  // sums say whose share it is in.
+  template <typename M, typename A>
+  __device__ __forceinline__ int find(M measure, A aim) {
+    const uint64_t target = aim(block_sum(own_sum(measure)));
+    uint64_t base = 0, upto = 0;
+    int w = -1;
+    do {  // at most 16 waves; their sums exceed target
+      base = upto;
+      upto += s.sum[++w];
+    } while (upto <= target && w < kSmWaves - 1);
+    const int from = begin + w * per_wave;
+    return find_share(from, min(from + per_wave, end), base, target, measure);
+  }
+  __device__ __forceinline__ int listed_token() {  // every kept token is in the list
     const int ns = (V + 255) / 256;
     __syncthreads();
-    for (int e = t; e < ns; e += kSmThreads) seg[e] = 0;
+    for (int e = t; e < ns; e += kSmThreads) s.seg[e] = 0;
     __syncthreads();
     uint64_t sum = 0;
     for (int e = t; e < nlist; e += kSmThreads) {
-      const uint64_t w = kept((int)list_idx[e], sm_logit(list_key[e]));
+      const uint64_t w = kept((int)s.list_idx[e], sm_logit(s.list_key[e]));
       sum += w;
-      if (w) atomicAdd(&seg[list_idx[e] >> 8], (unsigned long long)w);
+      if (w) atomicAdd(&s.seg[s.list_idx[e] >> 8], (unsigned long long)w);
     }
-    id = find_in(0, V, 0, goal(block_sum(sum)), kept);
-  } else {
-    id = find(kept, goal);
+    const uint64_t total = block_sum(sum);
+    return find_in(0, V, 0, goal(total), [&](int e, float l) { return kept(e, l); });
   }
-  if (t == 0) argmax_finish(i, id, a.out, a.ring, a.ring_rows, a.ring_len, a.expect, a.accept);
+  // A list that holds the first k tokens and whatever else: top-k, top-p and the token.
+  __device__ __forceinline__ int token_of_list() {
+    if (nlist <= kSmSort) {
+      cut_list(k, [&](uint64_t sum) { return need_of(sum); });
+    } else {
+      refine_list(0, (uint64_t)k, false);
+      if (has_p) refine_list(0, need_of(list_sum()), true);
+      if (ties_left) last_listed_tie();
+    }
+    return listed_token();
+  }
+
+  // The row's token, by this workgroup alone; largest() and parameters() came before.
+  __device__ __forceinline__ int token() {
+    bool all_listed = false;
+    if (has_k) {
+      // V / 4 threads, or 960 of the 1024, hold logits
+      if (V <= kSmSort || k <= min(kSmGuess, V / 4)) {
+        const int b = V <= kSmSort ? kSmBins - 1 : guess_bin((uint64_t)k);
+        if (collect(0, b, kSmSort)) return token_of_list();
+      }
+      __syncthreads();
+      s.hist[t] = 0;
+      __syncthreads();
+      each([&](int e, const float (&x)[4]) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          if (e + q < w_end) atomicAdd(&s.hist[bin_of(x[q])], 1ull);
+      });
+      __syncthreads();
+      uint64_t before;
+      const uint32_t b = find_bin(s.hist[t], 0, (uint64_t)k, before);
+      const uint64_t upto = before + s.hist[b];
+      if (upto <= LIST) {
+        collect(0, b, LIST);
+        return token_of_list();
+      }
+      if (collect(b, b, LIST)) refine_list(before, (uint64_t)k, false);
+      else refine_row((uint64_t)k, false);
+    }
+    if (has_p) {
+      const uint64_t own = weigh_bins(s.hist);
+      const uint64_t need = need_of(block_sum(own));
+      uint64_t before;
+      const int b = (int)find_bin(own, 0, need, before);
+      uint64_t upto = 0;
+      each([&](int e, const float (&x)[4]) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) upto += e + q < w_end && bin_of(x[q]) <= b;
+      });
+      if (!has_k && block_sum(upto) <= kSmSort) {
+        collect(0, b, kSmSort);
+        cut_list(nlist, [&](uint64_t) { return need; });
+        all_listed = true;
+      } else if (collect(b, b, LIST)) {
+        refine_list(before, need, true);
+      } else {
+        refine_row(need, true);
+      }
+    }
+    if (all_listed) return listed_token();
+    if (ties && ties_left) {
+      if (ties_listed) {
+        last_listed_tie();
+      } else {
+        const uint64_t nth = ties - 1;
+        last_tie = find([&](int, float l) -> uint64_t { return sm_key(l) == kk ? 1 : 0; },
+                        [&](uint64_t) { return nth; });
+        __syncthreads();
+      }
+    }
+    return find([&](int e, float l) { return kept(e, l); }, [&](uint64_t sum) { return goal(sum); });
+  }
+  // The kept tokens' weights by bin, in LDS; the thread's bin.
+  __device__ __forceinline__ uint64_t weigh_bins(unsigned long long* hist) {
+    const uint32_t k0 = kk;
+    __syncthreads();
+    hist[t] = 0;
+    __syncthreads();
+    each([&](int, const float (&x)[4]) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const uint64_t w = weight(x[q]);
+        if (w && sm_key(x[q]) > k0) atomicAdd(&hist[bin_of(x[q])], (unsigned long long)w);
+      }
+    });
+    if (t == 0 && ties) atomicAdd(&hist[bin_of(sm_logit(k0))], (unsigned long long)(ties * weight(sm_logit(k0))));
+    __syncthreads();
+    return hist[t];
+  }
+  __device__ __forceinline__ void finish(int id) {
+    if (t == 0) argmax_finish(i, id, a.out, a.ring, a.ring_rows, a.ring_len, a.expect, a.accept);
+  }
+};
+
+template <int CAP>
+__global__ __launch_bounds__(kSmThreads) void sample_kernel(SmArgs a) {
+  __shared__ __align__(16) SmShared<CAP, 2048> sh;
+  Sm<CAP, 2048> m(a, sh, blockIdx.x, 0, a.V);
+  m.largest();
+  m.finish(m.parameters() ? m.token() : m.first_best());
+}
+
+// --- long rows: grid (slab, row) but for the last ------------------------------
+using SmSlab = Sm<0, 2048>;
+using SmSlabShared = SmShared<0, 2048>;
+
+__global__ __launch_bounds__(kSmThreads) void sample_largest_kernel(SmArgs a, SmRowWs* wss) {
+  __shared__ __align__(16) SmSlabShared sh;
+  const int slab = blockIdx.x;
+  SmSlab m(a, sh, blockIdx.y, slab * kSmSlab, min((slab + 1) * kSmSlab, a.V));
+  SmRowWs& ws = wss[blockIdx.y];
+  m.largest();
+  if (m.t == 0) {
+    ws.max[slab] = m.best;
+    ws.min[slab] = m.low;
+    ws.nan[slab] = m.nan;
+  }
+  if (slab == 0) {
+    ws.hist[m.t] = 0;
+    if (m.t == 0) ws.count = 0;
+  }
+}
+
+// What the row's workgroup can do with the slabs' lists.
+__device__ __forceinline__ bool sm_listed(const SmSlab& m) { return m.has_k && m.k <= kSmGuess; }
+
+__device__ __forceinline__ void sm_append(SmSlab& m, SmRowWs& ws) {  // the slab's list to the row's
+  const uint32_t n = m.s.count;
+  if (m.t == 0) m.s.u32 = atomicAdd(&ws.count, n <= 2048 ? n : kSmRowList + 1);
+  __syncthreads();
+  const uint32_t at = m.s.u32;
+  for (uint32_t e = m.t; e < (uint32_t)m.nlist && at + e < kSmRowList; e += kSmThreads) {
+    ws.key[at + e] = m.s.list_key[e];
+    ws.idx[at + e] = m.s.list_idx[e];
+  }
+}
+
+// With top-k, the tokens that may be among the first k: each slab's first k and a few.
+// With top-p alone, the weights by bin.
+__global__ __launch_bounds__(kSmThreads) void sample_bins_kernel(SmArgs a, SmRowWs* wss) {
+  __shared__ __align__(16) SmSlabShared sh;
+  const int slab = blockIdx.x;
+  SmSlab m(a, sh, blockIdx.y, slab * kSmSlab, min((slab + 1) * kSmSlab, a.V));
+  SmRowWs& ws = wss[blockIdx.y];
+  m.largest_of(ws, gridDim.x);
+  if (!m.parameters()) return;
+  __syncthreads();  // the table
+  if (sm_listed(m)) {
+    m.mine = -INFINITY;
+    m.each([&](int, const float (&x)[4]) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) m.mine = fmaxf(m.mine, x[q]);
+    });
+    const int len = m.end - m.begin;
+    const int b = len <= kSmSort || m.k > min(kSmGuess, len / 4) ? kSmBins - 1 : m.guess_bin((uint64_t)m.k);
+    m.collect(0, b, 2048);
+    sm_append(m, ws);
+  } else if (m.has_p && !m.has_k) {
+    const uint64_t own = m.weigh_bins(sh.hist);
+    if (own) atomicAdd(&ws.hist[m.t], (unsigned long long)own);
+  }
+}
+
+// With top-p alone: the tokens of the border's bin.
+__global__ __launch_bounds__(kSmThreads) void sample_border_kernel(SmArgs a, SmRowWs* wss) {
+  __shared__ __align__(16) SmSlabShared sh;
+  const int slab = blockIdx.x;
+  SmSlab m(a, sh, blockIdx.y, slab * kSmSlab, min((slab + 1) * kSmSlab, a.V));
+  SmRowWs& ws = wss[blockIdx.y];
+  m.largest_of(ws, gridDim.x);
+  if (!m.parameters() || !m.has_p || m.has_k) return;
+  const uint64_t own = ws.hist[m.t];
+  const uint64_t need = m.need_of(m.block_sum(own));
+  uint64_t before;
+  const int b = (int)m.find_bin(own, 0, need, before);
+  m.collect(b, b, 2048);
+  sm_append(m, ws);
+}
+
+// Without top-k: the border, which every slab finds from the same list, and the kept
+// weight of each wave's share.
+__global__ __launch_bounds__(kSmThreads) void sample_shares_kernel(SmArgs a, SmRowWs* wss) {
+  __shared__ __align__(16) SmShared<0, kSmRowList> sh;
+  const int slab = blockIdx.x;
+  Sm<0, kSmRowList> m(a, sh, blockIdx.y, slab * kSmSlab, min((slab + 1) * kSmSlab, a.V));
+  SmRowWs& ws = wss[blockIdx.y];
+  m.largest_of(ws, gridDim.x);
+  if (!m.parameters() || m.has_k) return;
+  __syncthreads();  // the table
+  if (m.has_p) {
+    if (ws.count > kSmRowList) return;
+    m.nlist = (int)ws.count;
+    for (int e = m.t; e < m.nlist; e += kSmThreads) {
+      sh.list_key[e] = ws.key[e];
+      sh.list_idx[e] = ws.idx[e];
+    }
+    const uint64_t own = ws.hist[m.t];
+    const uint64_t need = m.need_of(m.block_sum(own));
+    uint64_t before;
+    m.find_bin(own, 0, need, before);
+    m.refine_list(before, need, true);
+    if (m.ties_left) m.last_listed_tie();
+    if (slab == 0 && m.t == 0) {
+      ws.kk = m.kk;
+      ws.last_tie = m.last_tie;
+    }
+  }
+  const uint64_t sum = sm_wave_sum(m.own_sum([&](int e, float l) { return m.kept(e, l); }));
+  if (m.lane == 0) ws.share[slab * kSmWaves + m.wave] = sum;
+}
+
+__global__ __launch_bounds__(kSmThreads) void sample_row_kernel(SmArgs a, SmRowWs* wss, int slabs) {
+  __shared__ __align__(16) SmShared<0, kSmRowList> sh;
+  SmRowWs& ws = wss[blockIdx.x];
+  Sm<0, kSmRowList> m(a, sh, blockIdx.x, 0, a.V);
+  m.largest_of(ws, slabs);
+  __syncthreads();  // the table
+  if (!m.parameters()) {  // the first slab that has it
+    const bool has = m.lane < slabs && (m.nan ? ws.nan[min(m.lane, slabs - 1)] != 0 : ws.max[min(m.lane, slabs - 1)] == m.best);
+    const int slab = __builtin_ctzll(__ballot(has));
+    Sm<0, kSmRowList> one(a, sh, blockIdx.x, slab * kSmSlab, min((slab + 1) * kSmSlab, a.V));
+    one.best = m.best;
+    one.nan = m.nan;
+    m.finish(one.first_best());
+    return;
+  }
+  const bool listed = m.has_k && m.k <= kSmGuess;
+  if ((listed || (m.has_p && !m.has_k)) ? ws.count > kSmRowList : m.has_k) {  // not prepared
+    m.largest();
+    m.finish(m.token());
+    return;
+  }
+  if (listed) {
+    m.nlist = (int)ws.count;
+    for (int e = m.t; e < m.nlist; e += kSmThreads) {
+      sh.list_key[e] = ws.key[e];
+      sh.list_idx[e] = ws.idx[e];
+    }
+    __syncthreads();
+    m.finish(m.token_of_list());
+    return;
+  }
+  if (m.has_p) {
+    m.kk = ws.kk;
+    m.last_tie = ws.last_tie;
+  }
+  // whose share the token is in: at most 1024 of them, one a thread
+  const uint64_t own = m.t < slabs * kSmWaves ? (uint64_t)ws.share[m.t] : 0;
+  const uint64_t target = m.goal(m.block_sum(own));
+  const uint64_t before = m.block_scan(own);
+  if (before <= target && before + own > target) {
+    sh.u32 = m.t;
+    sh.u64 = before;
+  }
+  __syncthreads();
+  const int slab = (int)sh.u32 / kSmWaves, w = (int)sh.u32 % kSmWaves;
+  const uint64_t base = sh.u64;
+  const int lo = slab * kSmSlab, hi = min(lo + kSmSlab, a.V), per_wave = (hi - lo + 63) / 64 * 4;
+  const int from = lo + w * per_wave;
+  __syncthreads();
+  m.finish(m.find_share(from, min(from + per_wave, hi), base, target, [&](int e, float l) { return m.kept(e, l); }));
 }
 
 }  // namespace wfd
 
 extern "C" {
 
+size_t wfd_sample_workspace_bytes(int n, int vocab) {
+  return n <= 0 || vocab <= wfd::kSmLong || vocab > wfd::kSmMaxVocab ? 0 : (size_t)n * sizeof(wfd::SmRowWs);
+}
+
 int wfd_sample(const float* logits, int64_t ld, const float* u, const float* temperature, const int32_t* top_k,
                const float* top_p, const float* min_p, int64_t* out, int64_t* ring, const int32_t* ring_rows,
-               int64_t ring_len, const int64_t* expect, int32_t* accept, int n, int vocab, hipStream_t stream) {
+               int64_t ring_len, const int64_t* expect, int32_t* accept, int n, int vocab, void* workspace,
+               size_t ws_bytes, hipStream_t stream) {
   using namespace wfd;
   if (n < 0 || vocab <= 0 || ld < vocab) {
     set_error("wfd_sample: bad shape n=%d vocab=%d ld=%lld", n, vocab, (long long)ld);
     return kBadArg;
   }
-  if (vocab > kSmMaxVocab) {
-    set_error("wfd_sample: vocab=%d (at most %d)", vocab, kSmMaxVocab);
+  if (vocab > kSmMaxVocab || n > 65535) {
+    set_error("wfd_sample: vocab=%d n=%d (at most %d and 65535)", vocab, n, kSmMaxVocab);
     return kUnsupported;
   }
   if (n == 0) return kOk;
-  if (!logits || !u || !out || (ring && (!ring_rows || ring_len <= 0)) || (!expect != !accept)) {
+  const size_t need = wfd_sample_workspace_bytes(n, vocab);
+  if (!logits || !u || !out || (ring && (!ring_rows || ring_len <= 0)) || (!expect != !accept) ||
+      (need && !workspace)) {
     set_error("wfd_sample: null pointer argument (ring needs ring_rows and a length; expect and accept go together)");
     return kBadArg;
+  }
+  if (need && ((uintptr_t)workspace & 15)) {
+    set_error("wfd_sample: workspace must be 16-byte aligned");
+    return kBadArg;
+  }
+  if (ws_bytes < need) {
+    set_error("wfd_sample: workspace %zu bytes < required %zu", ws_bytes, need);
+    return kWorkspace;
   }
   SmArgs a;
   a.logits = logits;
@@ -656,12 +958,21 @@ int wfd_sample(const float* logits, int64_t ld, const float* u, const float* tem
   a.expect = expect;
   a.accept = accept;
   a.V = vocab;
-  if (vocab <= 2 * kSmChunk)
-    hipLaunchKernelGGL(sample_kernel<2 * kSmChunk>, dim3(n), dim3(kSmThreads), 0, stream, a);
-  else if (vocab <= 8 * kSmChunk)
-    hipLaunchKernelGGL(sample_kernel<8 * kSmChunk>, dim3(n), dim3(kSmThreads), 0, stream, a);
-  else
-    hipLaunchKernelGGL(sample_kernel<0>, dim3(n), dim3(kSmThreads), 0, stream, a);
+  const dim3 block(kSmThreads);
+  if (vocab <= 2 * kSmChunk) {
+    hipLaunchKernelGGL(sample_kernel<2 * kSmChunk>, dim3(n), block, 0, stream, a);
+  } else if (vocab <= kSmLong) {
+    hipLaunchKernelGGL(sample_kernel<kSmLong>, dim3(n), block, 0, stream, a);
+  } else {
+    SmRowWs* ws = (SmRowWs*)workspace;
+    const int slabs = (vocab + kSmSlab - 1) / kSmSlab;
+    const dim3 grid(slabs, n);
+    hipLaunchKernelGGL(sample_largest_kernel, grid, block, 0, stream, a, ws);
+    hipLaunchKernelGGL(sample_bins_kernel, grid, block, 0, stream, a, ws);
+    if (top_p) hipLaunchKernelGGL(sample_border_kernel, grid, block, 0, stream, a, ws);
+    hipLaunchKernelGGL(sample_shares_kernel, grid, block, 0, stream, a, ws);
+    hipLaunchKernelGGL(sample_row_kernel, dim3(n), block, 0, stream, a, ws, slabs);
+  }
   return launch_status("wfd_sample");
 }
 

@@ -15,6 +15,7 @@ back, so the caller guarantees they index inside the buffers passed.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 import threading
 from collections import OrderedDict
@@ -301,8 +302,7 @@ def attn_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, p
     _need(out.shape == q.shape and out.dtype == q.dtype and out.is_contiguous(), "bad out")
     dt, lib = _dt(q), _lib.load()
     if workspace is None:
-        workspace = _workspace(lib.wfd_attn_shared_workspace_bytes(n, H, Hkv, Dh, prefix_len_max, kv_len_max),
-                               q.device)
+        workspace = _workspace(attn_shared_workspace_bytes(n, H, Hkv, Dh, prefix_len_max, kv_len_max), q.device)
     sc = 1.0 / math.sqrt(Dh) if scale is None else float(scale)
     rc = lib.wfd_attn_shared(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), br, prefix_row_base.data_ptr(),
                              prefix_len.data_ptr(), group_first.data_ptr(), ng, group_max, kv_row_base.data_ptr(),
@@ -313,6 +313,7 @@ def attn_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, p
     return out
 
 
+@functools.lru_cache(maxsize=1024)
 def attn_shared_workspace_bytes(n: int, H: int, Hkv: int, Dh: int, prefix_len_max: int, kv_len_max: int) -> int:
     return int(_lib.load().wfd_attn_shared_workspace_bytes(n, H, Hkv, Dh, prefix_len_max, kv_len_max))
 
@@ -921,13 +922,14 @@ def sample(logits: torch.Tensor, u: torch.Tensor, *, temperature: torch.Tensor |
            top_k: torch.Tensor | None = None, top_p: torch.Tensor | None = None, min_p: torch.Tensor | None = None,
            n: int | None = None, out: torch.Tensor | None = None, ring: torch.Tensor | None = None,
            ring_rows: torch.Tensor | None = None, expect: torch.Tensor | None = None,
-           accept: torch.Tensor | None = None, accept_mapped: tuple[int, int] | None = None) -> torch.Tensor:
+           accept: torch.Tensor | None = None, accept_mapped: tuple[int, int] | None = None,
+           workspace: torch.Tensor | None = None) -> torch.Tensor:
     """out[i] = the token drawn from logits[i] with the uniform number u[i]
     (wfd_sample has the definition): parameters per row, on the device
     (float32, top_k int32; None: off), temperature 0 greedy. The outputs are
     argmax's: with `ring`, ring[ring_rows[i]] = out[i]; with `expect`, accept
     flags of the drawn tokens."""
-    _need_current(logits, u, temperature, top_k, top_p, min_p, out, ring, ring_rows, expect, accept)
+    _need_current(logits, u, temperature, top_k, top_p, min_p, out, ring, ring_rows, expect, accept, workspace)
     _need(logits.dtype == torch.float32 and logits.dim() == 2 and logits.stride(1) == 1, "logits: float32 (n, V)")
     n = logits.shape[0] if n is None else n
     if not 0 <= n <= logits.shape[0]:
@@ -942,12 +944,22 @@ def sample(logits: torch.Tensor, u: torch.Tensor, *, temperature: torch.Tensor |
     if min_p is not None:
         _table("min_p", min_p, torch.float32, n)
     out, acc = _argmax_outputs(n, logits.device, out, ring, ring_rows, expect, accept, accept_mapped)
-    ld = logits.stride(0) if logits.shape[0] > 1 else logits.shape[1]
+    V = logits.shape[1]
+    ld = logits.stride(0) if logits.shape[0] > 1 else V
+    need = sample_workspace_bytes(n, V)
+    if workspace is None and need:
+        workspace = _workspace(need, logits.device)
     rc = _lib.load().wfd_sample(logits.data_ptr(), ld, u.data_ptr(), _p(temperature), _p(top_k), _p(top_p), _p(min_p),
                                 out.data_ptr(), _p(ring), _p(ring_rows), ring.numel() if ring is not None else 0,
-                                _p(expect), acc, n, logits.shape[1], _stream())
+                                _p(expect), acc, n, V, _p(workspace),
+                                0 if workspace is None else workspace.numel() * workspace.element_size(), _stream())
     _lib.check(rc, "wfd_sample")
     return out
+
+
+@functools.lru_cache(maxsize=1024)
+def sample_workspace_bytes(n: int, vocab: int) -> int:
+    return int(_lib.load().wfd_sample_workspace_bytes(n, vocab))
 
 
 def _argmax_outputs(n, device, out, ring, ring_rows, expect, accept, accept_mapped):
