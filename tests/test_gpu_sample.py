@@ -110,6 +110,19 @@ def test_bf16_logits_with_many_ties(gpu):
     check(gpu, logits, u, [0.7] * n, k, p)
 
 
+@pytest.mark.parametrize("V", [3000, 20000, 60000])
+def test_every_top_k_over_few_values(gpu, V):
+    """Every k around and between the ends of the runs of equal logits, to past a sorted list."""
+    g = torch.Generator().manual_seed(V)
+    row = (torch.randn(V, generator=g) * 2).bfloat16().float()
+    ends = torch.unique(row, return_counts=True)[1].flip(0).cumsum(0)
+    ends = ends[ends < 2500][::3].tolist()
+    k = sorted({e + d for e in ends for d in (-1, 0, 1) if e + d > 0})
+    rows = row.expand(len(k), V).contiguous()
+    check(gpu, rows, torch.rand(len(k), generator=g).tolist(), k=k)
+    check(gpu, rows, torch.rand(len(k), generator=g).tolist(), k=k, p=[0.9] * len(k))
+
+
 @pytest.mark.parametrize("V", [70, 9000, 33000])
 def test_masked_and_special_logits(gpu, V):
     g = torch.Generator().manual_seed(V)
@@ -133,6 +146,27 @@ def test_masked_and_special_logits(gpu, V):
         check(gpu, rows, us, t=[0.8] * 12, k=[4] * 12)
         check(gpu, rows, us, t=[1.3] * 12, p=[0.6] * 12)
         check(gpu, rows, us, p=[0.9] * 12, m=[0.3] * 12, k=[5] * 12)
+
+
+@pytest.mark.parametrize("V", [3000, 30000, 100000])
+@pytest.mark.parametrize("masked", [-INF, -1e9, -1e4])
+def test_whole_stretches_masked(gpu, V, masked):
+    """A grammar leaves a few tokens, far apart, of a row; fewer than top-k, or many."""
+    n = 24
+    g = torch.Generator().manual_seed(V)
+    rows = torch.randn(n, V, generator=g) * 2
+    for i in range(n):
+        left = [1, 3, 40, 900][i % 4]
+        keep = torch.randperm(V, generator=g)[:left] if i % 8 < 4 else torch.arange(V - left, V)
+        mask = torch.ones(V, dtype=torch.bool)
+        mask[keep] = False
+        rows[i, mask] = masked
+    u = torch.rand(n, generator=g).tolist()
+    for k in (5, 100, 500, 2000):
+        check(gpu, rows, u, k=[k] * n)
+        check(gpu, rows, u, [1.3] * n, [k] * n, [0.9] * n)
+    check(gpu, rows, u, p=[0.95] * n)
+    check(gpu, rows, u, [0.7] * n, m=[0.02] * n)
 
 
 def test_parameters_outside_their_ranges(gpu):

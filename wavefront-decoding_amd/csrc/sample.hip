@@ -254,6 +254,25 @@ struct Sm {
     return s.u32;
   }
 
+  __device__ __forceinline__ void block_range(uint32_t& lo, uint32_t& hi) {
+#pragma unroll
+    for (int m = 32; m >= 1; m >>= 1) {
+      lo = min(lo, (uint32_t)__shfl_xor((int)lo, m, 64));
+      hi = max(hi, (uint32_t)__shfl_xor((int)hi, m, 64));
+    }
+    __syncthreads();
+    if (lane == 0) {
+      s.lo[wave] = lo;
+      s.hi[wave] = hi;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kSmWaves; ++w) {
+      lo = min(lo, s.lo[w]);
+      hi = max(hi, s.hi[w]);
+    }
+  }
+
   // --- the row's largest logit, whether there is a NaN, the range of the bins --
   __device__ __forceinline__ void largest() {
     mine = -INFINITY;
@@ -369,8 +388,11 @@ struct Sm {
   }
 
   // --- the list ----------------------------------------------------------------
-  // Tokens of bins [b0, b1] to the list; false if they are more than room.
-  __device__ __forceinline__ bool collect(int b0, int b1, uint32_t room) {
+  // Tokens of bins [b0, b1] to the list; false if they are more than room. With
+  // `drawable`, without those whose weight is certainly 0 (masked ones, above all): they
+  // are never drawn, come last in the order and add to no sum.
+  __device__ __forceinline__ bool collect(int b0, int b1, uint32_t room, bool drawable) {
+    const float reach = drawable ? (float)inv : 0.f;
     __syncthreads();
     if (t == 0) s.count = 0;
     __syncthreads();
@@ -380,7 +402,7 @@ struct Sm {
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const int b = bin_of(x[q]);
-        in[q] = e + q < w_end && b >= b0 && b <= b1;
+        in[q] = e + q < w_end && b >= b0 && b <= b1 && !((best - x[q]) * reach > 47.f);
         n_in += in[q];
       }
       if (n_in) {
@@ -423,14 +445,9 @@ struct Sm {
         if (e + q < w_end) f(sm_key(x[q]));
     });
   }
-  // Sorts a list of at most kSmSort tokens and cuts it: of the n_kept first (all, without
-  // top-k) those whose weight reaches need(weight of these), with top-p.
-  template <typename N>
-  __device__ __forceinline__ void cut_list(int n_kept, N need) {
-    // larger keys first, lower indexes first among equals; nothing behind the list
-    __syncthreads();
-    uint64_t v = t < nlist ? ((uint64_t)s.list_key[t] << 32) | (uint32_t)~s.list_idx[t] : 0;
-    for (int size = 2; size < 2 * nlist; size <<= 1) {
+  // Values of threads t < n in falling order (n <= kSmSort; the others hold 0).
+  __device__ __forceinline__ uint64_t sorted(uint64_t v, int n) {
+    for (int size = 2; size < 2 * n; size <<= 1) {
       for (int step = size >> 1; step > 0; step >>= 1) {
         uint64_t o;
         if (step < 64) {
@@ -445,11 +462,20 @@ struct Sm {
         v = (first == falling) == (v > o) ? v : o;
       }
     }
+    return v;
+  }
+  // The token of a list of at most kSmSort: of its n_kept first (all of them, without
+  // top-k) those whose weight reaches need(weight of these), with top-p; of these the
+  // ones min_p leaves, by index.
+  template <typename N>
+  __device__ __forceinline__ int token_of_sorted(int n_kept, N need) {
     __syncthreads();
-    s.hist[t] = v;
-    const uint64_t w = t < nlist ? weight(sm_logit((uint32_t)(v >> 32))) : 0;
-    const uint64_t before = block_scan(w);
+    // larger keys first, lower indexes first among equals
+    const uint64_t v = sorted(t < nlist ? ((uint64_t)s.list_key[t] << 32) | (uint32_t)~s.list_idx[t] : 0, nlist);
+    const uint32_t key = (uint32_t)(v >> 32), idx = ~(uint32_t)v;
     if (has_p) {
+      const uint64_t w = t < nlist ? weight(sm_logit(key)) : 0;
+      const uint64_t before = block_scan(w);
       if (t == n_kept - 1) s.u64 = before + w;
       __syncthreads();
       const uint64_t least = need((uint64_t)s.u64);
@@ -457,10 +483,23 @@ struct Sm {
       __syncthreads();
       n_kept = (int)s.u32 + 1;
     }
-    const uint64_t last = s.hist[n_kept - 1];
-    kk = (uint32_t)(last >> 32);
-    last_tie = (int)~(uint32_t)last;
-    ties = 0;
+    if (V <= kSmLong) {  // the kept tokens' places among a hundred steps of the row
+      __syncthreads();
+      if (t == n_kept - 1) s.u64 = v;
+      __syncthreads();
+      kk = (uint32_t)(s.u64 >> 32);
+      last_tie = (int)~(uint32_t)s.u64;
+      ties = 0;
+      return listed_token();
+    }
+    const uint64_t by_index = sorted(t < n_kept ? ((uint64_t)~idx << 32) | key : 0, n_kept);
+    uint64_t w = t < n_kept ? weight(sm_logit((uint32_t)by_index)) : 0;
+    if (w < wmin) w = 0;
+    const uint64_t before = block_scan(w);
+    const uint64_t target = goal(block_sum(w));
+    if (before <= target && before + w > target) s.u32 = ~(uint32_t)(by_index >> 32);
+    __syncthreads();
+    return (int)s.u32;
   }
 
   // The shortest prefix of the kept tokens whose measure (1 or the weight), on top of
@@ -477,22 +516,7 @@ struct Sm {
         hi = max(hi, key);
       }
     });
-#pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) {
-      lo = min(lo, (uint32_t)__shfl_xor((int)lo, m, 64));
-      hi = max(hi, (uint32_t)__shfl_xor((int)hi, m, 64));
-    }
-    __syncthreads();
-    if (lane == 0) {
-      s.lo[wave] = lo;
-      s.hi[wave] = hi;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kSmWaves; ++w) {
-      lo = min(lo, s.lo[w]);
-      hi = max(hi, s.hi[w]);
-    }
+    block_range(lo, hi);
     // digits of hi - key, so that larger keys come first
     const int bits = 32 - __clz((int)((hi - lo) | 1u));
     int shift = bits;
@@ -643,26 +667,58 @@ struct Sm {
     const uint64_t total = block_sum(sum);
     return find_in(0, V, 0, goal(total), [&](int e, float l) { return kept(e, l); });
   }
-  // A list that holds the first k tokens and whatever else: top-k, top-p and the token.
-  __device__ __forceinline__ int token_of_list() {
-    if (nlist <= kSmSort) {
-      cut_list(k, [&](uint64_t sum) { return need_of(sum); });
-    } else {
-      refine_list(0, (uint64_t)k, false);
-      if (has_p) refine_list(0, need_of(list_sum()), true);
-      if (ties_left) last_listed_tie();
+  // Drops what no k-th token's bin reaches from a list that holds the first k tokens.
+  __device__ __forceinline__ void thin_list() {
+    __syncthreads();
+    s.hist[t] = 0;
+    __syncthreads();
+    uint32_t key[LIST / kSmThreads], idx[LIST / kSmThreads];
+#pragma unroll
+    for (int c = 0; c < LIST / kSmThreads; ++c) {
+      const int e = c * kSmThreads + t;
+      key[c] = e < nlist ? s.list_key[e] : 0;
+      idx[c] = e < nlist ? s.list_idx[e] : 0;
+      if (e < nlist) atomicAdd(&s.hist[bin_of(sm_logit(key[c]))], 1ull);
     }
+    if (t == 0) s.count = 0;
+    __syncthreads();
+    uint64_t before;
+    const int b = (int)find_bin(s.hist[t], 0, (uint64_t)k, before);
+#pragma unroll
+    for (int c = 0; c < LIST / kSmThreads; ++c)
+      if (c * kSmThreads + t < nlist && bin_of(sm_logit(key[c])) <= b) {
+        const uint32_t at = atomicAdd(&s.count, 1u);
+        s.list_key[at] = key[c];
+        s.list_idx[at] = idx[c];
+      }
+    __syncthreads();
+    nlist = (int)s.count;
+  }
+  // A list that holds the first k tokens, or all that can be drawn, and whatever else:
+  // top-k, top-p and the token.
+  __device__ __forceinline__ int token_of_list() {
+    if (nlist > kSmSort && nlist > k) thin_list();
+    if (nlist <= kSmSort) return token_of_sorted(min(k, nlist), [&](uint64_t sum) { return need_of(sum); });
+    if (nlist > k) {
+      refine_list(0, (uint64_t)k, false);
+    } else {  // all of the list, and nothing that is not in it
+      uint32_t lo = 0xffffffffu, hi = 0;
+      over_list([&](uint32_t key) { lo = min(lo, key); });
+      block_range(lo, hi);
+      kk = lo - 1;
+    }
+    if (has_p) refine_list(0, need_of(list_sum()), true);
+    if (ties_left) last_listed_tie();
     return listed_token();
   }
 
   // The row's token, by this workgroup alone; largest() and parameters() came before.
   __device__ __forceinline__ int token() {
-    bool all_listed = false;
     if (has_k) {
       // V / 4 threads, or 960 of the 1024, hold logits
       if (V <= kSmSort || k <= min(kSmGuess, V / 4)) {
         const int b = V <= kSmSort ? kSmBins - 1 : guess_bin((uint64_t)k);
-        if (collect(0, b, kSmSort)) return token_of_list();
+        if (collect(0, b, kSmSort, true)) return token_of_list();
       }
       __syncthreads();
       s.hist[t] = 0;
@@ -677,10 +733,10 @@ struct Sm {
       const uint32_t b = find_bin(s.hist[t], 0, (uint64_t)k, before);
       const uint64_t upto = before + s.hist[b];
       if (upto <= LIST) {
-        collect(0, b, LIST);
+        collect(0, b, LIST, true);
         return token_of_list();
       }
-      if (collect(b, b, LIST)) refine_list(before, (uint64_t)k, false);
+      if (collect(b, b, LIST, false)) refine_list(before, (uint64_t)k, false);
       else refine_row((uint64_t)k, false);
     }
     if (has_p) {
@@ -694,16 +750,14 @@ struct Sm {
         for (int q = 0; q < 4; ++q) upto += e + q < w_end && bin_of(x[q]) <= b;
       });
       if (!has_k && block_sum(upto) <= kSmSort) {
-        collect(0, b, kSmSort);
-        cut_list(nlist, [&](uint64_t) { return need; });
-        all_listed = true;
-      } else if (collect(b, b, LIST)) {
+        collect(0, b, kSmSort, true);
+        return token_of_sorted(nlist, [&](uint64_t) { return need; });
+      } else if (collect(b, b, LIST, true)) {
         refine_list(before, need, true);
       } else {
         refine_row(need, true);
       }
     }
-    if (all_listed) return listed_token();
     if (ties && ties_left) {
       if (ties_listed) {
         last_listed_tie();
@@ -799,7 +853,7 @@ __global__ __launch_bounds__(kSmThreads) void sample_bins_kernel(SmArgs a, SmRow
     });
     const int len = m.end - m.begin;
     const int b = len <= kSmSort || m.k > min(kSmGuess, len / 4) ? kSmBins - 1 : m.guess_bin((uint64_t)m.k);
-    m.collect(0, b, 2048);
+    m.collect(0, b, 2048, true);
     sm_append(m, ws);
   } else if (m.has_p && !m.has_k) {
     const uint64_t own = m.weigh_bins(sh.hist);
@@ -819,7 +873,7 @@ __global__ __launch_bounds__(kSmThreads) void sample_border_kernel(SmArgs a, SmR
   const uint64_t need = m.need_of(m.block_sum(own));
   uint64_t before;
   const int b = (int)m.find_bin(own, 0, need, before);
-  m.collect(b, b, 2048);
+  m.collect(b, b, 2048, true);
   sm_append(m, ws);
 }
 
@@ -968,7 +1022,7 @@ int wfd_sample(const float* logits, int64_t ld, const float* u, const float* tem
     const int slabs = (vocab + kSmSlab - 1) / kSmSlab;
     const dim3 grid(slabs, n);
     hipLaunchKernelGGL(sample_largest_kernel, grid, block, 0, stream, a, ws);
-    hipLaunchKernelGGL(sample_bins_kernel, grid, block, 0, stream, a, ws);
+    if (top_k || top_p) hipLaunchKernelGGL(sample_bins_kernel, grid, block, 0, stream, a, ws);
     if (top_p) hipLaunchKernelGGL(sample_border_kernel, grid, block, 0, stream, a, ws);
     hipLaunchKernelGGL(sample_shares_kernel, grid, block, 0, stream, a, ws);
     hipLaunchKernelGGL(sample_row_kernel, dim3(n), block, 0, stream, a, ws, slabs);
