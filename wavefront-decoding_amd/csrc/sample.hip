@@ -72,6 +72,7 @@ struct SmArgs {
 
 constexpr int kSmBins = 1024;   // one per thread
 constexpr int kSmSort = kSmThreads;  // entries of a list that is sorted
+constexpr int kSmCount = 256;        // and of one that is ordered by counting
 constexpr int kSmLong = 32768;       // longest row of one workgroup
 constexpr int kSmSlab = 8192;
 constexpr int kSmSlabs = kSmMaxVocab / kSmSlab;
@@ -393,16 +394,20 @@ struct Sm {
   // are never drawn, come last in the order and add to no sum.
   __device__ __forceinline__ bool collect(int b0, int b1, uint32_t room, bool drawable) {
     const float reach = drawable ? (float)inv : 0.f;
+    // bin_of's borders, on its own product: x in [b0, b1 + 1)
+    const float from = (float)b0, to = b1 >= kSmBins - 1 ? INFINITY : (float)(b1 + 1);
     __syncthreads();
     if (t == 0) s.count = 0;
     __syncthreads();
     each([&](int e, const float (&x)[4]) {
       bool in[4];
       int n_in = 0;
+      const int room_here = w_end - e;
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const int b = bin_of(x[q]);
-        in[q] = e + q < w_end && b >= b0 && b <= b1 && !((best - x[q]) * reach > 47.f);
+        const float d = best - x[q];
+        const float at = x[q] == best ? 0.f : d * scale;
+        in[q] = q < room_here && at >= from && (at < to || to == INFINITY) && !(d * reach > 47.f);
         n_in += in[q];
       }
       if (n_in) {
@@ -445,6 +450,27 @@ struct Sm {
         if (e + q < w_end) f(sm_key(x[q]));
     });
   }
+  // The list in falling order, one entry a thread (n <= kSmSort): larger keys first, lower
+  // indexes first among equals; 0 behind it. Up to kSmCount entries an entry's place is
+  // the number that come before it; 100 of them take 0.8 us so, 3.4 by the network.
+  __device__ __forceinline__ uint64_t sorted_list() {
+    const uint64_t v = t < nlist ? entry(t) : 0;
+    if (nlist > kSmCount) return sorted(v, nlist);
+    __syncthreads();
+    s.hist[t] = 0;
+    __syncthreads();
+    if (t < nlist) {
+      int place = 0;
+#pragma unroll 4
+      for (int e = 0; e < nlist; ++e) place += entry(e) > v;
+      s.hist[place] = v;
+    }
+    __syncthreads();
+    return s.hist[t];
+  }
+  __device__ __forceinline__ uint64_t entry(int e) const {
+    return ((uint64_t)s.list_key[e] << 32) | (uint32_t)~s.list_idx[e];
+  }
   // Values of threads t < n in falling order (n <= kSmSort; the others hold 0).
   __device__ __forceinline__ uint64_t sorted(uint64_t v, int n) {
     for (int size = 2; size < 2 * n; size <<= 1) {
@@ -470,8 +496,7 @@ struct Sm {
   template <typename N>
   __device__ __forceinline__ int token_of_sorted(int n_kept, N need) {
     __syncthreads();
-    // larger keys first, lower indexes first among equals
-    const uint64_t v = sorted(t < nlist ? ((uint64_t)s.list_key[t] << 32) | (uint32_t)~s.list_idx[t] : 0, nlist);
+    const uint64_t v = sorted_list();
     const uint32_t key = (uint32_t)(v >> 32), idx = ~(uint32_t)v;
     if (has_p) {
       const uint64_t w = t < nlist ? weight(sm_logit(key)) : 0;
@@ -482,6 +507,27 @@ struct Sm {
       if (before < least && before + w >= least) s.u32 = t;
       __syncthreads();
       n_kept = (int)s.u32 + 1;
+    }
+    if (n_kept <= kSmCount) {  // by the sum over the kept tokens of lower index
+      uint64_t w = t < n_kept ? weight(sm_logit(key)) : 0;
+      if (w < wmin) w = 0;
+      __syncthreads();
+      s.hist[t] = w;
+      if (t < n_kept) s.list_idx[t] = idx;
+      __syncthreads();
+      if (t < n_kept) {
+        uint64_t before = 0, total = 0;
+#pragma unroll 4
+        for (int e = 0; e < n_kept; ++e) {
+          const uint64_t o = s.hist[e];
+          total += o;
+          before += s.list_idx[e] < idx ? o : 0;
+        }
+        const uint64_t target = goal(total);
+        if (before <= target && before + w > target) s.u32 = idx;
+      }
+      __syncthreads();
+      return (int)s.u32;
     }
     if (V <= kSmLong) {  // the kept tokens' places among a hundred steps of the row
       __syncthreads();
