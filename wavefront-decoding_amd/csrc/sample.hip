@@ -18,8 +18,8 @@
 // the weight -- they are found without ordering the row: of the 1024 threads'
 // largest logits, at least k are no smaller than the k-th, so every one of the
 // first k tokens is at or above it, and few others are. Those go to a list in LDS,
-// which is sorted (one entry a thread), and top-k, top-p and min_p are positions
-// in it. Otherwise a histogram of the logits' distance from the largest says which
+// which is put in order (one entry a thread) if it is short, and top-k, top-p and
+// min_p are positions in it. Otherwise a histogram of the logits' distance from the largest says which
 // of 1024 bins the last kept token lies in, by count or by weight, and a radix
 // select over that bin's tokens (over the row, if they are too many) finds its
 // key; ties with it are kept in index order.
@@ -71,8 +71,8 @@ struct SmArgs {
 };
 
 constexpr int kSmBins = 1024;   // one per thread
-constexpr int kSmSort = kSmThreads;  // entries of a list that is sorted
-constexpr int kSmCount = 256;        // and of one that is ordered by counting
+constexpr int kSmFew = 256;          // entries of a list that is put in order
+constexpr int kSmShort = 2048;       // slabs of so few logits are listed whole
 constexpr int kSmLong = 32768;       // longest row of one workgroup
 constexpr int kSmSlab = 8192;
 constexpr int kSmSlabs = kSmMaxVocab / kSmSlab;
@@ -450,56 +450,31 @@ struct Sm {
         if (e + q < w_end) f(sm_key(x[q]));
     });
   }
-  // The list in falling order, one entry a thread (n <= kSmSort): larger keys first, lower
-  // indexes first among equals; 0 behind it. Up to kSmCount entries an entry's place is
-  // the number that come before it; 100 of them take 0.8 us so, 3.4 by the network.
-  __device__ __forceinline__ uint64_t sorted_list() {
-    const uint64_t v = t < nlist ? entry(t) : 0;
-    if (nlist > kSmCount) return sorted(v, nlist);
+  // The token of a list of at most kSmFew: of its n_kept first -- larger logits first,
+  // lower indexes first among equals -- those whose weight reaches need(weight of these),
+  // with top-p; of these the ones min_p leaves, by index. An entry's place is the number
+  // that come before it, the sum of the kept tokens of lower index likewise: 100 entries
+  // take 0.8 us each time, where a bitonic sort took 3.4.
+  __device__ __forceinline__ uint64_t entry(int e) const {
+    return ((uint64_t)s.list_key[e] << 32) | (uint32_t)~s.list_idx[e];
+  }
+  template <typename N>
+  __device__ __forceinline__ int token_of_few(int n_kept, N need) {
     __syncthreads();
     s.hist[t] = 0;
     __syncthreads();
     if (t < nlist) {
+      const uint64_t own = entry(t);
       int place = 0;
 #pragma unroll 4
-      for (int e = 0; e < nlist; ++e) place += entry(e) > v;
-      s.hist[place] = v;
+      for (int e = 0; e < nlist; ++e) place += entry(e) > own;
+      s.hist[place] = own;
     }
     __syncthreads();
-    return s.hist[t];
-  }
-  __device__ __forceinline__ uint64_t entry(int e) const {
-    return ((uint64_t)s.list_key[e] << 32) | (uint32_t)~s.list_idx[e];
-  }
-  // Values of threads t < n in falling order (n <= kSmSort; the others hold 0).
-  __device__ __forceinline__ uint64_t sorted(uint64_t v, int n) {
-    for (int size = 2; size < 2 * n; size <<= 1) {
-      for (int step = size >> 1; step > 0; step >>= 1) {
-        uint64_t o;
-        if (step < 64) {
-          o = sm_shfl_xor(v, step);
-        } else {
-          __syncthreads();
-          s.hist[t] = v;
-          __syncthreads();
-          o = s.hist[t ^ step];
-        }
-        const bool first = (t & step) == 0, falling = (t & size) == 0;
-        v = (first == falling) == (v > o) ? v : o;
-      }
-    }
-    return v;
-  }
-  // The token of a list of at most kSmSort: of its n_kept first (all of them, without
-  // top-k) those whose weight reaches need(weight of these), with top-p; of these the
-  // ones min_p leaves, by index.
-  template <typename N>
-  __device__ __forceinline__ int token_of_sorted(int n_kept, N need) {
-    __syncthreads();
-    const uint64_t v = sorted_list();
+    const uint64_t v = s.hist[t];
     const uint32_t key = (uint32_t)(v >> 32), idx = ~(uint32_t)v;
+    uint64_t w = t < nlist ? weight(sm_logit(key)) : 0;
     if (has_p) {
-      const uint64_t w = t < nlist ? weight(sm_logit(key)) : 0;
       const uint64_t before = block_scan(w);
       if (t == n_kept - 1) s.u64 = before + w;
       __syncthreads();
@@ -508,42 +483,22 @@ struct Sm {
       __syncthreads();
       n_kept = (int)s.u32 + 1;
     }
-    if (n_kept <= kSmCount) {  // by the sum over the kept tokens of lower index
-      uint64_t w = t < n_kept ? weight(sm_logit(key)) : 0;
-      if (w < wmin) w = 0;
-      __syncthreads();
-      s.hist[t] = w;
-      if (t < n_kept) s.list_idx[t] = idx;
-      __syncthreads();
-      if (t < n_kept) {
-        uint64_t before = 0, total = 0;
+    if (w < wmin || t >= n_kept) w = 0;
+    __syncthreads();
+    s.hist[t] = w;
+    if (t < n_kept) s.list_idx[t] = idx;
+    __syncthreads();
+    if (t < n_kept) {
+      uint64_t before = 0, total = 0;
 #pragma unroll 4
-        for (int e = 0; e < n_kept; ++e) {
-          const uint64_t o = s.hist[e];
-          total += o;
-          before += s.list_idx[e] < idx ? o : 0;
-        }
-        const uint64_t target = goal(total);
-        if (before <= target && before + w > target) s.u32 = idx;
+      for (int e = 0; e < n_kept; ++e) {
+        const uint64_t o = s.hist[e];
+        total += o;
+        before += s.list_idx[e] < idx ? o : 0;
       }
-      __syncthreads();
-      return (int)s.u32;
+      const uint64_t target = goal(total);
+      if (before <= target && before + w > target) s.u32 = idx;
     }
-    if (V <= kSmLong) {  // the kept tokens' places among a hundred steps of the row
-      __syncthreads();
-      if (t == n_kept - 1) s.u64 = v;
-      __syncthreads();
-      kk = (uint32_t)(s.u64 >> 32);
-      last_tie = (int)~(uint32_t)s.u64;
-      ties = 0;
-      return listed_token();
-    }
-    const uint64_t by_index = sorted(t < n_kept ? ((uint64_t)~idx << 32) | key : 0, n_kept);
-    uint64_t w = t < n_kept ? weight(sm_logit((uint32_t)by_index)) : 0;
-    if (w < wmin) w = 0;
-    const uint64_t before = block_scan(w);
-    const uint64_t target = goal(block_sum(w));
-    if (before <= target && before + w > target) s.u32 = ~(uint32_t)(by_index >> 32);
     __syncthreads();
     return (int)s.u32;
   }
@@ -743,8 +698,8 @@ struct Sm {
   // A list that holds the first k tokens, or all that can be drawn, and whatever else:
   // top-k, top-p and the token.
   __device__ __forceinline__ int token_of_list() {
-    if (nlist > kSmSort && nlist > k) thin_list();
-    if (nlist <= kSmSort) return token_of_sorted(min(k, nlist), [&](uint64_t sum) { return need_of(sum); });
+    if (nlist > kSmFew && nlist > k) thin_list();
+    if (nlist <= kSmFew) return token_of_few(min(k, nlist), [&](uint64_t sum) { return need_of(sum); });
     if (nlist > k) {
       refine_list(0, (uint64_t)k, false);
     } else {  // all of the list, and nothing that is not in it
@@ -762,9 +717,9 @@ struct Sm {
   __device__ __forceinline__ int token() {
     if (has_k) {
       // V / 4 threads, or 960 of the 1024, hold logits
-      if (V <= kSmSort || k <= min(kSmGuess, V / 4)) {
-        const int b = V <= kSmSort ? kSmBins - 1 : guess_bin((uint64_t)k);
-        if (collect(0, b, kSmSort, true)) return token_of_list();
+      if (V <= LIST || k <= min(kSmGuess, V / 4)) {
+        const int b = V <= LIST ? kSmBins - 1 : guess_bin((uint64_t)k);
+        if (collect(0, b, LIST, true)) return token_of_list();
       }
       __syncthreads();
       s.hist[t] = 0;
@@ -795,9 +750,12 @@ struct Sm {
 #pragma unroll
         for (int q = 0; q < 4; ++q) upto += e + q < w_end && bin_of(x[q]) <= b;
       });
-      if (!has_k && block_sum(upto) <= kSmSort) {
-        collect(0, b, kSmSort, true);
-        return token_of_sorted(nlist, [&](uint64_t) { return need; });
+      if (!has_k && block_sum(upto) <= LIST) {
+        collect(0, b, LIST, true);
+        if (nlist <= kSmFew) return token_of_few(nlist, [&](uint64_t) { return need; });
+        refine_list(0, need, true);
+        if (ties_left) last_listed_tie();
+        return listed_token();
       } else if (collect(b, b, LIST, true)) {
         refine_list(before, need, true);
       } else {
@@ -898,7 +856,7 @@ __global__ __launch_bounds__(kSmThreads) void sample_bins_kernel(SmArgs a, SmRow
       for (int q = 0; q < 4; ++q) m.mine = fmaxf(m.mine, x[q]);
     });
     const int len = m.end - m.begin;
-    const int b = len <= kSmSort || m.k > min(kSmGuess, len / 4) ? kSmBins - 1 : m.guess_bin((uint64_t)m.k);
+    const int b = len <= kSmShort || m.k > min(kSmGuess, len / 4) ? kSmBins - 1 : m.guess_bin((uint64_t)m.k);
     m.collect(0, b, 2048, true);
     sm_append(m, ws);
   } else if (m.has_p && !m.has_k) {
