@@ -50,21 +50,26 @@ class BatchStaticKVCache:
         # one extra trailing "trash" row (a whole block when head-major) absorbs
         # the appends of padding rows of a captured (fixed-width) launch and is
         # never part of any slot.
-        if head_major:
-            shape = (nblk + 1, n_kv_head, max_seq_len, head_dim)
-            self.flat_k = torch.zeros(shape, dtype=dtype, device=self.device)
-            self.flat_v = torch.zeros(shape, dtype=dtype, device=self.device)
-            view = lambda t: t[:nblk].view(n_slots, batch_size, n_kv_head, max_seq_len,  # noqa: E731
-                                           head_dim).permute(0, 1, 3, 2, 4)
-        else:
-            self.flat_k = torch.zeros(rows + 1, n_kv_head, head_dim, dtype=dtype, device=self.device)
-            self.flat_v = torch.zeros(rows + 1, n_kv_head, head_dim, dtype=dtype, device=self.device)
-            view = lambda t: t[:rows].view(n_slots, batch_size, max_seq_len, n_kv_head, head_dim)  # noqa: E731
+        self._allocate((nblk + 1, n_kv_head, max_seq_len, head_dim) if head_major
+                       else (rows + 1, n_kv_head, head_dim))
         self.trash_row = rows
-        self.K = view(self.flat_k)
-        self.V = view(self.flat_v)
         # logical per-(slot, seq) lengths: bookkeeping and bounds checks only
         self.seqlen = [[0] * batch_size for _ in range(n_slots)]
+
+    def _allocate(self, shape) -> None:
+        self.flat_k = torch.zeros(shape, dtype=self.dtype, device=self.device)
+        self.flat_v = torch.zeros(shape, dtype=self.dtype, device=self.device)
+        nblk, S = self.n_slots * self.B, self.S
+        if self.head_major:
+            view = lambda t: t[:nblk].view(self.n_slots, self.B, self.n_kv_head, S,  # noqa: E731
+                                           self.head_dim).permute(0, 1, 3, 2, 4)
+        else:
+            view = lambda t: t[: nblk * S].view(self.n_slots, self.B, S, self.n_kv_head, self.head_dim)  # noqa: E731
+        self.K = view(self.flat_k)
+        self.V = view(self.flat_v)
+
+    def _append(self, k: torch.Tensor, v: torch.Tensor, rows: torch.Tensor) -> None:
+        ops.kv_append(k, v, self.flat_k, self.flat_v, rows)
 
     # -- indexing -----------------------------------------------------------
     def row_base(self, slot: int, b: int) -> int:
@@ -107,8 +112,8 @@ class BatchStaticKVCache:
         seq_ids = list(range(self.B)) if seq_ids is None else list(seq_ids)
         rows = torch.tensor([self.flat_row(slot, b, p) for b in seq_ids for p in range(L)], dtype=torch.int64,
                             device=self.device)
-        ops.kv_append(k.reshape(-1, self.n_kv_head, self.head_dim).contiguous(),
-                      v.reshape(-1, self.n_kv_head, self.head_dim).contiguous(), self.flat_k, self.flat_v, rows)
+        self._append(k.reshape(-1, self.n_kv_head, self.head_dim).contiguous(),
+                     v.reshape(-1, self.n_kv_head, self.head_dim).contiguous(), rows)
         for b in seq_ids:
             self.seqlen[slot][b] = max(self.seqlen[slot][b], L)
 
@@ -118,7 +123,7 @@ class BatchStaticKVCache:
             self.note_write(sl, b, p)
         rows = torch.tensor([self.flat_row(sl, b, p) for sl, b, p in zip(slots, seq_ids, positions)],
                             dtype=torch.int64, device=self.device)
-        ops.kv_append(k.contiguous(), v.contiguous(), self.flat_k, self.flat_v, rows)
+        self._append(k.contiguous(), v.contiguous(), rows)
 
     def gather_pack(self, slots, seq_ids, uptos):
         """Compatibility form of the reference pack (batch_kv_cache.py:75-96):
@@ -141,6 +146,36 @@ class BatchStaticKVCache:
         """Forget every sequence (buffers are reused as they are; reads are
         bounded by the reading query's position, so stale rows are never read)."""
         self.seqlen = [[0] * self.B for _ in range(self.n_slots)]
+
+
+class QuantBatchKVCache(BatchStaticKVCache):
+    """The same slots in 8 bits: `flat` (ops.QuantKV) holds the rows as codes
+    with an exponent per row and head, written by ops.kv_append_q /
+    qkv_rope_append_q and read by ops.attn_decode_q at (row_base, kv_len);
+    (Dh + 1) / (2 Dh) of a bf16 cache's bytes. K / V views have no meaning
+    here: gather_pack reads values back, as `dtype`."""
+
+    def __init__(self, n_slots: int, batch_size: int, n_kv_head: int, head_dim: int, max_seq_len: int,
+                 dtype: torch.dtype, device, *, head_major: bool = True, code: torch.dtype = torch.float8_e4m3fn):
+        self.code = code
+        super().__init__(n_slots, batch_size, n_kv_head, head_dim, max_seq_len, dtype, device, head_major=head_major)
+
+    def _allocate(self, shape) -> None:
+        self.flat = ops.QuantKV.zeros(shape, code=self.code, device=self.device)
+
+    def _append(self, k: torch.Tensor, v: torch.Tensor, rows: torch.Tensor) -> None:
+        ops.kv_append_q(k, v, self.flat, rows)
+
+    @property
+    def nbytes(self) -> int:
+        return 2 * self.n_slots * self.B * self.S * self.n_kv_head * (self.head_dim + 1)
+
+    def gather_pack(self, slots, seq_ids, uptos):
+        lengths = [u + 1 for u in uptos]
+        cu = torch.tensor([0] + lengths, dtype=torch.int32).cumsum(0, dtype=torch.int32).to(self.device)
+        rows = torch.cat([torch.arange(ln) + self.row_base(sl, b) for sl, b, ln in zip(slots, seq_ids, lengths)])
+        k, v = ops.kv_read_q(self.flat, rows.to(self.device), dtype=self.dtype)
+        return k, v, cu, max(lengths)
 
 
 class StaticKVCache(BatchStaticKVCache):
