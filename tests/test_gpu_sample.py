@@ -284,3 +284,22 @@ def test_sampled_wavefront_is_sequential_sampling(gpu, kw):
         runs.append(want)
     if kw.get("temperature") != 0.0:
         assert runs[0] != runs[1]
+
+
+@pytest.mark.parametrize("V", [2000, 40000])
+def test_top_p_at_the_edge_of_a_bin(gpu, V):
+    """a tokens of one logit and the rest of a lower one, top-p at the first ones' share:
+    whether the second ones' bin is needed is a matter of the last bit of p."""
+    g = torch.Generator().manual_seed(V)
+    n = 96
+    logits = torch.zeros(n, V)
+    t, p = [], []
+    for i in range(n):
+        at = torch.randperm(V, generator=g)
+        a, gap = V // 3 + i, 1.0 + i / 64
+        logits[i, at[a:]] = -gap
+        t.append([1.0, 0.75, 1.5][i % 3])
+        share = np.float32(a / (a + (V - a) * math.exp(-gap / t[-1])))
+        p.append(float(np.nextafter(share, np.float32(i % 2), dtype=np.float32) if i % 4 < 2 else share))
+    check(gpu, logits, torch.rand(n, generator=g).tolist(), t, None, p)
+    check(gpu, logits, [LAST] * n, t, None, p)
