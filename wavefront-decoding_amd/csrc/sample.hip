@@ -126,12 +126,14 @@ struct SmRowWs {
   uint32_t key[kSmRowList], idx[kSmRowList];
 };
 
-// CAP > 0: the logits at hand are kept in LDS, at most CAP; 0: they are read again
-// in every pass (from L2). In registers, 32 a thread, the passes' code spilled.
+// CAP > 0: the logits at hand, at most CAP, are kept in LDS; < 0: at most -CAP, in
+// registers, whose loads are in flight until the first use (for the slabs' 8 a thread;
+// the one-workgroup kernel's code spilled with 8 too). 0: they are read again in every
+// pass (from L2).
 template <int CAP, int LIST>
 struct SmShared {
   unsigned long long hist[kSmBins];
-  unsigned long long seg[(CAP > 0 ? CAP : kSmMaxVocab) / 256];  // the running sums' steps, in index order
+  unsigned long long seg[(CAP > 0 ? CAP : CAP < 0 ? -CAP : kSmMaxVocab) / 256];  // the running sums' steps, in index order
   u32x4 keep[CAP > 0 ? CAP / 4 : 1];
   uint32_t list_key[LIST], list_idx[LIST];
   double tab[32];
@@ -166,6 +168,7 @@ struct Sm {
   uint32_t kk = 0;
   uint64_t ties = 0, ties_left = 0;
   int last_tie = 0x7fffffff;
+  float held[CAP < 0 ? -CAP / kSmChunk : 1][4];
   bool ties_listed = false;  // every token with key kk is in the list
   int nlist = 0;
 
@@ -174,7 +177,10 @@ struct Sm {
         lane(threadIdx.x & 63), V(args.V), begin(lo), end(hi), per_wave((hi - lo + 63) / 64 * 4),
         w_end(min(lo + (wave + 1) * per_wave, hi)), rounds((per_wave + 255) / 256),
         row(args.logits + (int64_t)row_i * args.ld), vec(((uintptr_t)(row + lo) & 15) == 0) {
-    if constexpr (CAP > 0) {  // every load first; a thread reads back only what it stores
+    if constexpr (CAP < 0) {
+#pragma unroll
+      for (int c = 0; c < -CAP / kSmChunk; ++c) fetch(c, held[c]);
+    } else if constexpr (CAP > 0) {  // every load first; a thread reads back only what it stores
       float x[CAP / kSmChunk][4];
 #pragma unroll
       for (int c = 0; c < CAP / kSmChunk; ++c) fetch(c, x[c]);
@@ -199,7 +205,11 @@ struct Sm {
   template <typename F>
   __device__ __forceinline__ void each(F f) {
     float x[4];
-    if constexpr (CAP > 0) {
+    if constexpr (CAP < 0) {
+#pragma unroll
+      for (int c = 0; c < -CAP / kSmChunk; ++c)
+        if (c < rounds) f(first_of(c), held[c]);
+    } else if constexpr (CAP > 0) {
       for (int c = 0; c < rounds; ++c) {
         Elem<float>::unpack(s.keep[c * kSmThreads + t], x);
         f(first_of(c), x);
@@ -885,8 +895,8 @@ __global__ __launch_bounds__(kSmThreads) void sample_kernel(SmArgs a) {
 }
 
 // --- long rows: grid (slab, row) but for the last ------------------------------
-using SmSlab = Sm<0, 2048>;
-using SmSlabShared = SmShared<0, 2048>;
+using SmSlab = Sm<-kSmSlab, 2048>;
+using SmSlabShared = SmShared<-kSmSlab, 2048>;
 
 __global__ __launch_bounds__(kSmThreads) void sample_largest_kernel(SmArgs a, SmRowWs* wss) {
   __shared__ __align__(16) SmSlabShared sh;
@@ -972,6 +982,18 @@ __global__ __launch_bounds__(kSmThreads) void sample_row_kernel(SmArgs a, SmRowW
   __shared__ __align__(16) SmShared<0, kSmRowList> sh;
   SmRowWs& ws = wss[blockIdx.x];
   Sm<0, kSmRowList> m(a, sh, blockIdx.x, 0, a.V);
+  // what the launches before left, all loads at once
+  const uint32_t count = ws.count;
+  const uint64_t bin = ws.hist[m.t];
+  uint64_t own = ws.share[min(m.t, slabs * kSmWaves - 1)];
+  const uint32_t key0 = ws.key[m.t], idx0 = ws.idx[m.t];
+  auto take_list = [&]() {
+    m.nlist = (int)count;
+    for (int e = m.t; e < m.nlist; e += kSmThreads) {
+      sh.list_key[e] = e < kSmThreads ? key0 : ws.key[e];
+      sh.list_idx[e] = e < kSmThreads ? idx0 : ws.idx[e];
+    }
+  };
   m.largest_of(ws, slabs);
   __syncthreads();  // the table
   if (!m.parameters()) {  // the first slab that has it
@@ -984,30 +1006,21 @@ __global__ __launch_bounds__(kSmThreads) void sample_row_kernel(SmArgs a, SmRowW
     return;
   }
   const bool listed = m.has_k && m.k <= kSmGuess;
-  if ((listed || (m.has_p && !m.has_k)) ? ws.count > kSmRowList : m.has_k) {  // not prepared
+  if ((listed || (m.has_p && !m.has_k)) ? count > kSmRowList : m.has_k) {  // not prepared
     m.largest();
     m.finish(m.token());
     return;
   }
   if (listed) {
-    m.nlist = (int)ws.count;
-    for (int e = m.t; e < m.nlist; e += kSmThreads) {
-      sh.list_key[e] = ws.key[e];
-      sh.list_idx[e] = ws.idx[e];
-    }
+    take_list();
     __syncthreads();
     m.finish(m.token_of_list());
     return;
   }
   // the shares, at most 1024, one a thread; with top-p the kept ones of the listed tokens added
-  uint64_t own = m.t < slabs * kSmWaves ? (uint64_t)ws.share[m.t] : 0;
+  if (m.t >= slabs * kSmWaves) own = 0;
   if (m.has_p) {
-    m.nlist = (int)ws.count;
-    for (int e = m.t; e < m.nlist; e += kSmThreads) {
-      sh.list_key[e] = ws.key[e];
-      sh.list_idx[e] = ws.idx[e];
-    }
-    const uint64_t bin = ws.hist[m.t];
+    take_list();
     const uint64_t need = m.need_of(m.block_sum(bin));
     uint64_t before;
     m.find_bin(bin, 0, need, before);
