@@ -12,7 +12,11 @@
 //
 // Bound by HBM: (Dh + 1) bytes of K and of V per key and kv head. P.V on the
 // VALU, as in wfd_attn_decode, took 1600 vector instructions per 64 keys of four
-// heads and held 64 rows over 32k keys at 3.3 TB/s; a tile here takes a fifth.
+// heads and held 64 rows over 32k keys at 3.3 TB/s; a tile here takes a fifth. 64
+// rows x 4 kv heads x 32.7k e4m3 keys: 400 us, 5.4 TB/s (reads alone, so above the
+// 4.9 of a copy); 112 rows x 16 heads x 128-1200 int8 keys 82 us, 3.8 TB/s (short
+// rows' first loads and merges); 8 rows of 512-778 keys 10.4 us, one tile after
+// another in 128 workgroups.
 // Work split as there: a workgroup of 8 waves owns one (1024-key split, kv head,
 // query row), its waves take 32-key tiles round-robin, each through LDS of its
 // own a tile ahead; the waves merge through LDS in fixed order and a row's splits
@@ -348,9 +352,9 @@ attn_q_split_kernel(AttnQArgs a) {
 // workgroup's where the rows alone make 1024 splits (two rounds of workgroups): it
 // finishes the row itself, with the combine kernel's arithmetic, and neither that
 // launch nor workgroups that find no keys are needed. 112 rows x 16 heads x 128-1200
-// keys: 104 -> 82 us. Longer rows keep a workgroup per split (64 rows x 4 heads x 32k
-// keys, four splits each: 400 -> 410 us), and so do fewer rows, whose splits are what
-// fills the chip.
+// keys: 104 -> 82 us, 64 x 16 x 1100-2000: 88 -> 86. Longer rows keep a workgroup per
+// split (64 rows x 4 heads x 32k keys, four splits each: 400 -> 410 us), and so do
+// fewer rows, whose splits are what fills the chip (8 x 16 x 1100-2000: 18.0 -> 21.3).
 constexpr int kAqRowSplits = 4;
 constexpr int kAqFill = 1024;
 static int splits_per_workgroup(int ms, int64_t rows) {

@@ -28,9 +28,13 @@ constexpr int kShTarget = 128;   // chunks x kv heads aimed at
 constexpr int kShMaxG = 16;
 constexpr int kShMaxHeads = 4096;  // a chunk's keys stay within 32-bit offsets of its first
 
-// Keys per chunk of a prefix of P keys: enough chunks for a workgroup per CU over
-// the kv heads while they are at least 128 keys; long prefixes take 1024, where
-// the parts' traffic is small against the keys'.
+// Keys per chunk of a prefix of P keys: 128 chunks over the kv heads, a workgroup
+// each for every second CU, while they are at least 128 keys: the parts' traffic
+// grows with the chunks, and a group's pairs and the other groups fill the rest.
+// 64 rows x 8000 keys x 16 heads, 100 rows over three prefixes of 20-32k x 4, and 64
+// over four of 2000 x 16 take 55 / 89 / 58 us, with 256 chunks 59 / 104 / 63, with 64
+// 55 / 87 / 57; 8 rows x 32000 x 4 30.3, 31.5 and 30.2. At most 1024 keys (512: 58 /
+// 105 / 59; 2048 as 1024), and 512 of a row's own (256: 60 / 92 / 56; 1024: 55 / 92 / 56).
 __host__ __device__ inline int prefix_chunk(int P, int Hkv) {
   const int64_t c = ((int64_t)P * Hkv + kShTarget - 1) / kShTarget;
   const int64_t r = (c + kShMinChunk - 1) / kShMinChunk * kShMinChunk;
@@ -269,6 +273,13 @@ __device__ __forceinline__ f32x16 sh_mfma32(const u32x4& x, const u32x4& y, f32x
 // lane half hf is key 16 (r / 8) + 8 hf + r % 8), so P never leaves its lane, and
 // V^T comes out of the row-major tile by transposing LDS reads. Keys past the
 // chunk read as zeros and score -inf.
+//
+// 64 rows x 8000 keys x 16 heads: 47 us and 7-9 for the merge (floor 41), of which the
+// loads alone take 43; 100 rows x 20-32k x 4 kv heads: 80 + 9, loads alone 60: each
+// tile of 32 pairs takes its prefix from the L2 again (740 MB, 12 TB/s), and products
+// and exponentials only partly hide behind them at two waves per SIMD. 64 pairs a
+// wave (69 / 129 us), eight waves sharing the tiles of 64 pairs (56 / 94) and two
+// chains of K Q^T (as one) were no faster.
 template <int DH>
 __global__ __launch_bounds__(64 * kShWaves) __attribute__((amdgpu_waves_per_eu(2))) void attn_shared_bf16_kernel(
     ShArgs a) {
