@@ -9,7 +9,8 @@ Layers, bottom-up:
   attention         the reference's attention-backend API (attn_dense,
                     attn_cutoff_multi, attn_varlen, attn_varlen_q1_padded,
                     set_backend/backend, compute_qkv) on the HIP kernels
-  kv_cache          StaticKVCache / BatchStaticKVCache over one flat device buffer
+  kv_cache          StaticKVCache / BatchStaticKVCache over one flat device buffer,
+                    QuantBatchKVCache over 8-bit codes
   model             synthetic looped-LM configs and seeded random-init weights
   engine            the device engine: P / R / C unions as fused launch
                     sequences, captured as hipGraphs (one replay per tick)
