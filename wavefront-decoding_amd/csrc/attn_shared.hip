@@ -6,8 +6,8 @@
 // Softmax over a union is a merge of softmaxes over its parts: a part leaves its
 // maximum m, sum l and unnormalised output o, and the row is sum o 2^(m - M) /
 // sum l 2^(m - M) over its parts. The prefix is cut into chunks of keys, a
-// workgroup computes one chunk for up to 32 (fp32: 16) (query row, query head)
-// pairs of a group and one kv head -- each key is read once for all of them -- and a row's
+// workgroup computes one chunk for up to 32 (query row, query head) pairs
+// of a group and one kv head -- each key is read once for all of them -- and a row's
 // own keys are cut likewise, for that row alone; attn_shared_combine merges a
 // row's parts in the order of its keys.
 //
@@ -18,8 +18,7 @@
 
 namespace wfd {
 
-constexpr int kShRowsF32 = 16;   // (query row, head) pairs per workgroup
-constexpr int kShRowsBF16 = 32;
+constexpr int kShRows = 32;      // (query row, head) pairs per workgroup
 constexpr int kShWaves = 4;      // key streams per workgroup
 constexpr int kShMinChunk = 128;
 constexpr int kShMaxChunk = 1024;
@@ -162,106 +161,62 @@ __device__ __forceinline__ void sh_leave(const ShArgs& a, const ShItem& it, cons
   }
 }
 
-// fp32: 16 pairs per workgroup on the fp32 MFMA (scores as in wfd_attn_decode;
-// P.V on the 16x16x4 form, P through LDS), operands straight from the cache.
-template <int DH>
-__global__ __launch_bounds__(64 * kShWaves) void attn_shared_f32_kernel(ShArgs a) {
-  using T = float;
-  constexpr int RT = kShRowsF32;
-  constexpr int V = Elem<T>::kVec;
-  constexpr int KSTEP = 4 * V;
-  constexpr int NDS = DH / KSTEP;
-  constexpr int NC = DH / 16;
-  __shared__ float p_lds[kShWaves][16][17];
-  __shared__ __align__(16) float o_lds[kShWaves][16][DH];
-  __shared__ float m_lds[kShWaves][16];
-  __shared__ float l_lds[kShWaves][16];
-  __shared__ int64_t at_lds[RT];
-  ShItem it;
-  if (!sh_item<RT>(a, it)) return;  // uniform
-  const int g = it.g, nr = it.nr, k0 = it.k0, k1 = it.k1;
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4;
-  const int64_t hb = kv_offset(it.base, g, a.Hkv, DH, a.br);
-  const int64_t rs = a.br > 1 ? (int64_t)DH : (int64_t)a.Hkv * DH;
-  const T* kb = (const T*)a.kc + hb;
-  const T* vb = (const T*)a.vc + hb;
-  u32x4 qf[NDS];
-#pragma unroll
-  for (int s = 0; s < NDS; ++s)
-    qf[s] = col < nr ? ld16((const T*)a.q + sh_pair(a, it, col) * DH + grp * V + s * KSTEP) : zero16();
-
-  float mrun[4], lrun[4];
-  f32x4 o[NC];
-#pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    mrun[r] = -INFINITY;
-    lrun[r] = 0.f;
-  }
-#pragma unroll
-  for (int c = 0; c < NC; ++c) o[c] = f32x4{0.f, 0.f, 0.f, 0.f};
-
-  for (int t0 = k0 + 16 * wave; t0 < k1; t0 += 16 * kShWaves) {
-    const T* kp = kb + (int64_t)min(t0 + col, k1 - 1) * rs + grp * V;
-    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int s = 0; s < NDS; ++s) acc = mfma_step<T>(qf[s], ld16(kp + s * KSTEP), acc);
-    float corr[4];
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const float sv = t0 + col < k1 ? acc[r] * a.scale_log2 : -INFINITY;
-      float mt = sv;
-#pragma unroll
-      for (int sh = 8; sh >= 1; sh >>= 1) mt = fmaxf(mt, __shfl_xor(mt, sh, 64));
-      const float mnew = fmaxf(mrun[r], mt);
-      corr[r] = mrun[r] == -INFINITY ? 0.f : exp2f(mrun[r] - mnew);
-      mrun[r] = mnew;
-      const float p = sv == -INFINITY ? 0.f : exp2f(sv - mnew);
-      float lt = p;
-#pragma unroll
-      for (int sh = 8; sh >= 1; sh >>= 1) lt += __shfl_xor(lt, sh, 64);
-      lrun[r] = fmaf(lrun[r], corr[r], lt);
-      p_lds[wave][4 * grp + r][col] = p;
-    }
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-#pragma unroll
-    for (int c = 0; c < NC; ++c)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) o[c][r] *= corr[r];
-#pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      const float p = p_lds[wave][col][4 * s + grp];
-      const int key = t0 + 4 * s + grp;
-      const T* vp = vb + (int64_t)min(key, k1 - 1) * rs + col;
-#pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        const float v = key < k1 ? Elem<T>::load(vp + 16 * c) : 0.f;
-        o[c] = __builtin_amdgcn_mfma_f32_16x16x4f32(p, v, o[c], 0, 0, 0);
-      }
-    }
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-  }
-#pragma unroll
-  for (int r = 0; r < 4; ++r) {
-#pragma unroll
-    for (int c = 0; c < NC; ++c) o_lds[wave][4 * grp + r][16 * c + col] = o[c][r];
-    if (col == 0) {
-      m_lds[wave][4 * grp + r] = mrun[r];
-      l_lds[wave][4 * grp + r] = lrun[r];
-    }
-  }
-  __syncthreads();
-  sh_leave<DH, DH, RT>(a, it, &o_lds[0][0][0], &m_lds[0][0], &l_lds[0][0], at_lds);
-}
-
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 __device__ __forceinline__ f32x16 sh_mfma32(const u32x4& x, const u32x4& y, f32x16 acc) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, y), acc, 0,
                                                  0, 0);
+}
+
+// One tile's scores (of the lane's pair) to probabilities, under the pair's reference
+// point: the maximum when it was last moved, which is when a tile exceeds it by more
+// than 2^8. Probabilities up to 2^8 lose nothing in fp32 sums or bf16, and most tiles
+// rescale nothing (with the running maximum itself some pair of the 32 moves in nearly
+// every tile). It depends on the pair's own scores only.
+template <int NDB>
+__device__ __forceinline__ void sh_softmax(f32x16& sc, f32x16 (&o)[NDB], float& mref, float& lrun, float scale) {
+  float mt = -INFINITY;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) mt = fmaxf(mt, sc[r]);
+  mt = fmaxf(mt, __shfl_xor(mt, 32, 64)) * scale;
+  if (__builtin_amdgcn_ballot_w64(mt > mref + 8.f)) {
+    const float mnew = mt > mref + 8.f ? mt : mref;
+    const float corr = mref == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mref - mnew);
+    mref = mnew;
+    lrun *= corr;
+#pragma unroll
+    for (int db = 0; db < NDB; ++db)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[db][r] *= corr;
+  }
+  const float ref = mref == -INFINITY ? 0.f : mref;
+  // v_exp_f32 flushes below 2^-126: far under what a sum that holds 2^-8 or more resolves
+  float lt = 0.f;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    sc[r] = __builtin_amdgcn_exp2f(fmaf(sc[r], scale, -ref));
+    lt += sc[r];
+  }
+  lrun += lt + __shfl_xor(lt, 32, 64);
+}
+
+// A wave's stream to LDS for the merge: lane (col, hf) holds pair col's columns
+// 32 db + 8 (r / 4) + 4 hf + r % 4.
+template <int DH, int OP, int RT>
+__device__ __forceinline__ void sh_keep(const ShItem& it, int wave, int col, int hf, const f32x16 (&o)[DH / 32],
+                                        float mref, float lrun, float* o_lds, float* m_lds, float* l_lds) {
+  if (col < it.nr) {
+#pragma unroll
+    for (int db = 0; db < DH / 32; ++db)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        *reinterpret_cast<f32x4*>(o_lds + (wave * RT + col) * OP + 32 * db + 8 * r + 4 * hf) =
+            f32x4{o[db][4 * r], o[db][4 * r + 1], o[db][4 * r + 2], o[db][4 * r + 3]};
+    if (hf == 0) {
+      m_lds[wave * RT + col] = mref;
+      l_lds[wave * RT + col] = lrun;
+    }
+  }
 }
 
 // bf16: 32 pairs per workgroup, one per column of the 32x32x16 MFMA, and four
@@ -283,7 +238,7 @@ __device__ __forceinline__ f32x16 sh_mfma32(const u32x4& x, const u32x4& y, f32x
 template <int DH>
 __global__ __launch_bounds__(64 * kShWaves) __attribute__((amdgpu_waves_per_eu(2))) void attn_shared_bf16_kernel(
     ShArgs a) {
-  constexpr int RT = kShRowsBF16;
+  constexpr int RT = kShRows;
   constexpr int TK = 32;
   constexpr int NDS = DH / 16;
   constexpr int NDB = DH / 32;
@@ -355,11 +310,6 @@ __global__ __launch_bounds__(64 * kShWaves) __attribute__((amdgpu_waves_per_eu(2
     return u32x4{x.x, x.y, y.x, y.y};
   };
 
-  // The reference point of a pair's exponentials: the maximum when it was last
-  // moved, which is when a tile exceeds it by more than 2^8. Probabilities up to
-  // 2^8 lose nothing in fp32 sums or bf16, and most tiles rescale nothing (with
-  // the running maximum itself some pair of the 32 moves in nearly every tile).
-  // It depends on the pair's own scores only.
   float mref = -INFINITY, lrun = 0.f;
   f32x16 o[NDB];
 #pragma unroll
@@ -388,29 +338,7 @@ __global__ __launch_bounds__(64 * kShWaves) __attribute__((amdgpu_waves_per_eu(2
       for (int r = 0; r < 16; ++r)
         if (t0 + 16 * (r >> 3) + 8 * hf + (r & 7) >= nk) sc[r] = -INFINITY;
     }
-    float mt = -INFINITY;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) mt = fmaxf(mt, sc[r]);
-    mt = fmaxf(mt, __shfl_xor(mt, 32, 64)) * scale;
-    if (__builtin_amdgcn_ballot_w64(mt > mref + 8.f)) {
-      const float mnew = mt > mref + 8.f ? mt : mref;
-      const float corr = mref == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mref - mnew);
-      mref = mnew;
-      lrun *= corr;
-#pragma unroll
-      for (int db = 0; db < NDB; ++db)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) o[db][r] *= corr;
-    }
-    const float ref = mref == -INFINITY ? 0.f : mref;
-    // v_exp_f32 flushes below 2^-126: far under a bf16 probability's resolution
-    float lt = 0.f;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      sc[r] = __builtin_amdgcn_exp2f(fmaf(sc[r], scale, -ref));
-      lt += sc[r];
-    }
-    lrun += lt + __shfl_xor(lt, 32, 64);
+    sh_softmax<NDB>(sc, o, mref, lrun, scale);
     // the one rounding before the output's: P meets V as bf16 (half a step: 2^-8
     // of P, at random signs), where fp32 products would take 8 times the MFMA time
     u32x4 pb[2];
@@ -429,20 +357,118 @@ __global__ __launch_bounds__(64 * kShWaves) __attribute__((amdgpu_waves_per_eu(2
 
   __syncthreads();  // every wave's tiles are done: the merge takes their LDS
   float* o_lds = reinterpret_cast<float*>(lds);
-  if (col < it.nr) {
-#pragma unroll
-    for (int db = 0; db < NDB; ++db)
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-        *reinterpret_cast<f32x4*>(o_lds + (wave * RT + col) * OP + 32 * db + 8 * r + 4 * hf) =
-            f32x4{o[db][4 * r], o[db][4 * r + 1], o[db][4 * r + 2], o[db][4 * r + 3]};
-    if (hf == 0) {
-      m_lds[wave * RT + col] = mref;
-      l_lds[wave * RT + col] = lrun;
-    }
-  }
+  sh_keep<DH, OP, RT>(it, wave, col, hf, o, mref, lrun, o_lds, m_lds, l_lds);
   __syncthreads();
   sh_leave<DH, OP, RT>(a, it, o_lds, m_lds, l_lds, at_lds);
+}
+
+// fp32: the same on the 32x32x2 MFMA. A lane's operands of K Q^T are four consecutive
+// columns at a time (lane half hf takes columns 8 j + 4 hf + e at step 4 j + e), its
+// S^T register r is key 8 (r / 4) + 4 hf + r % 4, which is also the key it supplies of
+// P^T at step r, and V^T is read from the row-major tile a value at a time, 32
+// consecutive ones a row. One workgroup per CU by LDS, a wave per SIMD.
+template <int DH>
+__global__ __launch_bounds__(64 * kShWaves) void attn_shared_f32_kernel(ShArgs a) {
+  constexpr int RT = kShRows;
+  constexpr int TK = 32;
+  constexpr int NDB = DH / 32;
+  constexpr int KP = DH + 4;    // LDS row pitches: K reads 16 bytes of 32 rows, V^T 128 bytes of rows
+  constexpr int VP = DH + 8;    // that are 4 apart
+  constexpr int CPR = DH / 4;   // 16-byte pieces per row
+  constexpr int RPI = 64 / CPR;
+  constexpr int NLD = TK / RPI;
+  constexpr int OP = DH + 4;
+  constexpr int kWaveEls = TK * (KP + VP);
+  static_assert(kWaveEls >= RT * OP, "the merge takes the tiles' LDS");
+  __shared__ __align__(16) float lds[kWaveEls * kShWaves];
+  __shared__ float m_lds[kShWaves * RT];
+  __shared__ float l_lds[kShWaves * RT];
+  __shared__ int64_t at_lds[RT];
+  ShItem it;
+  if (!sh_item<RT>(a, it)) return;  // uniform
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, col = lane & 31, hf = lane >> 5;
+  float* k_lds = lds + wave * kWaveEls;
+  float* v_lds = k_lds + TK * KP;
+
+  const int64_t rs = a.br > 1 ? (int64_t)DH : (int64_t)a.Hkv * DH;
+  const int64_t at = kv_offset(it.base, it.g, a.Hkv, DH, a.br) + it.k0 * rs;
+  const int nk = it.k1 - it.k0;
+  const uint32_t rsb = (uint32_t)(rs * sizeof(float));
+  const uint32_t span = (uint32_t)(nk - 1) * rsb + DH * sizeof(float);
+  auto rsrc = [&](const void* p) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>((const float*)p + at), (short)0, span, 0x00020000);
+  };
+  const __amdgpu_buffer_rsrc_t kr = rsrc(a.kc), vr = rsrc(a.vc);
+  const int lr = lane / CPR, lp = lane % CPR;
+  u32x4 kreg[NLD], vreg[NLD];
+  uint32_t off = (uint32_t)(TK * wave + lr) * rsb + (uint32_t)lp * 16u;
+  auto fetch = [&]() {  // this wave's next tile; zeros past the chunk
+#pragma unroll
+    for (int s = 0; s < NLD; ++s) {
+      kreg[s] = buf_ld16(kr, off + (uint32_t)(RPI * s) * rsb);
+      vreg[s] = buf_ld16(vr, off + (uint32_t)(RPI * s) * rsb);
+    }
+    off += (uint32_t)(TK * kShWaves) * rsb;
+  };
+  fetch();
+
+  const float scale = fmaxf(fabsf(a.scale_log2), 1e-37f);  // as in the bf16 kernel
+  const uint32_t flip = a.scale_log2 < 0.f ? 0x80000000u : 0u;
+  u32x4 qf[DH / 8];
+  {
+    const float* qp = (const float*)a.q + sh_pair(a, it, min(col, it.nr - 1)) * DH + 4 * hf;
+#pragma unroll
+    for (int s = 0; s < DH / 8; ++s) qf[s] = ld16(qp + 8 * s) ^ flip;
+  }
+  float mref = -INFINITY, lrun = 0.f;
+  f32x16 o[NDB];
+#pragma unroll
+  for (int c = 0; c < NDB; ++c)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o[c][r] = 0.f;
+
+  for (int t0 = TK * wave; t0 < nk; t0 += TK * kShWaves) {  // uniform over the wave
+#pragma unroll
+    for (int s = 0; s < NLD; ++s) {
+      *reinterpret_cast<u32x4*>(k_lds + (RPI * s + lr) * KP + 4 * lp) = kreg[s];
+      *reinterpret_cast<u32x4*>(v_lds + (RPI * s + lr) * VP + 4 * lp) = vreg[s];
+    }
+    fetch();
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    f32x16 sc;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) sc[r] = 0.f;
+#pragma unroll
+    for (int j = 0; j < DH / 8; ++j) {
+      const f32x4 kf = *reinterpret_cast<const f32x4*>(k_lds + col * KP + 8 * j + 4 * hf);
+      const f32x4 q4 = __builtin_bit_cast(f32x4, qf[j]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sc = __builtin_amdgcn_mfma_f32_32x32x2f32(kf[e], q4[e], sc, 0, 0, 0);
+    }
+    if (t0 + TK > nk) {  // the chunk's last tile (uniform)
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if (t0 + 8 * (r >> 2) + 4 * hf + (r & 3) >= nk) sc[r] = -INFINITY;
+    }
+    sh_softmax<NDB>(sc, o, mref, lrun, scale);
+    const float* vp = v_lds + 4 * hf * VP + col;
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+#pragma unroll
+      for (int db = 0; db < NDB; ++db)
+        o[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(vp[(8 * (r >> 2) + (r & 3)) * VP + 32 * db], sc[r], o[db], 0, 0, 0);
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();  // the next tile overwrites this one
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  }
+
+  __syncthreads();  // every wave's tiles are done: the merge takes their LDS
+  sh_keep<DH, OP, RT>(it, wave, col, hf, o, mref, lrun, lds, m_lds, l_lds);
+  __syncthreads();
+  sh_leave<DH, OP, RT>(a, it, lds, m_lds, l_lds, at_lds);
 }
 
 // One row's parts, prefix chunks then its own, merged in that order, kCombineBatch
@@ -496,17 +522,14 @@ __global__ __launch_bounds__(DH) void attn_shared_combine(ShArgs a) {
 }
 
 template <typename T, int DH>
-static void launch_shared(ShArgs a, int64_t pairs, hipStream_t st) {
+static void launch_shared(const ShArgs& a, hipStream_t st) {
   const int64_t nkeys = (int64_t)a.ng * a.pchunks * a.Hkv, own = (int64_t)a.n * a.ochunks * a.Hkv;
-  auto tiles = [&](int rt) { return (int)((pairs + rt - 1) / rt); };
-  auto grid = [&](int64_t prefix_tiles) { return dim3((unsigned)((nkeys + 7) / 8 * 8 * prefix_tiles + own)); };
-  const dim3 block(64 * kShWaves);
-  if constexpr (sizeof(T) == 4) {
-    a.tiles = tiles(kShRowsF32);
-    if (grid(a.tiles).x) hipLaunchKernelGGL((attn_shared_f32_kernel<DH>), grid(a.tiles), block, 0, st, a);
-  } else {
-    a.tiles = tiles(kShRowsBF16);
-    if (grid(a.tiles).x) hipLaunchKernelGGL((attn_shared_bf16_kernel<DH>), grid(a.tiles), block, 0, st, a);
+  const dim3 grid((unsigned)((nkeys + 7) / 8 * 8 * a.tiles + own)), block(64 * kShWaves);
+  if (grid.x) {
+    if constexpr (sizeof(T) == 4)
+      hipLaunchKernelGGL((attn_shared_f32_kernel<DH>), grid, block, 0, st, a);
+    else
+      hipLaunchKernelGGL((attn_shared_bf16_kernel<DH>), grid, block, 0, st, a);
   }
   hipLaunchKernelGGL((attn_shared_combine<T, DH>), dim3(a.H, a.n), dim3(DH), 0, st, a);
 }
@@ -576,8 +599,7 @@ int wfd_attn_shared(const void* q, const void* k_cache, const void* v_cache, int
   a.Hkv = Hkv;
   a.ng = ngroups;
   const int64_t pairs = (int64_t)(group_max < n ? group_max : n) * G;
-  const int rt = dtype == kBF16 ? kShRowsBF16 : kShRowsF32;
-  const int64_t tiles = (pairs + rt - 1) / rt;
+  const int64_t tiles = (pairs + kShRows - 1) / kShRows;
   a.pchunks = max_prefix_chunks(prefix_len_max, Hkv);
   a.ochunks = div_up(kv_len_max, kShOwnChunk);
   a.pmax = prefix_len_max;
@@ -592,10 +614,11 @@ int wfd_attn_shared(const void* q, const void* k_cache, const void* v_cache, int
               group_max, prefix_len_max, kv_len_max);
     return kUnsupported;
   }
+  a.tiles = (int)tiles;
   if (dtype == kBF16)
-    Dh == 64 ? launch_shared<bf16_t, 64>(a, pairs, stream) : launch_shared<bf16_t, 128>(a, pairs, stream);
+    Dh == 64 ? launch_shared<bf16_t, 64>(a, stream) : launch_shared<bf16_t, 128>(a, stream);
   else
-    Dh == 64 ? launch_shared<float, 64>(a, pairs, stream) : launch_shared<float, 128>(a, pairs, stream);
+    Dh == 64 ? launch_shared<float, 64>(a, stream) : launch_shared<float, 128>(a, stream);
   return launch_status(me);
 }
 
