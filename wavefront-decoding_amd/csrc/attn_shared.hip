@@ -365,20 +365,22 @@ __global__ __launch_bounds__(64 * kShWaves) __attribute__((amdgpu_waves_per_eu(2
 // fp32: the same on the 32x32x2 MFMA. A lane's operands of K Q^T are four consecutive
 // columns at a time (lane half hf takes columns 8 j + 4 hf + e at step 4 j + e), its
 // S^T register r is key 8 (r / 4) + 4 hf + r % 4, which is also the key it supplies of
-// P^T at step r, and V^T is read from the row-major tile a value at a time, 32
-// consecutive ones a row. One workgroup per CU by LDS, a wave per SIMD.
+// P^T at step r. K goes through LDS; V^T comes straight from the cache, 32 consecutive
+// values of a row to half of the lanes, loaded under the scores, and the next tile of K
+// under P V, into the registers that V leaves. 64 rows x 8000 keys x 16 heads: 125 us
+// (floor 82, its products 55 of them); V through LDS too, which leaves a wave per SIMD,
+// 152; 16 pairs on the 16x16x4 form, operands straight from the cache, 371.
 template <int DH>
-__global__ __launch_bounds__(64 * kShWaves) void attn_shared_f32_kernel(ShArgs a) {
+__global__ __launch_bounds__(64 * kShWaves) __attribute__((amdgpu_waves_per_eu(2))) void attn_shared_f32_kernel(ShArgs a) {
   constexpr int RT = kShRows;
   constexpr int TK = 32;
   constexpr int NDB = DH / 32;
-  constexpr int KP = DH + 4;    // LDS row pitches: K reads 16 bytes of 32 rows, V^T 128 bytes of rows
-  constexpr int VP = DH + 8;    // that are 4 apart
+  constexpr int KP = DH + 4;    // LDS row pitch: 16 bytes of 16 rows are spread over all banks
   constexpr int CPR = DH / 4;   // 16-byte pieces per row
   constexpr int RPI = 64 / CPR;
   constexpr int NLD = TK / RPI;
   constexpr int OP = DH + 4;
-  constexpr int kWaveEls = TK * (KP + VP);
+  constexpr int kWaveEls = TK * KP;
   static_assert(kWaveEls >= RT * OP, "the merge takes the tiles' LDS");
   __shared__ __align__(16) float lds[kWaveEls * kShWaves];
   __shared__ float m_lds[kShWaves * RT];
@@ -389,7 +391,6 @@ __global__ __launch_bounds__(64 * kShWaves) void attn_shared_f32_kernel(ShArgs a
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63, col = lane & 31, hf = lane >> 5;
   float* k_lds = lds + wave * kWaveEls;
-  float* v_lds = k_lds + TK * KP;
 
   const int64_t rs = a.br > 1 ? (int64_t)DH : (int64_t)a.Hkv * DH;
   const int64_t at = kv_offset(it.base, it.g, a.Hkv, DH, a.br) + it.k0 * rs;
@@ -401,17 +402,29 @@ __global__ __launch_bounds__(64 * kShWaves) void attn_shared_f32_kernel(ShArgs a
   };
   const __amdgpu_buffer_rsrc_t kr = rsrc(a.kc), vr = rsrc(a.vc);
   const int lr = lane / CPR, lp = lane % CPR;
-  u32x4 kreg[NLD], vreg[NLD];
-  uint32_t off = (uint32_t)(TK * wave + lr) * rsb + (uint32_t)lp * 16u;
-  auto fetch = [&]() {  // this wave's next tile; zeros past the chunk
+  u32x4 kreg[NLD];
+  float vreg[16][NDB];
+  uint32_t koff = (uint32_t)(TK * wave + lr) * rsb + (uint32_t)lp * 16u;
+  uint32_t voff = (uint32_t)(TK * wave + 4 * hf) * rsb + (uint32_t)col * 4u;
+  const uint32_t next = (uint32_t)(TK * kShWaves) * rsb;
+  // zeros past the chunk
+  auto fetch_k = [&](int q) {  // a quarter of this wave's next tile
 #pragma unroll
-    for (int s = 0; s < NLD; ++s) {
-      kreg[s] = buf_ld16(kr, off + (uint32_t)(RPI * s) * rsb);
-      vreg[s] = buf_ld16(vr, off + (uint32_t)(RPI * s) * rsb);
-    }
-    off += (uint32_t)(TK * kShWaves) * rsb;
+    for (int s = q * NLD / 4; s < (q + 1) * NLD / 4; ++s) kreg[s] = buf_ld16(kr, koff + (uint32_t)(RPI * s) * rsb);
   };
-  fetch();
+  auto fetch_v = [&]() {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const uint32_t row = voff + (uint32_t)(8 * (r >> 2) + (r & 3)) * rsb;
+#pragma unroll
+      for (int db = 0; db < NDB; ++db)
+        vreg[r][db] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(vr, row + 128u * db, 0, 0));
+    }
+    voff += next;
+  };
+#pragma unroll
+  for (int q = 0; q < 4; ++q) fetch_k(q);
+  koff += next;
 
   const float scale = fmaxf(fabsf(a.scale_log2), 1e-37f);  // as in the bf16 kernel
   const uint32_t flip = a.scale_log2 < 0.f ? 0x80000000u : 0u;
@@ -430,11 +443,8 @@ __global__ __launch_bounds__(64 * kShWaves) void attn_shared_f32_kernel(ShArgs a
 
   for (int t0 = TK * wave; t0 < nk; t0 += TK * kShWaves) {  // uniform over the wave
 #pragma unroll
-    for (int s = 0; s < NLD; ++s) {
-      *reinterpret_cast<u32x4*>(k_lds + (RPI * s + lr) * KP + 4 * lp) = kreg[s];
-      *reinterpret_cast<u32x4*>(v_lds + (RPI * s + lr) * VP + 4 * lp) = vreg[s];
-    }
-    fetch();
+    for (int s = 0; s < NLD; ++s) *reinterpret_cast<u32x4*>(k_lds + (RPI * s + lr) * KP + 4 * lp) = kreg[s];
+    fetch_v();
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
@@ -454,12 +464,17 @@ __global__ __launch_bounds__(64 * kShWaves) void attn_shared_f32_kernel(ShArgs a
         if (t0 + 8 * (r >> 2) + 4 * hf + (r & 3) >= nk) sc[r] = -INFINITY;
     }
     sh_softmax<NDB>(sc, o, mref, lrun, scale);
-    const float* vp = v_lds + 4 * hf * VP + col;
 #pragma unroll
-    for (int r = 0; r < 16; ++r)
+    for (int q = 0; q < 4; ++q) {  // the next tile of K takes the registers that V leaves
 #pragma unroll
-      for (int db = 0; db < NDB; ++db)
-        o[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(vp[(8 * (r >> 2) + (r & 3)) * VP + 32 * db], sc[r], o[db], 0, 0, 0);
+      for (int r = 4 * q; r < 4 * q + 4; ++r)
+#pragma unroll
+        for (int db = 0; db < NDB; ++db)
+          o[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(vreg[r][db], sc[r], o[db], 0, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
+      fetch_k(q);
+    }
+    koff += next;
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();  // the next tile overwrites this one
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
