@@ -60,12 +60,51 @@ __device__ __forceinline__ float sm_logit(uint32_t key) {
   return __uint_as_float((key >> 31) ? key ^ 0x80000000u : ~key);
 }
 
-__device__ __forceinline__ uint64_t sm_shfl_xor(uint64_t v, int m) {
-  return (uint64_t)__shfl_xor((unsigned long long)v, m, 64);
+// Wave-wide folds over neighbouring lanes' registers (DPP), a third of the latency of
+// shuffles through LDS; every lane of the wave calls them. fold(lanes 0..l) in lane l.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t sm_dpp(uint32_t v, uint32_t none) {
+  return (uint32_t)__builtin_amdgcn_update_dpp((int)none, (int)v, CTRL, ROWS, 0xf, false);
 }
-__device__ __forceinline__ uint64_t sm_shfl_up(uint64_t v, int m) {
-  return (uint64_t)__shfl_up((unsigned long long)v, m, 64);
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t sm_dpp_add(uint64_t v) {
+  return v + (((uint64_t)sm_dpp<CTRL, ROWS>((uint32_t)(v >> 32), 0) << 32) | sm_dpp<CTRL, ROWS>((uint32_t)v, 0));
 }
+__device__ __forceinline__ uint64_t sm_wave_scan(uint64_t v) {
+  v = sm_dpp_add<0x111, 0xf>(v);  // within rows of 16: from 1, 2, 4, 8 lanes before
+  v = sm_dpp_add<0x112, 0xf>(v);
+  v = sm_dpp_add<0x114, 0xf>(v);
+  v = sm_dpp_add<0x118, 0xf>(v);
+  v = sm_dpp_add<0x142, 0xa>(v);  // a row's last lane to the next row, of each half
+  return sm_dpp_add<0x143, 0xc>(v);  // lane 31 to the upper half
+}
+__device__ __forceinline__ uint64_t sm_last_lane(uint64_t v) {
+  return ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), 63) << 32) |
+         (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, 63);
+}
+__device__ __forceinline__ uint64_t sm_wave_sum(uint64_t v) { return sm_last_lane(sm_wave_scan(v)); }
+template <typename F>
+__device__ __forceinline__ uint32_t sm_wave_fold(uint32_t v, uint32_t none, F f) {
+  v = f(v, sm_dpp<0x111, 0xf>(v, none));
+  v = f(v, sm_dpp<0x112, 0xf>(v, none));
+  v = f(v, sm_dpp<0x114, 0xf>(v, none));
+  v = f(v, sm_dpp<0x118, 0xf>(v, none));
+  v = f(v, sm_dpp<0x142, 0xa>(v, none));
+  v = f(v, sm_dpp<0x143, 0xc>(v, none));
+  return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
+__device__ __forceinline__ uint32_t sm_wave_min(uint32_t v) {
+  return sm_wave_fold(v, 0xffffffffu, [](uint32_t x, uint32_t y) { return min(x, y); });
+}
+__device__ __forceinline__ uint32_t sm_wave_max(uint32_t v) {
+  return sm_wave_fold(v, 0u, [](uint32_t x, uint32_t y) { return max(x, y); });
+}
+__device__ __forceinline__ float sm_wave_max(float v) {
+  return __uint_as_float(sm_wave_fold(__float_as_uint(v), 0xff800000u, [](uint32_t x, uint32_t y) {
+    return __float_as_uint(fmaxf(__uint_as_float(x), __uint_as_float(y)));
+  }));
+}
+__device__ __forceinline__ float sm_wave_min(float v) { return -sm_wave_max(-v); }
 
 struct SmArgs {
   const float* logits;
@@ -90,17 +129,11 @@ constexpr int kSmRowList = 8192;     // tokens that the slabs of a row may list
 constexpr int kSmGuess = 600;        // top-k up to which the list is tried: ~900 tokens are at or above the 600th thread's
 constexpr float kSmMasked = -1e4f;  // logits down to here spread the bins; the others share the last
 
-__device__ __forceinline__ uint64_t sm_wave_sum(uint64_t v) {
-#pragma unroll
-  for (int m = 32; m >= 1; m >>= 1) v += sm_shfl_xor(v, m);
-  return v;
-}
-
 // 2^x for x <= 0 in units of 2^-44, rounded to nearest: x = m / 32 + r, 2^r by its
 // series to r^5 (the rest is below 3e-15 of it), 2^(m / 32) from the table with
-// the exponent added to its bits. Adding 1.5 2^52 (2^52) leaves the nearest integer
-// in the low bits of the sum.
-__device__ __forceinline__ uint64_t sm_exp2(double x, const double* __restrict__ tab) {
+// the exponent added to its bits. Adding 1.5 2^52 leaves the nearest integer in the
+// low bits of the sum, adding and subtracting 2^52 rounds to it.
+__device__ __forceinline__ double sm_exp2(double x, const double* __restrict__ tab) {
   x = fmax(x, -900.);  // also of NaN; far below the least weight
   const double t = fma(x, 32., 6755399441055744.);
   const int k = (int)(uint32_t)__double_as_longlong(t);
@@ -111,7 +144,7 @@ __device__ __forceinline__ uint64_t sm_exp2(double x, const double* __restrict__
   p = fma(p, r, 0.6931471805599453);
   p = fma(p, r, 1.0);
   const double two = __longlong_as_double(__double_as_longlong(tab[k & 31]) + ((long long)((k >> 5) + 44) << 52));
-  return (uint64_t)__double_as_longlong(fma(p, two, 4503599627370496.)) & 0xfffffffffffffull;
+  return fma(p, two, 4503599627370496.) - 4503599627370496.;
 }
 
 // floor(s f) for f in [0, 1), and whether anything was cut off
@@ -186,12 +219,6 @@ struct Sm {
     if constexpr (CAP < 0) {
 #pragma unroll
       for (int c = 0; c < -CAP / kSmChunk; ++c) fetch(c, held[c]);
-    } else if constexpr (CAP > 0) {  // every load first; a thread reads back only what it stores
-      float x[CAP / kSmChunk][4];
-#pragma unroll
-      for (int c = 0; c < CAP / kSmChunk; ++c) fetch(c, x[c]);
-#pragma unroll
-      for (int c = 0; c < CAP / kSmChunk; ++c) s.keep[c * kSmThreads + t] = Elem<float>::pack(x[c]);
     }
     if (t < 32) s.tab[t] = exp2((double)t * 0.03125);
   }
@@ -243,23 +270,15 @@ struct Sm {
     for (int w = 0; w < kSmWaves; ++w) all += s.sum[w];
     return all;
   }
-  __device__ __forceinline__ uint64_t wave_scan(uint64_t v) const {  // inclusive
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) {
-      const uint64_t o = sm_shfl_up(v, m);
-      if (lane >= m) v += o;
-    }
-    return v;
-  }
   __device__ __forceinline__ uint64_t block_scan(uint64_t v) {  // the sum of the threads' v before this one
-    const uint64_t inc = wave_scan(v);
+    const uint64_t inc = sm_wave_scan(v);
     __syncthreads();
     if (lane == 63) s.sum[wave] = inc;
     __syncthreads();
-    uint64_t before = lane < wave ? (uint64_t)s.sum[lane] : 0;  // 16 waves
+    uint64_t before = 0;
 #pragma unroll
-    for (int m = 8; m >= 1; m >>= 1) before += sm_shfl_xor(before, m);
-    return (uint64_t)__shfl((unsigned long long)before, 0, 64) + inc - v;
+    for (int w = 0; w < kSmWaves; ++w) before += w < wave ? (uint64_t)s.sum[w] : 0;
+    return before + inc - v;
   }
   // The bin (thread t holds bin t's sum v) in which base plus the running sum reaches need; before: the sum before it.
   __device__ __forceinline__ uint32_t find_bin(uint64_t v, uint64_t base, uint64_t need, uint64_t& before) {
@@ -274,11 +293,8 @@ struct Sm {
   }
 
   __device__ __forceinline__ void block_range(uint32_t& lo, uint32_t& hi) {
-#pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) {
-      lo = min(lo, (uint32_t)__shfl_xor((int)lo, m, 64));
-      hi = max(hi, (uint32_t)__shfl_xor((int)hi, m, 64));
-    }
+    lo = sm_wave_min(lo);
+    hi = sm_wave_max(hi);
     __syncthreads();
     if (lane == 0) {
       s.lo[wave] = lo;
@@ -297,20 +313,28 @@ struct Sm {
     mine = -INFINITY;
     float lo = INFINITY;
     bool bad = false;
-    each([&](int, const float (&x)[4]) {
+    auto look = [&](int, const float (&x)[4]) {
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         bad |= x[q] != x[q];
         mine = fmaxf(mine, x[q]);
         lo = fminf(lo, x[q] > kSmMasked ? x[q] : INFINITY);
       }
-    });
-    float hi = mine;
+    };
+    if constexpr (CAP > 0) {  // on their way to LDS, every load first; a thread reads back only what it stores
+      float x[CAP / kSmChunk][4];
 #pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) {
-      hi = fmaxf(hi, __shfl_xor(hi, m, 64));
-      lo = fminf(lo, __shfl_xor(lo, m, 64));
+      for (int c = 0; c < CAP / kSmChunk; ++c) fetch(c, x[c]);
+#pragma unroll
+      for (int c = 0; c < CAP / kSmChunk; ++c) {
+        s.keep[c * kSmThreads + t] = Elem<float>::pack(x[c]);
+        look(first_of(c), x[c]);
+      }
+    } else {
+      each(look);
     }
+    const float hi = sm_wave_max(mine);
+    lo = sm_wave_min(lo);
     bad = __ballot(bad) != 0;
     if (lane == 0) {
       s.max[wave] = hi;
@@ -338,11 +362,8 @@ struct Sm {
     nan = __ballot(ws.nan[l] != 0) != 0;
     best = ws.max[l];
     low = ws.min[l];
-#pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) {
-      best = fmaxf(best, __shfl_xor(best, m, 64));
-      low = fminf(low, __shfl_xor(low, m, 64));
-    }
+    best = sm_wave_max(best);
+    low = sm_wave_min(low);
   }
   // false: a greedy row, or one with a NaN or without any possible token
   __device__ __forceinline__ bool parameters() {
@@ -370,8 +391,7 @@ struct Sm {
       for (int q = 3; q >= 0; --q)
         if (e + q < w_end && (nan ? x[q] != x[q] : x[q] == best)) bi = min(bi, e + q);
     });
-#pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) bi = min(bi, __shfl_xor(bi, m, 64));
+    bi = (int)sm_wave_min((uint32_t)bi);
     __syncthreads();
     if (lane == 0) s.lo[wave] = (uint32_t)bi;
     __syncthreads();
@@ -380,9 +400,12 @@ struct Sm {
   }
 
   // --- weights and bins ------------------------------------------------------
-  __device__ __forceinline__ uint64_t weight(float l) const {
-    if (endless) return l == best ? (uint64_t)kSmOne : 0;
+  __device__ __forceinline__ double weight_d(float l) const {  // an integer
+    if (endless) return l == best ? kSmOne : 0.;
     return sm_exp2(((double)l - (double)best) * inv, s.tab);  // of the largest itself: exactly one
+  }
+  __device__ __forceinline__ uint64_t weight(float l) const {
+    return (uint64_t)__double_as_longlong(weight_d(l) + 4503599627370496.) & 0xfffffffffffffull;
   }
   __device__ __forceinline__ int bin_of(float l) const {  // by the distance from the largest
     return l == best ? 0 : (int)fminf((best - l) * scale, (float)(kSmBins - 1));
@@ -418,6 +441,9 @@ struct Sm {
     if (t == 0) s.count = 0;
     __syncthreads();
     each([&](int e, const float (&x)[4]) {
+      // bins go by the distance from the largest: if the nearest of the four is past `to`, all
+      // are (nothing is past the last bin)
+      if ((best - fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]))) * scale > to) return;
       bool in[4];
       int n_in = 0;
       const int room_here = w_end - e;
@@ -449,30 +475,37 @@ struct Sm {
   // min_p leaves; the tokens of bin b that weigh anything to the list, and their weight.
   // false: more than the list holds.
   struct Split {
-    uint64_t all = 0, before = 0, kept = 0, at = 0;  // the thread's
+    uint64_t all, before, kept, at;  // the thread's
   };
   __device__ __forceinline__ bool split(int b, Split& sp) {
     __syncthreads();
     if (t == 0) s.count = 0;
     __syncthreads();
+    // integers up to 512 logits x 2^44 a thread: exact in 53 bits
+    double all = 0., before = 0., at = 0., left_out = 0.;
+    const double least = (double)wmin;
     each([&](int e, const float (&x)[4]) {
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const uint64_t w = weight(x[q]);
+        const double w = weight_d(x[q]);
         const int bin = bin_of(x[q]);
-        sp.all += w;
-        sp.before += bin < b ? w : 0;
-        sp.kept += bin < b && w >= wmin ? w : 0;
-        if (bin == b && w) {
-          sp.at += w;
-          const uint32_t at = atomicAdd(&s.count, 1u);
-          if (at < LIST) {
-            s.list_key[at] = sm_key(x[q]);
-            s.list_idx[at] = e + q;
+        all += w;
+        before = fma(w, bin < b ? 1. : 0., before);
+        if (wmin && bin < b && w < least) left_out += w;
+        if (bin == b && w > 0.) {
+          at += w;
+          const uint32_t to = atomicAdd(&s.count, 1u);
+          if (to < LIST) {
+            s.list_key[to] = sm_key(x[q]);
+            s.list_idx[to] = e + q;
           }
         }
       }
     });
+    sp.all = (uint64_t)all;
+    sp.before = (uint64_t)before;
+    sp.at = (uint64_t)at;
+    sp.kept = (uint64_t)(before - left_out);
     __syncthreads();
     nlist = (int)min(s.count, (uint32_t)LIST);
     return s.count <= LIST;
@@ -669,16 +702,29 @@ struct Sm {
   }
 
   // --- the token ---------------------------------------------------------------
+  // The lane's 4 logits of step c, of 256, of a share [from, to) of the row; in LDS if
+  // it is wave `share`'s.
+  __device__ __forceinline__ void step_of(int from, int to, int share, int c, float (&x)[4]) const {
+    if constexpr (CAP > 0) {
+      if (share >= 0) {
+        Elem<float>::unpack(s.keep[c * kSmThreads + 64 * share + lane], x);
+        return;
+      }
+    }
+    const int e = from + 256 * c + 4 * lane;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) x[q] = e + q < to ? row[e + q] : 0.f;
+  }
   // Lowest index of [from, to), in steps of 256 that seg has the sums of, whose
   // running sum of measure(index, logit), from base on, exceeds target.
   template <typename M>
-  __device__ __forceinline__ int find_in(int from, int to, uint64_t base, uint64_t target, M measure) {
+  __device__ __forceinline__ int find_in(int from, int to, int share, uint64_t base, uint64_t target, M measure) {
     __syncthreads();
     if (wave == 0) {
       const int ns = (to - from + 255) / 256;
       for (int s0 = 0; s0 < ns; s0 += 64) {
         const uint64_t own = s0 + lane < ns ? (uint64_t)s.seg[s0 + lane] : 0;
-        const uint64_t inc = wave_scan(own);
+        const uint64_t inc = sm_wave_scan(own);
         const uint64_t run = base + inc - own;
         const uint64_t hit = __ballot(run <= target && run + own > target);
         if (hit) {
@@ -686,13 +732,15 @@ struct Sm {
           const uint64_t at = (uint64_t)__shfl((unsigned long long)run, b, 64);
           // the step's 256 logits again, 4 a lane
           const int e = from + (s0 + b) * 256 + 4 * lane;
+          float x[4];
+          step_of(from, to, share, s0 + b, x);
           uint64_t v[4], sum = 0;
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
-            v[q] = e + q < to ? measure(e + q, row[e + q]) : 0;
+            v[q] = e + q < to ? measure(e + q, x[q]) : 0;
             sum += v[q];
           }
-          uint64_t r2 = at + wave_scan(sum) - sum;
+          uint64_t r2 = at + sm_wave_scan(sum) - sum;
           if (r2 <= target && r2 + sum > target) {
             int q = 0;
             while (q < 3 && r2 + v[q] <= target) r2 += v[q++];
@@ -700,7 +748,7 @@ struct Sm {
           }
           break;
         }
-        base += (uint64_t)__shfl((unsigned long long)inc, 63, 64);
+        base += sm_last_lane(inc);
       }
     }
     __syncthreads();
@@ -708,16 +756,19 @@ struct Sm {
   }
   // The same over one share [from, to), whose steps the workgroup adds up first.
   template <typename M>
-  __device__ __forceinline__ int find_share(int from, int to, uint64_t base, uint64_t target, M measure) {
+  __device__ __forceinline__ int find_share(int from, int to, int share, uint64_t base, uint64_t target, M measure) {
+    __syncthreads();  // other threads' logits
     for (int c = wave; c * 256 < to - from; c += kSmWaves) {
       const int e = from + 256 * c + 4 * lane;
+      float x[4];
+      step_of(from, to, share, c, x);
       uint64_t v = 0;
 #pragma unroll
-      for (int q = 0; q < 4; ++q) v += e + q < to ? measure(e + q, row[e + q]) : 0;
+      for (int q = 0; q < 4; ++q) v += e + q < to ? measure(e + q, x[q]) : 0;
       v = sm_wave_sum(v);
       if (lane == 0) s.seg[c] = v;
     }
-    return find_in(from, to, base, target, measure);
+    return find_in(from, to, share, base, target, measure);
   }
   template <typename M>
   __device__ __forceinline__ uint64_t own_sum(M measure) {  // the thread's
@@ -743,7 +794,7 @@ struct Sm {
       upto += s.sum[++w];
     } while (upto <= target && w < kSmWaves - 1);
     const int from = begin + w * per_wave;
-    return find_share(from, min(from + per_wave, end), base, target, measure);
+    return find_share(from, min(from + per_wave, end), w, base, target, measure);
   }
   __device__ __forceinline__ int listed_token() {  // every kept token is in the list
     const int ns = (V + 255) / 256;
@@ -757,7 +808,7 @@ struct Sm {
       if (w) atomicAdd(&s.seg[s.list_idx[e] >> 8], (unsigned long long)w);
     }
     const uint64_t total = block_sum(sum);
-    return find_in(0, V, 0, goal(total), [&](int e, float l) { return kept(e, l); });
+    return find_in(0, V, -1, 0, goal(total), [&](int e, float l) { return kept(e, l); });
   }
   // Drops what no k-th token's bin reaches from a list that holds the first k tokens.
   __device__ __forceinline__ void thin_list() {
@@ -857,6 +908,11 @@ struct Sm {
       const int b = (int)find_bin(own, 0, need, before);
       if (collect(b, b, LIST, true)) refine_list(before, need, true);
       else refine_row(need, true);
+    }
+    if (!has_k && !has_p) {
+      Split sp;
+      split(kSmBins, sp);
+      return find_by_waves([&](int e, float l) { return kept(e, l); }, goal(block_sum(sp.kept)));
     }
     if (ties && ties_left) {
       if (ties_listed) {
@@ -1055,7 +1111,7 @@ __global__ __launch_bounds__(kSmThreads) void sample_row_kernel(SmArgs a, SmRowW
   const int lo = slab * kSmSlab, hi = min(lo + kSmSlab, a.V), per_wave = (hi - lo + 63) / 64 * 4;
   const int from = lo + w * per_wave;
   __syncthreads();
-  m.finish(m.find_share(from, min(from + per_wave, hi), base, target, [&](int e, float l) { return m.kept(e, l); }));
+  m.finish(m.find_share(from, min(from + per_wave, hi), -1, base, target, [&](int e, float l) { return m.kept(e, l); }));
 }
 
 }  // namespace wfd
