@@ -23,7 +23,7 @@
 // from the largest logit, that its last token lies in from 32-bit weights; one pass
 // over the exact ones then gives the row's sum, the waves' sums of the bins before
 // and the bin's tokens, in whose order the last one is found (the guess is checked
-// against the exact sums). Two exact passes took 100 rows 50 us instead of 37. Otherwise a histogram says which bin the last kept token lies in, by count or
+// against the exact sums; two exact passes took 100 rows a third longer). Otherwise a histogram says which bin the last kept token lies in, by count or
 // by weight, and a radix select over that bin's tokens (over the row, if they are
 // too many) finds its key; ties with it are kept in index order.
 //
@@ -34,12 +34,14 @@
 // token. What no slab could prepare (a top-k beyond kSmGuess, a list that
 // overflows) the last launch does by itself as for a short row. Slabs for rows of
 // 32000 took one top-p row from 32 to 30 us, but 100 of them from 38 to 43, and one
-// row with top-k from 18 to 24.
+// row with top-k from 18 to 24 (before the steps below were shortened for both).
 //
-// Bound by the one CU a row has (the logits themselves are microseconds): a pass of
-// exact weights is ~11 us of 32000, the rest a dozen steps that each wait for the
-// workgroup. 1 x 32000 with top-k and top-p 18 us, 100 x 32000 mixed 37, 16 x 128000
-// top-p 41 (4 + 8 + 10 + 18 us of launches), 8 x 128000 with top-k 30.
+// Bound by the one CU a row has (the logits themselves are microseconds), there by
+// instructions: 4 waves a SIMD issue one each 4 cycles apiece, so of 32000 logits the
+// exact weights, ~45 instructions each, take 8 us, the 32-bit ones 6, the candidates 4,
+// reading the row 3, and each step that waits for the workgroup 0.4. 1 x 32000 with
+// top-k and top-p 14.4 us, 100 x 32000 mixed 31, 16 x 128000 top-p 38 (4 + 8 + 10 + 16
+// in four launches), 8 x 128000 with top-k 25.
 #include "wfd_common.h"
 
 namespace wfd {
@@ -62,6 +64,7 @@ __device__ __forceinline__ float sm_logit(uint32_t key) {
 
 // Wave-wide folds over neighbouring lanes' registers (DPP), a third of the latency of
 // shuffles through LDS; every lane of the wave calls them. fold(lanes 0..l) in lane l.
+constexpr int kSmQuad1 = 0xb1, kSmQuad2 = 0x4e;  // lane l ^ 1, l ^ 2
 template <int CTRL, int ROWS>
 __device__ __forceinline__ uint32_t sm_dpp(uint32_t v, uint32_t none) {
   return (uint32_t)__builtin_amdgcn_update_dpp((int)none, (int)v, CTRL, ROWS, 0xf, false);
@@ -120,7 +123,7 @@ struct SmArgs {
 };
 
 constexpr int kSmBins = 1024;   // one per thread
-constexpr int kSmFew = 256;          // entries of a list that is put in order
+constexpr int kSmFew = kSmThreads / 4;  // entries of a list that is put in order
 constexpr int kSmShort = 2048;       // slabs of so few logits are listed whole
 constexpr int kSmLong = 32768;       // longest row of one workgroup
 constexpr int kSmSlab = 8192;
@@ -129,21 +132,22 @@ constexpr int kSmRowList = 8192;     // tokens that the slabs of a row may list
 constexpr int kSmGuess = 600;        // top-k up to which the list is tried: ~900 tokens are at or above the 600th thread's
 constexpr float kSmMasked = -1e4f;  // logits down to here spread the bins; the others share the last
 
-// 2^x for x <= 0 in units of 2^-44, rounded to nearest: x = m / 32 + r, 2^r by its
-// series to r^5 (the rest is below 3e-15 of it), 2^(m / 32) from the table with
+// 2^x for x <= 0 in units of 2^-44, rounded to an integer: x = m / 128 + r, 2^r by its
+// series to r^4 (the rest is below 2e-15 of it), 2^(44 + m / 128) from the table with
 // the exponent added to its bits. Adding 1.5 2^52 leaves the nearest integer in the
 // low bits of the sum, adding and subtracting 2^52 rounds to it.
+constexpr int kSmTable = 128;
 __device__ __forceinline__ double sm_exp2(double x, const double* __restrict__ tab) {
   x = fmax(x, -900.);  // also of NaN; far below the least weight
-  const double t = fma(x, 32., 6755399441055744.);
+  const double t = fma(x, (double)kSmTable, 6755399441055744.);
   const int k = (int)(uint32_t)__double_as_longlong(t);
-  const double r = fma(t - 6755399441055744., -0.03125, x);
-  double p = fma(r, 0.0013333558146428443, 0.009618129107628477);
-  p = fma(p, r, 0.05550410866482158);
+  const double r = fma(t - 6755399441055744., -1. / kSmTable, x);
+  double p = fma(r, 0.009618129107628477, 0.05550410866482158);
   p = fma(p, r, 0.24022650695910072);
   p = fma(p, r, 0.6931471805599453);
   p = fma(p, r, 1.0);
-  const double two = __longlong_as_double(__double_as_longlong(tab[k & 31]) + ((long long)((k >> 5) + 44) << 52));
+  const double two =
+      __longlong_as_double(__double_as_longlong(tab[k & (kSmTable - 1)]) + ((long long)(k & -kSmTable) << 45));
   return fma(p, two, 4503599627370496.) - 4503599627370496.;
 }
 
@@ -175,7 +179,7 @@ struct SmShared {
   unsigned long long seg[(CAP > 0 ? CAP : CAP < 0 ? -CAP : kSmMaxVocab) / 256];  // the running sums' steps, in index order
   u32x4 keep[CAP > 0 ? CAP / 4 : 1];
   uint32_t list_key[LIST], list_idx[LIST];
-  double tab[32];
+  double tab[kSmTable];
   float max[kSmWaves], min[kSmWaves];
   unsigned long long sum[kSmWaves];
   uint32_t lo[kSmWaves], hi[kSmWaves];
@@ -220,7 +224,7 @@ struct Sm {
 #pragma unroll
       for (int c = 0; c < -CAP / kSmChunk; ++c) fetch(c, held[c]);
     }
-    if (t < 32) s.tab[t] = exp2((double)t * 0.03125);
+    if (t < kSmTable) s.tab[t] = exp2((double)t * (1. / kSmTable)) * kSmOne;
   }
 
   __device__ __forceinline__ int first_of(int c) const { return begin + wave * per_wave + 256 * c + 4 * lane; }
@@ -404,6 +408,15 @@ struct Sm {
     if (endless) return l == best ? kSmOne : 0.;
     return sm_exp2(((double)l - (double)best) * inv, s.tab);  // of the largest itself: exactly one
   }
+  __device__ __forceinline__ void weights(const float (&x)[4], double (&w)[4]) const {
+    if (endless) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) w[q] = x[q] == best ? kSmOne : 0.;
+    } else {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) w[q] = sm_exp2(((double)x[q] - (double)best) * inv, s.tab);
+    }
+  }
   __device__ __forceinline__ uint64_t weight(float l) const {
     return (uint64_t)__double_as_longlong(weight_d(l) + 4503599627370496.) & 0xfffffffffffffull;
   }
@@ -429,43 +442,57 @@ struct Sm {
     return sm_mul_frac(total, u, rest);
   }
 
+  // The least logit of bins 0..b (bin_of falls as the logit rises): a 64-ary search over
+  // the keys by one wave.
+  __device__ __forceinline__ float least_of(int b) const {
+    if (b < 0) return NAN;  // none compares at or above it
+    if (b >= kSmBins - 1) return -INFINITY;
+    uint32_t lo = 0, hi = sm_key(best);  // bin_of(best) is 0; keys below -inf's are NaN, in the last bin
+    while (lo < hi) {
+      const uint32_t step = (hi - lo) / 64 + 1;
+      const uint32_t at = min(lo + lane * step, hi);
+      const uint64_t in = __ballot(bin_of(sm_logit(at)) <= b);
+      if (in == 0) {
+        lo += 63 * step + 1;
+      } else {
+        const uint32_t f = __builtin_ctzll(in);
+        hi = min(lo + f * step, hi);
+        if (f) lo += (f - 1) * step + 1;
+      }
+    }
+    return sm_logit(hi);
+  }
+  // The logits of bins [b0, b1] are x with x >= from and not x >= past; the list is empty then.
+  __device__ __forceinline__ void bin_range(int b0, int b1, float& from, float& past) {
+    __syncthreads();
+    if (wave < 2) {
+      const float l = least_of(wave == 0 ? b1 : b0 - 1);
+      if (lane == 0) s.max[wave] = l;
+    }
+    if (t == 0) s.count = 0;
+    __syncthreads();
+    from = s.max[0];
+    past = s.max[1];
+  }
+  __device__ __forceinline__ void list(int e, float l) {
+    const uint32_t at = atomicAdd(&s.count, 1u);
+    if (at < LIST) {
+      s.list_key[at] = sm_key(l);
+      s.list_idx[at] = e;
+    }
+  }
   // --- the list ----------------------------------------------------------------
   // Tokens of bins [b0, b1] to the list; false if they are more than room. With
   // `drawable`, without those whose weight is certainly 0 (masked ones, above all): they
   // are never drawn, come last in the order and add to no sum.
   __device__ __forceinline__ bool collect(int b0, int b1, uint32_t room, bool drawable) {
     const float reach = drawable ? (float)inv : 0.f;
-    // bin_of's borders, on its own product: x in [b0, b1 + 1)
-    const float from = (float)b0, to = b1 >= kSmBins - 1 ? INFINITY : (float)(b1 + 1);
-    __syncthreads();
-    if (t == 0) s.count = 0;
-    __syncthreads();
+    float from, past;
+    bin_range(b0, b1, from, past);
     each([&](int e, const float (&x)[4]) {
-      // bins go by the distance from the largest: if the nearest of the four is past `to`, all
-      // are (nothing is past the last bin)
-      if ((best - fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]))) * scale > to) return;
-      bool in[4];
-      int n_in = 0;
-      const int room_here = w_end - e;
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const float d = best - x[q];
-        const float at = x[q] == best ? 0.f : d * scale;
-        in[q] = q < room_here && at >= from && (at < to || to == INFINITY) && !(d * reach > 47.f);
-        n_in += in[q];
-      }
-      if (n_in) {
-        uint32_t at = atomicAdd(&s.count, (uint32_t)n_in);
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-          if (in[q]) {
-            if (at < LIST) {
-              s.list_key[at] = sm_key(x[q]);
-              s.list_idx[at] = e + q;
-            }
-            ++at;
-          }
-      }
+      for (int q = 0; q < 4; ++q)
+        if (x[q] >= from && !(x[q] >= past) && e + q < w_end && !((best - x[q]) * reach > 47.f)) list(e + q, x[q]);
     });
     __syncthreads();
     nlist = (int)min(s.count, (uint32_t)LIST);
@@ -478,29 +505,30 @@ struct Sm {
     uint64_t all, before, kept, at;  // the thread's
   };
   __device__ __forceinline__ bool split(int b, Split& sp) {
-    __syncthreads();
-    if (t == 0) s.count = 0;
-    __syncthreads();
+    float from, past;
+    bin_range(b, b, from, past);
     // integers up to 512 logits x 2^44 a thread: exact in 53 bits
     double all = 0., before = 0., at = 0., left_out = 0.;
     const double least = (double)wmin;
     each([&](int e, const float (&x)[4]) {
+      double w[4];
+      weights(x, w);
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const double w = weight_d(x[q]);
-        const int bin = bin_of(x[q]);
-        all += w;
-        before = fma(w, bin < b ? 1. : 0., before);
-        if (wmin && bin < b && w < least) left_out += w;
-        if (bin == b && w > 0.) {
-          at += w;
-          const uint32_t to = atomicAdd(&s.count, 1u);
-          if (to < LIST) {
-            s.list_key[to] = sm_key(x[q]);
-            s.list_idx[to] = e + q;
-          }
-        }
+        all += w[q];
+        before = fma(w[q], x[q] >= past ? 1. : 0., before);
       }
+      if (wmin) {  // uniform
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          if (x[q] >= past && w[q] < least) left_out += w[q];
+      }
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        if (x[q] >= from && !(x[q] >= past) && w[q] > 0.) {
+          at += w[q];
+          list(e + q, x[q]);
+        }
     });
     sp.all = (uint64_t)all;
     sp.before = (uint64_t)before;
@@ -512,6 +540,7 @@ struct Sm {
   }
   // The bin in which top-p probably ends, by 32-bit weights in units of 2^-31.
   __device__ __forceinline__ int likely_bin() {
+    if (endless) return 0;
     const float f = (float)fmin(inv, 1e30);
     __syncthreads();
     s.hist[t] = 0;
@@ -519,9 +548,9 @@ struct Sm {
     each([&](int, const float (&x)[4]) {
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const float w = endless ? (x[q] == best ? 1.f : 0.f) : __builtin_amdgcn_exp2f((x[q] - best) * f);
-        const uint32_t m = (uint32_t)(w * 2147483648.f);
-        if (m) atomicAdd(&s.hist[bin_of(x[q])], (unsigned long long)m);
+        const float d = best - x[q];
+        const uint32_t m = (uint32_t)__builtin_amdgcn_exp2f(fmaf(d, -f, 31.f));
+        if (m) atomicAdd(&s.hist[(int)fminf(d * scale, (float)(kSmBins - 1))], (unsigned long long)m);
       }
     });
     __syncthreads();
@@ -555,8 +584,7 @@ struct Sm {
   // The token of a list of at most kSmFew: of its n_kept first -- larger logits first,
   // lower indexes first among equals -- those whose weight reaches need(weight of these),
   // with top-p; of these the ones min_p leaves, by index. An entry's place is the number
-  // that come before it, the sum of the kept tokens of lower index likewise: 100 entries
-  // take 0.8 us each time, where a bitonic sort took 3.4.
+  // that come before it, the sum of the kept tokens of lower index likewise.
   __device__ __forceinline__ uint64_t entry(int e) const {
     return ((uint64_t)s.list_key[e] << 32) | (uint32_t)~s.list_idx[e];
   }
@@ -564,13 +592,16 @@ struct Sm {
     __syncthreads();
     s.hist[t] = 0;
     __syncthreads();
-    if (t < nlist) {
-      const uint64_t own = entry(t);
-      int place = 0;
+    const int mine_e = t >> 2;  // four threads an entry, a quarter of the comparisons each
+    const uint64_t own = mine_e < nlist ? entry(mine_e) : 0;
+    uint32_t place = 0;
+    if (mine_e < nlist) {
 #pragma unroll 4
-      for (int e = 0; e < nlist; ++e) place += entry(e) > own;
-      s.hist[place] = own;
+      for (int e = t & 3; e < nlist; e += 4) place += entry(e) > own;
     }
+    place += sm_dpp<kSmQuad1, 0xf>(place, 0);
+    place += sm_dpp<kSmQuad2, 0xf>(place, 0);
+    if ((t & 3) == 0 && mine_e < nlist) s.hist[place] = own;
     __syncthreads();
     return s.hist[t];
   }
@@ -593,16 +624,23 @@ struct Sm {
     s.hist[t] = w;
     if (t < n_kept) s.list_idx[t] = idx;
     __syncthreads();
-    if (t < n_kept) {
-      uint64_t before = 0, total = 0;
+    const int e0 = t >> 2;
+    const bool in = e0 < n_kept;
+    const uint32_t idx0 = in ? s.list_idx[e0] : 0;
+    uint64_t before = 0, total = 0;
+    if (in) {
 #pragma unroll 4
-      for (int e = 0; e < n_kept; ++e) {
+      for (int e = t & 3; e < n_kept; e += 4) {
         const uint64_t o = s.hist[e];
         total += o;
-        before += s.list_idx[e] < idx ? o : 0;
+        before += s.list_idx[e] < idx0 ? o : 0;
       }
+    }
+    total = sm_dpp_add<kSmQuad2, 0xf>(sm_dpp_add<kSmQuad1, 0xf>(total));
+    before = sm_dpp_add<kSmQuad2, 0xf>(sm_dpp_add<kSmQuad1, 0xf>(before));
+    if (in && (t & 3) == 0) {
       const uint64_t target = goal(total);
-      if (before <= target && before + w > target) s.u32 = idx;
+      if (before <= target && before + (uint64_t)s.hist[e0] > target) s.u32 = idx0;
     }
     __syncthreads();
     return (int)s.u32;
