@@ -185,6 +185,28 @@ def test_attention_lengths_and_layouts(gpu, code, dtype, H, Hkv, Dh, block):
     assert not out[0].any() and not out[-1].any()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("H,Hkv,Dh", [(8, 4, 64), (16, 4, 128)])
+def test_attention_of_many_rows_is_that_of_each_alone(gpu, dtype, H, Hkv, Dh):
+    """Rows enough that a workgroup takes all splits of one: the bits of a row alone, whose
+    splits are merged by another launch, and of a call whose longest row could be longer."""
+    S, n = 4000, 150
+    cache, (k, v) = _filled(2 * S, Hkv, Dh, "int8", gpu, 3)
+    g = _gen(Dh)
+    lens = torch.randint(-1, S + 1, (n,), generator=g)
+    lens[:8] = torch.tensor([0, 1, 1024, 1025, 2048, 2049, S, -5])
+    base = torch.randint(0, S, (n,), generator=g)
+    q = (torch.randn(n, H, Dh, generator=g) * 2).to(dtype)
+    args = lambda at: (q[at].to(gpu), cache, base[at].to(gpu), lens[at].int().to(gpu))  # noqa: E731
+    out = ops.attn_decode_q(*args(slice(None)), kv_len_max=S)
+    assert torch.equal(ops.attn_decode_q(*args(slice(None)), kv_len_max=2 * S), out)
+    for i in [*range(12), 60, 149]:
+        assert torch.equal(ops.attn_decode_q(*args(slice(i, i + 1)), kv_len_max=S)[0], out[i])
+        span = slice(int(base[i]), int(base[i]) + max(int(lens[i]), 0))
+        check_attention(out[i], *attend(q[i].double(), k[span].transpose(0, 1), v[span].transpose(0, 1),
+                                        1 / math.sqrt(Dh), 2.0 ** -16 if dtype == torch.bfloat16 else 0.0))
+
+
 @pytest.mark.parametrize("code", CODES)
 def test_attention_reads_no_row_past_its_length(gpu, code):
     """Rows behind the length hold NaN codes and the non-finite mark: no effect. A
