@@ -23,9 +23,10 @@
 // from the largest logit, that its last token lies in from 32-bit weights; one pass
 // over the exact ones then gives the row's sum, the waves' sums of the bins before
 // and the bin's tokens, in whose order the last one is found (the guess is checked
-// against the exact sums; two exact passes took 100 rows a third longer). Otherwise a histogram says which bin the last kept token lies in, by count or
-// by weight, and a radix select over that bin's tokens (over the row, if they are
-// too many) finds its key; ties with it are kept in index order.
+// against the exact sums; two exact passes took 100 rows a third longer). Otherwise a
+// histogram says which bin the last kept token lies in, by count or by weight, and a
+// radix select over that bin's tokens (over the row, if they are too many) finds its
+// key; ties with it are kept in index order.
 //
 // Rows of up to 32768 logits are one workgroup's, which keeps them in LDS. Longer
 // ones are cut into slabs of 8192, a workgroup each, in four launches that leave
@@ -33,8 +34,8 @@
 // the histogram; the weights before the border's bin and its tokens; the row's
 // token. What no slab could prepare (a top-k beyond kSmGuess, a list that
 // overflows) the last launch does by itself as for a short row. Slabs for rows of
-// 32000 took one top-p row from 32 to 30 us, but 100 of them from 38 to 43, and one
-// row with top-k from 18 to 24 (before the steps below were shortened for both).
+// 32000 took one top-p row from 26.8 to 27.5 us, 32 of them from 33.9 to 30.8, but 100
+// from 31.9 to 39.5, and one row with top-k from 14.4 to 21.
 //
 // Bound by the one CU a row has (the logits themselves are microseconds), there by
 // instructions: 4 waves a SIMD issue one each 4 cycles apiece, so of 32000 logits the
@@ -549,7 +550,7 @@ struct Sm {
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const float d = best - x[q];
-        const uint32_t m = (uint32_t)__builtin_amdgcn_exp2f(fmaf(d, -f, 31.f));
+        const uint32_t m = (uint32_t)__builtin_amdgcn_exp2f(fmaxf(fmaf(d, -f, 31.f), -1.f));  // inf * 0 is 0 here
         if (m) atomicAdd(&s.hist[(int)fminf(d * scale, (float)(kSmBins - 1))], (unsigned long long)m);
       }
     });
