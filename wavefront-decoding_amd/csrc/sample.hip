@@ -74,18 +74,21 @@ template <int CTRL, int ROWS>
 __device__ __forceinline__ uint64_t sm_dpp_add(uint64_t v) {
   return v + (((uint64_t)sm_dpp<CTRL, ROWS>((uint32_t)(v >> 32), 0) << 32) | sm_dpp<CTRL, ROWS>((uint32_t)v, 0));
 }
-__device__ __forceinline__ uint64_t sm_wave_scan(uint64_t v) {
-  v = sm_dpp_add<0x111, 0xf>(v);  // within rows of 16: from 1, 2, 4, 8 lanes before
+__device__ __forceinline__ uint64_t sm_row_scan(uint64_t v) {  // within rows of 16 lanes
+  v = sm_dpp_add<0x111, 0xf>(v);  // from 1, 2, 4, 8 lanes before
   v = sm_dpp_add<0x112, 0xf>(v);
   v = sm_dpp_add<0x114, 0xf>(v);
-  v = sm_dpp_add<0x118, 0xf>(v);
-  v = sm_dpp_add<0x142, 0xa>(v);  // a row's last lane to the next row, of each half
-  return sm_dpp_add<0x143, 0xc>(v);  // lane 31 to the upper half
+  return sm_dpp_add<0x118, 0xf>(v);
 }
-__device__ __forceinline__ uint64_t sm_last_lane(uint64_t v) {
-  return ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), 63) << 32) |
-         (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, 63);
+__device__ __forceinline__ uint64_t sm_wave_scan(uint64_t v) {
+  v = sm_dpp_add<0x142, 0xa>(sm_row_scan(v));  // a row's last lane to the next row, of each half
+  return sm_dpp_add<0x143, 0xc>(v);            // lane 31 to the upper half
 }
+__device__ __forceinline__ uint64_t sm_lane(uint64_t v, int lane) {  // lane: uniform
+  return ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32) |
+         (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, lane);
+}
+__device__ __forceinline__ uint64_t sm_last_lane(uint64_t v) { return sm_lane(v, 63); }
 __device__ __forceinline__ uint64_t sm_wave_sum(uint64_t v) { return sm_last_lane(sm_wave_scan(v)); }
 template <typename F>
 __device__ __forceinline__ uint32_t sm_wave_fold(uint32_t v, uint32_t none, F f) {
@@ -182,7 +185,8 @@ struct SmShared {
   uint32_t list_key[LIST], list_idx[LIST];
   double tab[kSmTable];
   float max[kSmWaves], min[kSmWaves];
-  unsigned long long sum[kSmWaves];
+  unsigned long long sum[4][kSmWaves];
+  unsigned long long share[kSmWaves];  // kept weights of the waves' shares
   uint32_t lo[kSmWaves], hi[kSmWaves];
   unsigned long long u64;
   uint32_t u32, count;
@@ -265,29 +269,52 @@ struct Sm {
   }
 
   // --- the workgroup's sums -------------------------------------------------
+  // The waves' sums are 16 lanes of each wave, which adds them up for itself: 16 adds by
+  // every wave took twice the time.
   __device__ __forceinline__ uint64_t block_sum(uint64_t v) {
     v = sm_wave_sum(v);
     __syncthreads();
-    if (lane == 0) s.sum[wave] = v;
+    if (lane == 0) s.sum[0][wave] = v;
     __syncthreads();
-    uint64_t all = 0;
-#pragma unroll
-    for (int w = 0; w < kSmWaves; ++w) all += s.sum[w];
-    return all;
+    return sm_lane(sm_row_scan(s.sum[0][lane & 15]), 15);
   }
-  __device__ __forceinline__ uint64_t block_scan(uint64_t v) {  // the sum of the threads' v before this one
+  __device__ __forceinline__ void block_sums(uint64_t (&v)[4]) {  // v[3] by waves is left in share
+#pragma unroll
+    for (int q = 0; q < 4; ++q) v[q] = sm_wave_sum(v[q]);
+    __syncthreads();
+    if (lane == 0) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) s.sum[q][wave] = v[q];
+      s.share[wave] = v[3];
+    }
+    __syncthreads();
+    const uint64_t run = sm_row_scan(s.sum[lane >> 4][lane & 15]);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) v[q] = sm_lane(run, 16 * q + 15);
+  }
+  __device__ __forceinline__ uint64_t block_scan(uint64_t v, uint64_t& total) {  // the sum of the threads' v before this one
     const uint64_t inc = sm_wave_scan(v);
     __syncthreads();
-    if (lane == 63) s.sum[wave] = inc;
+    if (lane == 63) s.sum[0][wave] = inc;
     __syncthreads();
-    uint64_t before = 0;
-#pragma unroll
-    for (int w = 0; w < kSmWaves; ++w) before += w < wave ? (uint64_t)s.sum[w] : 0;
-    return before + inc - v;
+    const uint64_t run = sm_row_scan(s.sum[0][lane & 15]);
+    total = sm_lane(run, 15);
+    return (wave ? sm_lane(run, wave - 1) : 0) + inc - v;
+  }
+  // The shares' sum, for find_by_waves.
+  __device__ __forceinline__ uint64_t share_sum(uint64_t v) {
+    v = sm_wave_sum(v);
+    __syncthreads();
+    if (lane == 0) s.share[wave] = v;
+    __syncthreads();
+    return sm_lane(sm_row_scan(s.share[lane & 15]), 15);
   }
   // The bin (thread t holds bin t's sum v) in which base plus the running sum reaches need; before: the sum before it.
   __device__ __forceinline__ uint32_t find_bin(uint64_t v, uint64_t base, uint64_t need, uint64_t& before) {
-    const uint64_t run = base + block_scan(v);
+    uint64_t total;
+    return bin_at(v, base + block_scan(v, total), need, before);
+  }
+  __device__ __forceinline__ uint32_t bin_at(uint64_t v, uint64_t run, uint64_t need, uint64_t& before) {
     if (run < need && run + v >= need) {
       s.u32 = t;
       s.u64 = run;
@@ -295,6 +322,13 @@ struct Sm {
     __syncthreads();
     before = s.u64;
     return s.u32;
+  }
+  // The bin in which top-p of all bins' weight is reached.
+  __device__ __forceinline__ uint32_t top_p_bin(uint64_t v, uint64_t& need, uint64_t& before) {
+    uint64_t total;
+    const uint64_t run = block_scan(v, total);
+    need = need_of(total);
+    return bin_at(v, run, need, before);
   }
 
   __device__ __forceinline__ void block_range(uint32_t& lo, uint32_t& hi) {
@@ -306,11 +340,8 @@ struct Sm {
       s.hi[wave] = hi;
     }
     __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kSmWaves; ++w) {
-      lo = min(lo, s.lo[w]);
-      hi = max(hi, s.hi[w]);
-    }
+    lo = sm_wave_min(s.lo[lane & 15]);
+    hi = sm_wave_max(s.hi[lane & 15]);
   }
 
   // --- the row's largest logit, whether there is a NaN, the range of the bins --
@@ -347,15 +378,9 @@ struct Sm {
       s.lo[wave] = bad;
     }
     __syncthreads();
-    nan = false;
-    best = -INFINITY;
-    low = INFINITY;
-#pragma unroll
-    for (int w = 0; w < kSmWaves; ++w) {
-      nan |= s.lo[w] != 0;
-      best = fmaxf(best, s.max[w]);
-      low = fminf(low, s.min[w]);
-    }
+    nan = __ballot(s.lo[lane & 15] != 0) != 0;
+    best = sm_wave_max(s.max[lane & 15]);
+    low = sm_wave_min(s.min[lane & 15]);
     __syncthreads();
   }
   // The same of a long row, from its slabs'.
@@ -555,9 +580,8 @@ struct Sm {
       }
     });
     __syncthreads();
-    const uint64_t own = s.hist[t];
-    uint64_t before;
-    return (int)find_bin(own, 0, need_of(block_sum(own)), before);
+    uint64_t need, before;
+    return (int)top_p_bin(s.hist[t], need, before);
   }
   // The bin that holds the k-th of the threads' largest logits (of `mine`, of the threads
   // that hold any): every one of the first k tokens is in it or before.
@@ -612,7 +636,8 @@ struct Sm {
     const uint32_t key = (uint32_t)(v >> 32), idx = ~(uint32_t)v;
     uint64_t w = t < nlist ? weight(sm_logit(key)) : 0;
     if (has_p) {
-      const uint64_t before = block_scan(w);
+      uint64_t all;
+      const uint64_t before = block_scan(w, all);
       if (t == n_kept - 1) s.u64 = before + w;
       __syncthreads();
       const uint64_t least = need((uint64_t)s.u64);
@@ -709,7 +734,8 @@ struct Sm {
     }
     const uint64_t v = ordered_few();
     const uint64_t w = t < nlist ? weight(sm_logit((uint32_t)(v >> 32))) : 0;
-    const uint64_t before = base + block_scan(w);
+    uint64_t all;
+    const uint64_t before = base + block_scan(w, all);
     if (before < need && before + w >= need) s.u64 = v;
     __syncthreads();
     kk = (uint32_t)(s.u64 >> 32);
@@ -822,7 +848,7 @@ struct Sm {
   // sums say whose share it is in.
   template <typename M, typename A>
   __device__ __forceinline__ int find(M measure, A aim) {
-    return find_by_waves(measure, aim(block_sum(own_sum(measure))));
+    return find_by_waves(measure, aim(share_sum(own_sum(measure))));
   }
   template <typename M>
   __device__ __forceinline__ int find_by_waves(M measure, uint64_t target) {  // from the waves' sums
@@ -830,7 +856,7 @@ struct Sm {
     int w = -1;
     do {  // at most 16 waves; their sums exceed target
       base = upto;
-      upto += s.sum[++w];
+      upto += s.share[++w];
     } while (upto <= target && w < kSmWaves - 1);
     const int from = begin + w * per_wave;
     return find_share(from, min(from + per_wave, end), w, base, target, measure);
@@ -924,34 +950,32 @@ struct Sm {
     if (has_p && !has_k) {
       Split sp;
       const bool fits = split(likely_bin(), sp);
-      const uint64_t need = need_of(block_sum(sp.all)), before = block_sum(sp.before);
-      if (fits && before < need && before + block_sum(sp.at) >= need) {
+      uint64_t v[4] = {sp.all, sp.before, sp.at, sp.kept};
+      block_sums(v);
+      const uint64_t need = need_of(v[0]), before = v[1];
+      if (fits && before < need && before + v[2] >= need) {
         border(before, need);
-        block_sum(sp.kept);  // the waves' sums, to which each adds its listed tokens
+        uint64_t more = 0;  // kept ones of the listed tokens
         for (int e = t; e < nlist; e += kSmThreads) {
           const int idx = (int)s.list_idx[e];
           const uint64_t w = kept(idx, sm_logit(s.list_key[e]));
-          if (w) atomicAdd(&s.sum[(idx - begin) / per_wave], (unsigned long long)w);
+          if (w) atomicAdd(&s.share[(idx - begin) / per_wave], (unsigned long long)w);
+          more += w;
         }
-        __syncthreads();
-        uint64_t total = 0;
-#pragma unroll
-        for (int w = 0; w < kSmWaves; ++w) total += s.sum[w];
-        return find_by_waves([&](int e, float l) { return kept(e, l); }, goal(total));
+        return find_by_waves([&](int e, float l) { return kept(e, l); }, goal(v[3] + block_sum(more)));
       }
     }
     if (has_p) {  // behind a top-k, or with a bin of too many tokens, or at a bin's edge
       const uint64_t own = weigh_bins(s.hist);
-      const uint64_t need = need_of(block_sum(own));
-      uint64_t before;
-      const int b = (int)find_bin(own, 0, need, before);
+      uint64_t need, before;
+      const int b = (int)top_p_bin(own, need, before);
       if (collect(b, b, LIST, true)) refine_list(before, need, true);
       else refine_row(need, true);
     }
     if (!has_k && !has_p) {
       Split sp;
       split(kSmBins, sp);
-      return find_by_waves([&](int e, float l) { return kept(e, l); }, goal(block_sum(sp.kept)));
+      return find_by_waves([&](int e, float l) { return kept(e, l); }, goal(share_sum(sp.kept)));
     }
     if (ties && ties_left) {
       if (ties_listed) {
@@ -1068,9 +1092,8 @@ __global__ __launch_bounds__(kSmThreads) void sample_shares_kernel(SmArgs a, SmR
   __syncthreads();  // the table
   int b = kSmBins;
   if (m.has_p) {
-    const uint64_t own = ws.hist[m.t];
-    uint64_t before;
-    b = (int)m.find_bin(own, 0, m.need_of(m.block_sum(own)), before);
+    uint64_t need, before;
+    b = (int)m.top_p_bin(ws.hist[m.t], need, before);
   }
   SmSlab::Split sp;
   m.split(b, sp);
@@ -1122,9 +1145,8 @@ __global__ __launch_bounds__(kSmThreads) void sample_row_kernel(SmArgs a, SmRowW
   if (m.t >= slabs * kSmWaves) own = 0;
   if (m.has_p) {
     take_list();
-    const uint64_t need = m.need_of(m.block_sum(bin));
-    uint64_t before;
-    m.find_bin(bin, 0, need, before);
+    uint64_t need, before;
+    m.top_p_bin(bin, need, before);
     m.border(before, need);
     __syncthreads();
     sh.hist[m.t] = own;
@@ -1138,8 +1160,8 @@ __global__ __launch_bounds__(kSmThreads) void sample_row_kernel(SmArgs a, SmRowW
     __syncthreads();
     own = sh.hist[m.t];
   }
-  const uint64_t target = m.goal(m.block_sum(own));
-  const uint64_t before = m.block_scan(own);
+  uint64_t total;
+  const uint64_t before = m.block_scan(own, total), target = m.goal(total);
   if (before <= target && before + own > target) {
     sh.u32 = m.t;
     sh.u64 = before;
