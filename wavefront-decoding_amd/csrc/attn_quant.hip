@@ -13,9 +13,9 @@
 // Bound by HBM: (Dh + 1) bytes of K and of V per key and kv head. P.V on the
 // VALU, as in wfd_attn_decode, took 1600 vector instructions per 64 keys of four
 // heads and held 64 rows over 32k keys at 3.3 TB/s; a tile here takes a fifth. 64
-// rows x 4 kv heads x 32.7k e4m3 keys: 400 us, 5.4 TB/s (reads alone, so above the
-// 4.9 of a copy); 112 rows x 16 heads x 128-1200 int8 keys 82 us, 3.8 TB/s (short
-// rows' first loads and merges); 8 rows of 512-778 keys 10.4 us, one tile after
+// rows x 4 kv heads x 32.7k e4m3 keys: 375-400 us, 5.4-5.7 TB/s (reads alone, so above
+// the 4.9 of a copy); 112 rows x 16 heads x 128-1200 int8 keys 78-82 us, 3.8-4.0 TB/s
+// (short rows' first loads and merges); 8 rows of 512-778 keys 10.4 us, one tile after
 // another in 128 workgroups.
 // Work split as there: a workgroup of 8 waves owns one (1024-key split, kv head,
 // query row), its waves take 32-key tiles round-robin, each through LDS of its

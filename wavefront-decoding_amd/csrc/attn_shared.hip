@@ -32,9 +32,9 @@ constexpr int kShMaxHeads = 4096;  // a chunk's keys stay within 32-bit offsets 
 // each for every second CU, while they are at least 128 keys: the parts' traffic
 // grows with the chunks, and a group's pairs and the other groups fill the rest.
 // 64 rows x 8000 keys x 16 heads, 100 rows over three prefixes of 20-32k x 4, and 64
-// over four of 2000 x 16 take 55 / 89 / 58 us, with 256 chunks 59 / 104 / 63, with 64
-// 55 / 87 / 57; 8 rows x 32000 x 4 30.3, 31.5 and 30.2. At most 1024 keys (512: 58 /
-// 105 / 59; 2048 as 1024), and 512 of a row's own (256: 60 / 92 / 56; 1024: 55 / 92 / 56).
+// over four of 2000 x 16 take 53 / 85-88 / 57 us, with 256 chunks 54 / 98 / 60, with 64
+// 54 / 84 / 57; 8 rows x 32000 x 4 26.7, 25.9 and 26.6. At most 1024 keys (512: 55 / 96 /
+// 57; 2048 as 1024), and 512 of a row's own (256: 57 / 90 / 54; 1024: 53 / 88 / 54).
 __host__ __device__ inline int prefix_chunk(int P, int Hkv) {
   const int64_t c = ((int64_t)P * Hkv + kShTarget - 1) / kShTarget;
   const int64_t r = (c + kShMinChunk - 1) / kShMinChunk * kShMinChunk;
@@ -230,12 +230,12 @@ __device__ __forceinline__ void sh_keep(const ShItem& it, int wave, int col, int
 // V^T comes out of the row-major tile by transposing LDS reads. Keys past the
 // chunk read as zeros and score -inf.
 //
-// 64 rows x 8000 keys x 16 heads: 47 us and 7-9 for the merge (floor 41), of which the
-// loads alone take 43; 100 rows x 20-32k x 4 kv heads: 80 + 9, loads alone 60: each
+// 64 rows x 8000 keys x 16 heads: 48 us and 5 for the merge (floor 41), of which the
+// loads alone take 43; 100 rows x 20-32k x 4 kv heads: 79 + 7, loads alone 60: each
 // tile of 32 pairs takes its prefix from the L2 again (740 MB, 12 TB/s), and products
 // and exponentials only partly hide behind them at two waves per SIMD. 64 pairs a
-// wave (69 / 129 us), eight waves sharing the tiles of 64 pairs (56 / 94) and two
-// chains of K Q^T (as one) were no faster.
+// wave (57 -> 69 and 100 -> 129 us), eight waves sharing the tiles of 64 pairs (55 -> 56
+// and 89 -> 94) and two chains of K Q^T (as one) were no faster.
 template <int DH>
 __global__ __launch_bounds__(64 * kShWaves) __attribute__((amdgpu_waves_per_eu(2))) void attn_shared_bf16_kernel(
     ShArgs a) {

@@ -40,9 +40,9 @@
 // Bound by the one CU a row has (the logits themselves are microseconds), there by
 // instructions: 4 waves a SIMD issue one each 4 cycles apiece, so of 32000 logits the
 // exact weights, ~45 instructions each, take 8 us, the 32-bit ones 6, the candidates 4,
-// reading the row 3, and each step that waits for the workgroup 0.4. 1 x 32000 with
-// top-k and top-p 14.4 us, 100 x 32000 mixed 31, 16 x 128000 top-p 38 (4 + 8 + 10 + 16
-// in four launches), 8 x 128000 with top-k 25.
+// reading the row 3, and each step that waits for the workgroup 0.3. 1 x 32000 with
+// top-k and top-p 13 us, 100 x 32000 mixed 28, 16 x 128000 top-p 33 (4 + 8 + 9 + 13 in
+// four launches), 8 x 128000 with top-k 23.
 #include "wfd_common.h"
 
 namespace wfd {
