@@ -34,8 +34,8 @@
 // the histogram; the weights before the border's bin and its tokens; the row's
 // token. What no slab could prepare (a top-k beyond kSmGuess, a list that
 // overflows) the last launch does by itself as for a short row. Slabs for rows of
-// 32000 took one top-p row from 26.8 to 27.5 us, 32 of them from 33.9 to 30.8, but 100
-// from 31.9 to 39.5, and one row with top-k from 14.4 to 21.
+// 32000 took 32 top-p rows from 30.8 to 26.7 us, but 100 of them from 28.8 to 35, one
+// as long, and one row with top-k from 13 to 19.
 //
 // Bound by the one CU a row has (the logits themselves are microseconds), there by
 // instructions: 4 waves a SIMD issue one each 4 cycles apiece, so of 32000 logits the

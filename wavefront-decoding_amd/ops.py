@@ -53,13 +53,14 @@ def _need(cond: bool, msg: str) -> None:
         raise _lib.WfdError(msg)
 
 
-def _need_current(*ts: torch.Tensor | None) -> None:
-    """GPU tensors, all on the device whose stream the launch goes to."""
+def _need_current(*ts: torch.Tensor | None) -> int:
+    """GPU tensors, all on the current device: the stream the launch goes to."""
     dev = torch.cuda.current_device()
     for t in ts:
         if t is not None and t.get_device() != dev:
             _need_cuda(t)
             raise _lib.WfdError(f"operand on {t.device}, but the current device is cuda:{dev}")
+    return torch._C._cuda_getCurrentRawStream(dev)
 
 
 def _table(name: str, t: torch.Tensor, dtype: torch.dtype, size: int) -> None:
@@ -142,6 +143,9 @@ _MAX_WORKSPACES = 32
 
 def attn_workspace_bytes(n: int, H: int, Dh: int, kv_len_max: int) -> int:
     return int(_lib.load().wfd_attn_workspace_bytes(n, H, Dh, kv_len_max))
+
+
+_attn_workspace_bytes = functools.lru_cache(maxsize=1024)(attn_workspace_bytes)
 
 
 def _raw_stream(device: torch.device) -> int:
@@ -280,7 +284,8 @@ def attn_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, p
     row its own rows kv_row_base[i] + [0, kv_len[i]). prefix_len_max and
     kv_len_max bound the lengths (0: none has any), group_max a group's rows
     (None: n)."""
-    _need_current(q, k_cache, v_cache, prefix_row_base, prefix_len, group_first, kv_row_base, kv_len, out, workspace)
+    stream = _need_current(q, k_cache, v_cache, prefix_row_base, prefix_len, group_first, kv_row_base, kv_len, out,
+                           workspace)
     _need(q.dim() == 3 and q.is_contiguous(), "q must be contiguous (n, H, Dh)")
     n, H, Dh = q.shape
     Hkv, cDh, br = kv_layout(k_cache, v_cache)
@@ -299,7 +304,8 @@ def attn_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, p
     _need(group_max >= 0, "group_max must be >= 0")
     if out is None:
         out = torch.empty_like(q)
-    _need(out.shape == q.shape and out.dtype == q.dtype and out.is_contiguous(), "bad out")
+    else:
+        _need(out.shape == q.shape and out.dtype == q.dtype and out.is_contiguous(), "bad out")
     dt, lib = _dt(q), _lib.load()
     if workspace is None:
         workspace = _workspace(attn_shared_workspace_bytes(n, H, Hkv, Dh, prefix_len_max, kv_len_max), q.device)
@@ -308,7 +314,7 @@ def attn_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, p
                              prefix_len.data_ptr(), group_first.data_ptr(), ng, group_max, kv_row_base.data_ptr(),
                              kv_len.data_ptr(), out.data_ptr(), n, H, Hkv, Dh, dt, sc, int(prefix_len_max),
                              int(kv_len_max), workspace.data_ptr(), workspace.numel() * workspace.element_size(),
-                             _stream())
+                             stream)
     _lib.check(rc, "wfd_attn_shared")
     return out
 
@@ -489,7 +495,7 @@ def kv_append_q(k: torch.Tensor, v: torch.Tensor, cache: QuantKV, flat_row: torc
     """Cache row flat_row[i] = k[i] / v[i], quantised (wfd_kv_append_q): k, v
     (n, Hkv, Dh), each row contiguous (views of a fused qkv row will do);
     flat_row int64, distinct rows."""
-    _need_current(k, v, flat_row, cache.k)
+    stream = _need_current(k, v, flat_row, cache.k)
     n = k.shape[0]
     _kv_rows(k, cache, "k")
     _kv_rows(v, cache, "v")
@@ -498,7 +504,7 @@ def kv_append_q(k: torch.Tensor, v: torch.Tensor, cache: QuantKV, flat_row: torc
     width = cache.Hkv * cache.Dh
     ldk, ldv = (t.stride(0) if n > 1 else width for t in (k, v))
     rc = _lib.load().wfd_kv_append_q(k.data_ptr(), ldk, v.data_ptr(), ldv, *cache._ptrs, cache.code,
-                                     cache.block_rows, flat_row.data_ptr(), n, cache.Hkv, cache.Dh, _dt(k), _stream())
+                                     cache.block_rows, flat_row.data_ptr(), n, cache.Hkv, cache.Dh, _dt(k), stream)
     _lib.check(rc, "wfd_kv_append_q")
 
 
@@ -507,7 +513,7 @@ def qkv_rope_append_q(qkv: torch.Tensor, pos: torch.Tensor, rope_cos: torch.Tens
                       q_out: torch.Tensor | None = None) -> torch.Tensor:
     """qkv_rope_append into an 8-bit cache (wfd_qkv_rope_append_q): returns the
     rotated q (the same bits), k (rotated) and v go to rows flat_row."""
-    _need_current(qkv, pos, rope_cos, rope_sin, flat_row, q_out, cache.k)
+    stream = _need_current(qkv, pos, rope_cos, rope_sin, flat_row, q_out, cache.k)
     n = qkv.shape[0]
     _need(qkv.dim() == 2 and qkv.stride(1) == 1 and qkv.shape[1] >= (H + 2 * Hkv) * Dh, "qkv (n, (H+2Hkv)Dh)")
     _table("pos", pos, torch.int32, n)
@@ -515,15 +521,16 @@ def qkv_rope_append_q(qkv: torch.Tensor, pos: torch.Tensor, rope_cos: torch.Tens
     _need(rope_cos.dtype == torch.float32 == rope_sin.dtype and rope_cos.shape == rope_sin.shape
           and rope_cos.dim() == 2 and rope_cos.shape[1] == Dh // 2 and rope_cos.is_contiguous()
           and rope_sin.is_contiguous(), "rope tables: float32 (S, Dh/2)")
-    _need((cache.Hkv, cache.Dh) == (Hkv, Dh), "cache shape mismatch")
+    _need(cache.Hkv == Hkv and cache.Dh == Dh, "cache shape mismatch")
     if q_out is None:
-        q_out = torch.empty(n, H, Dh, dtype=qkv.dtype, device=qkv.device)
-    _need(q_out.is_contiguous() and q_out.numel() >= n * H * Dh and q_out.dtype == qkv.dtype, "q_out (n, H, Dh)")
+        q_out = qkv.new_empty((n, H, Dh))
+    else:
+        _need(q_out.is_contiguous() and q_out.numel() >= n * H * Dh and q_out.dtype == qkv.dtype, "q_out (n, H, Dh)")
     ldq = qkv.stride(0) if n > 1 else (H + 2 * Hkv) * Dh
     rc = _lib.load().wfd_qkv_rope_append_q(qkv.data_ptr(), ldq, pos.data_ptr(), rope_cos.data_ptr(),
                                            rope_sin.data_ptr(), rope_cos.shape[0], flat_row.data_ptr(),
                                            q_out.data_ptr(), *cache._ptrs, cache.code, cache.block_rows, n, H, Hkv,
-                                           Dh, _dt(qkv), _stream())
+                                           Dh, _dt(qkv), stream)
     _lib.check(rc, "wfd_qkv_rope_append_q")
     return q_out
 
@@ -531,18 +538,21 @@ def qkv_rope_append_q(qkv: torch.Tensor, pos: torch.Tensor, rope_cos: torch.Tens
 def kv_read_q(cache: QuantKV, flat_row: torch.Tensor, *, dtype: torch.dtype = torch.bfloat16,
               k_out: torch.Tensor | None = None, v_out: torch.Tensor | None = None):
     """(k, v), each (n, Hkv, Dh) of `dtype`: the values of cache rows flat_row (wfd_kv_read_q)."""
-    _need_current(flat_row, k_out, v_out, cache.k)
+    stream = _need_current(flat_row, k_out, v_out, cache.k)
     _need(flat_row.dtype == torch.int64 and flat_row.dim() == 1 and flat_row.is_contiguous(), "flat_row: int64 (n,)")
     if dtype not in _DT:
         raise _lib.WfdError(f"unsupported dtype {dtype} (float32 / bfloat16)")
-    n, shape = flat_row.numel(), (flat_row.numel(), cache.Hkv, cache.Dh)
-    k_out, v_out = (torch.empty(shape, dtype=dtype, device=cache.k.device) if t is None else t
-                    for t in (k_out, v_out))
+    n = flat_row.numel()
+    shape = (n, cache.Hkv, cache.Dh)
     for name, t in (("k_out", k_out), ("v_out", v_out)):
-        if not (t.shape == shape and t.is_contiguous() and t.dtype == dtype):
+        if t is not None and not (t.shape == shape and t.is_contiguous() and t.dtype == dtype):
             raise _lib.WfdError(f"{name}: (n, Hkv, Dh) of {dtype}")
+    if k_out is None:
+        k_out = torch.empty(shape, dtype=dtype, device=cache.k.device)
+    if v_out is None:
+        v_out = torch.empty_like(k_out)
     rc = _lib.load().wfd_kv_read_q(*cache._ptrs, cache.code, cache.block_rows, flat_row.data_ptr(),
-                                   k_out.data_ptr(), v_out.data_ptr(), n, cache.Hkv, cache.Dh, _DT[dtype], _stream())
+                                   k_out.data_ptr(), v_out.data_ptr(), n, cache.Hkv, cache.Dh, _DT[dtype], stream)
     _lib.check(rc, "wfd_kv_read_q")
     return k_out, v_out
 
@@ -552,7 +562,7 @@ def attn_decode_q(q: torch.Tensor, cache: QuantKV, kv_row_base: torch.Tensor, kv
                   workspace: torch.Tensor | None = None) -> torch.Tensor:
     """attn_decode over an 8-bit cache (wfd_attn_decode_q): q (n, H, Dh), query i
     reads cache rows kv_row_base[i] + [0, kv_len[i])."""
-    _need_current(q, kv_row_base, kv_len, out, workspace, cache.k)
+    stream = _need_current(q, kv_row_base, kv_len, out, workspace, cache.k)
     _need(q.dim() == 3 and q.is_contiguous(), "q must be contiguous (n, H, Dh)")
     n, H, Dh = q.shape
     _need(cache.Dh == Dh, "q and cache head_dim mismatch")
@@ -563,15 +573,16 @@ def attn_decode_q(q: torch.Tensor, cache: QuantKV, kv_row_base: torch.Tensor, kv
     _need(kv_len_max >= 1, "kv_len_max must be >= 1")
     if out is None:
         out = torch.empty_like(q)
-    _need(out.shape == q.shape and out.dtype == q.dtype and out.is_contiguous(), "bad out")
+    else:
+        _need(out.shape == q.shape and out.dtype == q.dtype and out.is_contiguous(), "bad out")
     dt = _dt(q)
     if workspace is None:
-        workspace = attn_workspace(n, H, Dh, kv_len_max, q.device)
+        workspace = _workspace(_attn_workspace_bytes(n, H, Dh, int(kv_len_max)), q.device)
     sc = 1.0 / math.sqrt(Dh) if scale is None else float(scale)
     rc = _lib.load().wfd_attn_decode_q(q.data_ptr(), *cache._ptrs, cache.code, cache.block_rows,
                                        kv_row_base.data_ptr(), kv_len.data_ptr(), out.data_ptr(), n, H, cache.Hkv, Dh,
                                        dt, sc, int(kv_len_max), workspace.data_ptr(),
-                                       workspace.numel() * workspace.element_size(), _stream())
+                                       workspace.numel() * workspace.element_size(), stream)
     _lib.check(rc, "wfd_attn_decode_q")
     return out
 
@@ -929,7 +940,7 @@ def sample(logits: torch.Tensor, u: torch.Tensor, *, temperature: torch.Tensor |
     (float32, top_k int32; None: off), temperature 0 greedy. The outputs are
     argmax's: with `ring`, ring[ring_rows[i]] = out[i]; with `expect`, accept
     flags of the drawn tokens."""
-    _need_current(logits, u, temperature, top_k, top_p, min_p, out, ring, ring_rows, expect, accept, workspace)
+    stream = _need_current(logits, u, temperature, top_k, top_p, min_p, out, ring, ring_rows, expect, accept, workspace)
     _need(logits.dtype == torch.float32 and logits.dim() == 2 and logits.stride(1) == 1, "logits: float32 (n, V)")
     n = logits.shape[0] if n is None else n
     if not 0 <= n <= logits.shape[0]:
@@ -952,7 +963,7 @@ def sample(logits: torch.Tensor, u: torch.Tensor, *, temperature: torch.Tensor |
     rc = _lib.load().wfd_sample(logits.data_ptr(), ld, u.data_ptr(), _p(temperature), _p(top_k), _p(top_p), _p(min_p),
                                 out.data_ptr(), _p(ring), _p(ring_rows), ring.numel() if ring is not None else 0,
                                 _p(expect), acc, n, V, _p(workspace),
-                                0 if workspace is None else workspace.numel() * workspace.element_size(), _stream())
+                                0 if workspace is None else workspace.numel() * workspace.element_size(), stream)
     _lib.check(rc, "wfd_sample")
     return out
 
