@@ -303,3 +303,20 @@ def test_top_p_at_the_edge_of_a_bin(gpu, V):
         p.append(float(np.nextafter(share, np.float32(i % 2), dtype=np.float32) if i % 4 < 2 else share))
     check(gpu, logits, torch.rand(n, generator=g).tolist(), t, None, p)
     check(gpu, logits, [LAST] * n, t, None, p)
+
+
+@pytest.mark.parametrize("V", [300, 20000, 60000])
+@pytest.mark.parametrize("t", [INF, 1e30, 1e-30, 1e-45])
+def test_extreme_temperatures_over_masked_rows(gpu, V, t):
+    g = torch.Generator().manual_seed(V)
+    n = 6
+    rows = torch.randn(n, V, generator=g) * 3
+    rows[1, ::2] = -INF
+    rows[2, : V - 7] = -INF
+    rows[3, 5:] = torch.finfo(torch.float32).min
+    rows[4, [1, V - 1]] = rows[4].max() + 1  # two largest
+    u = torch.rand(n, generator=g).tolist()
+    check(gpu, rows, u, [t] * n)
+    check(gpu, rows, u, [t] * n, None, [0.6] * n)
+    check(gpu, rows, u, [t] * n, [50] * n, [0.6] * n)
+    check(gpu, rows, u, [t] * n, None, [0.9] * n, [0.5] * n)

@@ -14,11 +14,10 @@
 // kernel's layout, the companions or the run -- and a border is off by 2^-45 per
 // token. u, p and their products with the sums are exact (64 x 64 -> 128 bits).
 //
-// Where the kept tokens are few -- top-k, or a top-p whose tokens hold enough of
-// the weight -- they are found without ordering the row: of the 1024 threads'
-// largest logits, at least k are no smaller than the k-th, so every one of the
-// first k tokens is at or above it, and few others are. Those go to a list in LDS,
-// which is put in order (one entry a thread) if it is short, and top-k, top-p and
+// Where top-k keeps few tokens they are found without ordering the row: of the 1024
+// threads' largest logits, at least k are no smaller than the k-th, so every one of
+// the first k tokens is at or above it, and few others are. Those go to a list in LDS,
+// which is put in order (four threads an entry) if it is short, and top-k, top-p and
 // min_p are positions in it. A top-p alone guesses the bin, of 1024 by the distance
 // from the largest logit, that its last token lies in from 32-bit weights; one pass
 // over the exact ones then gives the row's sum, the waves' sums of the bins before
