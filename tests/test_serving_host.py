@@ -196,6 +196,18 @@ def test_sampler_parameters_and_numbers():
     assert (made.seed, made.temperature, made.top_k, made.top_p) == (5, 0.5, 7, 1.0)
 
 
+def test_batch_schedulers_refuse_to_sample():
+    """They compare greedy ids, on the device where they can: a sampling policy would decode greedily."""
+    from wavefront_decoding_amd.policy import SampledPolicy
+    from wavefront_decoding_amd.scheduler_batch import generate_dtv_batch, generate_wavefront_batch
+
+    policy = SampledPolicy(8, 2)
+    with pytest.raises(ValueError, match="greedily"):
+        generate_wavefront_batch(None, None, 4, policy)
+    with pytest.raises(ValueError, match="greedily"):
+        generate_dtv_batch(None, None, 4, policy, 2)
+
+
 # ---------------------------------------------------------------------------
 # shared prefixes
 # ---------------------------------------------------------------------------

@@ -280,6 +280,11 @@ def _settle(lane: Lane, verifies, draft, gold: dict, cache, decide) -> None:
         lane.enqueue(gold[id(draft)], draft.position + 1)
 
 
+def _need_greedy(policy: SsdPolicy) -> None:
+    if policy.mode != "greedy":
+        raise ValueError(f"the batch schedulers decode greedily, not {policy.mode!r} (scheduler.py samples)")
+
+
 @torch.no_grad()
 def generate_wavefront_batch(blocks, prompt_ids, max_new_tokens, policy: SsdPolicy, emus=None,
                              prefilled: SharedPrefill | None = None) -> BatchTrace:
@@ -290,6 +295,7 @@ def generate_wavefront_batch(blocks, prompt_ids, max_new_tokens, policy: SsdPoli
     kernel compares them, and the tick reads back one accept flag per C row
     while every id stays on the device (read once at the end). Other blocks
     compare the ids on the host."""
+    _need_greedy(policy)
     emulated = emus is not None and all(e is not None for e in emus)
     greedy = emus is None or all(e is None for e in emus)
     on_device = greedy and getattr(blocks, "device_accept", False) and hasattr(blocks, "run_passes")
@@ -382,6 +388,7 @@ def generate_dtv_batch(blocks, prompt_ids, max_new_tokens, policy: SsdPolicy, dr
     lane past it; if all k hold, the last source's argmax is a free bonus
     token. Lanes drift apart freely; P, R and C run once per tick over the
     union of what every live lane needs."""
+    _need_greedy(policy)
     if draft_length < 1 or draft_length + 1 > getattr(blocks, "max_in_flight", draft_length + 1):
         raise ValueError(f"draft_length={draft_length}: a round keeps draft_length + 1 sources in flight, "
                          f"at most {getattr(blocks, 'max_in_flight', '?')} fit")
