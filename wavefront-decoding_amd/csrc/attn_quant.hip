@@ -20,7 +20,7 @@
 // Work split as there: a workgroup of 8 waves owns one (1024-key split, kv head,
 // query row), its waves take 32-key tiles round-robin, each through LDS of its
 // own a tile ahead; the waves merge through LDS in fixed order and a row's splits
-// in attn_combine_kernel, all a function of kv_len only, so a row's bits do not
+// in attn_q_combine, all a function of kv_len only, so a row's bits do not
 // depend on the launch.
 #include "attn_combine.h"
 #include "quant.h"
@@ -327,7 +327,7 @@ attn_q_split_kernel(AttnQArgs a) {
   __syncthreads();  // the next split's tiles take the LDS; this one's partial is written
   }
   if (ns == 1 || nsp < ns) return;
-  // a row whose splits were all this workgroup's: attn_combine_kernel's sums, on
+  // a row whose splits were all this workgroup's: attn_merge_parts' sums, on
   // partials that this workgroup wrote
   for (int idx = threadIdx.x; idx < G * (DH / 4); idx += 64 * NW) {
     const int m = idx / (DH / 4), d = 4 * (idx % (DH / 4));
@@ -348,6 +348,15 @@ attn_q_split_kernel(AttnQArgs a) {
   }
 }
 
+template <typename T, int DH>
+__global__ __launch_bounds__(kMergeThreads) void attn_q_combine(AttnQArgs a) {
+  const int h = blockIdx.x, i = blockIdx.y;
+  const int ns = (min(a.kl[i], a.ms * kAttnSplit) + kAttnSplit - 1) / kAttnSplit;
+  if (ns <= 1) return;  // finished by its split's workgroup
+  const int64_t row = (int64_t)i * a.H + h;
+  attn_merge_parts<T, DH>(a.po, a.pml, ns, [&](int s) { return row * a.ms + s; }, (T*)a.out + row * DH);
+}
+
 // Splits a workgroup takes, one after the other. A row of up to four splits is one
 // workgroup's where the rows alone make 1024 splits (two rounds of workgroups): it
 // finishes the row itself, with the combine kernel's arithmetic, and neither that
@@ -366,8 +375,7 @@ static void launch_attn_q(const AttnQArgs& a, hipStream_t st) {
   const int wgs = (a.ms + a.spw - 1) / a.spw;
   hipLaunchKernelGGL((attn_q_split_kernel<T, CODE, DH>), dim3(wgs, a.Hkv, a.n), dim3(64 * kAqWaves), 0, st, a);
   if (wgs > 1)  // some query may span several workgroups
-    hipLaunchKernelGGL((attn_combine_kernel<T, DH, true>), dim3(a.H, a.n), dim3(DH), 0, st, a.po, a.pml, a.kl,
-                       (T*)a.out, a.H, a.ms);
+    hipLaunchKernelGGL((attn_q_combine<T, DH>), dim3(a.H, a.n), dim3(kMergeThreads), 0, st, a);
 }
 
 }  // namespace wfd

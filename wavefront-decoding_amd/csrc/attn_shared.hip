@@ -25,7 +25,6 @@ constexpr int kShMaxChunk = 1024;
 constexpr int kShOwnChunk = 512;
 constexpr int kShTarget = 128;   // chunks x kv heads aimed at
 constexpr int kShMaxG = 16;
-constexpr int kShCombine = 256;  // threads of the merge
 constexpr int kShMaxHeads = 4096;  // a chunk's keys stay within 32-bit offsets of its first
 
 // Keys per chunk of a prefix of P keys: 128 chunks over the kv heads, a workgroup
@@ -372,7 +371,8 @@ __global__ __launch_bounds__(64 * kShWaves) __attribute__((amdgpu_waves_per_eu(2
 // (floor 82; its products alone, by count, 55); V through LDS too, which leaves a wave per SIMD,
 // 152; 16 pairs on the 16x16x4 form, operands straight from the cache, 371.
 template <int DH>
-__global__ __launch_bounds__(64 * kShWaves) __attribute__((amdgpu_waves_per_eu(2))) void attn_shared_f32_kernel(ShArgs a) {
+__global__ __launch_bounds__(64 * kShWaves) __attribute__((amdgpu_waves_per_eu(2))) void attn_shared_f32_kernel(
+    ShArgs a) {
   constexpr int RT = kShRows;
   constexpr int TK = 32;
   constexpr int NDB = DH / 32;
@@ -487,19 +487,11 @@ __global__ __launch_bounds__(64 * kShWaves) __attribute__((amdgpu_waves_per_eu(2
   sh_leave<DH, OP, RT>(a, it, lds, m_lds, l_lds, at_lds);
 }
 
-// One row's parts, prefix chunks then its own: slot q of the workgroup, DH / 4 threads
-// of 4 columns, merges parts q, q + NS, ... in that order, four at a time (loads
-// together, one rescale of the sums), and the slots are merged in theirs. All parts of
-// up to 4 NS are in flight at once: 100 rows x 16 heads x ~30 parts 7.6 us, where a
-// thread per column took 11. The row's group is found by one wave-wide look at
-// group_first per 64 groups.
+// One row's parts, prefix chunks then its own. The row's group is found by one
+// wave-wide look at group_first per 64 groups.
 template <typename T, int DH>
-__global__ __launch_bounds__(kShCombine) void attn_shared_combine(ShArgs a) {
-  constexpr int TPS = DH / 4, NS = kShCombine / TPS, B = 4;
-  __shared__ __align__(16) float o_lds[NS][DH];
-  __shared__ float m_lds[NS], l_lds[NS];
+__global__ __launch_bounds__(kMergeThreads) void attn_shared_combine(ShArgs a) {
   const int h = blockIdx.x, i = blockIdx.y, lane = threadIdx.x & 63;
-  const int slot = threadIdx.x / TPS, d = 4 * (threadIdx.x % TPS);
   const int own = div_up(min(a.rlen[i], a.omax), kShOwnChunk);
   int P = 0;
   for (int j0 = 0; j0 < a.ng; j0 += 64) {  // uniform
@@ -510,60 +502,9 @@ __global__ __launch_bounds__(kShCombine) void attn_shared_combine(ShArgs a) {
   }
   P = min(P, a.pmax);
   const int np = P > 0 ? div_up(P, prefix_chunk(P, a.Hkv)) : 0;
-  const int ns = np + own;
-  const int64_t base = ((int64_t)i * a.H + h) * (a.pchunks + a.ochunks);
-  float M = -INFINITY, L = 0.f;
-  f32x4 O = {0.f, 0.f, 0.f, 0.f};
-  for (int s0 = slot; s0 < ns; s0 += B * NS) {
-    float mv[B], lv[B];
-    f32x4 ov[B];
-    float mb = M;
-#pragma unroll
-    for (int b = 0; b < B; ++b) {
-      const int s = min(s0 + b * NS, ns - 1);
-      const int64_t p = base + (s < np ? s : a.pchunks + s - np);
-      const float2 ml = *reinterpret_cast<const float2*>(a.pml + 2 * p);
-      ov[b] = *reinterpret_cast<const f32x4*>(a.po + p * DH + d);
-      mv[b] = s0 + b * NS < ns ? ml.x : -INFINITY;
-      lv[b] = ml.y;
-    }
-#pragma unroll
-    for (int b = 0; b < B; ++b) mb = fmaxf(mb, mv[b]);
-    const float corr = M == -INFINITY ? 1.f : exp2f(M - mb);  // nothing but zeros (or a NaN to keep) so far
-    L *= corr;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) O[e] *= corr;
-    M = mb;
-#pragma unroll
-    for (int b = 0; b < B; ++b) {
-      if (s0 + b * NS < ns) {
-        const float f = mv[b] == -INFINITY ? 0.f : exp2f(mv[b] - M);
-        L = fmaf(lv[b], f, L);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) O[e] = fmaf(ov[b][e], f, O[e]);
-      }
-    }
-  }
-  *reinterpret_cast<f32x4*>(&o_lds[slot][d]) = O;
-  if (d == 0) {
-    m_lds[slot] = M;
-    l_lds[slot] = L;
-  }
-  __syncthreads();
-  if (threadIdx.x >= DH) return;
-  const int c = threadIdx.x;
-  M = -INFINITY;
-  L = 0.f;
-  float out = 0.f;
-#pragma unroll
-  for (int q = 0; q < NS; ++q) M = fmaxf(M, m_lds[q]);
-#pragma unroll
-  for (int q = 0; q < NS; ++q) {
-    const float f = m_lds[q] == -INFINITY ? 0.f : exp2f(m_lds[q] - M);
-    L = fmaf(l_lds[q], f, L);
-    out = fmaf(o_lds[q][c], f, out);
-  }
-  Elem<T>::store((T*)a.out + ((int64_t)i * a.H + h) * DH + c, attn_finish_nan(out, L));
+  const int64_t row = (int64_t)i * a.H + h, base = row * (a.pchunks + a.ochunks);
+  attn_merge_parts<T, DH>(a.po, a.pml, np + own, [&](int s) { return base + (s < np ? s : a.pchunks + s - np); },
+                          (T*)a.out + row * DH);
 }
 
 template <typename T, int DH>
@@ -576,7 +517,7 @@ static void launch_shared(const ShArgs& a, hipStream_t st) {
     else
       hipLaunchKernelGGL((attn_shared_bf16_kernel<DH>), grid, block, 0, st, a);
   }
-  hipLaunchKernelGGL((attn_shared_combine<T, DH>), dim3(a.H, a.n), dim3(kShCombine), 0, st, a);
+  hipLaunchKernelGGL((attn_shared_combine<T, DH>), dim3(a.H, a.n), dim3(kMergeThreads), 0, st, a);
 }
 
 }  // namespace wfd
@@ -597,8 +538,8 @@ int wfd_attn_shared(const void* q, const void* k_cache, const void* v_cache, int
                     size_t ws_bytes, hipStream_t stream) {
   using namespace wfd;
   const char* me = "wfd_attn_shared";
-  if (n < 0 || H <= 0 || Hkv <= 0 || H % Hkv != 0 || H > kShMaxHeads || ngroups < 0 || group_max < 0 || kv_block_rows < 0 ||
-      prefix_len_max < 0 || kv_len_max < 0) {
+  if (n < 0 || H <= 0 || Hkv <= 0 || H % Hkv != 0 || H > kShMaxHeads || ngroups < 0 || group_max < 0 ||
+      kv_block_rows < 0 || prefix_len_max < 0 || kv_len_max < 0) {
     set_error("%s: bad shape n=%d H=%d Hkv=%d ngroups=%d group_max=%d prefix_len_max=%d kv_len_max=%d", me, n, H, Hkv,
               ngroups, group_max, prefix_len_max, kv_len_max);
     return kBadArg;

@@ -132,7 +132,7 @@ constexpr int kSmLong = 32768;       // longest row of one workgroup
 constexpr int kSmSlab = 8192;
 constexpr int kSmSlabs = kSmMaxVocab / kSmSlab;
 constexpr int kSmRowList = 8192;     // tokens that the slabs of a row may list
-constexpr int kSmGuess = 600;        // top-k up to which the list is tried: ~900 tokens are at or above the 600th thread's
+constexpr int kSmGuess = 600;        // top-k to which the list is tried: ~900 tokens reach the 600th thread's
 constexpr float kSmMasked = -1e4f;  // logits down to here spread the bins; the others share the last
 
 // 2^x for x <= 0 in units of 2^-44, rounded to an integer: x = m / 128 + r, 2^r by its
@@ -179,7 +179,7 @@ struct SmRowWs {
 template <int CAP, int LIST>
 struct SmShared {
   unsigned long long hist[kSmBins];
-  unsigned long long seg[(CAP > 0 ? CAP : CAP < 0 ? -CAP : kSmMaxVocab) / 256];  // the running sums' steps, in index order
+  unsigned long long seg[(CAP > 0 ? CAP : CAP < 0 ? -CAP : kSmMaxVocab) / 256];  // the running sums' steps
   u32x4 keep[CAP > 0 ? CAP / 4 : 1];
   uint32_t list_key[LIST], list_idx[LIST];
   double tab[kSmTable];
@@ -291,7 +291,8 @@ struct Sm {
 #pragma unroll
     for (int q = 0; q < 4; ++q) v[q] = sm_lane(run, 16 * q + 15);
   }
-  __device__ __forceinline__ uint64_t block_scan(uint64_t v, uint64_t& total) {  // the sum of the threads' v before this one
+  // The sum of the threads' v before this one.
+  __device__ __forceinline__ uint64_t block_scan(uint64_t v, uint64_t& total) {
     const uint64_t inc = sm_wave_scan(v);
     __syncthreads();
     if (lane == 63) s.sum[0][wave] = inc;
@@ -457,7 +458,7 @@ struct Sm {
     const uint64_t w = weight(l);
     return w >= wmin ? w : 0;
   }
-  __device__ __forceinline__ uint64_t need_of(uint64_t sum) const {  // the weight that top-p asks of sum, at least the least
+  __device__ __forceinline__ uint64_t need_of(uint64_t sum) const {  // what top-p asks of sum, at least 1
     bool rest;
     const uint64_t need = sm_mul_frac(sum, p > 0.f ? p : 0.f, rest);
     return rest || need == 0 ? need + 1 : need;
@@ -1120,7 +1121,8 @@ __global__ __launch_bounds__(kSmThreads) void sample_row_kernel(SmArgs a, SmRowW
   m.largest_of(ws, slabs);
   __syncthreads();  // the table
   if (!m.parameters()) {  // the first slab that has it
-    const bool has = m.lane < slabs && (m.nan ? ws.nan[min(m.lane, slabs - 1)] != 0 : ws.max[min(m.lane, slabs - 1)] == m.best);
+    const int l = min(m.lane, slabs - 1);
+    const bool has = m.lane < slabs && (m.nan ? ws.nan[l] != 0 : ws.max[l] == m.best);
     const int slab = __builtin_ctzll(__ballot(has));
     Sm<0, kSmRowList> one(a, sh, blockIdx.x, slab * kSmSlab, min((slab + 1) * kSmSlab, a.V));
     one.best = m.best;
@@ -1171,7 +1173,8 @@ __global__ __launch_bounds__(kSmThreads) void sample_row_kernel(SmArgs a, SmRowW
   const int lo = slab * kSmSlab, hi = min(lo + kSmSlab, a.V), per_wave = (hi - lo + 63) / 64 * 4;
   const int from = lo + w * per_wave;
   __syncthreads();
-  m.finish(m.find_share(from, min(from + per_wave, hi), -1, base, target, [&](int e, float l) { return m.kept(e, l); }));
+  m.finish(m.find_share(from, min(from + per_wave, hi), -1, base, target,
+                        [&](int e, float l) { return m.kept(e, l); }));
 }
 
 }  // namespace wfd
