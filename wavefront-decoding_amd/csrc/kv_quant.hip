@@ -5,7 +5,7 @@
 // few shuffles within those lanes, the codes leave as 8 bytes a lane and the
 // exponent as one byte from the row's first lane. Bound by memory: every value
 // is read once and every code written once. 8192 bf16 rows of 16 heads x 128 take
-// 23.5 us to write (4.3 TB/s; a large copy reaches 4.9) and 19.6 to read back; the
+// 21 us to write (4.8 TB/s; a large copy reaches 4.9) and 19.6 to read back; the
 // few rows of a decode step 2.7 us a launch, the launch itself.
 #include <type_traits>
 
@@ -58,6 +58,12 @@ __device__ __forceinline__ void write_row(const float (&x)[8], int sub, int64_t 
   if (sub == 0) exps[off / (8 * LPR)] = (uint8_t)b;
 }
 
+// bf16 lanes take a K and a V row, 32 bytes of loads in flight as an fp32 lane has of
+// one: 8192 rows x 16 heads x 128 in 21 us where a row a lane group took 23.8 (fp32
+// pairs: 72.6 -> 76).
+template <typename T>
+constexpr bool kAppendPair = sizeof(T) == 2;
+
 template <typename T, int CODE, int DH>
 __global__ __launch_bounds__(kQThreads) void kv_append_q_kernel(const T* __restrict__ k, int64_t ldk,
                                                                 const T* __restrict__ v, int64_t ldv,
@@ -67,16 +73,28 @@ __global__ __launch_bounds__(kQThreads) void kv_append_q_kernel(const T* __restr
                                                                 const int64_t* __restrict__ flat_row, int n,
                                                                 int Hkv) {
   constexpr int LPR = DH / 8;
-  const int64_t unit = ((int64_t)blockIdx.x * kQThreads + threadIdx.x) / LPR;  // (token, K or V, head)
+  const int64_t unit = ((int64_t)blockIdx.x * kQThreads + threadIdx.x) / LPR;
   const int sub = threadIdx.x % LPR;
-  const int i = (int)(unit / (2 * Hkv));
-  if (i >= n) return;
-  const int r = (int)(unit - (int64_t)i * 2 * Hkv);
-  const bool isv = r >= Hkv;
-  const int h = isv ? r - Hkv : r;
-  float x[8];
-  load8((isv ? v + i * ldv : k + i * ldk) + h * DH + 8 * sub, x);
-  write_row<CODE, LPR>(x, sub, kv_offset(flat_row[i], h, Hkv, DH, block_rows), isv ? vc : kc, isv ? ve : ke);
+  if constexpr (kAppendPair<T>) {  // (token, head): K and V
+    const int i = (int)(unit / Hkv);
+    if (i >= n) return;
+    const int h = (int)(unit - (int64_t)i * Hkv);
+    float x[8], y[8];
+    load8(k + i * ldk + h * DH + 8 * sub, x);
+    load8(v + i * ldv + h * DH + 8 * sub, y);
+    const int64_t off = kv_offset(flat_row[i], h, Hkv, DH, block_rows);
+    write_row<CODE, LPR>(x, sub, off, kc, ke);
+    write_row<CODE, LPR>(y, sub, off, vc, ve);
+  } else {  // (token, K or V, head)
+    const int i = (int)(unit / (2 * Hkv));
+    if (i >= n) return;
+    const int r = (int)(unit - (int64_t)i * 2 * Hkv);
+    const bool isv = r >= Hkv;
+    const int h = isv ? r - Hkv : r;
+    float x[8];
+    load8((isv ? v + i * ldv : k + i * ldk) + h * DH + 8 * sub, x);
+    write_row<CODE, LPR>(x, sub, kv_offset(flat_row[i], h, Hkv, DH, block_rows), isv ? vc : kc, isv ? ve : ke);
+  }
 }
 
 // y to the float on its side of zero, last bit set if anything was cut off:
@@ -217,7 +235,7 @@ int wfd_kv_append_q(const void* k, int64_t ldk, const void* v, int64_t ldv, void
     set_error("%s: k, v, their row pitches and the codes must be 16-byte aligned", me);
     return kBadArg;
   }
-  const unsigned grid = q_grid((int64_t)n * 2 * Hkv, Dh);
+  const unsigned grid = q_grid((int64_t)n * Hkv * (dtype == kBF16 ? 1 : 2), Dh);
   if (!grid) {
     set_error("%s: n=%d Hkv=%d beyond the grid", me, n, Hkv);
     return kUnsupported;
