@@ -210,7 +210,7 @@ int wfd_attn_varlen(const void* q, const void* k, const void* v, const int32_t* 
  * any) and group_max >= every group's rows size the grid. workspace >=
  * wfd_attn_shared_workspace_bytes(...). Dh 64 or 128, H / Hkv up to 16, any
  * scale; at most 65535 rows. fp32 statistics, sums and division; for bf16 the
- * probabilities meet V as bf16 (as in wfd_attn_prefill). A row's bits depend on
+ * probabilities meet V with 16 significant bits. A row's bits depend on
  * its own q, keys and lengths and on Hkv, not on its group's other rows (they
  * are not wfd_attn_decode's, whose key order differs). Infinities and NaN in K
  * and V reach only the rows that attend them.

@@ -138,8 +138,7 @@ class Answers:
 
     def check(self, ticks):
         """Every operator of every step, from its own inputs, against its definition."""
-        # half steps of the probabilities: bf16 in one term (shared), in two (8-bit)
-        p_step = 2.0 ** -16 if self.code else 2.0 ** -8
+        p_step = 2.0 ** -16  # probabilities meet V in two bf16 terms
         H, HKV, DH = self.H, self.HKV, self.DH
         slots = [tuple(self.keys(b, self.own + len(ticks))) for b in range(self.n)]
         for t, (qkv, q, o, logits, u, ids) in enumerate(ticks):

@@ -33,7 +33,8 @@ constexpr int kShMaxHeads = 4096;  // a chunk's keys stay within 32-bit offsets 
 // 64 rows x 8000 keys x 16 heads, 100 rows over three prefixes of 20-32k x 4, and 64
 // over four of 2000 x 16 take 53 / 85-88 / 57 us, with 256 chunks 54 / 98 / 60, with 64
 // 54 / 84 / 57; 8 rows x 32000 x 4 26.7, 25.9 and 26.6. At most 1024 keys (512: 55 / 96 /
-// 57; 2048 as 1024), and 512 of a row's own (256: 57 / 90 / 54; 1024: 53 / 88 / 54).
+// 57; 2048 as 1024), and 512 of a row's own (256: 57 / 90 / 54; 1024: 53 / 88 / 54;
+// all with P in one term).
 __host__ __device__ inline int prefix_chunk(int P, int Hkv) {
   const int64_t c = ((int64_t)P * Hkv + kShTarget - 1) / kShTarget;
   const int64_t r = (c + kShMinChunk - 1) / kShMinChunk * kShMinChunk;
@@ -230,7 +231,7 @@ __device__ __forceinline__ void sh_keep(const ShItem& it, int wave, int col, int
 // chunk read as zeros and score -inf.
 //
 // 64 rows x 8000 keys x 16 heads: 48 us and 5 for the merge (floor 41), of which the
-// loads alone take 43; 100 rows x 20-32k x 4 kv heads: 79 + 7, loads alone 60: each
+// loads alone take 43; 100 rows x 20-32k x 4 kv heads: 82-86 + 7, loads alone 60: each
 // tile of 32 pairs takes its prefix from the L2 again (740 MB, 12 TB/s), and products
 // and exponentials only partly hide behind them at two waves per SIMD. 64 pairs a
 // wave (57 -> 69 and 100 -> 129 us), eight waves sharing the tiles of 64 pairs (55 -> 56
@@ -339,17 +340,25 @@ __global__ __launch_bounds__(64 * kShWaves) __attribute__((amdgpu_waves_per_eu(2
         if (t0 + 16 * (r >> 3) + 8 * hf + (r & 7) >= nk) sc[r] = -INFINITY;
     }
     sh_softmax<NDB>(sc, o, mref, lrun, scale);
-    // the one rounding before the output's: P meets V as bf16 (half a step: 2^-8
-    // of P, at random signs), where fp32 products would take 8 times the MFMA time
-    u32x4 pb[2];
+    // P meets V in two bf16 terms, half a step of 2^-16 of it. In one (2^-8, at random
+    // signs) the output was 0.0023 of its norm off instead of 0.0017, which is its own
+    // rounding, for 0-5 % less time; fp32 products take 8 times the MFMA time.
 #pragma unroll
-    for (int s = 0; s < 2; ++s)
+    for (int s = 0; s < 2; ++s) {
+      u32x4 hi, lo;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) pb[s][e] = f32x2_to_bf16x2_bits(sc[8 * s + 2 * e], sc[8 * s + 2 * e + 1]);
+      for (int e = 0; e < 4; ++e) {
+        const float x = sc[8 * s + 2 * e], y = sc[8 * s + 2 * e + 1];
+        hi[e] = f32x2_to_bf16x2_bits(x, y);
+        lo[e] = f32x2_to_bf16x2_bits(x - __uint_as_float(hi[e] << 16), y - __uint_as_float(hi[e] & 0xffff0000u));
+      }
 #pragma unroll
-    for (int s = 0; s < 2; ++s)
-#pragma unroll
-      for (int db = 0; db < NDB; ++db) o[db] = sh_mfma32(vt_frag(db, s), pb[s], o[db]);
+      for (int db = 0; db < NDB; ++db) {
+        const u32x4 vf = vt_frag(db, s);
+        o[db] = sh_mfma32(vf, lo, o[db]);
+        o[db] = sh_mfma32(vf, hi, o[db]);
+      }
+    }
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();  // the next tile overwrites this one
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
