@@ -213,7 +213,8 @@ int wfd_attn_varlen(const void* q, const void* k, const void* v, const int32_t* 
  * probabilities meet V with 16 significant bits. A row's bits depend on
  * its own q, keys and lengths and on Hkv, not on its group's other rows (they
  * are not wfd_attn_decode's, whose key order differs). Infinities and NaN in K
- * and V reach only the rows that attend them.
+ * and V reach only the rows that attend them, an infinity in V as itself (opposite
+ * ones, and one whose probability is 0 in fp32, as NaN).
  * Replaces: what wfd_attn_decode replaces for sequences whose prompts are equal;
  *   the reference stores and reads such a prompt once per sequence
  *   (src/decoding/huginn_blocks_batch.py:179-203,265-285).

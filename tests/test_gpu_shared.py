@@ -225,3 +225,32 @@ def test_captured_call_with_moving_lengths(gpu):
         torch.cuda.synchronize()
         assert torch.equal(captured, eager)
         c.check(eager)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("H,Hkv,Dh", [(4, 4, 64), (8, 2, 128)])
+def test_infinities_in_v_come_out_as_themselves(gpu, dtype, H, Hkv, Dh):
+    """An infinity in V is the row's result in that column, opposite ones and NaN are NaN, and
+    every other value keeps its bits, beside a row whose query is NaN too."""
+    groups = [(0, 900, 30), (900, 40, 12)]
+    own = [(1000 + 5 * i, (7 * i) % 60) for i in range(42)]
+    c = Case(gpu, dtype, H, Hkv, Dh, 1300, groups, own, seed=Dh)
+    c.q[4, H - 1, 3] = math.nan
+    want = c.run().cpu()
+    c.v[17, 0, 1] = c.v[899, 0, 1] = c.v[300, 0, 2] = math.inf
+    c.v[18, 0, 3] = c.v[400, 0, 4] = c.v[899, 0, 4] = -math.inf
+    c.v[300, 0, 5], c.v[301, 0, 5], c.v[310, 0, 6] = math.inf, -math.inf, math.nan
+    c.v[500, 0, 7], c.v[501, 0, 7] = math.inf, math.nan
+    c.v[905, Hkv - 1, :8] = math.inf
+    c.v[1000 + 5 * 9, 0, 8] = -math.inf  # a row's own key
+    got = c.run().cpu()
+    infinite = 0
+    for i in range(42):
+        at = c.keys(i)
+        ref, _ = attend(c.q[i].double(), c.k[at].double().transpose(0, 1), c.v[at].double().transpose(0, 1),
+                        1 / math.sqrt(Dh))
+        special = ~torch.isfinite(ref)
+        infinite += int(ref.isinf().sum())
+        assert torch.equal(got[i][special].double().nan_to_num(nan=7.0), ref[special].nan_to_num(nan=7.0))
+        assert torch.equal(got[i][~special], want[i][~special])
+    assert infinite > 200

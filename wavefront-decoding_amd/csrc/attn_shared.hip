@@ -124,10 +124,11 @@ __device__ __forceinline__ int64_t sh_pair(const ShArgs& a, const ShItem& it, in
 // Merges the workgroup's key streams, one per wave, and leaves the part: o_lds
 // [wave][pair][DH, pitch OP], m / l [wave][pair]. A thread first has one pair's
 // weights and place (it would otherwise compute them for every value), then takes
-// four columns of a pair at a time.
+// four columns of a pair at a time. With `again` it only replaces the NaN that it left
+// before (a thread has the same values both times) where the streams now hold an infinity.
 template <int DH, int OP, int RT>
 __device__ __forceinline__ void sh_leave(const ShArgs& a, const ShItem& it, const float* o_lds, const float* m_lds,
-                                         float* l_lds, int64_t* at_lds) {
+                                         float* l_lds, int64_t* at_lds, bool again) {
   const int ms = a.pchunks + a.ochunks;
   if (threadIdx.x < it.nr) {
     const int r = threadIdx.x;
@@ -158,7 +159,13 @@ __device__ __forceinline__ void sh_leave(const ShArgs& a, const ShItem& it, cons
 #pragma unroll
       for (int e = 0; e < 4; ++e) O[e] = fmaf(ow[e], f, O[e]);
     }
-    *reinterpret_cast<f32x4*>(a.po + at_lds[r] * DH + d) = O;
+    f32x4* left = reinterpret_cast<f32x4*>(a.po + at_lds[r] * DH + d);
+    if (again) {  // uniform
+      const f32x4 was = *left;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) O[e] = was[e] != was[e] && fabsf(O[e]) == INFINITY ? O[e] : was[e];
+    }
+    *left = O;
   }
 }
 
@@ -255,6 +262,7 @@ __global__ __launch_bounds__(64 * kShWaves) __attribute__((amdgpu_waves_per_eu(2
   __shared__ float m_lds[kShWaves * RT];
   __shared__ float l_lds[kShWaves * RT];
   __shared__ int64_t at_lds[RT];
+  __shared__ int nan_lds;
   ShItem it;
   if (!sh_item<RT>(a, it)) return;  // uniform
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -275,8 +283,10 @@ __global__ __launch_bounds__(64 * kShWaves) __attribute__((amdgpu_waves_per_eu(2
   const int lr = lane / CPR, lp = lane % CPR;  // row within a load, piece
   u32x4 kreg[NLD], vreg[NLD];
   uint32_t off[NLD];
+  auto first_tile = [&]() {
 #pragma unroll
-  for (int s = 0; s < NLD; ++s) off[s] = (uint32_t)(TK * wave + RPI * s + lr) * rsb + (uint32_t)lp * 16u;
+    for (int s = 0; s < NLD; ++s) off[s] = (uint32_t)(TK * wave + RPI * s + lr) * rsb + (uint32_t)lp * 16u;
+  };
   auto fetch = [&]() {  // this wave's next tile; zeros past the chunk
 #pragma unroll
     for (int s = 0; s < NLD; ++s) {
@@ -285,6 +295,7 @@ __global__ __launch_bounds__(64 * kShWaves) __attribute__((amdgpu_waves_per_eu(2
       off[s] += (uint32_t)(TK * kShWaves) * rsb;
     }
   };
+  first_tile();
   fetch();
 
   // Q as the B operand; a negative scale's sign goes to q, so that scores order as
@@ -311,6 +322,13 @@ __global__ __launch_bounds__(64 * kShWaves) __attribute__((amdgpu_waves_per_eu(2
     return u32x4{x.x, x.y, y.x, y.y};
   };
 
+  // A second pass over the chunk where the first left a NaN: the low terms below have
+  // either sign, and zero, so that an infinity in V comes out as a NaN. With the high
+  // term, of p's sign, in their place it is itself unless the sum is a NaN all the same.
+  // Asking costs 0.3 us a launch (4 rows x 512 keys 10.2 -> 10.5), nothing past the noise
+  // in the long cases.
+  bool again = false;
+  for (;;) {  // uniform over the workgroup
   float mref = -INFINITY, lrun = 0.f;
   f32x16 o[NDB];
 #pragma unroll
@@ -351,6 +369,7 @@ __global__ __launch_bounds__(64 * kShWaves) __attribute__((amdgpu_waves_per_eu(2
         const float x = sc[8 * s + 2 * e], y = sc[8 * s + 2 * e + 1];
         hi[e] = f32x2_to_bf16x2_bits(x, y);
         lo[e] = f32x2_to_bf16x2_bits(x - __uint_as_float(hi[e] << 16), y - __uint_as_float(hi[e] & 0xffff0000u));
+        lo[e] = again ? hi[e] : lo[e];
       }
 #pragma unroll
       for (int db = 0; db < NDB; ++db) {
@@ -364,11 +383,27 @@ __global__ __launch_bounds__(64 * kShWaves) __attribute__((amdgpu_waves_per_eu(2
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
   }
 
+  if (threadIdx.x == 0) nan_lds = 0;
   __syncthreads();  // every wave's tiles are done: the merge takes their LDS
   float* o_lds = reinterpret_cast<float*>(lds);
   sh_keep<DH, OP, RT>(it, wave, col, hf, o, mref, lrun, o_lds, m_lds, l_lds);
+  float sum[NDB] = {};  // NaN if any of them is
+#pragma unroll
+  for (int r = 0; r < 16; ++r)
+#pragma unroll
+    for (int db = 0; db < NDB; ++db) sum[db] += o[db][r];
+#pragma unroll
+  for (int db = 1; db < NDB; ++db) sum[0] += sum[db];
+  if (sum[0] != sum[0]) nan_lds = 1;
   __syncthreads();
-  sh_leave<DH, OP, RT>(a, it, o_lds, m_lds, l_lds, at_lds);
+  const bool more = !again && nan_lds;
+  sh_leave<DH, OP, RT>(a, it, o_lds, m_lds, l_lds, at_lds, again);
+  if (!more) break;
+  again = true;
+  __syncthreads();
+  first_tile();
+  fetch();
+  }
 }
 
 // fp32: the same on the 32x32x2 MFMA. A lane's operands of K Q^T are four consecutive
@@ -493,7 +528,7 @@ __global__ __launch_bounds__(64 * kShWaves) __attribute__((amdgpu_waves_per_eu(2
   __syncthreads();  // every wave's tiles are done: the merge takes their LDS
   sh_keep<DH, OP, RT>(it, wave, col, hf, o, mref, lrun, lds, m_lds, l_lds);
   __syncthreads();
-  sh_leave<DH, OP, RT>(a, it, lds, m_lds, l_lds, at_lds);
+  sh_leave<DH, OP, RT>(a, it, lds, m_lds, l_lds, at_lds, false);
 }
 
 // One row's parts, prefix chunks then its own. The row's group is found by one
