@@ -267,7 +267,8 @@ int wfd_kv_append(const void* k, const void* v, void* k_cache, void* v_cache, in
  * 1.9 * 2^127 to infinity.) The codes have the layout kv_block_rows gives a
  * cache of one byte per element, the exponent bytes the same layout without Dh:
  * (rows, Hkv), or (rows / B, Hkv, B). Dh 64 or 128; codes 16-byte aligned.
- * It takes (Dh + 1) / (2 Dh) of a bf16 cache's bytes.
+ * It takes (Dh + 1) / (2 Dh) of a bf16 cache's bytes. Calls of 2^34 values
+ * of K or more (rotating q too: n (H + 2 Hkv) Dh of 2^35) may be refused.
  *
  * wfd_kv_append_q: cache row flat_row[i] = k[i] / v[i], (Hkv, Dh) of `dtype` at
  * row pitches ldk / ldv (elements). Rows of flat_row are distinct, except that

@@ -262,3 +262,18 @@ def test_shared_alignment_workspace_and_grid_are_checked():
     assert call(size=16) == -4 and b"workspace" in lib.wfd_last_error()
     assert call(n=70000, size=1 << 60) == -2 and b"beyond the grid" in lib.wfd_last_error()
     assert call(n=60000, gm=60000, ng=60000, pm=1 << 24, size=1 << 60) == -2
+
+
+@pytest.mark.skipif(torch.cuda.device_count() > 0, reason="made-up device addresses: run only where no GPU is "
+                    "visible, so a regressed check cannot launch a kernel on them")
+def test_quant_calls_past_the_grid_are_refused():
+    """2^24 workgroups of 256 threads are more than a launch takes in x."""
+    lib = _lib.load()
+    p, W = [4096] * 4, 1 << 24
+    app = lambda n, dt: lib.wfd_kv_append_q(4096, 128, 4096, 128, *p, 0, 0, 4096, n, 2, 64, dt, None)  # noqa: E731
+    read = lambda n: lib.wfd_kv_read_q(*p, 0, 0, 4096, 4096, 4096, n, 2, 64, 1, None)  # noqa: E731
+    rope = lambda n: lib.wfd_qkv_rope_append_q(4096, 512, 4096, 4096, 4096, 8, 4096, 4096, *p, 0, 0, n, 4, 2, 64,  # noqa: E731
+                                               1, None)
+    for call, rows in ((lambda n: app(n, 1), 16), (lambda n: app(n, 0), 8), (read, 8), (rope, 4)):  # rows a workgroup
+        assert call(rows * W) == -2 and b"beyond the grid" in lib.wfd_last_error()
+        assert call(rows * (W - 1) + 1) == -2

@@ -182,10 +182,11 @@ __global__ __launch_bounds__(kQThreads) void kv_read_q_kernel(const uint8_t* __r
   store8((isv ? v_out : k_out) + ((int64_t)i * Hkv + h) * DH + 8 * sub, x);
 }
 
-// Workgroups over `units` rows of Dh values; 0 if they are past the grid.
+// Workgroups over `units` rows of Dh values; 0 if they are past the grid, whose threads
+// in x stay below 2^32.
 static unsigned q_grid(int64_t units, int Dh) {
   const int64_t wgs = (units * (Dh / 8) + kQThreads - 1) / kQThreads;
-  return wgs <= 0x7fffffff ? (unsigned)wgs : 0u;
+  return wgs * kQThreads <= 0xffffffffll ? (unsigned)wgs : 0u;
 }
 
 // Runs f<T, CODE, DH>() for the run-time type, code and head size (checked before).
