@@ -254,3 +254,19 @@ def test_infinities_in_v_come_out_as_themselves(gpu, dtype, H, Hkv, Dh):
         assert torch.equal(got[i][special].double().nan_to_num(nan=7.0), ref[special].nan_to_num(nan=7.0))
         assert torch.equal(got[i][~special], want[i][~special])
     assert infinite > 200
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_more_workgroups_than_a_grid_row(gpu, dtype):
+    """Empty groups, and bounds far above the lengths, until the workgroups pass 2^24: the
+    bits of the call that counts only what is there."""
+    groups = [(0, 1100, 300), (1100, 77, 200)]
+    own = [(1200 + i, i % 40) for i in range(512)]
+    c = Case(gpu, dtype, 16, 4, 64, 1800, groups, own, seed=7)
+    want = c.run()
+    q, k, v, base, length, first, *rest = c.args()
+    empty = 2098  # groups between the two
+    base, length = (torch.cat([t[:1], t[1:].expand(empty), t[1:]]) for t in (base, length))
+    first = torch.cat([first[:1], first[1:2].expand(empty + 1), first[2:]])
+    got = ops.attn_shared(q, k, v, base, length, first, *rest, prefix_len_max=32768, kv_len_max=600)
+    assert torch.equal(got, want)

@@ -61,6 +61,7 @@ struct ShArgs {
   void* out;
   float *po, *pml;
   int n, H, Hkv, ng, tiles, pchunks, ochunks, pmax, omax;
+  uint32_t items;
   float scale_log2;
 };
 
@@ -73,13 +74,14 @@ struct ShItem {
 };
 
 // The workgroup's item; false if it has none (a shorter prefix, a smaller group).
-// Prefix items first, RT pairs each. The tiles of one (group, chunk, head) read
+// Prefix items first, RT pairs each. The items are the grid's workgroups in order, x first. The tiles of one (group, chunk, head) read
 // the same keys: they are 8 workgroups apart, so they run on one XCD at about the
 // same time, and one of them brings the keys to its L2.
 template <int RT>
 __device__ __forceinline__ bool sh_item(const ShArgs& a, ShItem& it) {
   const uint32_t G = a.H / a.Hkv;
-  const uint32_t x = blockIdx.x;  // the host keeps the grid below 2^31
+  const uint32_t x = blockIdx.y * gridDim.x + blockIdx.x;  // the host keeps the items below 2^31
+  if (x >= a.items) return false;  // the grid's last row
   const uint32_t nkeys = (uint32_t)a.ng * a.pchunks * a.Hkv;
   const uint32_t nprefix = (nkeys + 7) / 8 * 8 * a.tiles;
   if (x < nprefix) {
@@ -551,15 +553,20 @@ __global__ __launch_bounds__(kMergeThreads) void attn_shared_combine(ShArgs a) {
                           (T*)a.out + row * DH);
 }
 
+// A launch has fewer than 2^32 threads in x. A multiple of 8, as sh_item's order wants.
+constexpr uint32_t kShGridX = 1u << 23;
+
 template <typename T, int DH>
-static void launch_shared(const ShArgs& a, hipStream_t st) {
+static void launch_shared(ShArgs& a, hipStream_t st) {
   const int64_t nkeys = (int64_t)a.ng * a.pchunks * a.Hkv, own = (int64_t)a.n * a.ochunks * a.Hkv;
-  const dim3 grid((unsigned)((nkeys + 7) / 8 * 8 * a.tiles + own)), block(64 * kShWaves);
-  if (grid.x) {
+  a.items = (uint32_t)((nkeys + 7) / 8 * 8 * a.tiles + own);
+  const dim3 grid(a.items < kShGridX ? a.items : kShGridX, (a.items + kShGridX - 1) / kShGridX), block(64 * kShWaves);
+  if (a.items) {
     if constexpr (sizeof(T) == 4)
       hipLaunchKernelGGL((attn_shared_f32_kernel<DH>), grid, block, 0, st, a);
     else
       hipLaunchKernelGGL((attn_shared_bf16_kernel<DH>), grid, block, 0, st, a);
+    if (hipPeekAtLastError() != hipSuccess) return;  // no parts to merge
   }
   hipLaunchKernelGGL((attn_shared_combine<T, DH>), dim3(a.H, a.n), dim3(kMergeThreads), 0, st, a);
 }
