@@ -270,3 +270,12 @@ def test_more_workgroups_than_a_grid_row(gpu, dtype):
     first = torch.cat([first[:1], first[1:2].expand(empty + 1), first[2:]])
     got = ops.attn_shared(q, k, v, base, length, first, *rest, prefix_len_max=32768, kv_len_max=600)
     assert torch.equal(got, want)
+
+
+def test_bounds_of_the_largest_length(gpu):
+    """2^31 - 1 as "no bound": every key counts, the bits are those of close bounds."""
+    c = Case(gpu, torch.bfloat16, 1, 1, 64, 42000, [(0, 40000, 2)], [(40000, 1500), (41000, 7)], seed=8)
+    want = c.run()
+    top = 2 ** 31 - 1
+    ws = torch.empty(ops.attn_shared_workspace_bytes(2, 1, 1, 64, top, top), dtype=torch.uint8, device=gpu)  # 3.3 GB
+    assert torch.equal(c.run(prefix_len_max=top, kv_len_max=top, workspace=ws), want)

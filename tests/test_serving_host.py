@@ -277,3 +277,16 @@ def test_quant_calls_past_the_grid_are_refused():
     for call, rows in ((lambda n: app(n, 1), 16), (lambda n: app(n, 0), 8), (read, 8), (rope, 4)):  # rows a workgroup
         assert call(rows * W) == -2 and b"beyond the grid" in lib.wfd_last_error()
         assert call(rows * (W - 1) + 1) == -2
+
+
+def test_shared_workspace_of_lengths_up_to_the_largest():
+    """The parts of bounds next to 2^31 are counted, not wrapped; what the call refuses has none."""
+    ws = _lib.load().wfd_attn_shared_workspace_bytes
+    size = lambda parts, Dh: sum(-(-x // 256) * 256 for x in (parts * Dh * 4, parts * 8))  # noqa: E731
+    top = 2 ** 31 - 1
+    for length in (top, top - 127, top - 128, top - 511, top - 1022, top - 1023, top - 1024, top - 2048):
+        assert ws(4, 16, 4, 128, length, 0) == size(4 * 16 * -(-length // 1024), 128)
+        assert ws(4, 16, 4, 64, 0, length) == size(4 * 16 * -(-length // 512), 64)
+    assert ws(65535, 4096, 4096, 128, top, top) == size(65535 * 4096 * (2 ** 21 + 2 ** 22), 128)
+    for n, H, Dh in ((65536, 4, 64), (4, 4097, 64), (4, 4, 1 << 20), (top, top, top)):
+        assert ws(n, H, H, Dh, top, top) == 0

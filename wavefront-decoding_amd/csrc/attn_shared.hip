@@ -25,6 +25,7 @@ constexpr int kShMaxChunk = 1024;
 constexpr int kShOwnChunk = 512;
 constexpr int kShTarget = 128;   // chunks x kv heads aimed at
 constexpr int kShMaxG = 16;
+constexpr int kShMaxRows = 65535;  // the merge's grid
 constexpr int kShMaxHeads = 4096;  // a chunk's keys stay within 32-bit offsets of its first
 
 // Keys per chunk of a prefix of P keys: 128 chunks over the kv heads, a workgroup
@@ -41,7 +42,7 @@ __host__ __device__ inline int prefix_chunk(int P, int Hkv) {
   return (int)(r < kShMinChunk ? kShMinChunk : (r > kShMaxChunk ? kShMaxChunk : r));
 }
 
-__host__ __device__ inline int div_up(int a, int b) { return a <= 0 ? 0 : (a + b - 1) / b; }
+__host__ __device__ inline int div_up(int a, int b) { return a <= 0 ? 0 : (a - 1) / b + 1; }
 
 // The most chunks any prefix of up to P keys makes (a chunk has at least
 // P Hkv / kShTarget keys unless it has 1024).
@@ -92,13 +93,13 @@ __device__ __forceinline__ bool sh_item(const ShArgs& a, ShItem& it) {
     it.g = (int)(kg % a.Hkv);
     const uint32_t jc = kg / a.Hkv;
     const int c = (int)(jc % a.pchunks), j = (int)(jc / a.pchunks);
-    const int P = min(a.plen[j], a.pmax);
+    const int P = max(min(a.plen[j], a.pmax), 0);
     const int ck = prefix_chunk(P, a.Hkv);
     it.row0 = a.gfirst[j];
     it.p0 = tile * RT;
     it.nr = min((min(a.gfirst[j + 1], a.n) - it.row0) * (int)G - it.p0, RT);
-    it.k0 = c * ck;
-    it.k1 = min(it.k0 + ck, P);
+    it.k0 = c * ck;  // below 2^31: there are at most 2^21 chunks of 1024
+    it.k1 = it.k0 + min(ck, P - it.k0);
     it.part = c;
     it.base = a.pbase[j];
   } else {
@@ -110,7 +111,7 @@ __device__ __forceinline__ bool sh_item(const ShArgs& a, ShItem& it) {
     it.p0 = 0;
     it.nr = (int)G;
     it.k0 = c * kShOwnChunk;
-    it.k1 = min(it.k0 + kShOwnChunk, min(a.rlen[it.row0], a.omax));
+    it.k1 = it.k0 + min(kShOwnChunk, max(min(a.rlen[it.row0], a.omax), 0) - it.k0);
     it.part = a.pchunks + c;
     it.base = a.rbase[it.row0];
   }
@@ -577,7 +578,10 @@ extern "C" {
 
 size_t wfd_attn_shared_workspace_bytes(int n, int H, int Hkv, int Dh, int prefix_len_max, int kv_len_max) {
   using namespace wfd;
-  if (n <= 0 || H <= 0 || Hkv <= 0 || Dh <= 0 || prefix_len_max < 0 || kv_len_max < 0) return 0;
+  // 0 for what the call refuses; the largest it takes is below 2^61
+  if (n <= 0 || n > kShMaxRows || H <= 0 || H > kShMaxHeads || Hkv <= 0 || Dh <= 0 || Dh > 128 || prefix_len_max < 0 ||
+      kv_len_max < 0)
+    return 0;
   const size_t parts = (size_t)n * H * (max_prefix_chunks(prefix_len_max, Hkv) + div_up(kv_len_max, kShOwnChunk));
   return align256(parts * Dh * sizeof(float)) + align256(parts * 2 * sizeof(float));
 }
@@ -646,7 +650,7 @@ int wfd_attn_shared(const void* q, const void* k_cache, const void* v_cache, int
   a.pml = (float*)((char*)workspace + align256((size_t)n * H * (a.pchunks + a.ochunks) * Dh * sizeof(float)));
   // in double: the product of four counts may pass 64 bits
   const double most = (((double)ngroups * a.pchunks * Hkv + 8) * (double)tiles + (double)n * a.ochunks * Hkv);
-  if (most > 2147483647.0 || n > 65535) {
+  if (most > 2147483647.0 || n > kShMaxRows) {
     set_error("%s: n=%d ngroups=%d group_max=%d prefix_len_max=%d kv_len_max=%d beyond the grid", me, n, ngroups,
               group_max, prefix_len_max, kv_len_max);
     return kUnsupported;
