@@ -304,8 +304,8 @@ int wfd_kv_read_q(const void* k_codes, const void* v_codes, const uint8_t* k_exp
  * without rounding), with fp32 statistics, sums and division; probabilities meet
  * V with 16 significant bits (fp32 queries: 24). A key row marked non-finite
  * makes the rows that attend it NaN, no others. H / Hkv up to 16, H up to 4096,
- * at most 65535 rows, any scale; workspace >= wfd_attn_workspace_bytes(n, H, Dh,
- * kv_len_max). A row's bits depend on that row only.
+ * at most 65535 rows, kv_len_max up to 2^31 - 1024, any scale; workspace >=
+ * wfd_attn_workspace_bytes(n, H, Dh, kv_len_max). A row's bits depend on that row only.
  * Replaces: what wfd_attn_decode replaces, over caches the reference does not have.
  */
 int wfd_attn_decode_q(const void* q, const void* k_codes, const void* v_codes, const uint8_t* k_exp,

@@ -290,3 +290,12 @@ def test_shared_workspace_of_lengths_up_to_the_largest():
     assert ws(65535, 4096, 4096, 128, top, top) == size(65535 * 4096 * (2 ** 21 + 2 ** 22), 128)
     for n, H, Dh in ((65536, 4, 64), (4, 4097, 64), (4, 4, 1 << 20), (top, top, top)):
         assert ws(n, H, H, Dh, top, top) == 0
+
+
+def test_quant_attention_counts_whole_splits():
+    lib = _lib.load()
+    call = lambda m: lib.wfd_attn_decode_q(None, None, None, None, None, 0, 0, None, None, None, 1, 4, 2, 64, 1,  # noqa: E731
+                                           0.1, m, None, 0, None)
+    for m in (2 ** 31 - 1, 2 ** 31 - 1023):
+        assert call(m) == -2 and b"beyond the grid" in lib.wfd_last_error()
+    assert call(2 ** 31 - 1024) == -1 and b"null pointer" in lib.wfd_last_error()

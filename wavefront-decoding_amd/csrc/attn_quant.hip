@@ -400,8 +400,8 @@ int wfd_attn_decode_q(const void* q, const void* k_codes, const void* v_codes, c
     set_error("%s: unsupported dtype=%d G=%d (G = H / Hkv up to %d)", me, dtype, G, kAqMaxG);
     return kUnsupported;
   }
-  if (n > 65535) {
-    set_error("%s: n=%d beyond the grid (65535 rows)", me, n);
+  if (n > 65535 || kv_len_max > INT32_MAX - (kAttnSplit - 1)) {  // whole splits below 2^31
+    set_error("%s: n=%d kv_len_max=%d beyond the grid (65535 rows, 2^31 - 1024 keys)", me, n, kv_len_max);
     return kUnsupported;
   }
   if (n == 0) return kOk;
