@@ -292,6 +292,39 @@ def test_shared_workspace_of_lengths_up_to_the_largest():
         assert ws(n, H, H, Dh, top, top) == 0
 
 
+def test_counts_beyond_32_bits_are_refused_not_cut_off(front, monkeypatch):
+    """2^32 + 5 would reach the library as 5, a bound below the lengths."""
+    i32, i64 = (lambda n: _m(n, dtype=torch.int32)), (lambda n: _m(n, dtype=torch.int64))
+    q, cache = _m(6, 4, 64), _m(100, 2, 64)
+    shared = lambda **kw: ops.attn_shared(q, cache, cache, i64(2), i32(2), i32(3), i64(6), i32(6),  # noqa: E731
+                                          **(dict(prefix_len_max=50, kv_len_max=10) | kw))
+    for n in (2 ** 31, 2 ** 32 + 5):
+        for kw in (dict(prefix_len_max=n), dict(kv_len_max=n)):
+            with pytest.raises(_lib.WfdError, match="above 2147483647"):
+                shared(**kw)
+        with pytest.raises(_lib.WfdError, match="above"):
+            ops.attn_decode_q(q, _q(), i64(6), i32(6), kv_len_max=n)
+    with pytest.raises(_lib.WfdError, match="above 2147482624"):
+        ops.attn_decode_q(q, _q(), i64(6), i32(6), kv_len_max=2 ** 31 - 1023)
+    u = _m(4, dtype=torch.float32)
+    with pytest.raises(_lib.WfdError, match="vocabulary 4294967301"):
+        ops.sample(_m(4, 2 ** 32 + 5, dtype=torch.float32), u)
+    with pytest.raises(_lib.WfdError, match="rows 4294967301"):
+        ops.sample(_m(2 ** 32 + 5, 1, dtype=torch.float32), _m(2 ** 32 + 5, dtype=torch.float32))
+    # a group holds at most the call's rows, whatever bound is given
+    sent = []
+
+    class Lib:
+        wfd_attn_shared_workspace_bytes = staticmethod(lambda *a: 16)
+        wfd_attn_shared = staticmethod(lambda *a: sent.append(a) or 0)
+
+    monkeypatch.setattr(_lib, "load", Lib)
+    monkeypatch.setattr(ops, "_workspace", lambda need, device: _m(need, dtype=torch.uint8))
+    for given, used in ((2 ** 32, 6), (None, 6), (3, 3), (0, 0)):
+        shared(group_max=given)
+        assert sent[-1][8] == used
+
+
 def test_quant_attention_counts_whole_splits():
     lib = _lib.load()
     call = lambda m: lib.wfd_attn_decode_q(None, None, None, None, None, 0, 0, None, None, None, 1, 4, 2, 64, 1,  # noqa: E731

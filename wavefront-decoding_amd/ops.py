@@ -63,6 +63,15 @@ def _need_current(*ts: torch.Tensor | None) -> int:
     return torch._C._cuda_getCurrentRawStream(dev)
 
 
+_I32_MAX = 2 ** 31 - 1
+
+
+def _fits(name: str, value: int, most: int = _I32_MAX) -> None:
+    """The library takes 32-bit counts, and a larger one would reach it cut off."""
+    if value > most:
+        raise _lib.WfdError(f"{name} {value} above {most}")
+
+
 def _table(name: str, t: torch.Tensor, dtype: torch.dtype, size: int) -> None:
     if t.dtype != dtype or t.numel() < size or not t.is_contiguous():
         raise _lib.WfdError(f"{name}: {dtype} contiguous (>= {size},)")
@@ -297,10 +306,12 @@ def attn_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, p
     _table("kv_row_base", kv_row_base, torch.int64, n)
     _table("kv_len", kv_len, torch.int32, n)
     _need(prefix_len_max >= 0 and kv_len_max >= 0, "prefix_len_max and kv_len_max must be >= 0")
+    _fits("prefix_len_max", prefix_len_max)
+    _fits("kv_len_max", kv_len_max)
     if 1 < br < max(prefix_len_max, kv_len_max):
         raise _lib.WfdError(f"prefix_len_max {prefix_len_max} or kv_len_max {kv_len_max} exceeds the cache block "
                             f"({br} rows)")
-    group_max = n if group_max is None else int(group_max)
+    group_max = n if group_max is None else min(int(group_max), n)
     _need(group_max >= 0, "group_max must be >= 0")
     if out is None:
         out = torch.empty_like(q)
@@ -571,6 +582,7 @@ def attn_decode_q(q: torch.Tensor, cache: QuantKV, kv_row_base: torch.Tensor, kv
     _table("kv_row_base", kv_row_base, torch.int64, n)
     _table("kv_len", kv_len, torch.int32, n)
     _need(kv_len_max >= 1, "kv_len_max must be >= 1")
+    _fits("kv_len_max", kv_len_max, _I32_MAX - 1023)  # whole splits of 1024 keys below 2^31
     if out is None:
         out = torch.empty_like(q)
     else:
@@ -956,6 +968,8 @@ def sample(logits: torch.Tensor, u: torch.Tensor, *, temperature: torch.Tensor |
         _table("min_p", min_p, torch.float32, n)
     out, acc = _argmax_outputs(n, logits.device, out, ring, ring_rows, expect, accept, accept_mapped)
     V = logits.shape[1]
+    _fits("rows", n)
+    _fits("vocabulary", V)
     ld = logits.stride(0) if logits.shape[0] > 1 else V
     need = sample_workspace_bytes(n, V)
     if workspace is None and need:
