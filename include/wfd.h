@@ -207,10 +207,11 @@ int wfd_attn_varlen(const void* q, const void* k, const void* v, const int32_t* 
  * block, and so do a row's own keys). Device tables: prefix_row_base int64 and
  * prefix_len int32 (ngroups), group_first int32 (ngroups + 1), kv_row_base int64
  * and kv_len int32 (n). prefix_len_max, kv_len_max >= the lengths (0: none has
- * any) and group_max >= every group's rows size the grid. workspace >=
- * wfd_attn_shared_workspace_bytes(...). Dh 64 or 128, H / Hkv up to 16, any
- * scale; at most 65535 rows. fp32 statistics, sums and division; for bf16 the
- * probabilities meet V with 16 significant bits. A row's bits depend on
+ * any) and group_max >= every group's rows size the grid; longer lengths count as
+ * these, and a row past its group's first group_max, of a prefix with keys, is NaN.
+ * workspace >= wfd_attn_shared_workspace_bytes(...). Dh 64 or 128, H / Hkv up to 16,
+ * H up to 4096, any scale; at most 65535 rows. fp32 statistics, sums and division;
+ * for bf16 the probabilities meet V with 16 significant bits. A row's bits depend on
  * its own q, keys and lengths and on Hkv, not on its group's other rows (they
  * are not wfd_attn_decode's, whose key order differs). Infinities and NaN in K
  * and V reach only the rows that attend them, an infinity in V as itself (opposite

@@ -279,3 +279,20 @@ def test_bounds_of_the_largest_length(gpu):
     top = 2 ** 31 - 1
     ws = torch.empty(ops.attn_shared_workspace_bytes(2, 1, 1, 64, top, top), dtype=torch.uint8, device=gpu)  # 3.3 GB
     assert torch.equal(c.run(prefix_len_max=top, kv_len_max=top, workspace=ws), want)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("group_max", [0, 1, 7, 8, 9, 30])
+def test_rows_past_group_max_are_nan(gpu, dtype, group_max):
+    """Nothing was computed for them: not a merge of what the workspace held. Rows of an
+    empty prefix, and rows of no group, need no prefix and are what they are."""
+    groups = [(0, 500, 40), (500, 200, 8), (700, 0, 35)]
+    own = [(800 + i, 1 + i % 20) for i in range(90)]
+    c = Case(gpu, dtype, 8, 2, 64, 1000, groups, own, seed=9)
+    want = c.run()
+    ws = torch.zeros(ops.attn_shared_workspace_bytes(90, 8, 2, 64, 500, 20), dtype=torch.uint8, device=gpu)
+    got = c.run(group_max=group_max, workspace=ws)
+    lost = torch.zeros(90, dtype=torch.bool)
+    lost[group_max:40] = True
+    lost[40 + group_max:48] = True
+    assert bool(got[lost].isnan().all()) and torch.equal(got[~lost], want[~lost])

@@ -61,7 +61,7 @@ struct ShArgs {
   const int32_t* rlen;
   void* out;
   float *po, *pml;
-  int n, H, Hkv, ng, tiles, pchunks, ochunks, pmax, omax;
+  int n, H, Hkv, ng, gmax, tiles, pchunks, ochunks, pmax, omax;
   uint32_t items;
   float scale_log2;
 };
@@ -535,21 +535,30 @@ __global__ __launch_bounds__(64 * kShWaves) __attribute__((amdgpu_waves_per_eu(2
 }
 
 // One row's parts, prefix chunks then its own. The row's group is found by one
-// wave-wide look at group_first per 64 groups.
+// wave-wide look at group_first per 64 groups. A row past the rows that the grid was
+// sized for has no prefix parts: it is NaN, not a merge of what the workspace held.
 template <typename T, int DH>
 __global__ __launch_bounds__(kMergeThreads) void attn_shared_combine(ShArgs a) {
   const int h = blockIdx.x, i = blockIdx.y, lane = threadIdx.x & 63;
   const int own = div_up(min(a.rlen[i], a.omax), kShOwnChunk);
-  int P = 0;
+  int P = 0, at = 0;
   for (int j0 = 0; j0 < a.ng; j0 += 64) {  // uniform
     const int j = min(j0 + lane, a.ng - 1);
-    const uint64_t hit = __ballot(j0 + lane < a.ng && a.gfirst[j] <= i && i < a.gfirst[j + 1]);
+    const int first = a.gfirst[j];
+    const uint64_t hit = __ballot(j0 + lane < a.ng && first <= i && i < a.gfirst[j + 1]);
     const int len = a.plen[j];
-    if (hit) P = __shfl(len, __builtin_ctzll(hit), 64);
+    if (hit) {
+      P = __shfl(len, __builtin_ctzll(hit), 64);
+      at = i - __shfl(first, __builtin_ctzll(hit), 64);
+    }
   }
   P = min(P, a.pmax);
   const int np = P > 0 ? div_up(P, prefix_chunk(P, a.Hkv)) : 0;
   const int64_t row = (int64_t)i * a.H + h, base = row * (a.pchunks + a.ochunks);
+  if (np && at >= a.gmax) {  // uniform
+    if (threadIdx.x < DH) Elem<T>::store((T*)a.out + row * DH + threadIdx.x, NAN);
+    return;
+  }
   attn_merge_parts<T, DH>(a.po, a.pml, np + own, [&](int s) { return base + (s < np ? s : a.pchunks + s - np); },
                           (T*)a.out + row * DH);
 }
@@ -639,6 +648,7 @@ int wfd_attn_shared(const void* q, const void* k_cache, const void* v_cache, int
   a.H = H;
   a.Hkv = Hkv;
   a.ng = ngroups;
+  a.gmax = group_max;
   const int64_t pairs = (int64_t)(group_max < n ? group_max : n) * G;
   const int64_t tiles = (pairs + kShRows - 1) / kShRows;
   a.pchunks = max_prefix_chunks(prefix_len_max, Hkv);

@@ -292,7 +292,7 @@ def attn_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, p
     prefix_row_base[j] + [0, prefix_len[j]), read once for the group, and each
     row its own rows kv_row_base[i] + [0, kv_len[i]). prefix_len_max and
     kv_len_max bound the lengths (0: none has any), group_max a group's rows
-    (None: n)."""
+    (None: n); a row past that bound, of a prefix with keys, is NaN."""
     stream = _need_current(q, k_cache, v_cache, prefix_row_base, prefix_len, group_first, kv_row_base, kv_len, out,
                            workspace)
     _need(q.dim() == 3 and q.is_contiguous(), "q must be contiguous (n, H, Dh)")
