@@ -551,7 +551,7 @@ int wfd_argmax(const float* logits, int64_t ld, int64_t* out, int64_t* ring, con
  * tokens ordered by logit, largest first, the lower index first among equals,
  * these are kept: the first top_k[i]; of these the shortest run whose sum of w
  * reaches top_p[i] of theirs; of these the ones with w_j >= min_p[i], the first
- * always. The token is the lowest kept index at which the running sum of w over
+ * always (above 1, where its equals go too, it is alone). The token is the lowest kept index at which the running sum of w over
  * the kept tokens, in index order, exceeds u[i] times their sum. So the same
  * logits and the same u give the same token wherever the row is, and a draft
  * can be verified by drawing it again. w is rounded to a multiple of 2^-44 (below

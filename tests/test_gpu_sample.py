@@ -320,3 +320,27 @@ def test_extreme_temperatures_over_masked_rows(gpu, V, t):
     check(gpu, rows, u, [t] * n, None, [0.6] * n)
     check(gpu, rows, u, [t] * n, [50] * n, [0.6] * n)
     check(gpu, rows, u, [t] * n, None, [0.9] * n, [0.5] * n)
+
+
+@pytest.mark.parametrize("V", [5, 300, 20000, 60000])
+def test_min_p_above_one_keeps_the_first_token_alone(gpu, V):
+    """No weight reaches it, and only the first of the order stays whatever its weight: not
+    the others as large. At 1 these stay."""
+    g = torch.Generator().manual_seed(V)
+    n = 8
+    rows = torch.randn(n, V, generator=g).clamp(max=3.0)
+    at = torch.stack([torch.randperm(V, generator=g)[:3].sort().values for _ in range(n)])
+    rows.scatter_(1, at, 5.0)
+    rows[5].scatter_(0, at[5], INF)
+    rows[6] = -INF
+    rows[7] = 0.0
+    first = at[:, 0].tolist()
+    first[6] = first[7] = 0
+    for u in (0.0, 0.5, LAST):
+        us = [u] * n
+        for kw in (dict(), dict(top_p=[0.9] * n), dict(top_k=[4] * n), dict(top_k=[50] * n, top_p=[0.9] * n)):
+            for m in (1.0000001, 2.0, INF):
+                assert draw(gpu, rows, us, min_p=[m] * n, **kw) == first
+            if not kw:
+                last = draw(gpu, rows, us, min_p=[1.0] * n)
+                assert last[:6] == [int(a[min(2, int(u * 3))]) for a in at[:6]]

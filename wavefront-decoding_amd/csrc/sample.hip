@@ -395,7 +395,7 @@ struct Sm {
     best = sm_wave_max(best);
     low = sm_wave_min(low);
   }
-  // false: a greedy row, or one with a NaN or without any possible token
+  // false: a row of one token, the first of its order (greedy ones), or with a NaN or without any possible token
   __device__ __forceinline__ bool parameters() {
     T = a.temperature ? a.temperature[i] : 1.f;
     if (nan || !(T > 0.f) || best == -INFINITY) return false;
@@ -406,8 +406,9 @@ struct Sm {
     p = a.top_p ? a.top_p[i] : 1.f;
     has_p = p < 1.f;
     minp = a.min_p ? a.min_p[i] : 0.f;
+    if (minp > 1.f) return false;  // no weight reaches it: the first token alone, the greedy one
     // on the integer weights' scale: w >= min_p for w on or above it
-    wmin = minp > 0.f ? (minp < 1.f ? (uint64_t)ceil((double)minp * kSmOne) : (uint64_t)kSmOne) : 0;
+    wmin = minp > 0.f ? (uint64_t)ceil((double)minp * kSmOne) : 0;
     u = a.u[i];
     u = u > 0.f ? (u < 1.f ? u : 0.99999994f) : 0.f;
     scale = best > low ? (float)(kSmBins - 2) / (best - low) : 1.f;
