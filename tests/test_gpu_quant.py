@@ -316,3 +316,19 @@ def test_empty_calls(gpu):
     cos = z(4, 32, d=torch.float32)
     assert ops.qkv_rope_append_q(z(0, 512), z(0, d=torch.int32), cos, cos, z(0, d=torch.int64), cache, 4, 2,
                                  64).shape == (0, 4, 64)
+
+
+def test_cache_tensors_moved_in_place(gpu):
+    """The kernels work where the cache's tensors are, not where they were."""
+    n, Hkv, Dh = 9, 2, 64
+    cache = _cache(16, Hkv, Dh, "int8", gpu)
+    k, v = (torch.randn(n, Hkv, Dh, generator=_gen(s)).bfloat16() for s in (1, 2))
+    rows = torch.arange(n, device=gpu)
+    ops.kv_append_q(k.to(gpu), v.to(gpu), cache, rows)
+    old = cache.k.data
+    before = old.clone()
+    cache.k.data = torch.zeros_like(old)
+    ops.kv_append_q(v.to(gpu), v.to(gpu), cache, rows)
+    assert torch.equal(old, before)
+    for got in ops.kv_read_q(cache, rows):
+        assert torch.equal(got.cpu(), quantise(v, "int8")[0].bfloat16())

@@ -332,3 +332,23 @@ def test_quant_attention_counts_whole_splits():
     for m in (2 ** 31 - 1, 2 ** 31 - 1023):
         assert call(m) == -2 and b"beyond the grid" in lib.wfd_last_error()
     assert call(2 ** 31 - 1024) == -1 and b"null pointer" in lib.wfd_last_error()
+
+
+def test_quant_cache_follows_its_tensors():
+    """Its tensors cannot be exchanged, and ones that were resized or moved in place are used
+    where they are, after the checks of a new cache."""
+    c = ops.QuantKV.zeros((8, 2, 64), code=torch.int8, device="cpu")
+    for name in ("k", "v", "k_exp", "v_exp", "tensors"):
+        with pytest.raises(AttributeError):
+            setattr(c, name, getattr(c, name))
+    where = lambda: tuple(t.data_ptr() for t in c.tensors)  # noqa: E731
+    assert c.pointers() == where()
+    c.k.data = torch.zeros(8, 2, 64, dtype=torch.int8)
+    c.v_exp.set_(torch.zeros(8, 2, dtype=torch.uint8))
+    assert c.pointers() == where()
+    for t, shape in zip(c.tensors, ((4096, 4, 64),) * 2 + ((4096, 4),) * 2):
+        t.resize_(shape)
+    assert c.pointers() == where() and (c.Hkv, c.Dh) == (4, 64)
+    c.v.resize_(40960, 4, 64)
+    with pytest.raises(_lib.WfdError, match="differ in shape"):
+        c.pointers()

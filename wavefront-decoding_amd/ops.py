@@ -467,20 +467,38 @@ class QuantKV:
     """An 8-bit KV cache (wfd_kv_append_q): codes `k` / `v` (float8_e4m3fn or
     int8) in either layout of kv_layout, and the exponent bytes `k_exp` /
     `v_exp` (uint8), the codes' shape without its last dimension; a value is
-    code * 2^(exp - 127)."""
+    code * 2^(exp - 127). Its tensors are fixed (other ones are another cache);
+    where their memory is when a call is made is looked up then."""
 
-    __slots__ = ("k", "v", "k_exp", "v_exp", "code", "Hkv", "Dh", "block_rows", "tensors", "_ptrs")
+    __slots__ = ("_tensors", "code", "Hkv", "Dh", "block_rows", "_ptrs")
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_exp: torch.Tensor, v_exp: torch.Tensor):
+        self._tensors = (k, v, k_exp, v_exp)
+        self._check()
+
+    def _check(self) -> None:
+        k, v, k_exp, v_exp = self._tensors
         _need(k.dtype in _CODES, f"8-bit cache: codes float8_e4m3fn or int8, not {k.dtype}")
         self.Hkv, self.Dh, self.block_rows = kv_layout(k, v)
         for t in (k_exp, v_exp):
             _need(t.dtype == torch.uint8 and t.is_contiguous() and t.shape == k.shape[:-1],
                   "8-bit cache: exponents uint8, contiguous, shaped like the codes without their last dimension")
         _need(k.device == v.device == k_exp.device == v_exp.device, "8-bit cache: its tensors are on one device")
-        self.k, self.v, self.k_exp, self.v_exp, self.code = k, v, k_exp, v_exp, _CODES[k.dtype]
-        self.tensors = (k, v, k_exp, v_exp)
-        self._ptrs = tuple(t.data_ptr() for t in self.tensors)
+        self.code = _CODES[k.dtype]
+        self._ptrs = tuple(t.data_ptr() for t in self._tensors)
+
+    tensors = property(lambda self: self._tensors)
+    k = property(lambda self: self._tensors[0])
+    v = property(lambda self: self._tensors[1])
+    k_exp = property(lambda self: self._tensors[2])
+    v_exp = property(lambda self: self._tensors[3])
+
+    def pointers(self) -> tuple[int, int, int, int]:
+        """Where the tensors are now; those that were resized or given other storage are checked again."""
+        k, v, k_exp, v_exp = self._tensors
+        if (k.data_ptr(), v.data_ptr(), k_exp.data_ptr(), v_exp.data_ptr()) != self._ptrs:
+            self._check()
+        return self._ptrs
 
     @classmethod
     def zeros(cls, shape, *, code: torch.dtype = torch.float8_e4m3fn, device="cuda") -> "QuantKV":
@@ -507,6 +525,7 @@ def kv_append_q(k: torch.Tensor, v: torch.Tensor, cache: QuantKV, flat_row: torc
     (n, Hkv, Dh), each row contiguous (views of a fused qkv row will do);
     flat_row int64, distinct rows."""
     stream = _need_current(k, v, flat_row, cache.k)
+    ptrs = cache.pointers()
     n = k.shape[0]
     _kv_rows(k, cache, "k")
     _kv_rows(v, cache, "v")
@@ -514,7 +533,7 @@ def kv_append_q(k: torch.Tensor, v: torch.Tensor, cache: QuantKV, flat_row: torc
     _table("flat_row", flat_row, torch.int64, n)
     width = cache.Hkv * cache.Dh
     ldk, ldv = (t.stride(0) if n > 1 else width for t in (k, v))
-    rc = _lib.load().wfd_kv_append_q(k.data_ptr(), ldk, v.data_ptr(), ldv, *cache._ptrs, cache.code,
+    rc = _lib.load().wfd_kv_append_q(k.data_ptr(), ldk, v.data_ptr(), ldv, *ptrs, cache.code,
                                      cache.block_rows, flat_row.data_ptr(), n, cache.Hkv, cache.Dh, _dt(k), stream)
     _lib.check(rc, "wfd_kv_append_q")
 
@@ -525,6 +544,7 @@ def qkv_rope_append_q(qkv: torch.Tensor, pos: torch.Tensor, rope_cos: torch.Tens
     """qkv_rope_append into an 8-bit cache (wfd_qkv_rope_append_q): returns the
     rotated q (the same bits), k (rotated) and v go to rows flat_row."""
     stream = _need_current(qkv, pos, rope_cos, rope_sin, flat_row, q_out, cache.k)
+    ptrs = cache.pointers()
     n = qkv.shape[0]
     _need(qkv.dim() == 2 and qkv.stride(1) == 1 and qkv.shape[1] >= (H + 2 * Hkv) * Dh, "qkv (n, (H+2Hkv)Dh)")
     _table("pos", pos, torch.int32, n)
@@ -540,7 +560,7 @@ def qkv_rope_append_q(qkv: torch.Tensor, pos: torch.Tensor, rope_cos: torch.Tens
     ldq = qkv.stride(0) if n > 1 else (H + 2 * Hkv) * Dh
     rc = _lib.load().wfd_qkv_rope_append_q(qkv.data_ptr(), ldq, pos.data_ptr(), rope_cos.data_ptr(),
                                            rope_sin.data_ptr(), rope_cos.shape[0], flat_row.data_ptr(),
-                                           q_out.data_ptr(), *cache._ptrs, cache.code, cache.block_rows, n, H, Hkv,
+                                           q_out.data_ptr(), *ptrs, cache.code, cache.block_rows, n, H, Hkv,
                                            Dh, _dt(qkv), stream)
     _lib.check(rc, "wfd_qkv_rope_append_q")
     return q_out
@@ -550,6 +570,7 @@ def kv_read_q(cache: QuantKV, flat_row: torch.Tensor, *, dtype: torch.dtype = to
               k_out: torch.Tensor | None = None, v_out: torch.Tensor | None = None):
     """(k, v), each (n, Hkv, Dh) of `dtype`: the values of cache rows flat_row (wfd_kv_read_q)."""
     stream = _need_current(flat_row, k_out, v_out, cache.k)
+    ptrs = cache.pointers()
     _need(flat_row.dtype == torch.int64 and flat_row.dim() == 1 and flat_row.is_contiguous(), "flat_row: int64 (n,)")
     if dtype not in _DT:
         raise _lib.WfdError(f"unsupported dtype {dtype} (float32 / bfloat16)")
@@ -562,7 +583,7 @@ def kv_read_q(cache: QuantKV, flat_row: torch.Tensor, *, dtype: torch.dtype = to
         k_out = torch.empty(shape, dtype=dtype, device=cache.k.device)
     if v_out is None:
         v_out = torch.empty_like(k_out)
-    rc = _lib.load().wfd_kv_read_q(*cache._ptrs, cache.code, cache.block_rows, flat_row.data_ptr(),
+    rc = _lib.load().wfd_kv_read_q(*ptrs, cache.code, cache.block_rows, flat_row.data_ptr(),
                                    k_out.data_ptr(), v_out.data_ptr(), n, cache.Hkv, cache.Dh, _DT[dtype], stream)
     _lib.check(rc, "wfd_kv_read_q")
     return k_out, v_out
@@ -574,6 +595,7 @@ def attn_decode_q(q: torch.Tensor, cache: QuantKV, kv_row_base: torch.Tensor, kv
     """attn_decode over an 8-bit cache (wfd_attn_decode_q): q (n, H, Dh), query i
     reads cache rows kv_row_base[i] + [0, kv_len[i])."""
     stream = _need_current(q, kv_row_base, kv_len, out, workspace, cache.k)
+    ptrs = cache.pointers()
     _need(q.dim() == 3 and q.is_contiguous(), "q must be contiguous (n, H, Dh)")
     n, H, Dh = q.shape
     _need(cache.Dh == Dh, "q and cache head_dim mismatch")
@@ -591,7 +613,7 @@ def attn_decode_q(q: torch.Tensor, cache: QuantKV, kv_row_base: torch.Tensor, kv
     if workspace is None:
         workspace = _workspace(_attn_workspace_bytes(n, H, Dh, int(kv_len_max)), q.device)
     sc = 1.0 / math.sqrt(Dh) if scale is None else float(scale)
-    rc = _lib.load().wfd_attn_decode_q(q.data_ptr(), *cache._ptrs, cache.code, cache.block_rows,
+    rc = _lib.load().wfd_attn_decode_q(q.data_ptr(), *ptrs, cache.code, cache.block_rows,
                                        kv_row_base.data_ptr(), kv_len.data_ptr(), out.data_ptr(), n, H, cache.Hkv, Dh,
                                        dt, sc, int(kv_len_max), workspace.data_ptr(),
                                        workspace.numel() * workspace.element_size(), stream)
