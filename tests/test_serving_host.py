@@ -352,3 +352,29 @@ def test_quant_cache_follows_its_tensors():
     c.v.resize_(40960, 4, 64)
     with pytest.raises(_lib.WfdError, match="differ in shape"):
         c.pointers()
+
+
+@pytest.mark.parametrize("head_major", [True, False])
+def test_quant_slots_read_back_only_what_they_hold(monkeypatch, head_major):
+    """Ids count from the end below 0, as in the unquantised cache, and rows outside the slots
+    never reach the kernel, which trusts them."""
+    from wavefront_decoding_amd.kv_cache import BatchStaticKVCache, QuantBatchKVCache
+
+    cache = QuantBatchKVCache(3, 2, 1, 64, 10, torch.bfloat16, "cpu", head_major=head_major)
+    plain = BatchStaticKVCache(3, 2, 1, 64, 10, torch.float32, "cpu", head_major=head_major)
+    plain.K[:, :, :, 0, 0] = torch.arange(60.0).view(3, 2, 10)  # every row's number
+    asked = []
+
+    def read(flat, rows, dtype):
+        assert not rows.numel() or 0 <= int(rows.min()) and int(rows.max()) < 60
+        asked.append(rows.tolist())
+        return rows, rows
+
+    monkeypatch.setattr(ops, "kv_read_q", read)
+    for at in (([0, 2], [1, 0], [3, 9]), ([-1, -3], [-1, 1], [0, 4]), ([1], [0], [-1])):
+        cache.gather_pack(*at)
+        assert asked.pop() == plain.gather_pack(*at)[0][:, 0, 0].tolist()
+    for at in (([3], [0], [0]), ([-4], [0], [0]), ([0], [2], [0]), ([0], [-3], [0]), ([0], [0], [10]), ([2], [1], [-2])):
+        with pytest.raises(IndexError):
+            cache.gather_pack(*at)
+    assert not asked

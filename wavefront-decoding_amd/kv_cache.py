@@ -172,8 +172,14 @@ class QuantBatchKVCache(BatchStaticKVCache):
 
     def gather_pack(self, slots, seq_ids, uptos):
         lengths = [u + 1 for u in uptos]
+        for upto in uptos:
+            if not -1 <= upto < self.S:
+                raise IndexError(f"position {upto} exceeds max_seq_len={self.S}")
+        # ids as indexes of the K / V views of the unquantised slots: from the end below 0
+        slot, seq = range(self.n_slots), range(self.B)
         cu = torch.tensor([0] + lengths, dtype=torch.int32).cumsum(0, dtype=torch.int32).to(self.device)
-        rows = torch.cat([torch.arange(ln) + self.row_base(sl, b) for sl, b, ln in zip(slots, seq_ids, lengths)])
+        rows = torch.cat([torch.arange(ln) + self.row_base(slot[sl], seq[b])
+                          for sl, b, ln in zip(slots, seq_ids, lengths)])
         k, v = ops.kv_read_q(self.flat, rows.to(self.device), dtype=self.dtype)
         return k, v, cu, max(lengths)
 
