@@ -378,3 +378,26 @@ def test_quant_slots_read_back_only_what_they_hold(monkeypatch, head_major):
         with pytest.raises(IndexError):
             cache.gather_pack(*at)
     assert not asked
+
+
+@pytest.mark.parametrize("quant", [False, True])
+def test_slots_are_written_only_where_they_are(monkeypatch, quant):
+    """Slots and sequences past the cache are an IndexError before any row is written, and
+    count from the end below 0."""
+    from wavefront_decoding_amd.kv_cache import BatchStaticKVCache, QuantBatchKVCache
+
+    cls = QuantBatchKVCache if quant else BatchStaticKVCache
+    cache = cls(3, 2, 1, 64, 10, torch.bfloat16, "cpu")
+    wrote = []
+    monkeypatch.setattr(ops, "kv_append", lambda k, v, fk, fv, rows: wrote.append(rows.tolist()))
+    monkeypatch.setattr(ops, "kv_append_q", lambda k, v, flat, rows: wrote.append(rows.tolist()))
+    k, t = torch.zeros(1, 2, 1, 64), torch.zeros(1, 1, 64)
+    for slot, b in ((3, 0), (-4, 0), (0, 2), (0, -3)):
+        with pytest.raises(IndexError):
+            cache.write_prefill(slot, k, k, seq_ids=[b])
+        with pytest.raises(IndexError):
+            cache.write_tokens([slot], [b], [0], t, t)
+    assert not wrote and cache.seqlen == [[0, 0]] * 3
+    cache.write_prefill(-1, k, k, seq_ids=[-2])
+    cache.write_tokens([-3], [-1], [4], t, t)
+    assert wrote == [[40, 41], [14]] and cache.seqlen == [[0, 5], [0, 0], [2, 0]]

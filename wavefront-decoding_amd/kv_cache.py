@@ -109,7 +109,8 @@ class BatchStaticKVCache:
         L = k.shape[1]
         if L > self.S:
             raise IndexError(f"prefill length {L} exceeds max_seq_len={self.S}")
-        seq_ids = list(range(self.B)) if seq_ids is None else list(seq_ids)
+        slot = range(self.n_slots)[slot]  # before any row of it is written; from the end below 0
+        seq_ids = list(range(self.B)) if seq_ids is None else [range(self.B)[b] for b in seq_ids]
         rows = torch.tensor([self.flat_row(slot, b, p) for b in seq_ids for p in range(L)], dtype=torch.int64,
                             device=self.device)
         self._append(k.reshape(-1, self.n_kv_head, self.head_dim).contiguous(),
@@ -119,6 +120,8 @@ class BatchStaticKVCache:
 
     def write_tokens(self, slots, seq_ids, positions, k: torch.Tensor, v: torch.Tensor) -> None:
         """Scatter n tokens: k, v (n, Hkv, Dh) -> (slots[i], seq_ids[i], positions[i])."""
+        slots = [range(self.n_slots)[sl] for sl in slots]
+        seq_ids = [range(self.B)[b] for b in seq_ids]
         for sl, b, p in zip(slots, seq_ids, positions):
             self.note_write(sl, b, p)
         rows = torch.tensor([self.flat_row(sl, b, p) for sl, b, p in zip(slots, seq_ids, positions)],
