@@ -296,3 +296,11 @@ def test_rows_past_group_max_are_nan(gpu, dtype, group_max):
     lost[group_max:40] = True
     lost[40 + group_max:48] = True
     assert bool(got[lost].isnan().all()) and torch.equal(got[~lost], want[~lost])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_a_nan_scale_gives_nan(gpu, dtype):
+    c = Case(gpu, dtype, 8, 2, 128, 900, [(0, 600, 5), (600, 0, 2)], [(600 + 9 * i, 8 * (i % 3)) for i in range(9)])
+    got = c.run(scale=math.nan)
+    keys = torch.tensor([len(c.keys(i)) > 0 for i in range(9)])
+    assert not bool(keys.all()) and bool(got[keys].isnan().all()) and not bool(got[~keys].any())

@@ -179,6 +179,11 @@ __device__ __forceinline__ f32x16 sh_mfma32(const u32x4& x, const u32x4& y, f32x
                                                  0, 0);
 }
 
+// The scale's size; zero is a tiny one, under which -inf stays -inf, and NaN is NaN.
+__device__ __forceinline__ float sh_scale(const ShArgs& a) {
+  return a.scale_log2 != a.scale_log2 ? a.scale_log2 : fmaxf(fabsf(a.scale_log2), 1e-37f);
+}
+
 // One tile's scores (of the lane's pair) to probabilities, under the pair's reference
 // point: the maximum when it was last moved, which is when a tile exceeds it by more
 // than 2^8. Probabilities up to 2^8 lose nothing in fp32 sums or bf16, and most tiles
@@ -302,8 +307,8 @@ __global__ __launch_bounds__(64 * kShWaves) __attribute__((amdgpu_waves_per_eu(2
   fetch();
 
   // Q as the B operand; a negative scale's sign goes to q, so that scores order as
-  // their products do, and a zero one is a tiny one, under which -inf stays -inf
-  const float scale = fmaxf(fabsf(a.scale_log2), 1e-37f);
+  // their products do
+  const float scale = sh_scale(a);
   const uint32_t flip = a.scale_log2 < 0.f ? 0x80008000u : 0u;
   u32x4 qf[NDS];
   {
@@ -474,7 +479,7 @@ __global__ __launch_bounds__(64 * kShWaves) __attribute__((amdgpu_waves_per_eu(2
   for (int q = 0; q < 4; ++q) fetch_k(q);
   koff += next;
 
-  const float scale = fmaxf(fabsf(a.scale_log2), 1e-37f);  // as in the bf16 kernel
+  const float scale = sh_scale(a);  // as in the bf16 kernel
   const uint32_t flip = a.scale_log2 < 0.f ? 0x80000000u : 0u;
   u32x4 qf[DH / 8];
   {
