@@ -401,3 +401,16 @@ def test_slots_are_written_only_where_they_are(monkeypatch, quant):
     cache.write_prefill(-1, k, k, seq_ids=[-2])
     cache.write_tokens([-3], [-1], [4], t, t)
     assert wrote == [[40, 41], [14]] and cache.seqlen == [[0, 5], [0, 0], [2, 0]]
+
+
+@pytest.mark.skipif(torch.cuda.device_count() > 0, reason="what is said where no GPU is visible")
+def test_host_tensors_are_refused_without_a_gpu():
+    t, rows = torch.zeros(2, 2, 64, dtype=torch.bfloat16), torch.zeros(2, dtype=torch.int64)
+    cache, u = ops.QuantKV.zeros((8, 2, 64), device="cpu"), torch.zeros(2)
+    for call in (lambda: ops.kv_append_q(t, t, cache, rows), lambda: ops.kv_read_q(cache, rows),
+                 lambda: ops.qkv_rope_append_q(t.view(2, 128), rows.int(), u, u, rows, cache, 2, 2, 64),
+                 lambda: ops.attn_decode_q(t, cache, rows, rows.int(), kv_len_max=4), lambda: ops.sample(t[0].float(), u),
+                 lambda: ops.attn_shared(t, t, t, rows, rows.int(), rows.int(), rows, rows.int(), prefix_len_max=1,
+                                         kv_len_max=1)):
+        with pytest.raises(_lib.WfdError, match="GPU tensors"):
+            call()

@@ -53,10 +53,12 @@ def _need(cond: bool, msg: str) -> None:
         raise _lib.WfdError(msg)
 
 
-def _need_current(*ts: torch.Tensor | None) -> int:
+def _need_current(first: torch.Tensor, *ts: torch.Tensor | None) -> int:
     """GPU tensors, all on the current device: the stream the launch goes to."""
+    if first.get_device() < 0:  # where there is no GPU, no device is current either
+        _need_cuda(first)
     dev = torch.cuda.current_device()
-    for t in ts:
+    for t in (first, *ts):
         if t is not None and t.get_device() != dev:
             _need_cuda(t)
             raise _lib.WfdError(f"operand on {t.device}, but the current device is cuda:{dev}")
