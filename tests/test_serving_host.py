@@ -414,3 +414,13 @@ def test_host_tensors_are_refused_without_a_gpu():
                                          kv_len_max=1)):
         with pytest.raises(_lib.WfdError, match="GPU tensors"):
             call()
+
+
+def test_sampler_takes_any_top_k(monkeypatch):
+    """More than any vocabulary is off, also past what the operator's 32 bits hold."""
+    from wavefront_decoding_amd.acceptance import SeededSampler
+
+    sent = []
+    monkeypatch.setattr(ops, "sample", lambda row, u, top_k, **kw: sent.append(top_k.tolist()) or torch.tensor([7]))
+    for k, used in ((5, 5), (2 ** 31 - 1, 2 ** 31 - 1), (2 ** 31, 2 ** 31 - 1), (10 ** 12, 2 ** 31 - 1)):
+        assert SeededSampler(0, top_k=k)(torch.zeros(9), 3) == 7 and sent[-1] == [used]

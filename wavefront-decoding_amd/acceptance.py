@@ -89,7 +89,8 @@ class SeededSampler(TokenSampler):
         have = self._on_device.setdefault(device, {})
         if not have:
             have["temperature"] = torch.tensor([self.temperature], device=device)
-            have["top_k"] = torch.tensor([self.top_k], dtype=torch.int32, device=device) if self.top_k else None
+            k = min(self.top_k, 2 ** 31 - 1)  # beyond any vocabulary: off
+            have["top_k"] = torch.tensor([k], dtype=torch.int32, device=device) if k else None
             have["top_p"] = torch.tensor([self.top_p], device=device) if self.top_p < 1.0 else None
             have["min_p"] = torch.tensor([self.min_p], device=device) if self.min_p else None
         if index not in have:
