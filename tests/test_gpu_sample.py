@@ -2,6 +2,7 @@
 from __future__ import annotations
 
 import math
+from fractions import Fraction
 
 import numpy as np
 import pytest
@@ -344,3 +345,52 @@ def test_min_p_above_one_keeps_the_first_token_alone(gpu, V):
             if not kw:
                 last = draw(gpu, rows, us, min_p=[1.0] * n)
                 assert last[:6] == [int(a[min(2, int(u * 3))]) for a in at[:6]]
+
+
+def ref_int(l, u, t=1.0, k=0, p=1.0) -> int:
+    """The definition with its weights as integers, multiples of 2^-44 of the largest, and every
+    sum and product exact."""
+    l = np.asarray(l, dtype=np.float32).astype(np.float64)
+    w = np.rint(np.exp((l - l.max()) / t) * 2.0 ** 44).astype(np.uint64)
+    order = np.lexsort((np.arange(l.size), -l))
+    if 0 < k < l.size:
+        order = order[:k]
+    if p < 1:
+        cum = np.cumsum(w[order], dtype=np.uint64)  # at most 2^63
+        need = math.ceil(Fraction(p) * int(cum[-1]))
+        order = order[: int(np.searchsorted(cum, np.uint64(max(need, 1)), side="left")) + 1]
+    kept = np.sort(order)
+    cum = np.cumsum(w[kept], dtype=np.uint64)
+    return int(kept[np.searchsorted(cum, np.uint64(math.floor(Fraction(u) * int(cum[-1]))), side="right")])
+
+
+@pytest.mark.parametrize("V", [1 << 19, (1 << 19) - 1, (1 << 19) - 8191])
+def test_largest_vocabularies_flat(gpu, V):
+    """Weights of one, whose sum reaches 2^63 and a thread's 2^53; the list overflows, so the row
+    is drawn by one workgroup with top-p, and with a top-k past the lists'."""
+    us = [0.0, 2.0 ** -24, 0.25, 0.7, LAST]
+    flat = torch.zeros(len(us), V)
+    token = lambda n: [math.floor(Fraction(f32(u)) * n) for u in us]  # noqa: E731
+    assert draw(gpu, flat, us) == token(V)
+    for k in (1, 600, 601, 5000, V - 1):
+        assert draw(gpu, flat, us, top_k=[k] * len(us)) == token(k)
+    for p in (2.0 ** -30, 0.3, LAST):
+        kept = max(1, math.ceil(Fraction(f32(p)) * V))
+        assert draw(gpu, flat, us, top_p=[p] * len(us)) == token(kept)
+        kept = math.ceil(Fraction(f32(p)) * 5000)
+        assert draw(gpu, flat, us, top_p=[p] * len(us), top_k=[5000] * len(us)) == token(kept)
+
+
+@pytest.mark.parametrize("V", [1 << 19, (1 << 19) - 1])
+@pytest.mark.parametrize("std", [0.2, 2.0])
+def test_largest_vocabularies_random(gpu, V, std):
+    g = torch.Generator().manual_seed(V)
+    n = 4
+    rows = torch.randn(n, V, generator=g) * std
+    t = [1.0, 0.7, 1.3, 0.5]
+    host = rows.numpy()
+    for k, p in ((0, 1.0), (0, 0.9), (0, 0.3), (40, 1.0), (300, 0.95), (600, 1.0), (601, 1.0), (601, 0.9),
+                 (20000, 0.5), (300000, 0.99)):
+        for u in (torch.rand(n, generator=g).tolist(), [LAST] * n):
+            got = draw(gpu, rows, u, temperature=t, top_k=[k] * n, top_p=[p] * n)
+            assert got == [ref_int(host[i], f32(u[i]), f32(t[i]), k, f32(p)) for i in range(n)], (k, p, u)

@@ -304,3 +304,27 @@ def test_a_nan_scale_gives_nan(gpu, dtype):
     got = c.run(scale=math.nan)
     keys = torch.tensor([len(c.keys(i)) > 0 for i in range(9)])
     assert not bool(keys.all()) and bool(got[keys].isnan().all()) and not bool(got[~keys].any())
+
+
+def test_rows_past_32_bit_offsets_to_the_last_bits(gpu):
+    """The bound of two bf16 terms a probability, far into a cache, in both layouts."""
+    Dh, rows, B = 64, (1 << 26) + 4096, 2048  # more than 2^32 elements
+    g = _gen(11)
+    tail = [torch.randn(B, 1, Dh, generator=g).bfloat16() for _ in range(2)]
+    q = torch.randn(3, 2, Dh, generator=g).bfloat16()
+    d = lambda x, dt: torch.tensor(x, dtype=dt, device=gpu)  # noqa: E731
+    base, outs = rows - B, []
+    for shape in ((rows, 1, Dh), (rows // B, 1, B, Dh)):
+        k, v = (torch.empty(shape, dtype=torch.bfloat16, device=gpu) for _ in range(2))
+        for t, x in zip((k, v), tail):
+            t.view(rows, 1, Dh)[-B:] = x.to(gpu)
+        outs.append(ops.attn_shared(q.to(gpu), k, v, d([base], torch.int64), d([1500], torch.int32),
+                                    d([0, 3], torch.int32), d([base + 1500 + 100 * i for i in range(3)], torch.int64),
+                                    d([90, 0, 5], torch.int32), prefix_len_max=1500, kv_len_max=90))
+        del k, v
+    assert torch.equal(*outs)
+    for i, L in enumerate((90, 0, 5)):
+        at = list(range(1500)) + list(range(1500 + 100 * i, 1500 + 100 * i + L))
+        check_attention(outs[0][i], *attend(q[i].double(), tail[0][at].double().transpose(0, 1),
+                                            tail[1][at].double().transpose(0, 1), 1 / math.sqrt(Dh),
+                                            P_STEP[torch.bfloat16]))
