@@ -9,6 +9,9 @@
 // P^T, the query heads of the kv head as the 16 columns. fp32 queries are split
 // into three bf16 terms, which hold all their bits; probabilities into two (a
 // half step of 2^-16 of each) or, for fp32, three. Statistics and sums are fp32.
+// A third term for bf16 outputs too moves their distance from the exact ones in the
+// seventh digit (0.00166 of the norm, their own rounding): 64 rows x 32.7k keys 393 ->
+// 424 us, 8 rows 10.5 -> 11.2.
 //
 // Bound by HBM: (Dh + 1) bytes of K and of V per key and kv head. P.V on the
 // VALU, as in wfd_attn_decode, took 1600 vector instructions per 64 keys of four

@@ -31,11 +31,14 @@ constexpr int kShMaxHeads = 4096;  // a chunk's keys stay within 32-bit offsets 
 // Keys per chunk of a prefix of P keys: 128 chunks over the kv heads, a workgroup
 // each for every second CU, while they are at least 128 keys: the parts' traffic
 // grows with the chunks, and a group's pairs and the other groups fill the rest.
-// 64 rows x 8000 keys x 16 heads, 100 rows over three prefixes of 20-32k x 4, and 64
-// over four of 2000 x 16 take 53 / 85-88 / 57 us, with 256 chunks 54 / 98 / 60, with 64
-// 54 / 84 / 57; 8 rows x 32000 x 4 26.7, 25.9 and 26.6. At most 1024 keys (512: 55 / 96 /
-// 57; 2048 as 1024), and 512 of a row's own (256: 57 / 90 / 54; 1024: 53 / 88 / 54;
-// all with P in one term).
+// In us, with 64 / 128 / 256 chunks (rows x keys x kv heads):
+//   few rows:  4 x 2000 x 16  14.1 / 12.6 / 13.8    4 x 8000 x 4    15.0 / 13.8 / 15.5
+//              4 x 16000 x 2  16.0 / 14.9 / 18.2    16 x 4000 x 16  23.7 / 18.8 / 17.7
+//              8 x 32000 x 4  27.5 / 27.5 / 27.4
+//   many:      64 x 8000 x 16 56 / 56 / 59          64 over 4 x 2000 x 16  44 / 47 / 54
+//              100 over 3 x 20-32k x 4  92-94 / 92-97 / 109
+// At most 1024 keys (512: 58 for 64 x 8000, 105 for the 100 rows; 2048: 55, 95), and 512
+// of a row's own (256: 60 and 98; 1024: 56 and 95).
 __host__ __device__ inline int prefix_chunk(int P, int Hkv) {
   const int64_t c = ((int64_t)P * Hkv + kShTarget - 1) / kShTarget;
   const int64_t r = (c + kShMinChunk - 1) / kShMinChunk * kShMinChunk;
@@ -245,12 +248,12 @@ __device__ __forceinline__ void sh_keep(const ShItem& it, int wave, int col, int
 // V^T comes out of the row-major tile by transposing LDS reads. Keys past the
 // chunk read as zeros and score -inf.
 //
-// 64 rows x 8000 keys x 16 heads: 48 us and 5 for the merge (floor 41), of which the
-// loads alone take 43; 100 rows x 20-32k x 4 kv heads: 82-86 + 7, loads alone 60: each
+// 64 rows x 8000 keys x 16 heads: 50 us and 5 for the merge (floor 41), of which the
+// loads alone take 43; 100 rows x 20-32k x 4 kv heads: 84-88 + 8, loads alone 60: each
 // tile of 32 pairs takes its prefix from the L2 again (740 MB, 12 TB/s), and products
 // and exponentials only partly hide behind them at two waves per SIMD. 64 pairs a
 // wave (57 -> 69 and 100 -> 129 us), eight waves sharing the tiles of 64 pairs (55 -> 56
-// and 89 -> 94) and two chains of K Q^T (as one) were no faster.
+// and 89 -> 94) and two chains of K Q^T (as one) were no faster, all with P in one term.
 template <int DH>
 __global__ __launch_bounds__(64 * kShWaves) __attribute__((amdgpu_waves_per_eu(2))) void attn_shared_bf16_kernel(
     ShArgs a) {
@@ -367,8 +370,9 @@ __global__ __launch_bounds__(64 * kShWaves) __attribute__((amdgpu_waves_per_eu(2
     }
     sh_softmax<NDB>(sc, o, mref, lrun, scale);
     // P meets V in two bf16 terms, half a step of 2^-16 of it. In one (2^-8, at random
-    // signs) the output was 0.0023 of its norm off instead of 0.0017, which is its own
-    // rounding, for 0-5 % less time; fp32 products take 8 times the MFMA time.
+    // signs) the output was 0.0023 of its norm off instead of 0.00166, which is its own
+    // rounding, for 0-5 % less time; a third term changes that in the seventh digit and
+    // costs 100 rows x 20-32k 90 -> 99 us; fp32 products take 8 times the MFMA time.
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       u32x4 hi, lo;
@@ -419,8 +423,8 @@ __global__ __launch_bounds__(64 * kShWaves) __attribute__((amdgpu_waves_per_eu(2
 // S^T register r is key 8 (r / 4) + 4 hf + r % 4, which is also the key it supplies of
 // P^T at step r. K goes through LDS; V^T comes straight from the cache, 32 consecutive
 // values of a row to half of the lanes, loaded under the scores, and the next tile of K
-// under P V, into the registers that V leaves. 64 rows x 8000 keys x 16 heads: 125 us
-// (floor 82; its products alone, by count, 55); V through LDS too, which leaves a wave per SIMD,
+// under P V, into the registers that V leaves. 64 rows x 8000 keys x 16 heads: 124-139
+// us (floor 82; its products alone, by count, 55); V through LDS too, which leaves a wave per SIMD,
 // 152; 16 pairs on the 16x16x4 form, operands straight from the cache, 371.
 template <int DH>
 __global__ __launch_bounds__(64 * kShWaves) __attribute__((amdgpu_waves_per_eu(2))) void attn_shared_f32_kernel(

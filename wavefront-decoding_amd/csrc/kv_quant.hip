@@ -5,8 +5,8 @@
 // few shuffles within those lanes, the codes leave as 8 bytes a lane and the
 // exponent as one byte from the row's first lane. Bound by memory: every value
 // is read once and every code written once. 8192 bf16 rows of 16 heads x 128 take
-// 21 us to write (4.8 TB/s; a large copy reaches 4.9) and 19.6 to read back; the
-// few rows of a decode step 2.7 us a launch, the launch itself.
+// 20.6 us to write (4.9 TB/s, as a large copy) and 19.2 to read back, fp32 ones 34 and
+// 29; the few rows of a decode step 2.7 us a launch, the launch itself.
 #include <type_traits>
 
 #include "quant.h"
@@ -59,8 +59,8 @@ __device__ __forceinline__ void write_row(const float (&x)[8], int sub, int64_t 
 }
 
 // bf16 lanes take a K and a V row, 32 bytes of loads in flight as an fp32 lane has of
-// one: 8192 rows x 16 heads x 128 in 21 us where a row a lane group took 23.8 (fp32
-// pairs: 72.6 -> 76).
+// one: the write of 8192 rows x 16 heads x 128 in 20.6 us where a row a lane group took
+// 24.6; fp32 34 us (4.9 TB/s) either way, and with the read back 74 us against 75.5.
 template <typename T>
 constexpr bool kAppendPair = sizeof(T) == 2;
 

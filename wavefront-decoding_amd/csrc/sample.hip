@@ -132,7 +132,13 @@ constexpr int kSmLong = 32768;       // longest row of one workgroup
 constexpr int kSmSlab = 8192;
 constexpr int kSmSlabs = kSmMaxVocab / kSmSlab;
 constexpr int kSmRowList = 8192;     // tokens that the slabs of a row may list
-constexpr int kSmGuess = 600;        // top-k to which the list is tried: ~900 tokens reach the 600th thread's
+// Top-k to which the list is tried: ~900 tokens reach the 600th thread's. The slabs of a
+// long row list as many each, and past kSmRowList in all the last launch draws the row
+// alone, as it does for a larger top-k without having tried. 16 rows, top-k 50 / 200 / 300
+// / 600 / 601 in us:  65536 logits 20 / 25 / 27 / 29 / 45;  128000 21 / 26 / 29 / 57 / 65;
+// 262144 27 / 34 / 75 / 79 / 98;  524288 39 / 118 / 126 / 130 / 171. Tried to 200 only,
+// top-k 300 of these takes 42 / 62 / 94 / 166; never, 50 takes 34 / 52 / 85 / 154.
+constexpr int kSmGuess = 600;
 constexpr float kSmMasked = -1e4f;  // logits down to here spread the bins; the others share the last
 
 // 2^x for x <= 0 in units of 2^-44, rounded to an integer: x = m / 128 + r, 2^r by its

@@ -5,9 +5,10 @@ every iteration is one R tick over the whole wave; P runs for tokens queued
 by the previous iteration; C runs when the tick brought a token to its draft
 point (step == T_draft, copied) or commit point (step == T_total, moved).
 The verify at position N finalizes N+1 against the token already speculated
-there: equal argmax -> accept; otherwise commit the argmax, roll back every
-slot at/after N+1 and re-enter the corrected token (cascade). A boundary
-(nothing speculated at N+1 yet) commits the argmax directly. After an
+there: equal to the sampler's token of the full-depth logits (greedy: their
+argmax) -> accept; otherwise commit that token, roll back every slot at/after
+N+1 and re-enter it (cascade). A boundary (nothing speculated at N+1 yet)
+commits it directly. After an
 accepted (or boundary) settle, the draft logits of this tick seed the next
 leading-edge token.
 
@@ -55,15 +56,17 @@ def _sync(device) -> None:
 @torch.no_grad()
 def generate_wavefront_dynamic(blocks, prompt_ids: torch.Tensor, max_new_tokens: int, policy: SsdPolicy,
                                eos_token_id: int | None = None) -> tuple[list[int], GenerationTrace]:
-    """Greedy lossless WFD for one sequence. Stops at max_new_tokens or when a
-    committed token equals eos_token_id. Returns (tokens, trace)."""
+    """Lossless WFD for one sequence, greedy or drawn as the policy says: the
+    committed tokens are those of sequential decoding with its sampler. Stops at
+    max_new_tokens or when a committed token equals eos_token_id. Returns
+    (tokens, trace)."""
     return wavefront_single(blocks, prompt_ids, max_new_tokens, policy, None, eos_token_id)
 
 
 def _decide(sampler, emu, draft_token: int, draft_probs, logits, position: int) -> tuple[bool, int]:
-    """(accept, gold) for a draft at `position`: the greedy comparison, or the
+    """(accept, gold) for a draft at `position`: the sampler's comparison, or the
     next Bernoulli draw of an emulated-acceptance stream (gold is still the
-    full-depth argmax, committed on a reject)."""
+    sampler's token of the full-depth logits, committed on a reject)."""
     if emu is None:
         return sampler.verify(draft_token, draft_probs, logits, position)
     return emu.draw(), sampler(logits, position)
@@ -71,7 +74,7 @@ def _decide(sampler, emu, draft_token: int, draft_probs, logits, position: int) 
 
 def wavefront_single(blocks, prompt_ids: torch.Tensor, max_new_tokens: int, policy: SsdPolicy, emu=None,
                      eos_token_id: int | None = None) -> tuple[list[int], GenerationTrace]:
-    """The WFD loop behind generate_wavefront_dynamic (emu None: greedy
+    """The WFD loop behind generate_wavefront_dynamic (emu None: the sampler's
     comparisons) and generate_wavefront_emu (each accept decided by emu.draw())."""
     trace = GenerationTrace()
     device = prompt_ids.device
@@ -159,16 +162,17 @@ def _finish(trace: GenerationTrace, device, t0: float, warm: float | None):
 def generate_draft_then_verify(blocks, prompt_ids: torch.Tensor, max_new_tokens: int, policy: SsdPolicy,
                                draft_length: int, eos_token_id: int | None = None
                                ) -> tuple[list[int], GenerationTrace]:
-    """Greedy draft-then-verify with nested reuse for one sequence
-    (src/decoding/scheduler.py:227-367). Each round forwards sources p..p+K one
-    after another at the shallow depth T_draft (a source's shallow argmax is
-    the next source's token and the draft for its position), then continues
-    all K+1 sources together to T_total -- the shallow recurrence is the prefix
-    of the full one, nothing is recomputed -- and verifies the drafts in order
-    against the full-depth argmaxes: the first mismatch commits the gold token
-    and drops every slot row from there on; if all K match, the last source's
-    gold is a free bonus token. Lossless: every committed token is a
-    full-depth argmax. Stops at max_new_tokens or a committed eos_token_id."""
+    """Draft-then-verify with nested reuse for one sequence, greedy or drawn as
+    the policy says (src/decoding/scheduler.py:227-367). Each round forwards
+    sources p..p+K one after another at the shallow depth T_draft (the sampler's
+    token of a source's shallow logits is the next source's token and the draft
+    for its position), then continues all K+1 sources together to T_total -- the
+    shallow recurrence is the prefix of the full one, nothing is recomputed --
+    and verifies the drafts in order against the sampler's tokens of the
+    full-depth logits: the first mismatch commits the gold token and drops every
+    slot row from there on; if all K match, the last source's gold is a free
+    bonus token. Lossless: every committed token is the sampler's of full-depth
+    logits. Stops at max_new_tokens or a committed eos_token_id."""
     return dtv_single(blocks, prompt_ids, max_new_tokens, policy, draft_length, None, eos_token_id)
 
 

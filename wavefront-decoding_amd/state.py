@@ -32,7 +32,7 @@ class ActiveToken:
     is_alive: bool = True
     hidden: Optional[object] = None         # optional host handle; the state lives at `row`
     static_state: Optional[object] = None
-    draft_probs: Optional[object] = None    # temperature sampling is out of scope (greedy only)
+    draft_probs: Optional[object] = None    # unused: a draft is verified by drawing its position again
     should_exit: bool = False               # adaptive early exit is out of scope: always False
 
 
