@@ -120,8 +120,8 @@ class BatchStaticKVCache:
 
     def write_tokens(self, slots, seq_ids, positions, k: torch.Tensor, v: torch.Tensor) -> None:
         """Scatter n tokens: k, v (n, Hkv, Dh) -> (slots[i], seq_ids[i], positions[i])."""
-        slots = [range(self.n_slots)[sl] for sl in slots]
-        seq_ids = [range(self.B)[b] for b in seq_ids]
+        slot, seq = range(self.n_slots), range(self.B)
+        slots, seq_ids = [slot[sl] for sl in slots], [seq[b] for b in seq_ids]
         for sl, b, p in zip(slots, seq_ids, positions):
             self.note_write(sl, b, p)
         rows = torch.tensor([self.flat_row(sl, b, p) for sl, b, p in zip(slots, seq_ids, positions)],
