@@ -212,6 +212,28 @@ def test_a_row_alone_has_the_same_bits(gpu):
             assert all(torch.equal(a[0], b[r]) for a, b in zip(one, many)), (V, r)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("V", [2064385, 2097172])
+def test_last_slab_shorter_than_the_top(gpu, dtype, V):
+    """Vocabularies whose last slab of 32768 has 1 or 20 logits: the tokens come from logits alone, whatever the
+    workspace held, also where the row is searched one token after the other."""
+    l = _logits(gpu, 4, V, dtype, seed=7, masked=False)
+    l[0, V - 1] = 60.0
+    l[1, V - 1] = math.nan
+    l[2, 5] = math.nan
+    l[3] = -math.inf
+    top = 64
+    need = ops.logprobs_workspace_bytes(4, V, top)
+    for fill in (0xff, 0x7f):
+        ws = torch.full((need,), fill, dtype=torch.uint8, device=gpu)
+        _, _, tv, ti = ops.logprobs(l, top=top, workspace=ws)
+        for r in range(4):
+            x = l[r].float()
+            order = torch.sort(torch.where(x.isnan(), math.inf, x), descending=True, stable=True)[1][:top]
+            assert torch.equal(ti[r], order), (fill, r)
+        assert tv[0].isfinite().all() and tv[1:].isnan().all()
+
+
 def test_far_rows(gpu):
     """Rows past 2^31 logits of the tensor."""
     V = 128000

@@ -325,6 +325,9 @@ __global__ __launch_bounds__(TH) __attribute__((amdgpu_waves_per_eu(8))) void lo
         a.top_id[u * a.top + k] = j;
       }
     };
+    // a slab of fewer logits than a.top leaves the rest as key 0, which ranks behind every logit
+    if (a.parts > 1)
+      for (int k = len + tid; k < a.top; k += TH) a.tops[u * a.top + k] = 0;
     if (wave == 0) t = over_waves(t_lds[tid & (W - 1)], add);
     if (tid == 0) {
       if (a.parts > 1) {
@@ -373,7 +376,7 @@ __global__ __launch_bounds__(TH) __attribute__((amdgpu_waves_per_eu(8))) void lo
     if (a.top && (nan || count > kLpList)) {  // uniform
       float lv = 0.f;
       int li = -1;
-      for (int k = 0; k < a.top; ++k) {
+      for (int k = 0; k < min(a.top, len); ++k) {
         float bv = -INFINITY;
         int bi = INT_MAX;
         for (int j = tid; j < len; j += TH) {
