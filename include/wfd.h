@@ -334,6 +334,7 @@ int wfd_attn_decode_q(const void* q, const void* k_codes, const void* v_codes, c
  * (n, H, Dh), k rotated and v to their pages. A row at a position below 0 or past
  * the rope tables is not stored, and its q is NaN; the tables are 16-byte aligned.
  * wfd_kv_append_paged: k, v rows (Hkv, Dh) at pitches ldk, ldv as they are.
+ * Both take up to 2^24 - 1 rows.
  * Two rows of one call are never at one place, unless the tables share a page that
  * both write: one of them is kept, whole per 16 bytes.
  * Replaces: what wfd_qkv_rope_append and wfd_kv_append replace, over a cache the

@@ -147,3 +147,14 @@ def test_c_entry_points_refuse():
         assert logp(**kw) == -1, kw
     assert logp(dtype=3) == -2 and logp(V=100, ld=100, top=65) == -2 and logp(n=0) == 0 and logp(logits=16) == 0
     assert logp(logits=16, out=16, ids=16, V=40000, ld=40000) == -4
+
+
+def test_appends_refuse_rows_beyond_the_grid():
+    """A row is a workgroup of 256 threads, and a launch has fewer than 2^32 of these."""
+    lib = _lib.load()
+    for n, rc in ((2 ** 24, -2), (2 ** 31 - 1, -2)):
+        assert lib.wfd_kv_append_paged(16, 64, 16, 64, 16, 16, 1, 16, 4, 4, 9, 16, 16, 16, 0, n, 1, 64, 1, None) == rc
+        assert b"beyond the grid" in lib.wfd_last_error()
+        assert lib.wfd_qkv_rope_append_paged(16, 192, 16, 16, 1, 16, 4, 4, 9, 16, 16, 16, 8, 16, 16, 16, 0, n, 1, 1,
+                                             64, 1, None) == rc
+        assert b"beyond the grid" in lib.wfd_last_error()

@@ -5,7 +5,7 @@
 // 16-byte pieces a thread, then each wave finds the row's sequence by a look at cu_q (64
 // entries a load), its position, its page, and the sines and cosines of that position,
 // four (fp32: two) pairs a load. Bound by memory, every value read once and written once:
-// 8180 rows of 16 + 2 * 16 heads of 128 bf16 39 us (5.2 TB/s, a large copy's rate; 51 us
+// 8332 rows of 16 + 2 * 16 heads of 128 bf16 39 us (5.2 TB/s, a large copy's rate; 51 us
 // with the values asked for after the place is known and the table read number by
 // number). 8 rows 3.5 us, the launch and that chain of loads (4.3).
 #include "pages.h"
@@ -13,6 +13,7 @@
 namespace wfd {
 
 constexpr int kPgThreads = 256;
+constexpr int kPgMaxRows = (1 << 24) - 1;  // a workgroup each: a launch has fewer than 2^32 threads
 constexpr int kPgAhead = 3;  // pieces of a thread asked for before the row's place is known
 
 struct PgRow {
@@ -149,6 +150,10 @@ int wfd_qkv_rope_append_paged(const void* qkv, int64_t ldq, const int32_t* cu_q,
               (long long)ldq);
     return kBadArg;
   }
+  if (n > kPgMaxRows) {
+    set_error("%s: n=%d beyond the grid (up to %d rows)", me, n, kPgMaxRows);
+    return kUnsupported;
+  }
   if (n == 0 || nseq == 0) return kOk;
   if (!qkv || !cu_q || !kv_len || !rope_cos || !rope_sin || !q_out || (pages_per_seq && !page_table) ||
       (num_pages && (!k_pages || !v_pages))) {
@@ -189,6 +194,10 @@ int wfd_kv_append_paged(const void* k, int64_t ldk, const void* v, int64_t ldv, 
   if (n < 0 || ldk < (int64_t)Hkv * Dh || ldv < (int64_t)Hkv * Dh || ldk % vec || ldv % vec) {
     set_error("%s: bad shape n=%d Hkv=%d Dh=%d ldk=%lld ldv=%lld", me, n, Hkv, Dh, (long long)ldk, (long long)ldv);
     return kBadArg;
+  }
+  if (n > kPgMaxRows) {
+    set_error("%s: n=%d beyond the grid (up to %d rows)", me, n, kPgMaxRows);
+    return kUnsupported;
   }
   if (n == 0 || nseq == 0 || pages_per_seq == 0 || num_pages == 0) return kOk;
   if (!k || !v || !cu_q || !kv_len || !page_table || !k_pages || !v_pages) {
