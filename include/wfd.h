@@ -363,8 +363,11 @@ int wfd_kv_append_paged(const void* k, int64_t ldk, const void* v, int64_t ldv, 
  * 32, any scale. workspace >= wfd_attn_paged_workspace_bytes(...), 16-byte aligned.
  * fp32 statistics, sums and division; probabilities meet V with 16 significant bits
  * (fp32: 24), in sequences of more than 64 rows x H / Hkv with 8, where their
- * products bound the call. A row's bits depend on its own sequence's
- * rows, length and pages' contents and on the head counts, window and sinks, not on
+ * products bound the call. In sequences of up to 64 rows x H / Hkv a row's bits
+ * depend on its query, its position, the keys it attends, the head counts, window and
+ * sinks alone: the rows of a draft have the bits of the single tokens that they verify
+ * (but for an infinity in V under a probability below 2^-126, which makes infinity or
+ * NaN). In longer ones they depend on the sequence's row count and length too; never on
  * the other sequences of the call or on where the pages are. Infinities and NaN in K
  * and V reach only the rows that attend them.
  * Replaces: attn_varlen over gathered prefixes (src/decoding/fa4_attention.py:301-366,

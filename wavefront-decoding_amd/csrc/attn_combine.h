@@ -72,8 +72,7 @@ __global__ __launch_bounds__(DH) void attn_combine_kernel(const float* __restric
 // 100 rows x 16 heads x ~30 parts 7.6 us, where a thread per column took 11.
 constexpr int kMergeThreads = 256;
 
-// KEYED: the row has keys, so a sum of zero is of scores that are all -inf (NaN).
-template <typename T, int DH, bool KEYED = false, typename At>
+template <typename T, int DH, typename At>
 __device__ __forceinline__ void attn_merge_parts(const float* __restrict__ po, const float* __restrict__ pml, int ns,
                                                  At at, T* __restrict__ row) {
   constexpr int TPS = DH / 4, NS = kMergeThreads / TPS, B = 4;
@@ -131,7 +130,7 @@ __device__ __forceinline__ void attn_merge_parts(const float* __restrict__ po, c
     L = fmaf(l_lds[q], f, L);
     out = fmaf(o_lds[q][c], f, out);
   }
-  Elem<T>::store(row + c, KEYED ? out / L : attn_finish_nan(out, L));
+  Elem<T>::store(row + c, attn_finish_nan(out, L));
 }
 
 // Row r of a packed varlen call (the FA varlen convention): query row r of

@@ -11,8 +11,12 @@
 // softmaxes over its parts: a part leaves its maximum m, sum l and unnormalised
 // output o, and attn_paged_combine adds them up.
 //
-// How a sequence is cut follows from its own rows, length and the head counts, and
-// a row's arithmetic from that, so a row's bits do not depend on the rest of the call.
+// A sequence of few rows (up to kPaFewPairs pairs of a kv head) is cut at key positions
+// that are the same for every row, and a wave of a part takes every fourth block of it by
+// the block's place in the sequence. What a tile holds beside a row then adds hidden keys to
+// it and nothing else, and a hidden key changes no bit: a row has the bits it has alone,
+// as the next token of its context. A sequence of more rows is cut by its own rows and
+// length. In either case the rest of the call has no part in it.
 #include <type_traits>
 
 #include "attn_combine.h"
@@ -33,23 +37,25 @@ constexpr int kPaManyRows = kPaRows * kPaWaves;
 // divisions in that 112 single rows took 141 us for 134.
 constexpr int kPaLogBlock = 5, kPaBlock = 1 << kPaLogBlock;
 constexpr int kPaManyLogBlock = 6, kPaManyBlock = 1 << kPaManyLogBlock;
-// Keys per part, where there are several. Few rows, least: one row of 16 heads over 1000 keys 13.7
-// us (with 512: 16); most: one row over 8000 keys 24 us (with 2048: 34). Many rows: 128 of 16
+// Few rows: parts of 512 keys up to key 32768 / Hkv, of 1024 behind it; under a window of 512. One
+// row of 16 heads over 1000 keys takes 16.9 us, 8 over 511 to 777 18.3, 64 over 500 / 600 keys 45.6
+// / 70, 8 of 4 kv heads over 1000 to 1200 17.1. With near parts of 256: 13.9, 18.4, 51 / 64, 15.2,
+// and 16 drafts of 8 rows over 500 to 3000 keys 48.5 for 39.6. With 1024 throughout: 18.5, 16.6,
+// 45.6 / 53, 23.6, and one row over 2000 keys 22.7 for 17.1, as with half as many near parts; with
+// twice as many 64 rows over 32700 keys, 4 kv heads, 773 for 767 (1024: 746). Windows with parts
+// of 1024: 64 rows, window 1024, 48.7 for 37.7, window 4096 122 for 117.
+constexpr int kPaLogNear = 4, kPaLogFar = 5;  // blocks of either
+constexpr int kPaNear = 64;                   // near parts x kv heads
+// fp32 sequences of more pairs: parts x tiles x kv heads that are aimed at, and the least keys of a part.
+constexpr int kPaTarget = 64;
+constexpr int kPaMinPart = 256;
+// Many rows: two workgroups a CU (512 rows behind 7600 keys 75 us, with half as many 91; with the
+// parts' sizes rounded up to powers of two 80 behind 7700) of at least 512 keys: 128 rows of 16
 // heads over 1000 keys 25 us (with 1024: 36, with 256: 22), 32 such sequences 133 (134, 172);
 // twice that for a sequence of 64 (tile, kv head)s, four times for one of 96 (4 x 512 rows over
 // 2048 keys, 4 kv heads, 71 us for 83; 300 rows of 16 heads over 1000 keys, of 48, would take 38
 // for 29).
-constexpr int kPaMinPart = 256;
-constexpr int kPaMaxPart = 1024;
 constexpr int kPaManyMinPart = 512;
-// Keys up to which few bf16 rows stay whole: a second launch costs more than their parts save. One
-// row of 16 heads over 300 / 500 / 760 keys 10.8 / 12.2 / 15.3 us for 13.0 / 13.3 / 13.5, 64 such
-// rows 30 / 44 / 76 for 37 / 47 / 84. (fp32 blocks take longer: 33 sequences' drafts 26.4, not 28.)
-constexpr int kPaWhole = 768;
-// Parts x tiles x kv heads of a sequence that are aimed at. Few rows: 64 (with 32 one row over
-// 2000 keys takes 20 us for 16). Many: two workgroups a CU (512 rows behind 7600 keys 75 us, with
-// half as many 91; with the parts' sizes rounded up to powers of two 80 behind 7700).
-constexpr int kPaLogTarget = 6, kPaTarget = 1 << kPaLogTarget;
 constexpr int kPaManyLogTarget = 9, kPaManyTarget = 1 << kPaManyLogTarget;
 // Workgroups of a launch, which take the items in turn: of few rows those that the card holds
 // at once (the host knows bounds of the items only; with four times as many 33 sequences' drafts
@@ -57,6 +63,23 @@ constexpr int kPaManyLogTarget = 9, kPaManyTarget = 1 << kPaManyLogTarget;
 constexpr int kPaResident = 512;
 constexpr int kPaManyGrid = 8192;
 constexpr int kPaMergeGrid = 2048;
+
+// Where a sequence's blocks are cut: `near` parts of 2^kPaLogNear blocks from position 0 on, behind
+// them parts of 2^lf.
+struct PaCut {
+  int near, lf;
+  __host__ __device__ int of(int block) const {
+    const int nb = near << kPaLogNear;
+    return block < nb ? block >> kPaLogNear : near + ((block - nb) >> lf);
+  }
+  __host__ __device__ int start(int part) const {
+    return part < near ? part << kPaLogNear : (near << kPaLogNear) + ((part - near) << lf);
+  }
+};
+
+inline PaCut pa_few_cut(int Hkv, int window) {
+  return window ? PaCut{0, kPaLogNear} : PaCut{(kPaNear + Hkv - 1) / Hkv, kPaLogFar};
+}
 
 struct PaArgs {
   const void *q, *kp, *vp;
@@ -72,6 +95,7 @@ struct PaArgs {
   uint32_t many_wgs, many_lead;  // of a kv head
   int few_rows;          // rows kept per sequence, 0: by the row's number
   int many_pairs;        // slots kept per sequence, 0: by the row's number
+  PaCut cut;             // of few rows
   float scale_log2;
 };
 
@@ -86,29 +110,37 @@ __host__ __device__ inline int pa_blocks(int len, int rows, int window, int sink
   return some < all ? some : all;
 }
 
-// Blocks per part, the least number that leaves a sequence of `tiles` tiles of `blocks` blocks
-// at most the target's parts; of few rows the least power of two.
-__host__ __device__ inline int pa_part(bool many, int tiles, int blocks, int Hkv) {
-  const int lt = many ? kPaManyLogTarget : kPaLogTarget;
+// Blocks per part of many rows, the least number that leaves a sequence of `tiles` tiles of
+// `blocks` blocks at most the target's parts.
+__host__ __device__ inline int pa_part(int tiles, int blocks, int Hkv) {
   const int wide = tiles * Hkv;  // with many of them a part saves less than its merge costs
   const int more = wide >= 96 ? 4 : (wide >= 64 ? 2 : 1);
-  const int least = many ? more * kPaManyMinPart / kPaManyBlock : kPaMinPart / kPaBlock;
-  const int64_t p = ((int64_t)blocks * Hkv * tiles + (1 << lt) - 1) >> lt;
-  const bool bound = !many && tiles * kPaRows <= kPaFewPairs;  // at most kPaMaxPart keys
-  const int most = bound ? kPaMaxPart / kPaBlock : 1 << 29;
-  const int r = (int)(p < least ? least : (p < most ? p : most));
-  return many ? r : 1 << (32 - __builtin_clz((unsigned)(r - 1)));
+  const int least = more * kPaManyMinPart / kPaManyBlock;
+  const int64_t p = ((int64_t)blocks * Hkv * tiles + kPaManyTarget - 1) >> kPaManyLogTarget;
+  return (int)(p < least ? least : (p < (1 << 29) ? p : 1 << 29));
 }
-__host__ __device__ inline int pa_parts(bool many, int blocks, int part) {  // of a list of blocks
-  const uint32_t x = (uint32_t)blocks + (uint32_t)part - 1;
-  return (int)(many ? x / (uint32_t)part : x >> __builtin_ctz((unsigned)part));
+__host__ __device__ inline int pa_parts(int blocks, int part) {  // of a list of blocks
+  return (int)(((uint32_t)blocks + (uint32_t)part - 1) / (uint32_t)part);
+}
+
+// Parts that a tile of `rows` rows sees at most of `len` positions.
+__host__ __device__ inline int pa_most_parts(PaCut cut, int len, int rows, int window, int sinks) {
+  if (len <= 0) return 1;
+  const int all = cut.of((len - 1) >> kPaLogBlock) + 1;
+  if (!window) return all;
+  const int ls = cut.near && kPaLogNear < cut.lf ? kPaLogNear : cut.lf;
+  const int run = (int)(((uint32_t)window + rows - 1 + kPaBlock - 1) >> kPaLogBlock) + 1;  // blocks in a row
+  const int some = (sinks ? cut.of((sinks - 1) >> kPaLogBlock) + 1 : 0) + ((run - 2 + (1 << ls)) >> ls) + 1;
+  return some < all ? some : all;
 }
 
 struct PaSeq {
   int b, q0, nq, ne;  // the sequence, its first row, its rows, those within the bound
   int pos0;           // the first row's position
   bool many;
-  int tiles, part;    // its tiles, their blocks per part
+  int tiles;
+  int part;           // many: blocks per part of a tile
+  PaCut cut;          // otherwise: of the sequence
   int parts;          // at most, of a tile
 };
 
@@ -121,23 +153,43 @@ __device__ __forceinline__ PaSeq pa_seq(const PaArgs& a, int b, int c0, int c1, 
   kv = max(kv, 0);
   s.pos0 = kv - (c1 - c0);
   s.ne = min(max(s.nq, 0), a.qmax);
-  s.many = sizeof(T) == 2 && s.ne * a.G > kPaFewPairs;
-  const int rows = s.many ? a.many_tile : a.few_tile;
-  const int blocks =
-      pa_blocks(min(kv, a.kmax), rows, a.window, a.sinks, s.many ? kPaManyLogBlock : kPaLogBlock);
+  const bool large = s.ne * a.G > kPaFewPairs;
+  s.many = sizeof(T) == 2 && large;
+  const int rows = s.many ? a.many_tile : a.few_tile, len = min(kv, a.kmax);
   s.tiles = s.ne <= rows ? min(s.ne, 1) : (int)((uint32_t)(s.ne - 1) / (uint32_t)rows) + 1;
-  const bool whole = sizeof(T) == 2 && !s.many && blocks <= kPaWhole / kPaBlock;
-  s.part = whole ? kPaMaxPart / kPaBlock : pa_part(s.many, s.tiles, blocks, a.Hkv);
-  s.parts = max(pa_parts(s.many, blocks, s.part), 1);
+  s.cut = a.cut;
+  if (s.many) {
+    const int blocks = pa_blocks(len, rows, a.window, a.sinks, kPaManyLogBlock);
+    s.part = pa_part(s.tiles, blocks, a.Hkv);
+    s.parts = max(pa_parts(blocks, s.part), 1);
+    return s;
+  }
+  s.part = 0;
+  if (sizeof(T) == 4 && large) {
+    const int wide = s.tiles * a.Hkv;
+    const int blocks = pa_blocks(len, rows, a.window, a.sinks, kPaLogBlock);
+    const int p = wide >= kPaTarget ? 1 << 26 : max((int)(((uint32_t)blocks * wide + kPaTarget - 1) / kPaTarget), kPaMinPart / kPaBlock);
+    s.cut = PaCut{0, 32 - __builtin_clz((unsigned)(p - 1))};
+  }
+  s.parts = pa_most_parts(s.cut, len, rows, a.window, a.sinks);
+  if (a.window && len > 0) {  // uniform; the parts from the first row's window on, and the sinks'
+    const int lo = max(max(s.pos0, 0) - a.window + 1, 0) >> kPaLogBlock;
+    const int some = (a.sinks ? s.cut.of((a.sinks - 1) >> kPaLogBlock) + 1 : 0) +
+                     max(s.cut.of((len - 1) >> kPaLogBlock) - s.cut.of(lo), 0) + 1;
+    s.parts = min(s.parts, some);
+  }
   return s;
 }
 
-// A tile of rows: the list of its visible blocks.
+// A tile of rows, and its visible blocks: those with sinks, and a run to its last row. Of many
+// rows they are a list that is cut into parts; of few the parts are those of the sequence that
+// hold any.
 struct PaTile {
   int i0, nr;       // its first row in the sequence and the number of its pairs
   int pmin, pmax;   // first and last position, the last below kmax
-  int ns, first, nt;  // blocks with sinks, the first block of the window, blocks in all
-  int in0, in1;     // the blocks [in0, in1) of the list that every row sees whole
+  int ns, first, nt;  // blocks with sinks, the first block of the run, blocks in all
+  int in0, in1;     // the blocks [in0, in1) that every row sees whole: many, of the list; few, of the sequence
+  int sink_parts, first_part;  // few: parts with sinks, the run's first other part
   int parts;        // one at least
 };
 
@@ -151,17 +203,43 @@ __device__ __forceinline__ PaTile pa_tile(const PaArgs& a, const PaSeq& s, int t
   t.nr = count * a.G;
   t.pmin = s.pos0 + t.i0;
   t.pmax = min(t.pmin + count - 1, a.kmax - 1);
-  t.ns = t.first = t.nt = t.in0 = t.in1 = 0;
+  t.ns = t.first = t.nt = t.in0 = t.in1 = t.sink_parts = t.first_part = 0;
   t.parts = 1;
   if (count <= 0 || t.pmax < 0) return t;
   const int lo = a.window ? max(max(t.pmin, 0) - a.window + 1, 0) : 0;
   t.ns = (min(a.sinks, lo) + BLOCK - 1) / BLOCK;
   t.first = max(min(lo, t.pmax) / BLOCK, t.ns);
   t.nt = t.ns + t.pmax / BLOCK + 1 - t.first;
-  t.in0 = t.ns + max((a.window ? max(t.pmax - a.window + BLOCK, 0) / BLOCK : 0) - t.first, 0);
-  t.in1 = t.ns + (t.pmin + 1 > 0 ? (t.pmin + 1) / BLOCK : 0) - t.first;
-  t.parts = pa_parts(MANY, t.nt, s.part);
+  t.in0 = max(a.window ? max(t.pmax - a.window + BLOCK, 0) / BLOCK : 0, t.first);
+  t.in1 = t.pmin + 1 > 0 ? (t.pmin + 1) / BLOCK : 0;
+  if constexpr (MANY) {
+    t.in0 += t.ns - t.first;
+    t.in1 += t.ns - t.first;
+    t.parts = pa_parts(t.nt, s.part);
+  } else {
+    t.sink_parts = t.ns ? s.cut.of(t.ns - 1) + 1 : 0;
+    t.first_part = max(s.cut.of(t.first), t.sink_parts);
+    t.parts = t.sink_parts + max(s.cut.of(t.pmax / BLOCK) - t.first_part + 1, 0);
+  }
   return t;
+}
+
+// A wave's blocks of a part of few rows: every fourth of the sequence, `lead` of them with sinks.
+struct PaBlocks {
+  int sink, lead, run, count;
+  __device__ __forceinline__ int at(int i) const { return i < lead ? sink + 4 * i : run + 4 * (i - lead); }
+};
+__device__ __forceinline__ PaBlocks pa_wave_blocks(const PaSeq& s, const PaTile& t, int part, int wave) {
+  static_assert(kPaWaves == 4 && kPaLogNear >= 2 && kPaMinPart / kPaBlock >= 4, "a part's first block is wave 0's");
+  const int q = part < t.sink_parts ? part : part - t.sink_parts + t.first_part;
+  const int b0 = s.cut.start(q), b1 = s.cut.start(q + 1);
+  PaBlocks w;
+  w.sink = b0 + wave;
+  w.lead = max((min(b1, t.ns) - w.sink + 3) >> 2, 0);
+  const int from = max(b0, t.first);
+  w.run = from + ((wave - from) & 3);
+  w.count = w.lead + (t.nt > 0 ? max((min(b1, t.pmax / kPaBlock + 1) - w.run + 3) >> 2, 0) : 0);
+  return w;
 }
 
 // The slot of part 0 of row q0 + i, head h.
@@ -380,10 +458,10 @@ __device__ __forceinline__ void pa_wave_fence() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-// Where the blocks of a list are, for a wave: lane l has 16-key group l of the wave's next
-// 64 / GPB blocks (GPB groups each; block i of them is at place c0 + i STEP of the list), as
-// the byte offset of its first row from the pool's start. A group past the tile's last key
-// counts as that key's, one in no page of the pool as page 0's.
+// Where a wave's blocks are: lane l has 16-key group l of its next 64 / GPB blocks (GPB groups
+// each; block(i) is the number of the i-th), as the byte offset of its first row from the
+// pool's start. A group past the tile's last key counts as that key's, one in no page of the
+// pool as page 0's.
 struct PaPages {
   uint32_t lo, hi;
   uint64_t bad;  // groups in no page
@@ -393,12 +471,11 @@ struct PaPages {
     return (const char*)pool + o;
   }
 };
-template <typename T, int BLOCK, int STEP>
-__device__ __forceinline__ PaPages pa_pages(const PaArgs& a, const PaSeq& s, const PaTile& t, int c0, int64_t head) {
+template <typename T, int BLOCK, typename F>
+__device__ __forceinline__ PaPages pa_pages(const PaArgs& a, const PaSeq& s, const PaTile& t, int64_t head, F block) {
   constexpr int GPB = BLOCK / 16;
   const int lane = threadIdx.x & 63;
-  const int64_t c = (int64_t)c0 + (int64_t)(lane / GPB) * STEP;
-  const int blk = c < t.ns ? (int)c : (int)min(c - t.ns + t.first, (int64_t)(t.pmax / BLOCK));
+  const int blk = min(block(lane / GPB), t.pmax / BLOCK);
   const int key = min(blk * BLOCK + 16 * (lane % GPB), t.pmax & ~15);
   const uint32_t id = (uint32_t)a.m.table[(int64_t)s.b * a.m.ld + (key >> a.m.log2_rows)];
   const bool bad = id >= a.m.pages;
@@ -413,9 +490,21 @@ __device__ __forceinline__ PaPages pa_pages(const PaArgs& a, const PaSeq& s, con
 
 // The last row that may be read of a group of a block: those past the tile's last key are that key's.
 template <int BLOCK>
-__device__ __forceinline__ int pa_last_row(const PaTile& t, int c, int group) {
+__device__ __forceinline__ int pa_last_row(const PaTile& t, bool last_block, int group) {
   const int last = t.pmax % BLOCK - 16 * group;
-  return c < t.nt - 1 || last > 15 ? 15 : (last < 0 ? t.pmax & 15 : last);
+  return !last_block || last > 15 ? 15 : (last < 0 ? t.pmax & 15 : last);
+}
+
+// The transposed fragment of V from rows at a lane's place in a row-major block of LDS, rows VP elements apart.
+template <int VP>
+__device__ __forceinline__ u32x4 pa_vt_frag(const bf16_t* p) {
+  typedef short s16x4 __attribute__((ext_vector_type(4)));
+  typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+  typedef const __attribute__((address_space(3))) void* lds_ptr;
+  const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(lds_ptr)p);
+  const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(lds_ptr)(p + 4 * VP));
+  const uint2 x = __builtin_bit_cast(uint2, lo), y = __builtin_bit_cast(uint2, hi);
+  return u32x4{x.x, x.y, y.x, y.y};
 }
 
 // The workgroup's key streams, one per wave, merged: to the rows themselves, or as a
@@ -495,11 +584,8 @@ __device__ __forceinline__ void pa_keep(int nr, int wave, int col, int hf, const
   }
 }
 
-// A block's place in the tile's list to its first key.
-template <int BLOCK>
-__device__ __forceinline__ int pa_key(const PaTile& t, int c) {
-  return (c < t.ns ? c : c - t.ns + t.first) * BLOCK;
-}
+// The block at a place of a tile's list.
+__device__ __forceinline__ int pa_listed(const PaTile& t, int c) { return c < t.ns ? c : c - t.ns + t.first; }
 
 // bf16, few rows: bound by the keys and values, each read once per tile of 32 pairs (64 rows of
 // 4 heads x 4 over 32700 keys 742 us, 5.8 TB/s; 112 rows of 16 heads over 127 to 1199 keys 129
@@ -507,8 +593,7 @@ __device__ __forceinline__ int pa_key(const PaTile& t, int c) {
 // merge and, past kPaWhole keys, a second launch that merges the parts (8 rows over 512 to 777
 // keys 16.5 us, 19.4 when each had three parts).
 // Up to 32 pairs per workgroup, one per column of the 32x32x16 MFMA, and
-// four waves that each stream 32-key blocks (wave w blocks w, w + 4, ... of the part)
-// through LDS of their own: whole rows to registers a block ahead, to LDS as loaded,
+// four waves that each stream 32-key blocks (pa_wave_blocks) through LDS of their own: whole rows to registers a block ahead, to LDS as loaded,
 // no workgroup barrier before the merge. A wave computes S^T = K Q^T and O^T = V^T P^T;
 // the K rows of a block are taken in the order that makes a lane's S^T registers the 8
 // consecutive keys its P^T operand wants (result register r of lane half hf is key
@@ -553,16 +638,7 @@ __device__ __forceinline__ void pa_few_bf16(const PaArgs& a, PaFewLds<DH>& lds, 
   const int krow = 16 * (col >> 4) + 8 * ((col >> 2) & 1) + 4 * ((col >> 3) & 1) + (col & 3);
   const int tg = lane >> 4, ti = lane & 15;
   const int v_lane = ((tg >> 1) * 8 + (ti >> 2)) * VP + 16 * (tg & 1) + 4 * (ti & 3);
-  auto vt_frag = [&](int db, int s) {
-    typedef short s16x4 __attribute__((ext_vector_type(4)));
-    typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-    typedef const __attribute__((address_space(3))) void* lds_ptr;
-    const bf16_t* p = v_lds + v_lane + 16 * s * VP + 32 * db;
-    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(lds_ptr)p);
-    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(lds_ptr)(p + 4 * VP));
-    const uint2 x = __builtin_bit_cast(uint2, lo), y = __builtin_bit_cast(uint2, hi);
-    return u32x4{x.x, x.y, y.x, y.y};
-  };
+  auto vt_frag = [&](int db, int s) { return pa_vt_frag<VP>(v_lds + v_lane + 16 * s * VP + 32 * db); };
   const int g = blockIdx.x;
   const int64_t head = g * a.m.head_els;
 
@@ -574,18 +650,19 @@ __device__ __forceinline__ void pa_few_bf16(const PaArgs& a, PaFewLds<DH>& lds, 
     if (!pa_item<bf16_t, false>(a, u, s, t, part, first)) return;
     if (first && s.ne < s.nq) pa_rows_past<bf16_t, DH>(a, s, g);
     if (t.nr <= 0 || part >= t.parts) continue;
-    const int c0 = part * s.part, c1 = min(c0 + s.part, t.nt);
+    const PaBlocks mine = pa_wave_blocks(s, t, part, wave);
 
     u32x4 kreg[NLD], vreg[NLD];
     PaPages pages;
-    int ahead = 0, bad = 0;  // blocks of this wave fetched so far
-    auto fetch = [&](int c) {  // this wave's next block
-      const int i = ahead++ & 31;
-      if (i == 0) pages = pa_pages<bf16_t, TK, kPaWaves>(a, s, t, c, head);
+    int bad = 0;
+    auto fetch = [&](int c) {
+      const int i = c & 31;
+      if (i == 0) pages = pa_pages<bf16_t, TK>(a, s, t, head, [&](int x) { return mine.at(c + x); });
+      const bool end = mine.at(c) == t.pmax / TK;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const char *kb = pages.at(a.kp, 2 * i + h), *vb = pages.at(a.vp, 2 * i + h);
-        const int last = pa_last_row<TK>(t, c, h);
+        const int last = pa_last_row<TK>(t, end, h);
 #pragma unroll
         for (int e = 0; e < NLD / 2; ++e) {
           const uint32_t off = __umul24((uint32_t)min(RPI * e + lr, last), rsb) + (uint32_t)lp * 16u;
@@ -604,7 +681,7 @@ __device__ __forceinline__ void pa_few_bf16(const PaArgs& a, PaFewLds<DH>& lds, 
 #pragma unroll
       for (int k = 0; k < NDS; ++k) qf[k] = ld16(qp + 16 * k);
     }
-    if (c0 + wave < c1) fetch(c0 + wave);
+    if (mine.count > 0) fetch(0);
     pa_flip(qf, flip);
     float mref = -INFINITY, lrun = 0.f;
     f32x16 o[NDB];
@@ -613,9 +690,9 @@ __device__ __forceinline__ void pa_few_bf16(const PaArgs& a, PaFewLds<DH>& lds, 
 #pragma unroll
       for (int r = 0; r < 16; ++r) o[c][r] = 0.f;
 
-    for (int c = c0 + wave; c < c1; c += kPaWaves) {  // uniform over the wave
-      const int k0 = pa_key<TK>(t, c);
-      const bool all = c >= t.in0 && c < t.in1;
+    for (int c = 0; c < mine.count; ++c) {  // uniform over the wave
+      const int blk = mine.at(c), k0 = blk * TK;
+      const bool all = blk >= t.in0 && blk < t.in1;
       uint32_t odd = 0;  // keys whose V is not finite
       if (!all) {
 #pragma unroll
@@ -634,7 +711,7 @@ __device__ __forceinline__ void pa_few_bf16(const PaArgs& a, PaFewLds<DH>& lds, 
         *reinterpret_cast<u32x4*>(v_lds + (RPI * i + lr) * VP + 8 * lp) = vreg[i];
       }
       const int bad_now = bad;
-      if (c + kPaWaves < c1) fetch(c + kPaWaves);
+      if (c + 1 < mine.count) fetch(c + 1);
       pa_wave_fence();
       f32x16 sc[1];
 #pragma unroll
@@ -753,16 +830,17 @@ __device__ __forceinline__ void pa_f32_part(const PaArgs& a, const PaSeq& s, con
   const uint32_t k_lane = (uint32_t)(i16 * RB + 16 * (kg ^ i16));
   const uint32_t rsb = (uint32_t)a.m.row_els * sizeof(float);
   const int64_t head = g * a.m.head_els;
-  const int c0 = part * s.part, c1 = min(c0 + s.part, t.nt);
+  const PaBlocks mine = pa_wave_blocks(s, t, part, wave);
 
   PaPages pages;
-  int ahead = 0, next = 0, bad = 0;  // blocks of this wave found so far
-  int last[2];                       // the last row to read of either group
-  auto find = [&](int c) {           // this wave's next block
-    next = ahead++ & 31;
-    if (next == 0) pages = pa_pages<float, TK, kPaWaves>(a, s, t, c, head);
-    last[0] = pa_last_row<TK>(t, c, 0);
-    last[1] = pa_last_row<TK>(t, c, 1);
+  int next = 0, bad = 0;
+  int last[2];  // the last row to read of either group
+  auto find = [&](int c) {
+    next = c & 31;
+    if (next == 0) pages = pa_pages<float, TK>(a, s, t, head, [&](int x) { return mine.at(c + x); });
+    const bool end = mine.at(c) == t.pmax / TK;
+    last[0] = pa_last_row<TK>(t, end, 0);
+    last[1] = pa_last_row<TK>(t, end, 1);
     bad = (int)(pages.bad >> (2 * next) & 3);
   };
   auto fetch_k = [&]() {
@@ -784,8 +862,8 @@ __device__ __forceinline__ void pa_f32_part(const PaArgs& a, const PaSeq& s, con
 #pragma unroll
     for (int j = 0; j < NJ; ++j) qf[n][j] = ld16(qp + 16 * j);
   }
-  if (c0 + wave < c1) {
-    find(c0 + wave);
+  if (mine.count > 0) {
+    find(0);
     fetch_k();
   }
 #pragma unroll
@@ -802,7 +880,7 @@ __device__ __forceinline__ void pa_f32_part(const PaArgs& a, const PaSeq& s, con
       for (int e = 0; e < 4; ++e) o[n][q][e] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 
-  for (int c = c0 + wave; c < c1; c += kPaWaves) {  // uniform over the wave
+  for (int c = 0; c < mine.count; ++c) {  // uniform over the wave
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // K is there
     f32x4 v[8][NQ];
 #pragma unroll
@@ -839,8 +917,8 @@ __device__ __forceinline__ void pa_f32_part(const PaArgs& a, const PaSeq& s, con
             sc[n][h] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[j & 1][h][e], __uint_as_float(qf[n][j][e]), sc[n][h], 0,
                                                             0, 0);
     }
-    const int k0 = pa_key<TK>(t, c);
-    const bool all = c >= t.in0 && c < t.in1;
+    const int blk = mine.at(c), k0 = blk * TK;
+    const bool all = blk >= t.in0 && blk < t.in1;
     if (bad_now) {  // uniform
 #pragma unroll
       for (int n = 0; n < NT; ++n)
@@ -904,9 +982,9 @@ __device__ __forceinline__ void pa_f32_part(const PaArgs& a, const PaSeq& s, con
     for (int k = 0; k < 8; ++k)
 #pragma unroll
       for (int q = 0; q < NQ; ++q) asm volatile("" : "+v"(v[k][q]));
-    if (c + kPaWaves < c1) {  // uniform
+    if (c + 1 < mine.count) {  // uniform
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // this block's K is read
-      find(c + kPaWaves);
+      find(c + 1);
       fetch_k();
     }
 #pragma unroll
@@ -1032,16 +1110,7 @@ __device__ __forceinline__ void pa_many_bf16(const PaArgs& a, PaManyLds<DH>& lds
   const int krow = 16 * (col >> 4) + 8 * ((col >> 2) & 1) + 4 * ((col >> 3) & 1) + (col & 3);
   const int tg = lane >> 4, ti = lane & 15;
   const int v_lane = ((tg >> 1) * 8 + (ti >> 2)) * VP + 16 * (tg & 1) + 4 * (ti & 3);
-  auto vt_frag = [&](int b, int db, int k) {
-    typedef short s16x4 __attribute__((ext_vector_type(4)));
-    typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-    typedef const __attribute__((address_space(3))) void* lds_ptr;
-    const bf16_t* p = &v_lds[b][v_lane + 16 * k * VP + 32 * db];
-    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(lds_ptr)p);
-    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(lds_ptr)(p + 4 * VP));
-    const uint2 x = __builtin_bit_cast(uint2, lo), y = __builtin_bit_cast(uint2, hi);
-    return u32x4{x.x, x.y, y.x, y.y};
-  };
+  auto vt_frag = [&](int b, int db, int k) { return pa_vt_frag<VP>(&v_lds[b][v_lane + 16 * k * VP + 32 * db]); };
   const int g = blockIdx.x;
   const int64_t head = g * a.m.head_els;
 
@@ -1060,10 +1129,10 @@ __device__ __forceinline__ void pa_many_bf16(const PaArgs& a, PaManyLds<DH>& lds
     int bad = 0;
     auto fetch = [&](int c) {
       const int i16 = (c - c0) & 15;
-      if (i16 == 0) pages = pa_pages<bf16_t, TK, 1>(a, s, t, c, head);
+      if (i16 == 0) pages = pa_pages<bf16_t, TK>(a, s, t, head, [&](int x) { return pa_listed(t, c + x); });
 #pragma unroll
       for (int i = 0; i < NLD; ++i) {
-        const uint32_t off = __umul24((uint32_t)min(lr & 15, pa_last_row<TK>(t, c, group(i))), rsb) +
+        const uint32_t off = __umul24((uint32_t)min(lr & 15, pa_last_row<TK>(t, c == t.nt - 1, group(i))), rsb) +
                              (uint32_t)lp * 16u;
         kreg[i] = ld16(pages.at(a.kp, 4 * i16 + group(i)) + off);
         vreg[i] = ld16(pages.at(a.vp, 4 * i16 + group(i)) + off);
@@ -1118,7 +1187,7 @@ __device__ __forceinline__ void pa_many_bf16(const PaArgs& a, PaManyLds<DH>& lds
     auto block = [&](auto edge, int c) {
       constexpr bool EDGE = decltype(edge)::value;
       const int b = (c - c0) & 1;
-      [[maybe_unused]] const int k0 = pa_key<TK>(t, c);
+      [[maybe_unused]] const int k0 = pa_listed(t, c) * TK;
       // some row of the wave sees some key (uniform over the wave)
       bool any = live;
       if constexpr (EDGE)
@@ -1249,16 +1318,28 @@ __global__ __launch_bounds__(64 * kPaWaves) __attribute__((amdgpu_waves_per_eu(2
     pa_few_bf16<DH>(a, lds.few, merge, y - a.many_lead, few);
 }
 
-// The parts of the rows that have several. Up to kPaWide parts a (row, head) is merged by
-// DH / 4 threads of four columns, one fma per part in their order on the largest maximum;
-// more by a workgroup (attn_merge_parts). Bound by the parts' bytes: 2170 rows of 16 heads,
-// up to 5 parts of those of prompts, 27 us; 8 rows of 3 parts 4 us, the launch and its search.
+// The parts of the rows that have several, merged. A row that has keys in up to kPaWide of them
+// takes DH / 4 threads of four columns, one fma per part in the parts' order on the largest
+// maximum; a row of more a workgroup, whose slot x takes the parts of the sequence that are x
+// modulo its slots, in their order, before the slots are merged in theirs. A part without a key
+// that the row sees (its maximum is -inf) changes nothing in either, so a row's bits do not
+// depend on the parts that its tile has beside its own. Bound by the parts' bytes.
 constexpr int kPaWide = 16;
+constexpr int kPaMergeThreads = 256;
+
+// Parts in which the row at position pos sees a key.
+__device__ __forceinline__ int pa_own_parts(const PaArgs& a, const PaSeq& s, int pos) {
+  const int lo = a.window ? max(pos - a.window + 1, 0) : 0, ns = (min(a.sinks, lo) + kPaBlock - 1) >> kPaLogBlock;
+  const int sink_parts = ns ? s.cut.of(ns - 1) + 1 : 0;
+  return sink_parts + max(s.cut.of(pos >> kPaLogBlock) - max(s.cut.of(lo >> kPaLogBlock), sink_parts) + 1, 0);
+}
 
 template <typename T, int DH>
-__global__ __launch_bounds__(kMergeThreads) void attn_paged_combine(PaArgs a) {
-  constexpr int TPP = DH / 4, PP = kMergeThreads / TPP, B = 4;
-  const int H = a.H;
+__global__ __launch_bounds__(kPaMergeThreads) void attn_paged_combine(PaArgs a) {
+  constexpr int TPP = DH / 4, PP = kPaMergeThreads / TPP, B = 4;
+  __shared__ __align__(16) float o_lds[PP][DH];
+  __shared__ float m_lds[PP], l_lds[PP];
+  const int H = a.H, d = 4 * (threadIdx.x % TPP), slot = threadIdx.x / TPP;
   auto units = [&](const PaSeq& q) {
     return q.parts <= 1 ? 0 : (q.parts > kPaWide ? q.ne * H : (q.ne * H + PP - 1) / PP);
   };
@@ -1266,46 +1347,96 @@ __global__ __launch_bounds__(kMergeThreads) void attn_paged_combine(PaArgs a) {
     PaSeq s;
     int pair;
     if (!pa_find<T>(a, u, units, s, pair)) return;
-    const bool wide = s.parts > kPaWide;
-    if (!wide) pair = pair * PP + threadIdx.x / TPP;
+    const bool one = s.parts > kPaWide;  // pair of the workgroup
+    if (!one) pair = pair * PP + slot;
     if (pair >= s.ne * H) continue;  // no barrier ahead unless the unit is one pair
     const int i = pair / H, h = pair - i * H, pos = s.pos0 + i;
-    const int np = s.many ? pa_tile<true>(a, s, i / a.many_tile).parts : pa_tile<false>(a, s, i / a.few_tile).parts;
+    int np, sink_parts = 0, first_part = 0, own;
+    if (s.many) {
+      own = np = pa_tile<true>(a, s, i / a.many_tile).parts;
+    } else {
+      const PaTile t = pa_tile<false>(a, s, i / a.few_tile);
+      np = t.parts;
+      sink_parts = t.sink_parts;
+      first_part = t.first_part;
+      own = pa_own_parts(a, s, min(max(pos, 0), a.kmax - 1));
+    }
     if (np <= 1) continue;  // finished by its workgroup
     const int64_t base = pa_slot(a, s, i, h);
     T* row = (T*)a.out + ((int64_t)(s.q0 + i) * H + h) * DH;
-    if (wide) {
-      if (pos < 0 || pos >= a.kmax) {
-        if (threadIdx.x < DH) Elem<T>::store(row + threadIdx.x, pos < 0 ? 0.f : NAN);
-        continue;
-      }
-      attn_merge_parts<T, DH, true>(a.po, a.pml, np, [&](int p) { return base + p; }, row);
-      __syncthreads();  // its LDS, before the next row's
-      continue;
-    }
-    const int d = 4 * (threadIdx.x % TPP);
     const float2* ml = reinterpret_cast<const float2*>(a.pml) + base;
     const float* po = a.po + base * DH + d;
     float M = -INFINITY, L = 0.f;
     f32x4 O = {0.f, 0.f, 0.f, 0.f};
-    for (int p = 0; p < np; ++p) M = fmaxf(M, ml[p].x);
-    for (int p0 = 0; p0 < np; p0 += B) {
-      float2 w[B];
-      f32x4 v[B];
+    if (one && own > kPaWide) {  // uniform
+      const int lead = max((sink_parts - slot + PP - 1) / PP, 0);
+      const int run = sink_parts + ((slot - first_part) & (PP - 1));
+      const int count = lead + max((np - run + PP - 1) / PP, 0);
+      auto place = [&](int e) { return e < lead ? slot + PP * e : run + PP * (e - lead); };
+      for (int e0 = 0; e0 < count; e0 += B) {
+        float2 w[B];
+        f32x4 v[B];
 #pragma unroll
-      for (int b = 0; b < B; ++b) {
-        w[b] = ml[min(p0 + b, np - 1)];
-        v[b] = *reinterpret_cast<const f32x4*>(po + (int64_t)min(p0 + b, np - 1) * DH);
-      }
-#pragma unroll
-      for (int b = 0; b < B; ++b)
-        if (p0 + b < np) {
-          const float f = w[b].x == -INFINITY ? 0.f : exp2f(w[b].x - M);
-          L = fmaf(w[b].y, f, L);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) O[e] = fmaf(v[b][e], f, O[e]);
+        for (int b = 0; b < B; ++b) {
+          const int p = place(min(e0 + b, count - 1));
+          w[b] = ml[p];
+          v[b] = *reinterpret_cast<const f32x4*>(po + (int64_t)p * DH);
         }
+#pragma unroll
+        for (int b = 0; b < B; ++b)
+          if (e0 + b < count) {
+            const float mn = fmaxf(M, w[b].x);
+            const float corr = M == -INFINITY ? 1.f : exp2f(M - mn);  // nothing but zeros (or a NaN to keep) so far
+            const float f = w[b].x == -INFINITY ? 0.f : exp2f(w[b].x - mn);
+            M = mn;
+            L = fmaf(w[b].y, f, L * corr);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) O[e] = fmaf(v[b][e], f, O[e] * corr);
+          }
+      }
+      *reinterpret_cast<f32x4*>(&o_lds[slot][d]) = O;
+      if (d == 0) {
+        m_lds[slot] = M;
+        l_lds[slot] = L;
+      }
+      __syncthreads();
+      if (threadIdx.x < TPP) {
+        M = -INFINITY;
+        L = 0.f;
+        O = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int x = 0; x < PP; ++x) M = fmaxf(M, m_lds[x]);
+#pragma unroll
+        for (int x = 0; x < PP; ++x) {
+          const float f = m_lds[x] == -INFINITY ? 0.f : exp2f(m_lds[x] - M);
+          L = fmaf(l_lds[x], f, L);
+          const f32x4 v = *reinterpret_cast<const f32x4*>(&o_lds[x][d]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) O[e] = fmaf(v[e], f, O[e]);
+        }
+      }
+      __syncthreads();  // before the next row's
+    } else if (!one || slot == 0) {
+      for (int p = 0; p < np; ++p) M = fmaxf(M, ml[p].x);
+      for (int p0 = 0; p0 < np; p0 += B) {
+        float2 w[B];
+        f32x4 v[B];
+#pragma unroll
+        for (int b = 0; b < B; ++b) {
+          w[b] = ml[min(p0 + b, np - 1)];
+          v[b] = *reinterpret_cast<const f32x4*>(po + (int64_t)min(p0 + b, np - 1) * DH);
+        }
+#pragma unroll
+        for (int b = 0; b < B; ++b)
+          if (p0 + b < np) {
+            const float f = w[b].x == -INFINITY ? 0.f : exp2f(w[b].x - M);
+            L = fmaf(w[b].y, f, L);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) O[e] = fmaf(v[b][e], f, O[e]);
+          }
+      }
     }
+    if (one && slot) continue;
 #pragma unroll
     for (int e = 0; e < 4; ++e) O[e] = pa_finish(a, pos, O[e], L);
     if constexpr (sizeof(T) == 2)
@@ -1322,14 +1453,18 @@ struct PaPlan {
   int64_t few_slots, many_pairs, many_slots, few_units, many_units;
 };
 
-// The most parts of a tile: of a sequence with more tiles they are fewer.
-static int pa_most_parts(bool many, int blocks, int Hkv) {
-  const int least = many ? kPaManyMinPart / kPaManyBlock : kPaMinPart / kPaBlock;
-  const int target = many ? kPaManyTarget : kPaTarget;
-  int p = pa_div_up(target, Hkv);  // unless a part is at its least or largest
-  if (pa_div_up(blocks, least) < p) p = pa_div_up(blocks, least);
-  if (!many && pa_div_up(blocks, kPaMaxPart / kPaBlock) > p) p = pa_div_up(blocks, kPaMaxPart / kPaBlock);
-  return p > 1 ? p : 1;
+// The most parts of a tile of many rows: of a sequence with more tiles they are fewer.
+static int pa_most_many(int blocks, int Hkv) {
+  const int p = pa_div_up(kPaManyTarget, Hkv), all = pa_div_up(blocks, kPaManyMinPart / kPaManyBlock);
+  return p < all ? p : (all > 1 ? all : 1);
+}
+
+// The same in a sequence of fp32 rows that are not few: it has more than two tiles.
+static int pa_most_f32(int kmax, int Hkv, int rows, int window, int sinks) {
+  const int wide = 3 * Hkv;
+  if (wide >= kPaTarget) return 1;
+  const int p = pa_most_parts(PaCut{0, 3}, kmax, rows, window, sinks), most = kPaTarget / wide + 4;
+  return p < most ? p : most;
 }
 
 static PaPlan pa_plan(int n, int nseq, int H, int Hkv, int dtype, int qmax, int kmax, int window, int sinks) {
@@ -1343,13 +1478,16 @@ static PaPlan pa_plan(int n, int nseq, int H, int Hkv, int dtype, int qmax, int 
   // the few-row kernel's rows of a sequence
   const int most = bf16 && qmax > kPaFewPairs / G ? kPaFewPairs / G : qmax;
   const int64_t rows = (int64_t)nseq * most < n ? (int64_t)nseq * most : n;
-  const int blocks = pa_blocks(kmax, p.few_tile, window, sinks, kPaLogBlock);
-  p.few_per = bf16 && blocks <= kPaWhole / kPaBlock ? 1 : pa_most_parts(false, blocks, Hkv);
+  p.few_per = pa_most_parts(pa_few_cut(Hkv, window), kmax, p.few_tile, window, sinks);
+  if (!bf16 && (int64_t)qmax * G > kPaFewPairs) {
+    const int f = pa_most_f32(kmax, Hkv, p.few_tile, window, sinks);
+    if (f > p.few_per) p.few_per = f;
+  }
   p.few_rows = rows < n ? most : 0;
   p.few_slots = p.few_per > 1 ? rows * H * p.few_per : 0;
   p.few_units = (rows / p.few_tile + nseq) * p.few_per;
   if (p.many) {
-    p.many_per = pa_most_parts(true, pa_blocks(kmax, p.many_tile, window, sinks, kPaManyLogBlock), Hkv);
+    p.many_per = pa_most_many(pa_blocks(kmax, p.many_tile, window, sinks, kPaManyLogBlock), Hkv);
     // of one sequence: where a tile has several parts, tiles Hkv parts < 2 target
     const int64_t one = (int64_t)2 * kPaManyTarget * kPaManyRows;
     const int64_t by_seq = (int64_t)nseq * one, by_row = (int64_t)n * H * p.many_per;
@@ -1382,7 +1520,7 @@ static void launch_paged(PaArgs a, const PaPlan& p, hipStream_t st) {
   if (hipPeekAtLastError() != hipSuccess) return;  // no parts to merge
   if (p.few_per > 1 || p.many_per > 1)
     hipLaunchKernelGGL((attn_paged_combine<T, DH>), dim3(pa_grid((int64_t)a.n * a.H, kPaMergeGrid)),
-                       dim3(kMergeThreads), 0, st, a);
+                       dim3(kPaMergeThreads), 0, st, a);
 }
 
 }  // namespace wfd
@@ -1472,6 +1610,7 @@ int wfd_attn_paged(const void* q, const void* k_pages, const void* v_pages, int6
   a.pml = (float*)((char*)workspace + align256(slots * Dh * sizeof(float)));
   a.many_at = p.few_slots;
   a.g_magic = 65536 / a.G + 1;
+  a.cut = pa_few_cut(Hkv, a.window);
   a.few_tile = p.few_tile;
   a.many_tile = p.many_tile;
   a.few_per = p.few_per;
