@@ -360,7 +360,10 @@ int wfd_kv_append_paged(const void* k, int64_t ldk, const void* v, int64_t ldv, 
  * and is zero. q_len_max >= every sequence's rows and kv_len_max >= every kv_len
  * size the grid; a row past its sequence's first q_len_max, or at a position of
  * kv_len_max or beyond, is NaN. kv_len_max <= pages_per_seq * page_rows. H / Hkv up to
- * 32, any scale. workspace >= wfd_attn_paged_workspace_bytes(...), 16-byte aligned.
+ * 32, any scale. workspace >= wfd_attn_paged_workspace_bytes(...), 16-byte aligned:
+ * what the bounds allow (rows x H x parts of 512 keys and more, Dh + 2 floats each),
+ * gigabytes for thousands of rows of many sequences with a kv_len_max of tens of
+ * thousands; tight bounds and fewer sequences a call, which change no bits, need less.
  * fp32 statistics, sums and division; probabilities meet V with 16 significant bits
  * (fp32: 24), in sequences of more than 64 rows x H / Hkv with 8, where their
  * products bound the call. In sequences of up to 64 rows x H / Hkv a row's bits

@@ -37,3 +37,20 @@ def test_a_draft_has_the_bits_of_single_tokens(gpu, dtype, window, sinks, heads,
                          sinks=sinks)
     same = (drafts == one).flatten(1).all(-1).tolist()
     assert all(same), [(seqs[b], p) for (b, p), ok in zip(rows, same) if not ok][:5]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("H,Hkv,Dh", [(16, 16, 64), (16, 4, 64), (8, 1, 64), (32, 1, 128), (6, 6, 128)])
+def test_parts_stay_in_the_workspace(gpu, dtype, H, Hkv, Dh):
+    """Calls of few and many rows with a workspace of just the named size, between bytes that stay as they are: the bits
+    of the same calls with one of their own."""
+    for seed, seqs in enumerate(([(300, 4000)], [(1, 9000), (3, 700)], [(70, 3000), (1, 1200), (9, 2500), (200, 200)],
+                                 [(1, 600 + 40 * i) for i in range(20)] + [(33, 2100)], [(65, 8000)] * 3)):
+        c = Pages(gpu, dtype, H, Hkv, Dh, seqs, page=64, seed=seed)
+        for window, sinks in ((0, 0), (700, 40)):
+            need = ops.attn_paged_workspace_bytes(c.n, len(seqs), H, Hkv, Dh, dtype, c.q_len_max, c.kv_len_max, window,
+                                                  sinks)
+            ws = torch.full((need + 8192,), 0x5a, dtype=torch.uint8, device=gpu)
+            got = c.attn(window=window, sinks=sinks, workspace=ws[4096: 4096 + need])
+            assert (ws[:4096] == 0x5a).all() and (ws[4096 + need:] == 0x5a).all(), (seqs[:3], window)
+            assert torch.equal(got, c.attn(window=window, sinks=sinks))

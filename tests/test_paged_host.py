@@ -158,3 +158,23 @@ def test_appends_refuse_rows_beyond_the_grid():
         assert lib.wfd_qkv_rope_append_paged(16, 192, 16, 16, 1, 16, 4, 4, 9, 16, 16, 16, 8, 16, 16, 16, 0, n, 1, 1,
                                              64, 1, None) == rc
         assert b"beyond the grid" in lib.wfd_last_error()
+
+
+def test_workspace_of_parts_that_can_exist():
+    """A slot of a part is Dh + 2 numbers. fp32 sequences of many rows are cut into few parts or none, and a row is of a
+    sequence of few rows or of one of many, never of both."""
+    f32, bf16 = torch.float32, torch.bfloat16
+    slot = lambda Dh: (Dh + 2) * 4  # noqa: E731
+    need = ops.attn_paged_workspace_bytes
+    # one sequence, every tile of it in one part or in few
+    assert need(16384, 1, 32, 1, 128, f32, 16384, 16384) <= 10240 * slot(128) + 512
+    assert need(4096, 1, 16, 4, 128, f32, 4096, 8192) <= 10240 * slot(128) + 512
+    assert need(4096, 1, 16, 4, 128, bf16, 4096, 8192) <= 131072 * slot(128) + 512
+    assert need(2000, 1, 64, 64, 64, f32, 2000, 2000, 100, 4) <= 64 * 64 * 5 * slot(64) + 512
+    # ragged ticks: per row and head, parts of 512 keys at most
+    for H, Hkv in ((16, 16), (16, 4), (32, 8)):
+        for rows, seqs, q in ((8192, 256, 512), (8192, 256, 2048), (4096, 64, 300)):
+            for dt in (f32, bf16):
+                assert need(rows, seqs, H, Hkv, 128, dt, q, 32768) <= rows * H * 64 * slot(128) + 512
+    # single tokens under a window: its parts, one more for where it begins, and the sinks'
+    assert need(64, 64, 16, 4, 128, bf16, 1, 32768, 4096, 4) <= 64 * 16 * 11 * slot(128) + 512

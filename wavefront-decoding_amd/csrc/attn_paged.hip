@@ -17,6 +17,7 @@
 // it and nothing else, and a hidden key changes no bit: a row has the bits it has alone,
 // as the next token of its context. A sequence of more rows is cut by its own rows and
 // length. In either case the rest of the call has no part in it.
+#include <algorithm>
 #include <type_traits>
 
 #include "attn_combine.h"
@@ -86,15 +87,13 @@ struct PaArgs {
   const int32_t *cu_q, *kv_len;
   void* out;
   PageMap m;
-  float *po, *pml;       // few rows' parts, then many rows'
-  int64_t many_at;       // the first of these
+  float *po, *pml;       // the parts' slots
+  int64_t seq_slots;     // slots kept per sequence; 0: row_per for every row and head
   int n, nseq, H, Hkv, G, qmax, kmax, window, sinks;
   int g_magic;           // x / G = x g_magic >> 16 for x < 128
   int few_tile, many_tile;  // rows of a tile
-  int few_per, many_per; // part slots per row and head
+  int row_per;
   uint32_t many_wgs, many_lead;  // of a kv head
-  int few_rows;          // rows kept per sequence, 0: by the row's number
-  int many_pairs;        // slots kept per sequence, 0: by the row's number
   PaCut cut;             // of few rows
   float scale_log2;
 };
@@ -244,12 +243,8 @@ __device__ __forceinline__ PaBlocks pa_wave_blocks(const PaSeq& s, const PaTile&
 
 // The slot of part 0 of row q0 + i, head h.
 __device__ __forceinline__ int64_t pa_slot(const PaArgs& a, const PaSeq& s, int i, int h) {
-  if (s.many) {
-    if (a.many_pairs) return a.many_at + (int64_t)s.b * a.many_pairs + ((int64_t)i * a.H + h) * s.parts;
-    return a.many_at + ((int64_t)(s.q0 + i) * a.H + h) * a.many_per;
-  }
-  const int64_t row = a.few_rows ? (int64_t)s.b * a.few_rows + i : s.q0 + i;
-  return (row * a.H + h) * a.few_per;
+  if (a.seq_slots) return s.b * a.seq_slots + ((int64_t)i * a.H + h) * s.parts;
+  return ((int64_t)(s.q0 + i) * a.H + h) * a.row_per;
 }
 
 // The sequence of unit u among the sequences' units(s), and the unit within it; false
@@ -1446,12 +1441,18 @@ __global__ __launch_bounds__(kPaMergeThreads) void attn_paged_combine(PaArgs a) 
   }
 }
 
-// How a launch is cut at most: what the host knows are bounds.
+// How a launch is cut at most: what the host knows are bounds. Slots are kept per row for the
+// most parts that any row has, or per sequence for what one has at most, whichever takes less.
 struct PaPlan {
   bool many;
-  int few_tile, many_tile, few_per, many_per, few_rows;
-  int64_t few_slots, many_pairs, many_slots, few_units, many_units;
+  int few_tile, many_tile, row_per;
+  int64_t seq_slots, slots, few_units, many_units;
 };
+// Slots of one sequence that is not of few rows, where its tiles have several parts: pairs of a
+// tile x tiles x kv heads x parts. Many rows: parts < target / (tiles Hkv) + 1, of which tiles Hkv
+// is below the target. fp32: parts < target / (tiles Hkv) + 4, with a window's and its sinks' ends.
+constexpr int64_t kPaManySlots = 2 * kPaManyTarget * kPaManyRows;
+constexpr int64_t kPaF32Slots = 5 * kPaTarget * kPaRows;
 
 // The most parts of a tile of many rows: of a sequence with more tiles they are fewer.
 static int pa_most_many(int blocks, int Hkv) {
@@ -1471,30 +1472,26 @@ static PaPlan pa_plan(int n, int nseq, int H, int Hkv, int dtype, int qmax, int 
   PaPlan p{};
   const int G = H / Hkv;
   if (qmax > n) qmax = n;
-  const bool bf16 = dtype == kBF16;
-  p.many = bf16 && (int64_t)qmax * G > kPaFewPairs;
+  const bool large = (int64_t)qmax * G > kPaFewPairs;
+  p.many = dtype == kBF16 && large;
   p.few_tile = kPaRows / G;
   p.many_tile = kPaManyRows / G;
-  // the few-row kernel's rows of a sequence
-  const int most = bf16 && qmax > kPaFewPairs / G ? kPaFewPairs / G : qmax;
-  const int64_t rows = (int64_t)nseq * most < n ? (int64_t)nseq * most : n;
-  p.few_per = pa_most_parts(pa_few_cut(Hkv, window), kmax, p.few_tile, window, sinks);
-  if (!bf16 && (int64_t)qmax * G > kPaFewPairs) {
-    const int f = pa_most_f32(kmax, Hkv, p.few_tile, window, sinks);
-    if (f > p.few_per) p.few_per = f;
+  const int few_rows = large ? kPaFewPairs / G : qmax;  // of a sequence
+  const int few = pa_most_parts(pa_few_cut(Hkv, window), kmax, p.few_tile, window, sinks);
+  int most = 1;  // of a tile of the other sequences
+  if (p.many) most = pa_most_many(pa_blocks(kmax, p.many_tile, window, sinks, kPaManyLogBlock), Hkv);
+  else if (large) most = pa_most_f32(kmax, Hkv, p.few_tile, window, sinks);
+  p.row_per = few > most ? few : most;
+  if (p.row_per > 1) {
+    int64_t one = few > 1 ? (int64_t)few_rows * H * few : 0;
+    if (most > 1) one = std::max(one, p.many ? kPaManySlots : kPaF32Slots);
+    const int64_t by_row = (int64_t)n * H * p.row_per;
+    p.seq_slots = nseq * one < by_row ? one : 0;
+    p.slots = p.seq_slots ? nseq * one : by_row;
   }
-  p.few_rows = rows < n ? most : 0;
-  p.few_slots = p.few_per > 1 ? rows * H * p.few_per : 0;
-  p.few_units = (rows / p.few_tile + nseq) * p.few_per;
-  if (p.many) {
-    p.many_per = pa_most_many(pa_blocks(kmax, p.many_tile, window, sinks, kPaManyLogBlock), Hkv);
-    // of one sequence: where a tile has several parts, tiles Hkv parts < 2 target
-    const int64_t one = (int64_t)2 * kPaManyTarget * kPaManyRows;
-    const int64_t by_seq = (int64_t)nseq * one, by_row = (int64_t)n * H * p.many_per;
-    p.many_pairs = by_seq < by_row ? one : 0;
-    p.many_slots = p.many_per > 1 ? (by_seq < by_row ? by_seq : by_row) : 0;
-    p.many_units = ((int64_t)n / p.many_tile + nseq) * p.many_per;
-  }
+  const int64_t rows = std::min((int64_t)nseq * (p.many ? few_rows : qmax), (int64_t)n);
+  p.few_units = (rows / p.few_tile + nseq) * (p.many ? few : p.row_per);
+  if (p.many) p.many_units = ((int64_t)n / p.many_tile + nseq) * most;
   return p;
 }
 
@@ -1518,7 +1515,7 @@ static void launch_paged(PaArgs a, const PaPlan& p, hipStream_t st) {
     hipLaunchKernelGGL((attn_paged_few_bf16<DH>), dim3(a.Hkv, few), block, 0, st, a);
   }
   if (hipPeekAtLastError() != hipSuccess) return;  // no parts to merge
-  if (p.few_per > 1 || p.many_per > 1)
+  if (p.row_per > 1)
     hipLaunchKernelGGL((attn_paged_combine<T, DH>), dim3(pa_grid((int64_t)a.n * a.H, kPaMergeGrid)),
                        dim3(kPaMergeThreads), 0, st, a);
 }
@@ -1537,7 +1534,7 @@ size_t wfd_attn_paged_workspace_bytes(int n, int nseq, int H, int Hkv, int Dh, i
   if (window >= kv_len_max) window = 0;
   if (sinks > kv_len_max) sinks = kv_len_max;
   const PaPlan p = pa_plan(n, nseq, H, Hkv, dtype, q_len_max, kv_len_max, window, sinks);
-  const size_t slots = (size_t)(p.few_slots + p.many_slots);
+  const size_t slots = (size_t)p.slots;
   return slots ? align256(slots * Dh * sizeof(float)) + align256(slots * 2 * sizeof(float)) : 0;
 }
 
@@ -1605,18 +1602,14 @@ int wfd_attn_paged(const void* q, const void* k_pages, const void* v_pages, int6
     set_error("%s: n=%d nseq=%d kv_len_max=%d beyond the grid", me, n, nseq, kv_len_max);
     return kUnsupported;
   }
-  const size_t slots = (size_t)(p.few_slots + p.many_slots);
   a.po = (float*)workspace;
-  a.pml = (float*)((char*)workspace + align256(slots * Dh * sizeof(float)));
-  a.many_at = p.few_slots;
+  a.pml = (float*)((char*)workspace + align256((size_t)p.slots * Dh * sizeof(float)));
+  a.seq_slots = p.seq_slots;
   a.g_magic = 65536 / a.G + 1;
   a.cut = pa_few_cut(Hkv, a.window);
   a.few_tile = p.few_tile;
   a.many_tile = p.many_tile;
-  a.few_per = p.few_per;
-  a.many_per = p.many_per;
-  a.few_rows = p.few_rows;
-  a.many_pairs = (int)p.many_pairs;
+  a.row_per = p.row_per;
   if (dtype == kBF16)
     Dh == 64 ? launch_paged<bf16_t, 64>(a, p, stream) : launch_paged<bf16_t, 128>(a, p, stream);
   else
