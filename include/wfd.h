@@ -364,15 +364,16 @@ int wfd_kv_append_paged(const void* k, int64_t ldk, const void* v, int64_t ldv, 
  * what the bounds allow (rows x H x parts of 512 keys and more, Dh + 2 floats each),
  * gigabytes for thousands of rows of many sequences with a kv_len_max of tens of
  * thousands; tight bounds and fewer sequences a call, which change no bits, need less.
- * fp32 statistics, sums and division; probabilities meet V with 16 significant bits
- * (fp32: 24), in sequences of more than 64 rows x H / Hkv with 8, where their
- * products bound the call. In sequences of up to 64 rows x H / Hkv a row's bits
- * depend on its query, its position, the keys it attends, the head counts, window and
- * sinks alone: the rows of a draft have the bits of the single tokens that they verify
- * (but for an infinity in V under a probability below 2^-126, which makes infinity or
- * NaN). In longer ones they depend on the sequence's row count and length too; never on
- * the other sequences of the call or on where the pages are. Infinities and NaN in K
- * and V reach only the rows that attend them.
+ * fp32 statistics, sums and division; bf16 probabilities meet V within 2^-15 of
+ * themselves, in sequences of more than 64 rows x H / Hkv rounded to 8 bits (2^-8),
+ * where their products bound the call; fp32 ones as they are. In sequences of up to
+ * 64 rows x H / Hkv a row's bits depend on its query, its position, the keys it
+ * attends, the head counts, window and sinks alone: the rows of a draft have the bits
+ * of the single tokens that they verify (but for an infinity in V under a probability
+ * below 2^-126, which makes infinity or NaN). In longer ones they depend on the
+ * sequence's row count and length too; never on the other sequences of the call or on
+ * where the pages are. Infinities and NaN in K and V reach only the rows that attend
+ * them.
  * Replaces: attn_varlen over gathered prefixes (src/decoding/fa4_attention.py:301-366,
  *   src/decoding/batch_kv_cache.py:75-96) for a cache in pages; the reference has no
  *   window.

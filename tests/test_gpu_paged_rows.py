@@ -54,3 +54,24 @@ def test_parts_stay_in_the_workspace(gpu, dtype, H, Hkv, Dh):
             got = c.attn(window=window, sinks=sinks, workspace=ws[4096: 4096 + need])
             assert (ws[:4096] == 0x5a).all() and (ws[4096 + need:] == 0x5a).all(), (seqs[:3], window)
             assert torch.equal(got, c.attn(window=window, sinks=sinks))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("window,sinks", [(0, 0), (90, 3)])
+def test_hundreds_of_sequences(gpu, dtype, window, sinks):
+    """The search for a row's sequence takes 64 sequences a step: rows of few and of many, empty sequences and ones
+    without new rows spread over several steps, parts among them."""
+    seqs = [((0, 1, 1, 3, 0, 1)[i % 6], 5 + (37 * i) % 400) for i in range(230)]
+    for i, seq in ((3, (90, 400)), (62, (1, 1500)), (63, (70, 90)), (64, (1, 2000)), (128, (100, 1800)), (140, (0, 0)),
+                   (191, (20, 700)), (192, (1, 1)), (228, (120, 600)), (229, (2, 3000))):
+        seqs[i] = seq
+    c = Pages(gpu, dtype, 2, 1, 64, seqs, page=32, seed=2, lead=2, tail=3)
+    out = torch.full_like(c.q, 7.0)
+    c.attn(out=out, window=window, sinks=sinks)
+    c.check(out, window=window, sinks=sinks, p_step=2.0 ** -8 if dtype == torch.bfloat16 else 0.0)
+    assert (out[:2] == 7.0).all() and (out[c.cu[-1]:] == 7.0).all()
+    for b in (62, 63, 64, 127, 128, 191, 192, 229):
+        m, L = seqs[b]
+        one = ops.attn_paged(c.q[c.cu[b]: c.cu[b + 1]].clone(), c.k, c.v, c.table[b: b + 1], c.ints([0, m]), c.ints([L]),
+                             q_len_max=max(m, 1), kv_len_max=L, window=window, sinks=sinks)
+        assert torch.equal(one, out[c.cu[b]: c.cu[b + 1]]), b
