@@ -40,6 +40,16 @@ def test_a_draft_has_the_bits_of_single_tokens(gpu, dtype, window, sinks, heads,
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+def test_bounds_change_no_bits(gpu, dtype):
+    """kv_len_max decides whether a window covers every key, and the workspace: neither shows in a row."""
+    c = Pages(gpu, dtype, 32, 32, 64, [(1, 2500), (2, 1400), (1, 40), (1, 2900)], page=64, table_pad=100)
+    for window, sinks in ((0, 0), (3000, 0), (2900, 5), (1500, 9)):
+        ref = c.attn(window=window, sinks=sinks)
+        for most in (2901, 3000, 3001, 9000):
+            assert torch.equal(ref, c.attn(window=window, sinks=sinks, kv_len_max=most)), (window, most)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("H,Hkv,Dh", [(16, 16, 64), (16, 4, 64), (8, 1, 64), (32, 1, 128), (6, 6, 128)])
 def test_parts_stay_in_the_workspace(gpu, dtype, H, Hkv, Dh):
     """Calls of few and many rows with a workspace of just the named size, between bytes that stay as they are: the bits

@@ -78,6 +78,7 @@ struct PaCut {
   }
 };
 
+// window: the caller's, also where it covers all keys, so that kv_len_max does not decide on bits.
 inline PaCut pa_few_cut(int Hkv, int window) {
   return window ? PaCut{0, kPaLogNear} : PaCut{(kPaNear + Hkv - 1) / Hkv, kPaLogFar};
 }
@@ -1468,7 +1469,8 @@ static int pa_most_f32(int kmax, int Hkv, int rows, int window, int sinks) {
   return p < most ? p : most;
 }
 
-static PaPlan pa_plan(int n, int nseq, int H, int Hkv, int dtype, int qmax, int kmax, int window, int sinks) {
+static PaPlan pa_plan(int n, int nseq, int H, int Hkv, int dtype, int qmax, int kmax, PaCut cut, int window,
+                      int sinks) {
   PaPlan p{};
   const int G = H / Hkv;
   if (qmax > n) qmax = n;
@@ -1477,7 +1479,7 @@ static PaPlan pa_plan(int n, int nseq, int H, int Hkv, int dtype, int qmax, int 
   p.few_tile = kPaRows / G;
   p.many_tile = kPaManyRows / G;
   const int few_rows = large ? kPaFewPairs / G : qmax;  // of a sequence
-  const int few = pa_most_parts(pa_few_cut(Hkv, window), kmax, p.few_tile, window, sinks);
+  const int few = pa_most_parts(cut, kmax, p.few_tile, window, sinks);
   int most = 1;  // of a tile of the other sequences
   if (p.many) most = pa_most_many(pa_blocks(kmax, p.many_tile, window, sinks, kPaManyLogBlock), Hkv);
   else if (large) most = pa_most_f32(kmax, Hkv, p.few_tile, window, sinks);
@@ -1531,9 +1533,10 @@ size_t wfd_attn_paged_workspace_bytes(int n, int nseq, int H, int Hkv, int Dh, i
   if (n <= 0 || nseq <= 0 || H <= 0 || H > 4096 || Hkv <= 0 || H % Hkv || H / Hkv > kPaMaxG || Dh <= 0 || Dh > 128 ||
       q_len_max < 0 || kv_len_max <= 0 || window < 0 || sinks < 0)
     return 0;
+  const PaCut cut = pa_few_cut(Hkv, window);
   if (window >= kv_len_max) window = 0;
   if (sinks > kv_len_max) sinks = kv_len_max;
-  const PaPlan p = pa_plan(n, nseq, H, Hkv, dtype, q_len_max, kv_len_max, window, sinks);
+  const PaPlan p = pa_plan(n, nseq, H, Hkv, dtype, q_len_max, kv_len_max, cut, window, sinks);
   const size_t slots = (size_t)p.slots;
   return slots ? align256(slots * Dh * sizeof(float)) + align256(slots * 2 * sizeof(float)) : 0;
 }
@@ -1597,7 +1600,8 @@ int wfd_attn_paged(const void* q, const void* k_pages, const void* v_pages, int6
   a.window = window < kv_len_max ? window : 0;
   a.sinks = sinks < kv_len_max ? sinks : kv_len_max;
   a.scale_log2 = scale * 1.4426950408889634f;
-  const PaPlan p = pa_plan(n, nseq, H, Hkv, dtype, a.qmax, kv_len_max, a.window, a.sinks);
+  a.cut = pa_few_cut(Hkv, window);
+  const PaPlan p = pa_plan(n, nseq, H, Hkv, dtype, a.qmax, kv_len_max, a.cut, a.window, a.sinks);
   if (p.few_units > 0x7fffffff - 65536 || p.many_units > 0x7fffffff - 65536) {
     set_error("%s: n=%d nseq=%d kv_len_max=%d beyond the grid", me, n, nseq, kv_len_max);
     return kUnsupported;
@@ -1606,7 +1610,6 @@ int wfd_attn_paged(const void* q, const void* k_pages, const void* v_pages, int6
   a.pml = (float*)((char*)workspace + align256((size_t)p.slots * Dh * sizeof(float)));
   a.seq_slots = p.seq_slots;
   a.g_magic = 65536 / a.G + 1;
-  a.cut = pa_few_cut(Hkv, a.window);
   a.few_tile = p.few_tile;
   a.many_tile = p.many_tile;
   a.row_per = p.row_per;
