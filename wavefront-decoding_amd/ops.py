@@ -1153,7 +1153,6 @@ def sample_workspace_bytes(n: int, vocab: int) -> int:
 
 
 @functools.lru_cache(maxsize=1024)
-@functools.lru_cache(maxsize=1024)
 def logprobs_workspace_bytes(n: int, vocab: int, top: int) -> int:
     return int(_lib.load().wfd_logprobs_workspace_bytes(n, vocab, top))
 
