@@ -29,8 +29,8 @@ constexpr int kPaRows = 32;  // pairs of a wave: the columns of its 32x32 MFMA
 constexpr int kPaWaves = 4;
 constexpr int kPaMaxG = kPaRows;
 // A sequence's pairs per kv head up to which its rows are "few": read by 32 pairs at a time, with
-// no waiting for other waves. 16 rows of 4 heads over 1000 keys 15.0 us as few, 21.8 as many; 32
-// sequences of 24 such rows 45.6 as few, 31.6 as many.
+// no waiting for other waves. 16 rows of 4 heads over 1000 keys 18.1 us as few, 22.5 as many, 32
+// sequences of them 28.4 and 28.7; 24 such rows 18.0 and 23.3, 32 sequences of these 37.4 and 31.7.
 constexpr int kPaFewPairs = 64;
 constexpr int kPaManyRows = kPaRows * kPaWaves;
 // Keys per block of the few-row kernels and of the many-row one. Blocks, parts and targets are
@@ -52,10 +52,10 @@ constexpr int kPaTarget = 64;
 constexpr int kPaMinPart = 256;
 // Many rows: two workgroups a CU (512 rows behind 7600 keys 75 us, with half as many 91; with the
 // parts' sizes rounded up to powers of two 80 behind 7700) of at least 512 keys: 128 rows of 16
-// heads over 1000 keys 25 us (with 1024: 36, with 256: 22), 32 such sequences 133 (134, 172);
-// twice that for a sequence of 64 (tile, kv head)s, four times for one of 96 (4 x 512 rows over
-// 2048 keys, 4 kv heads, 71 us for 83; 300 rows of 16 heads over 1000 keys, of 48, would take 38
-// for 29).
+// heads over 1000 keys 25 us (with 1024: 36, with 256: 22), 32 such sequences 133 (134, 172).
+// Twice that for a sequence of 64 (tile, kv head)s, four times for one of 96: 500 rows of 16 heads
+// over 2000 keys 42 us for 34, four such sequences 66 for 75; 700 rows (96) 58 us, with twice 44,
+// once 40, four such sequences 76, 91, 99, eight 131, 162, 201.
 constexpr int kPaManyMinPart = 512;
 constexpr int kPaManyLogTarget = 9, kPaManyTarget = 1 << kPaManyLogTarget;
 // Workgroups of a launch, which take the items in turn: of few rows those that the card holds
@@ -584,10 +584,10 @@ __device__ __forceinline__ void pa_keep(int nr, int wave, int col, int hf, const
 __device__ __forceinline__ int pa_listed(const PaTile& t, int c) { return c < t.ns ? c : c - t.ns + t.first; }
 
 // bf16, few rows: bound by the keys and values, each read once per tile of 32 pairs (64 rows of
-// 4 heads x 4 over 32700 keys 742 us, 5.8 TB/s; 112 rows of 16 heads over 127 to 1199 keys 129
-// us, 4.7 TB/s), and for few short sequences by a chain of launch, search, page numbers, keys,
-// merge and, past kPaWhole keys, a second launch that merges the parts (8 rows over 512 to 777
-// keys 16.5 us, 19.4 when each had three parts).
+// 4 heads x 4 over 32700 keys 765 us, 5.6 TB/s; 112 rows of 16 heads over 127 to 1199 keys 124
+// us, 4.9 TB/s), and for few short sequences by a chain of launch, search, page numbers, keys,
+// merge and, where any row may have more than 512 keys, a second launch that merges the parts
+// (8 rows over 511 to 777 keys 18.6 us, 3.9 of them the second launch).
 // Up to 32 pairs per workgroup, one per column of the 32x32x16 MFMA, and
 // four waves that each stream 32-key blocks (pa_wave_blocks) through LDS of their own: whole rows to registers a block ahead, to LDS as loaded,
 // no workgroup barrier before the merge. A wave computes S^T = K Q^T and O^T = V^T P^T;
@@ -768,10 +768,11 @@ __global__ __launch_bounds__(64 * kPaWaves) __attribute__((amdgpu_waves_per_eu(2
 // its page, asked for before the scores; K goes straight to LDS, the next block's once the
 // scores are done, its 16-byte pieces of row r exchanged (piece p at p ^ r % 16) so that a
 // column of them is spread over all banks.
-// Bound by the keys and values, and by the products, 32 cycles each, whose columns few rows
-// leave mostly empty: 127 rows of 33 sequences, 4 heads of 64 over 40 to 2000 keys, 26 us (70
-// MB: 14 us at a copy's rate); 64 rows of 16 heads of 128 over 1000 to 4000 keys, 4 kv heads,
-// 170 us (131). On the 32x32x2 MFMA, K through registers and V in pieces of 4 bytes, 31 and 287.
+// Bound by the keys and values where there are enough of them (64 rows of 16 heads of 128 over
+// 1000 to 4000 keys, 4 kv heads, 156 us, 131 at a copy's rate), by two trips to memory a block,
+// K's and then V's, where a wave has few blocks: 127 rows of 33 sequences, 4 heads of 64 over 40
+// to 2000 keys, 24.5 us (70 MB: 14), 4 of them the merge. On the 32x32x2 MFMA, K through
+// registers and V in pieces of 4 bytes, 31 and 287.
 template <int DH>
 struct PaF32Lds {
   static constexpr int OP = DH + 4;
@@ -1067,7 +1068,7 @@ __global__ __launch_bounds__(64 * kPaWaves) __attribute__((amdgpu_waves_per_eu(2
 // heads (4 kv heads): 920 to 970 TFLOP/s, three quarters of a large library product's rate,
 // the MFMA busy for 37 % of the time, the VALU for 45 %; a workgroup alone on its CU takes
 // 0.63 of that. Under a window of 1024 a tile is 18 blocks, of which 5 lie at an edge, and
-// its first loads and its stores count: 16252 rows of 16 heads 230 us, 580 TFLOP/s.
+// its first loads and its stores count: 16252 rows of 16 heads 228 to 240 us, 560 to 580 TFLOP/s.
 // Measured and not better: eight waves with tiles of 256 pairs (the same, with a window 6 %
 // slower), blocks straight to LDS with the products of the next block between the
 // exponentials of this one (a window: 270 to 305 us), raised priority of one of the two
@@ -1295,7 +1296,7 @@ __device__ __forceinline__ void pa_many_bf16(const PaArgs& a, PaManyLds<DH>& lds
 
 // Both kinds of rows in one launch, so that those bound by memory and those bound by
 // products share the CUs (61 single rows and 3 pieces of prompts of 500 to 1100 rows, 4 kv
-// heads: 275 us, one kernel after the other 307, before parts filled the card exactly):
+// heads: 270 us; when it was 275 one kernel after the other took 307):
 // a.many_wgs of the workgroups of a kv head take many rows,
 // a.many_lead of them (one per CU) before those that take few, the others behind.
 template <int DH>
@@ -1319,7 +1320,8 @@ __global__ __launch_bounds__(64 * kPaWaves) __attribute__((amdgpu_waves_per_eu(2
 // maximum; a row of more a workgroup, whose slot x takes the parts of the sequence that are x
 // modulo its slots, in their order, before the slots are merged in theirs. A part without a key
 // that the row sees (its maximum is -inf) changes nothing in either, so a row's bits do not
-// depend on the parts that its tile has beside its own. Bound by the parts' bytes.
+// depend on the parts that its tile has beside its own. Bound by the parts' bytes: 2170 rows of
+// 16 heads, up to 5 parts of those of prompts, 24 us; 8 rows of 2 parts 3.9, the launch and its search.
 constexpr int kPaWide = 16;
 constexpr int kPaMergeThreads = 256;
 

@@ -21,10 +21,12 @@
 // place. A row with a NaN, or with more candidates than the list takes (equal logits by
 // the thousand), finds its tokens one after the other instead.
 //
-// Bound by the row's bytes, and by the exponentials, 7 instructions a logit, for bf16:
-// 2048 rows of 32000 fp32 logits 58 us (4.5 TB/s) without tokens, 66 with the 20 best
-// (75 before the next row was asked for early), bf16 45 and 64; one row 7 and 11 us,
-// most of it the way of its bytes and five exchanges through LDS.
+// Bound by the row's bytes, for bf16 by the instructions, 17 a logit, 7 of them the sums'
+// (the VALU is busy for 81 % of the time): 2048 rows of 32000 fp32 logits 58 us (4.5 TB/s)
+// without tokens, 71 with the 20 best (66 with the card not at its power limit; 75 before
+// the next row was asked for early), bf16 44 and 59; one row 7 and 11 us, most of it the
+// way of its bytes and five exchanges through LDS. Rows of 128000: 512 fp32 57 and 71 us
+// (4.6 TB/s), bf16 48 and 70, one fp32 row 10 and 16.
 #include "wfd_common.h"
 
 namespace wfd {
