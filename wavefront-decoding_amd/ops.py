@@ -732,7 +732,8 @@ def attn_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, pa
     The row at position p attends keys j <= p, with a `window` (0: none) those
     with j > p - window or j < sinks. kv_len_max bounds the lengths, q_len_max a
     sequence's rows (None: n); rows past these are NaN, rows of no sequence are
-    left as they were."""
+    left as they were. Rows of a sequence that brings up to 64 / (H / Hkv) of
+    them have the bits of single tokens."""
     stream = _need_current(q, k_pages, v_pages, page_table, cu_q, kv_len, out, workspace)
     _need(q.dim() == 3 and q.is_contiguous(), "q must be contiguous (n, H, Dh)")
     n, H, Dh = q.shape
