@@ -43,7 +43,7 @@ enum { WFD_E4M3 = 0, WFD_INT8 = 1 }; /* codes of an 8-bit slot cache */
 /* Message for the last failing call on this thread. */
 const char* wfd_last_error(void);
 /* Bumped when an entry point's signature changes, and up to 8 when one was added (the
-   later ones -- wfd_*_q, wfd_attn_shared, wfd_sample, wfd_*_paged, wfd_logprobs -- are
+   later ones -- wfd_*_q, wfd_attn_shared, wfd_sample, wfd_*_paged*, wfd_logprobs -- are
    found by their symbols; 5: wfd_argmax's accept flags, wfd_attn_varlen_rows; 6: wfd_linear_argmax, wfd_argmax_groups;
    7: folded norm pairs -- wfd_linear_prep, wfd_norm_prep, the row-scale argument of
    wfd_linear, wfd_linear_qkv_rope_append and wfd_linear_argmax; 8: wfd_attn_varlen,
@@ -374,6 +374,12 @@ int wfd_kv_append_paged(const void* k, int64_t ldk, const void* v, int64_t ldv, 
  * sequence's row count and length too; never on the other sequences of the call or on
  * where the pages are. Infinities and NaN in K and V reach only the rows that attend
  * them.
+ *
+ * wfd_attn_paged_by_row: the same with every sequence computed as one of few rows, so
+ * that every row of drafts and prompts of any length has the bits, and its
+ * probabilities the precision, of a single token. Sequences of many rows take about
+ * twice as long (bf16 products in two terms, keys read once per 32 pairs) and a
+ * workspace for the parts of all their rows (wfd_attn_paged_by_row_workspace_bytes).
  * Replaces: attn_varlen over gathered prefixes (src/decoding/fa4_attention.py:301-366,
  *   src/decoding/batch_kv_cache.py:75-96) for a cache in pages; the reference has no
  *   window.
@@ -385,6 +391,13 @@ int wfd_attn_paged(const void* q, const void* k_pages, const void* v_pages, int6
                    const int32_t* cu_q, const int32_t* kv_len, int nseq, void* out, int n, int H, int Hkv, int Dh,
                    int dtype, float scale, int q_len_max, int kv_len_max, int window, int sinks, void* workspace,
                    size_t ws_bytes, wfd_stream_t stream);
+size_t wfd_attn_paged_by_row_workspace_bytes(int n, int nseq, int H, int Hkv, int Dh, int dtype, int q_len_max,
+                                             int kv_len_max, int window, int sinks);
+int wfd_attn_paged_by_row(const void* q, const void* k_pages, const void* v_pages, int64_t kv_block_rows,
+                          const int32_t* page_table, int64_t ld_table, int pages_per_seq, int64_t num_pages,
+                          int page_rows, const int32_t* cu_q, const int32_t* kv_len, int nseq, void* out, int n, int H,
+                          int Hkv, int Dh, int dtype, float scale, int q_len_max, int kv_len_max, int window,
+                          int sinks, void* workspace, size_t ws_bytes, wfd_stream_t stream);
 
 /*
  * SwiGLU of n rows laid out [gate (F) | up (F)] with row stride ldg:

@@ -85,3 +85,43 @@ def test_hundreds_of_sequences(gpu, dtype, window, sinks):
         one = ops.attn_paged(c.q[c.cu[b]: c.cu[b + 1]].clone(), c.k, c.v, c.table[b: b + 1], c.ints([0, m]), c.ints([L]),
                              q_len_max=max(m, 1), kv_len_max=L, window=window, sinks=sinks)
         assert torch.equal(one, out[c.cu[b]: c.cu[b + 1]]), b
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("window,sinks", [(0, 0), (300, 4), (1030, 700)])
+@pytest.mark.parametrize("heads,seqs", [((16, 16, 128), [(200, 2700), (1, 900), (130, 130), (65, 600)]),
+                                        ((8, 1, 64), [(9, 700), (60, 9000), (100, 100)]),
+                                        ((32, 1, 64), [(3, 40), (16, 1500), (1, 513)]),
+                                        ((4, 2, 128), [(600, 600), (70, 17500), (0, 30)])])
+def test_by_row_every_row_has_the_bits_of_a_single_token(gpu, dtype, window, sinks, heads, seqs):
+    """Drafts, pieces of prompts and whole prompts, and the same rows one at a time."""
+    H, Hkv, Dh = heads
+    c = Pages(gpu, dtype, H, Hkv, Dh, seqs, page=64, seed=H, lead=1, tail=2)
+    out = torch.full_like(c.q, 7.0)
+    need = ops.attn_paged_workspace_bytes(c.n, len(seqs), H, Hkv, Dh, dtype, c.q_len_max, c.kv_len_max, window, sinks,
+                                          by_row=True)
+    ws = torch.full((need + 8192,), 0x5a, dtype=torch.uint8, device=gpu)
+    c.attn(out=out, window=window, sinks=sinks, by_row=True, workspace=ws[4096: 4096 + need])
+    assert (ws[:4096] == 0x5a).all() and (ws[4096 + need:] == 0x5a).all()
+    assert (out[:1] == 7.0).all() and (out[c.cu[-1]:] == 7.0).all()
+    rows = [(b, L - m + i + 1) for b, (m, L) in enumerate(seqs) for i in range(m)]
+    n = len(rows)
+    table = c.table[torch.tensor([b for b, _ in rows], device=gpu)]
+    one = ops.attn_paged(c.q[1: 1 + n].clone(), c.k, c.v, table, torch.arange(n + 1, dtype=torch.int32, device=gpu),
+                         c.ints([p for _, p in rows]), q_len_max=1, kv_len_max=c.kv_len_max, window=window,
+                         sinks=sinks)
+    same = (out[1: 1 + n] == one).flatten(1).all(-1).tolist()
+    assert all(same), [(seqs[b], p) for (b, p), ok in zip(rows, same) if not ok][:5]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_by_row_edges(gpu, dtype):
+    """Rows before position 0, past the bounds and of pages outside the pool, as without it."""
+    seqs = [(200, 70), (5, 3), (100, 300), (90, 200), (40, -7), (300, 900)]
+    c = Pages(gpu, dtype, 4, 2, 64, seqs, page=16, seed=8)
+    c.check(c.attn(by_row=True), p_step=2.0 ** -15 if dtype == torch.bfloat16 else 0.0)
+    plain, mine = (c.attn(q_len_max=95, kv_len_max=250, by_row=x) for x in (False, True))
+    assert torch.equal(plain.isnan(), mine.isnan()) and torch.equal(plain == 0, mine == 0)
+    c.table[3, 9] = -1
+    mine = c.attn(by_row=True)
+    assert torch.equal(mine.isnan(), c.attn().isnan()) and mine[c.cu[3] + 40:c.cu[4]].isnan().all()

@@ -178,3 +178,20 @@ def test_workspace_of_parts_that_can_exist():
                 assert need(rows, seqs, H, Hkv, 128, dt, q, 32768) <= rows * H * 64 * slot(128) + 512
     # single tokens under a window: its parts, one more for where it begins, and the sinks'
     assert need(64, 64, 16, 4, 128, bf16, 1, 32768, 4096, 4) <= 64 * 16 * 11 * slot(128) + 512
+
+
+def test_by_row_refuses_what_the_other_refuses():
+    lib = _lib.load()
+    for kw, rc in ((dict(nseq=-1), -1), (dict(rows=24), -1), (dict(Dh=96), -2), (dict(dtype=2), -2), (dict(km=65), -1),
+                   (dict(H=66), -2), (dict(), -1), (dict(ptr=8), -1), (dict(ptr=16, rows=1024, km=4096), -4)):
+        a = dict(n=1, nseq=1, H=4, Hkv=2, Dh=64, dtype=1, ld=4, per=4, pages=9, rows=16, km=64, ptr=None) | kw
+        p = a["ptr"]
+        assert lib.wfd_attn_paged_by_row(p, p, p, 0, p, a["ld"], a["per"], a["pages"], a["rows"], p, p, a["nseq"], p,
+                                         a["n"], a["H"], a["Hkv"], a["Dh"], a["dtype"], 0.1, 1, a["km"], 0, 0, None, 0,
+                                         None) == rc, kw
+        assert b"wfd_attn_paged_by_row" in lib.wfd_last_error(), kw
+    # parts for every row of a prompt, which fp32 sequences of many rows do without
+    need = ops.attn_paged_workspace_bytes
+    args = (2000, 1, 16, 16, 128, torch.float32, 2000, 2000)
+    assert need(*args) < need(*args, by_row=True) <= 2000 * 16 * 4 * 130 * 4 + 512
+    assert need(8, 1, 16, 16, 128, torch.bfloat16, 8, 2000) == need(8, 1, 16, 16, 128, torch.bfloat16, 8, 2000, by_row=True)

@@ -82,6 +82,7 @@ def test_probabilities_of_many_rows(gpu):
     for dtype, step in ((torch.bfloat16, 2.0 ** -8), (torch.float32, 0.0)):
         c = paired(gpu, dtype, 4, 4, 64, seqs)
         c.check(c.attn(), p_step=step)
+        c.check(c.attn(by_row=True), p_step=P_STEP_FEW[dtype])
 
 
 @pytest.mark.gpu

@@ -66,6 +66,9 @@ SIGNATURES: dict[str, tuple] = {
     "wfd_attn_paged_workspace_bytes": (_sz, [_i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32]),
     "wfd_attn_paged": (_i32, [_vp, _vp, _vp, _i64, _vp, _i64, _i32, _i64, _i32, _vp, _vp, _i32, _vp, _i32, _i32, _i32,
                               _i32, _i32, _f32, _i32, _i32, _i32, _i32, _vp, _sz, _vp]),
+    "wfd_attn_paged_by_row_workspace_bytes": (_sz, [_i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32]),
+    "wfd_attn_paged_by_row": (_i32, [_vp, _vp, _vp, _i64, _vp, _i64, _i32, _i64, _i32, _vp, _vp, _i32, _vp, _i32, _i32,
+                                     _i32, _i32, _i32, _f32, _i32, _i32, _i32, _i32, _vp, _sz, _vp]),
     "wfd_linear_k_multiple": (_i32, [_i32]),
     "wfd_linear_pack": (_i32, [_vp, _vp, _i32, _i32, _i32, _i32, _i32, _vp]),
     "wfd_linear": (_i32, [_vp, _vp, _i64, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _vp, _vp]),

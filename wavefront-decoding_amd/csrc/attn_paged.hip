@@ -16,7 +16,8 @@
 // the block's place in the sequence. What a tile holds beside a row then adds hidden keys to
 // it and nothing else, and a hidden key changes no bit: a row has the bits it has alone,
 // as the next token of its context. A sequence of more rows is cut by its own rows and
-// length. In either case the rest of the call has no part in it.
+// length, unless the caller asks for every row's own bits (wfd_attn_paged_by_row). In either
+// case the rest of the call has no part in it.
 #include <algorithm>
 #include <type_traits>
 
@@ -32,6 +33,7 @@ constexpr int kPaMaxG = kPaRows;
 // no waiting for other waves. 16 rows of 4 heads over 1000 keys 18.1 us as few, 22.5 as many, 32
 // sequences of them 28.4 and 28.7; 24 such rows 18.0 and 23.3, 32 sequences of these 37.4 and 31.7.
 constexpr int kPaFewPairs = 64;
+constexpr int kPaAllFew = 0x7fffffff;  // all of them, where every row is to have its own bits
 constexpr int kPaManyRows = kPaRows * kPaWaves;
 // Keys per block of the few-row kernels and of the many-row one. Blocks, parts and targets are
 // powers of two and counted by shifts: each workgroup looks for its own item, and with 64-bit
@@ -94,6 +96,7 @@ struct PaArgs {
   int g_magic;           // x / G = x g_magic >> 16 for x < 128
   int few_tile, many_tile;  // rows of a tile
   int row_per;
+  int few_pairs;         // kPaFewPairs, or kPaAllFew
   uint32_t many_wgs, many_lead;  // of a kv head
   PaCut cut;             // of few rows
   float scale_log2;
@@ -153,7 +156,7 @@ __device__ __forceinline__ PaSeq pa_seq(const PaArgs& a, int b, int c0, int c1, 
   kv = max(kv, 0);
   s.pos0 = kv - (c1 - c0);
   s.ne = min(max(s.nq, 0), a.qmax);
-  const bool large = s.ne * a.G > kPaFewPairs;
+  const bool large = s.ne * a.G > a.few_pairs;
   s.many = sizeof(T) == 2 && large;
   const int rows = s.many ? a.many_tile : a.few_tile, len = min(kv, a.kmax);
   s.tiles = s.ne <= rows ? min(s.ne, 1) : (int)((uint32_t)(s.ne - 1) / (uint32_t)rows) + 1;
@@ -1472,15 +1475,15 @@ static int pa_most_f32(int kmax, int Hkv, int rows, int window, int sinks) {
 }
 
 static PaPlan pa_plan(int n, int nseq, int H, int Hkv, int dtype, int qmax, int kmax, PaCut cut, int window,
-                      int sinks) {
+                      int sinks, int few_pairs) {
   PaPlan p{};
   const int G = H / Hkv;
   if (qmax > n) qmax = n;
-  const bool large = (int64_t)qmax * G > kPaFewPairs;
+  const bool large = (int64_t)qmax * G > few_pairs;
   p.many = dtype == kBF16 && large;
   p.few_tile = kPaRows / G;
   p.many_tile = kPaManyRows / G;
-  const int few_rows = large ? kPaFewPairs / G : qmax;  // of a sequence
+  const int few_rows = large ? few_pairs / G : qmax;  // of a sequence
   const int few = pa_most_parts(cut, kmax, p.few_tile, window, sinks);
   int most = 1;  // of a tile of the other sequences
   if (p.many) most = pa_most_many(pa_blocks(kmax, p.many_tile, window, sinks, kPaManyLogBlock), Hkv);
@@ -1524,13 +1527,8 @@ static void launch_paged(PaArgs a, const PaPlan& p, hipStream_t st) {
                        dim3(kPaMergeThreads), 0, st, a);
 }
 
-}  // namespace wfd
-
-extern "C" {
-
-size_t wfd_attn_paged_workspace_bytes(int n, int nseq, int H, int Hkv, int Dh, int dtype, int q_len_max,
-                                      int kv_len_max, int window, int sinks) {
-  using namespace wfd;
+static size_t pa_workspace(int n, int nseq, int H, int Hkv, int Dh, int dtype, int q_len_max, int kv_len_max,
+                           int window, int sinks, int few_pairs) {
   // 0 for what the call refuses
   if (n <= 0 || nseq <= 0 || H <= 0 || H > 4096 || Hkv <= 0 || H % Hkv || H / Hkv > kPaMaxG || Dh <= 0 || Dh > 128 ||
       q_len_max < 0 || kv_len_max <= 0 || window < 0 || sinks < 0)
@@ -1538,18 +1536,16 @@ size_t wfd_attn_paged_workspace_bytes(int n, int nseq, int H, int Hkv, int Dh, i
   const PaCut cut = pa_few_cut(Hkv, window);
   if (window >= kv_len_max) window = 0;
   if (sinks > kv_len_max) sinks = kv_len_max;
-  const PaPlan p = pa_plan(n, nseq, H, Hkv, dtype, q_len_max, kv_len_max, cut, window, sinks);
+  const PaPlan p = pa_plan(n, nseq, H, Hkv, dtype, q_len_max, kv_len_max, cut, window, sinks, few_pairs);
   const size_t slots = (size_t)p.slots;
   return slots ? align256(slots * Dh * sizeof(float)) + align256(slots * 2 * sizeof(float)) : 0;
 }
 
-int wfd_attn_paged(const void* q, const void* k_pages, const void* v_pages, int64_t kv_block_rows,
+static int pa_call(const char* me, const void* q, const void* k_pages, const void* v_pages, int64_t kv_block_rows,
                    const int32_t* page_table, int64_t ld_table, int pages_per_seq, int64_t num_pages, int page_rows,
                    const int32_t* cu_q, const int32_t* kv_len, int nseq, void* out, int n, int H, int Hkv, int Dh,
-                   int dtype, float scale, int q_len_max, int kv_len_max, int window, int sinks, void* workspace,
-                   size_t ws_bytes, hipStream_t stream) {
-  using namespace wfd;
-  const char* me = "wfd_attn_paged";
+                   int dtype, float scale, int q_len_max, int kv_len_max, int window, int sinks, int few_pairs,
+                   void* workspace, size_t ws_bytes, hipStream_t stream) {
   PaArgs a;
   const int rc = page_map(a.m, me, page_table, ld_table, pages_per_seq, num_pages, page_rows, kv_block_rows, nseq,
                           Hkv, Dh, dtype);
@@ -1576,7 +1572,8 @@ int wfd_attn_paged(const void* q, const void* k_pages, const void* v_pages, int6
     set_error("%s: q, the pages, out and workspace must be 16-byte aligned", me);
     return kBadArg;
   }
-  const size_t need = wfd_attn_paged_workspace_bytes(n, nseq, H, Hkv, Dh, dtype, q_len_max, kv_len_max, window, sinks);
+  const size_t need = pa_workspace(n, nseq, H, Hkv, Dh, dtype, q_len_max, kv_len_max, window, sinks,
+                                   few_pairs);
   if (need && (!workspace || ws_bytes < need)) {
     set_error("%s: workspace %zu bytes < required %zu", me, ws_bytes, need);
     return kWorkspace;
@@ -1603,7 +1600,7 @@ int wfd_attn_paged(const void* q, const void* k_pages, const void* v_pages, int6
   a.sinks = sinks < kv_len_max ? sinks : kv_len_max;
   a.scale_log2 = scale * 1.4426950408889634f;
   a.cut = pa_few_cut(Hkv, window);
-  const PaPlan p = pa_plan(n, nseq, H, Hkv, dtype, a.qmax, kv_len_max, a.cut, a.window, a.sinks);
+  const PaPlan p = pa_plan(n, nseq, H, Hkv, dtype, a.qmax, kv_len_max, a.cut, a.window, a.sinks, few_pairs);
   if (p.few_units > 0x7fffffff - 65536 || p.many_units > 0x7fffffff - 65536) {
     set_error("%s: n=%d nseq=%d kv_len_max=%d beyond the grid", me, n, nseq, kv_len_max);
     return kUnsupported;
@@ -1615,11 +1612,46 @@ int wfd_attn_paged(const void* q, const void* k_pages, const void* v_pages, int6
   a.few_tile = p.few_tile;
   a.many_tile = p.many_tile;
   a.row_per = p.row_per;
+  a.few_pairs = few_pairs;
   if (dtype == kBF16)
     Dh == 64 ? launch_paged<bf16_t, 64>(a, p, stream) : launch_paged<bf16_t, 128>(a, p, stream);
   else
     Dh == 64 ? launch_paged<float, 64>(a, p, stream) : launch_paged<float, 128>(a, p, stream);
   return launch_status(me);
+}
+
+}  // namespace wfd
+
+extern "C" {
+
+size_t wfd_attn_paged_workspace_bytes(int n, int nseq, int H, int Hkv, int Dh, int dtype, int q_len_max,
+                                      int kv_len_max, int window, int sinks) {
+  return wfd::pa_workspace(n, nseq, H, Hkv, Dh, dtype, q_len_max, kv_len_max, window, sinks, wfd::kPaFewPairs);
+}
+
+int wfd_attn_paged(const void* q, const void* k_pages, const void* v_pages, int64_t kv_block_rows,
+                   const int32_t* page_table, int64_t ld_table, int pages_per_seq, int64_t num_pages,
+                   int page_rows, const int32_t* cu_q, const int32_t* kv_len, int nseq, void* out, int n, int H,
+                   int Hkv, int Dh, int dtype, float scale, int q_len_max, int kv_len_max, int window,
+                   int sinks, void* workspace, size_t ws_bytes, hipStream_t stream) {
+  return wfd::pa_call("wfd_attn_paged", q, k_pages, v_pages, kv_block_rows, page_table, ld_table, pages_per_seq,
+                      num_pages, page_rows, cu_q, kv_len, nseq, out, n, H, Hkv, Dh, dtype, scale, q_len_max, kv_len_max,
+                      window, sinks, wfd::kPaFewPairs, workspace, ws_bytes, stream);
+}
+
+size_t wfd_attn_paged_by_row_workspace_bytes(int n, int nseq, int H, int Hkv, int Dh, int dtype, int q_len_max,
+                                             int kv_len_max, int window, int sinks) {
+  return wfd::pa_workspace(n, nseq, H, Hkv, Dh, dtype, q_len_max, kv_len_max, window, sinks, wfd::kPaAllFew);
+}
+
+int wfd_attn_paged_by_row(const void* q, const void* k_pages, const void* v_pages, int64_t kv_block_rows,
+                          const int32_t* page_table, int64_t ld_table, int pages_per_seq, int64_t num_pages,
+                          int page_rows, const int32_t* cu_q, const int32_t* kv_len, int nseq, void* out, int n, int H,
+                          int Hkv, int Dh, int dtype, float scale, int q_len_max, int kv_len_max, int window,
+                          int sinks, void* workspace, size_t ws_bytes, hipStream_t stream) {
+  return wfd::pa_call("wfd_attn_paged_by_row", q, k_pages, v_pages, kv_block_rows, page_table, ld_table, pages_per_seq,
+                      num_pages, page_rows, cu_q, kv_len, nseq, out, n, H, Hkv, Dh, dtype, scale, q_len_max, kv_len_max,
+                      window, sinks, wfd::kPaAllFew, workspace, ws_bytes, stream);
 }
 
 }  // extern "C"

@@ -718,22 +718,24 @@ def kv_append_paged(k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor, kv_len
 
 @functools.lru_cache(maxsize=1024)
 def attn_paged_workspace_bytes(n: int, nseq: int, H: int, Hkv: int, Dh: int, dtype: torch.dtype, q_len_max: int,
-                               kv_len_max: int, window: int = 0, sinks: int = 0) -> int:
-    return int(_lib.load().wfd_attn_paged_workspace_bytes(n, nseq, H, Hkv, Dh, _DT[dtype], q_len_max, kv_len_max,
-                                                          window, sinks))
+                               kv_len_max: int, window: int = 0, sinks: int = 0, by_row: bool = False) -> int:
+    lib = _lib.load()
+    need = lib.wfd_attn_paged_by_row_workspace_bytes if by_row else lib.wfd_attn_paged_workspace_bytes
+    return int(need(n, nseq, H, Hkv, Dh, _DT[dtype], q_len_max, kv_len_max, window, sinks))
 
 
 def attn_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
                cu_q: torch.Tensor, kv_len: torch.Tensor, *, kv_len_max: int, q_len_max: int | None = None,
-               window: int = 0, sinks: int = 0, page_rows: int | None = None, scale: float | None = None,
-               out: torch.Tensor | None = None, workspace: torch.Tensor | None = None) -> torch.Tensor:
+               window: int = 0, sinks: int = 0, by_row: bool = False, page_rows: int | None = None,
+               scale: float | None = None, out: torch.Tensor | None = None, workspace: torch.Tensor | None = None) -> torch.Tensor:
     """Attention of the newest tokens over a paged cache that holds them already
     (wfd_attn_paged): q (n, H, Dh), rows and pages as in qkv_rope_append_paged.
     The row at position p attends keys j <= p, with a `window` (0: none) those
     with j > p - window or j < sinks. kv_len_max bounds the lengths, q_len_max a
     sequence's rows (None: n); rows past these are NaN, rows of no sequence are
     left as they were. Rows of a sequence that brings up to 64 / (H / Hkv) of
-    them have the bits of single tokens."""
+    them have the bits of single tokens; with `by_row` (wfd_attn_paged_by_row,
+    slower for sequences of more) all have."""
     stream = _need_current(q, k_pages, v_pages, page_table, cu_q, kv_len, out, workspace)
     _need(q.dim() == 3 and q.is_contiguous(), "q must be contiguous (n, H, Dh)")
     n, H, Dh = q.shape
@@ -753,15 +755,16 @@ def attn_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, pa
     else:
         _need(out.shape == q.shape and out.dtype == q.dtype and out.is_contiguous(), "bad out")
     dt, lib = _dt(q), _lib.load()
-    need = attn_paged_workspace_bytes(n, nseq, H, lay[0], Dh, q.dtype, q_len_max, kv_len_max, window, sinks)
+    need = attn_paged_workspace_bytes(n, nseq, H, lay[0], Dh, q.dtype, q_len_max, kv_len_max, window, sinks,
+                                      by_row)
     if workspace is None and need:
         workspace = _workspace(need, q.device)
     sc = 1.0 / math.sqrt(Dh) if scale is None else float(scale)
-    rc = lib.wfd_attn_paged(q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), lay[2], *pages, cu_q.data_ptr(),
-                            kv_len.data_ptr(), nseq, out.data_ptr(), n, H, lay[0], Dh, dt, sc, q_len_max,
-                            int(kv_len_max), window, sinks, _p(workspace),
-                            0 if workspace is None else workspace.numel() * workspace.element_size(), stream)
-    _lib.check(rc, "wfd_attn_paged")
+    call = lib.wfd_attn_paged_by_row if by_row else lib.wfd_attn_paged
+    rc = call(q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), lay[2], *pages, cu_q.data_ptr(), kv_len.data_ptr(),
+              nseq, out.data_ptr(), n, H, lay[0], Dh, dt, sc, q_len_max, int(kv_len_max), window, sinks, _p(workspace),
+              0 if workspace is None else workspace.numel() * workspace.element_size(), stream)
+    _lib.check(rc, "wfd_attn_paged_by_row" if by_row else "wfd_attn_paged")
     return out
 
 
